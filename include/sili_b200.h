@@ -423,6 +423,99 @@ int sili_banded_attention_backward(const float* q, const float* k, const float* 
                                    float* dK, float* dV, int64_t groups, int64_t kv_groups, int64_t T, int64_t K,
                                    int64_t d, int64_t half_bandwidth, int causal, void* stream);
 
+/* ── serving: page tables, rotary positions, the 4-bit cache ─────────────
+ * What a decode or prompt step of a folded stack does around its
+ * projections.  No reference counterpart (the reference runs its attention on
+ * whole fp32 sequences).  Device arrays only; every call enqueues its work on
+ * `stream` (NULL: the default stream) and returns without waiting.  Element
+ * types of activations: */
+#define SILI_F32 0
+#define SILI_F16 1
+#define SILI_BF16 2
+
+/* Block tables and slot map of one step.  Request r holds cached[r] tokens in
+ * the pages table[r][0..] and brings fresh[r] more (negative counts as 0).
+ * The pages that the new tokens open are taken, in request order, from
+ * ring[(taken + j) mod ring_size], pool = {taken, given}: pages that ever left
+ * and came into the ring.  Written: those table entries; starts[n + 1], the
+ * new tokens' offsets; lens[n] = cached + fresh; per new token slots (page *
+ * page size + offset) and positions, -1 beyond the last token up to
+ * max_tokens; pool_out; status = {pages that lacked, tokens beyond
+ * max_tokens, pages beyond the table's width}.  A page that lacks is entered
+ * as -1 and its tokens' slots are -1; entries and tokens that lacked can be
+ * asked for again with the same lengths.  Running a call again with the same
+ * inputs writes the same values.  scratch: n + 1 ints, needed above 4096
+ * requests only.  Fewer than 2^31 new tokens. */
+int sili_page_tables(const int* cached, const int* fresh, int n_requests, int* table, int64_t table_stride, int width,
+                     const int* ring, int ring_size, const int64_t* pool, int page, int64_t max_tokens, int* starts,
+                     int* lens, int64_t* slots, int* positions, int64_t* pool_out, int64_t* status, int* scratch,
+                     void* stream);
+/* The pages of the requests with finished[r] != 0 go back to the ring (in
+ * request order, at (given + j) mod ring_size); their table entries become
+ * -1, their lens 0; entries of -1 are passed over.  scratch: n ints. */
+int sili_release_pages(const uint8_t* finished, int n_requests, int* lens, int* table, int64_t table_stride, int width,
+                       int* ring, int ring_size, const int64_t* pool, int page, int64_t* pool_out, int* scratch,
+                       void* stream);
+
+/* cos / sin [n_positions, rot / 2] of position * inv_freq[i] (host array of
+ * rot / 2 doubles; angles in 64 bits), times gain. */
+int sili_rotary_table(const double* inv_freq, int rot, int64_t n_positions, float gain, float* cos_out, float* sin_out,
+                      void* stream);
+/* Rotary positions: the first `rot` of each head's `dim` elements are turned,
+ * pair (a, b) -> (a c - b s, b c + a s) with c, s the table's row of the
+ * token's position; pairs are (i, i + rot/2), or (2i, 2i + 1) when
+ * interleaved; inverse turns back (the gradient).  The rest passes through.
+ * A token with a negative position (padding) gives zeros, one past the table
+ * NaN.  q and k: [tokens, heads, dim] with the last axis contiguous and
+ * strides in elements; either may have no heads; out may be the input.
+ * positions: int32, or int64 with pos64.  dim <= 1024. */
+int sili_rotary(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                int64_t qo_token_stride, int64_t qo_head_stride, int q_heads, const void* k, int64_t k_token_stride,
+                int64_t k_head_stride, void* k_out, int64_t ko_token_stride, int64_t ko_head_stride, int k_heads,
+                int64_t tokens, int dim, int rot, const float* cos, const float* sin, int64_t n_positions,
+                const void* positions, int pos64, int interleaved, int inverse, void* stream);
+
+/* The 4-bit cache: codes [n_pages, 2, kv_heads, page, dim / 2] and scales
+ * [n_pages, 2, kv_heads, page, dim / 32] (K, then V).  Groups of 32 values
+ * along the head share a scale: the byte below the sign of a half (amax / 6,
+ * rounded to three mantissa bits); codes are the layers' FP4 codes, element
+ * 2i in the low nibble; values saturate at 61440; a group holding an infinity
+ * or NaN reads back as NaN.  dim 64, 128 or 256.
+ *
+ * append: K (rotated first when rot > 0, rot a multiple of 16) and V of each
+ * token into its slot; slots outside [0, n_pages * page) are passed over; two
+ * tokens must not share one.  With q_heads > 0, q_out gets the rotated q. */
+int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                    int64_t qo_token_stride, int64_t qo_head_stride, int q_heads, const void* k, int64_t k_token_stride,
+                    int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int kv_heads,
+                    int64_t tokens, int dim, int rot, const float* cos, const float* sin, int64_t n_positions,
+                    const void* positions, int pos64, int interleaved, uint8_t* codes, uint8_t* scales, int64_t n_pages,
+                    int page, const int64_t* slots, void* stream);
+/* The values that the cache holds at the slots: k_out, v_out [tokens,
+ * kv_heads, dim]; zeros for slots outside the cache. */
+int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads, int dim,
+                  const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream);
+/* Causal attention over the cache.  Request r's lens[r] tokens lie in the
+ * pages table[r][0..]; its queries are the rows starts[r] .. starts[r + 1) of
+ * q [tokens, heads, dim] and stand at its last positions (starts NULL: one
+ * query a request, row r).  Query head h reads kv head h / (heads /
+ * kv_heads).  A query sees the keys up to its own position, with window > 0
+ * only the last `window` of them; keys of a page that is not there (an entry
+ * outside [0, n_pages)) are not seen.  out [tokens, heads, dim] =
+ * softmax(scale q k) v, rounded once; lse [tokens, heads] (may be NULL) the
+ * natural log of the softmax's sum.  A row that sees nothing, or belongs to
+ * no request, gives zeros and -inf.  most_new: the largest number of queries
+ * of a request, as the host knows it; it chooses the kernel, not the result.
+ * workspace: sili_kv4_attention_workspace bytes, zeroed once before its first
+ * call and left as a call leaves it; calls that may run at the same time need
+ * one each.  page: a multiple of 16. */
+int sili_kv4_attention_workspace(int64_t* bytes);
+int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
+                       int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads,
+                       const int* table, int64_t table_stride, int width, const int* lens, int requests,
+                       const int* starts, int most_new, float scale, int window, void* out, float* lse, void* workspace,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

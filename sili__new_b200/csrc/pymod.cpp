@@ -781,6 +781,66 @@ PYBIND11_MODULE(_cuda, m) {
     }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("groups"), py::arg("kv_groups"),
        py::arg("T"), py::arg("K"), py::arg("d"), py::arg("half_bandwidth"), py::arg("inner_k") = 0,
        py::arg("causal") = false, py::arg("stream") = 0);
+    // serving operators on device arrays (sili__new_b200.serving)
+    m.def("page_tables_ptr", [](uintptr_t cached, uintptr_t fresh, int n, uintptr_t table, int64_t stride, int width,
+                                uintptr_t ring, int ring_size, uintptr_t pool, int page, int64_t max_tokens,
+                                uintptr_t starts, uintptr_t lens, uintptr_t slots, uintptr_t positions,
+                                uintptr_t pool_out, uintptr_t status, uintptr_t scratch, uintptr_t stream) {
+        check(sili_page_tables((const int*)cached, (const int*)fresh, n, (int*)table, stride, width, (const int*)ring,
+                               ring_size, (const int64_t*)pool, page, max_tokens, (int*)starts, (int*)lens,
+                               (int64_t*)slots, (int*)positions, (int64_t*)pool_out, (int64_t*)status, (int*)scratch,
+                               (void*)stream));
+    });
+    m.def("release_pages_ptr", [](uintptr_t finished, int n, uintptr_t lens, uintptr_t table, int64_t stride, int width,
+                                  uintptr_t ring, int ring_size, uintptr_t pool, int page, uintptr_t pool_out,
+                                  uintptr_t scratch, uintptr_t stream) {
+        check(sili_release_pages((const uint8_t*)finished, n, (int*)lens, (int*)table, stride, width, (int*)ring,
+                                 ring_size, (const int64_t*)pool, page, (int64_t*)pool_out, (int*)scratch,
+                                 (void*)stream));
+    });
+    m.def("rotary_table_ptr", [](darr inv_freq, int64_t n_positions, float gain, uintptr_t c, uintptr_t s,
+                                 uintptr_t stream) {
+        check(sili_rotary_table(inv_freq.data(), 2 * (int)inv_freq.size(), n_positions, gain, (float*)c, (float*)s,
+                                (void*)stream));
+    });
+    m.def("rotary_ptr", [](int dtype, uintptr_t q, int64_t qt, int64_t qh, uintptr_t qo, int64_t qot, int64_t qoh,
+                           int q_heads, uintptr_t k, int64_t kt, int64_t kh, uintptr_t ko, int64_t kot, int64_t koh,
+                           int k_heads, int64_t tokens, int dim, int rot, uintptr_t c, uintptr_t s, int64_t n_positions,
+                           uintptr_t positions, bool pos64, bool interleaved, bool inverse, uintptr_t stream) {
+        check(sili_rotary(dtype, (const void*)q, qt, qh, (void*)qo, qot, qoh, q_heads, (const void*)k, kt, kh, (void*)ko,
+                          kot, koh, k_heads, tokens, dim, rot, (const float*)c, (const float*)s, n_positions,
+                          (const void*)positions, pos64, interleaved, inverse, (void*)stream));
+    });
+    m.def("kv4_append_ptr", [](int dtype, uintptr_t q, int64_t qt, int64_t qh, uintptr_t qo, int64_t qot, int64_t qoh,
+                               int q_heads, uintptr_t k, int64_t kt, int64_t kh, uintptr_t v, int64_t vt, int64_t vh,
+                               int kv_heads, int64_t tokens, int dim, int rot, uintptr_t c, uintptr_t s,
+                               int64_t n_positions, uintptr_t positions, bool pos64, bool interleaved, uintptr_t codes,
+                               uintptr_t scales, int64_t n_pages, int page, uintptr_t slots, uintptr_t stream) {
+        check(sili_kv4_append(dtype, (const void*)q, qt, qh, (void*)qo, qot, qoh, q_heads, (const void*)k, kt, kh,
+                              (const void*)v, vt, vh, kv_heads, tokens, dim, rot, (const float*)c, (const float*)s,
+                              n_positions, (const void*)positions, pos64, interleaved, (uint8_t*)codes,
+                              (uint8_t*)scales, n_pages, page, (const int64_t*)slots, (void*)stream));
+    });
+    m.def("kv4_read_ptr", [](int dtype, uintptr_t codes, uintptr_t scales, int64_t n_pages, int page, int kv_heads,
+                             int dim, uintptr_t slots, int64_t tokens, uintptr_t k, uintptr_t v, uintptr_t stream) {
+        check(sili_kv4_read(dtype, (const uint8_t*)codes, (const uint8_t*)scales, n_pages, page, kv_heads, dim,
+                            (const int64_t*)slots, tokens, (void*)k, (void*)v, (void*)stream));
+    });
+    m.def("kv4_attention_workspace", []() {
+        int64_t n = 0;
+        check(sili_kv4_attention_workspace(&n));
+        return n;
+    });
+    m.def("kv4_attention_ptr", [](int dtype, uintptr_t q, int64_t qt, int64_t qh, int64_t tokens, int heads, int dim,
+                                  uintptr_t codes, uintptr_t scales, int64_t n_pages, int page, int kv_heads,
+                                  uintptr_t table, int64_t stride, int width, uintptr_t lens, int requests,
+                                  uintptr_t starts, int most_new, float scale, int window, uintptr_t out, uintptr_t lse,
+                                  uintptr_t workspace, uintptr_t stream) {
+        check(sili_kv4_attention(dtype, (const void*)q, qt, qh, tokens, heads, dim, (const uint8_t*)codes,
+                                 (const uint8_t*)scales, n_pages, page, kv_heads, (const int*)table, stride, width,
+                                 (const int*)lens, requests, (const int*)starts, most_new, scale, window, (void*)out,
+                                 (float*)lse, (void*)workspace, (void*)stream));
+    });
     m.def("fp32_fma_peak", [](int device, int iters) {
         double tf = 0, ms = 0;
         check(sili_fp32_fma_peak(device, iters, &tf, &ms));
