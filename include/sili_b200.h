@@ -506,8 +506,8 @@ int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_
  * natural log of the softmax's sum.  A row that sees nothing, or belongs to
  * no request, gives zeros and -inf.  most_new: the largest number of queries
  * of a request, as the host knows it; it chooses the kernel, not the result.
- * workspace: sili_kv4_attention_workspace bytes, zeroed once before its first
- * call and left as a call leaves it; calls that may run at the same time need
+ * workspace: sili_kv4_attention_workspace bytes, the first 4096 of them zeroed
+ * once before its first call, and left as a call leaves it; calls that may run at the same time need
  * one each.  page: a multiple of 16. */
 int sili_kv4_attention_workspace(int64_t* bytes);
 int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,

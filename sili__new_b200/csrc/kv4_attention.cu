@@ -1,9 +1,38 @@
-// Attention over the 4-bit paged cache: one warp per (query token, head),
-// keys one by one, an online softmax in fp32.
+// Attention over the 4-bit paged cache on the warp's matrix instructions, for
+// decode steps (one or a few queries a request), for fp32 activations, and
+// for short prompts; long 16-bit prompts run in kv4_prompt.cu.
+//
+// For one kv head of one request, with rows rho = (query token, query head of
+// the group), the kernel accumulates the transposed products
+//   S^T [keys, rows] = K Q^T,   O^T [dim, rows] += V^T P^T
+// so that the cache is always the 16-row operand of mma.m16n8k16 and few
+// query rows fill the 8-wide one.  The 4-bit operands are turned into exact
+// halves in registers: cvt.f16x2.e2m1x2 of the stored bytes times the group's
+// scale (2 + 4 significant bits).  K bytes lie as the fragment wants them (a
+// thread's dim/4 consecutive elements are its share of every k step); V wants
+// two keys in one register, so the nibbles of two keys are interleaved before
+// the conversion (4 logic operations for 16 values).
+//
+// fp32 queries and probabilities are split into two halves (hi + lo, 22 bits,
+// after scaling a row by a power of two), 16-bit queries are exact in one;
+// probabilities are then rounded to one half (relative 2^-12, below the
+// output's own rounding).  Sums, maxima and outputs are fp32.  The running
+// maximum is moved only when a logit exceeds it by 2^7 (p <= 2^15 is still a
+// half): a warp vote in place of a reduction per tile.
+//
+// Work is cut evenly whatever the lengths: a unit is 128 keys of one (request,
+// kv head, row tile), all units are numbered in order, and each of the
+// launch's CTAs takes an equal run of them, found from the lengths on the
+// device.  A segment (all units of one row tile) that several CTAs share is
+// joined by whichever of them finishes last, in CTA order, so the result does
+// not depend on which that is.  Warps take 16 keys each (within one page) and
+// keep a ring of cp.async stages; the page of the next tile is fetched one
+// step ahead.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.cuh"
@@ -47,64 +76,705 @@ struct AttendArgs {
     int window;
     void* out;             // [tokens, heads, dim]
     float* lse;            // [tokens, heads] or null
+    void* workspace;
+    int page_shift;        // log2(page), or -1
 };
 
-template <typename T, int E>
-__global__ void __launch_bounds__(128) k_attend_simple(AttendArgs a) {
-    constexpr int kDim = 32 * E;
-    const int lane = threadIdx.x & 31;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= a.tokens * a.heads) return;
-    const int64_t t = id / a.heads;
-    const int h = (int)(id - t * a.heads), g = h / (a.heads / a.kv_heads);
-    int r = -1, ahead = 0;   // the token's request and how many of its tokens follow
-    if (a.starts) {
-        for (int i = 0; i < a.requests; ++i)
-            if (a.starts[i] <= t && t < a.starts[i + 1]) { r = i; ahead = (int)(a.starts[i + 1] - 1 - t); break; }
-    } else if (t < a.requests) {
-        r = (int)t;
+constexpr int kWarps = 8;
+constexpr int kUnit = 16 * kWarps;      // keys of a unit
+constexpr int kMaxStages = 4;
+constexpr int kMaxCtas = 2 * 148;       // two CTAs an SM; one for the wider row tiles
+// p = 2^(x - m + 8): room below (a half's subnormals start at 2^-32 of the largest) and above (x may exceed m by 7)
+constexpr float kLift = 8.f, kSlack = 7.f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kTicketBytes = 4096;
+
+constexpr int64_t workspace_bytes() {
+    // two partial results a CTA: rows * (dim + 2) floats
+    return kTicketBytes + (int64_t)kMaxCtas * 2 * 32 * 130 * 4;
+}
+
+template <int E, int NT>
+struct Layout {
+    static constexpr int kDim = 32 * E, kRowBytes = kDim / 2, kRows = 8 * NT;
+    static constexpr int kStages = E == 8 && NT == 2 ? 2 : kMaxStages;   // what shared memory holds beside the join space
+    static constexpr int kCodes = 16 * kRowBytes, kScales = 16 * E;
+    static constexpr int kStage = 2 * (kCodes + kScales);
+    static constexpr int kJoinRow = kDim + 4;           // floats; + 4 spreads the rows over the banks
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kJoin = kWarps * kRows * (kJoinRow + 2) * 4;
+};
+template <typename T, int E, int NT>
+constexpr int smem_bytes() {
+    using L = Layout<E, NT>;
+    constexpr int terms = sizeof(T) == 4 ? 2 : 1;
+    return L::kRing + L::kJoin + (NT > 1 ? NT * 2 * E * terms * 32 * 8 : 0);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t c;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// what is left of (lo, hi) after rounding to the halves h
+__device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t h) {
+    const float2 f = sili::half2_bits_to_float2(h);
+    return pack2(lo - f.x, hi - f.y);
+}
+
+// One request's share of the work.
+struct Req {
+    int row0, nq, len;     // first query row, queries, keys
+    int64_t pos0;          // position of the first query (negative: it sees nothing)
+    int k0, units, tiles;  // first unit of keys, units and row tiles
+};
+
+template <int ROWS>
+__device__ __forceinline__ Req request(const AttendArgs& a, int r) {
+    Req q;
+    int64_t s0 = r, s1 = r + 1;
+    if (a.starts) { s0 = a.starts[r]; s1 = a.starts[r + 1]; }
+    s0 = min(max(s0, (int64_t)0), a.tokens);
+    s1 = min(max(s1, s0), a.tokens);
+    q.row0 = (int)s0;
+    q.nq = (int)(s1 - s0);
+    const int all = max(a.lens[r], 0);
+    q.len = (int)min(min((int64_t)all, (int64_t)a.width * a.page), (int64_t)0x7FFFFF00);
+    q.pos0 = (int64_t)all - q.nq;
+    const int64_t from = a.window ? max(q.pos0 - a.window + 1, (int64_t)0) : 0;
+    q.k0 = (int)(from / kUnit);
+    q.units = max((q.len + kUnit - 1) / kUnit - q.k0, 1);
+    const int group = a.heads / a.kv_heads;
+    q.tiles = (q.nq * group + ROWS - 1) / ROWS;
+    return q;
+}
+__device__ __forceinline__ int64_t units_of(const AttendArgs& a, const Req& q) {
+    return (int64_t)q.units * q.tiles * a.kv_heads;
+}
+
+// A position in the numbered units: request, segment (kv head, row tile) and unit of keys.
+template <int ROWS>
+struct Cursor {
+    Req q;
+    int r, seg, u;
+    __device__ __forceinline__ void next(const AttendArgs& a) {
+        if (++u < q.k0 + q.units) return;
+        if (++seg == q.tiles * a.kv_heads) {
+            do {
+                if (++r >= a.requests) return;      // past the last unit; never read there
+                q = request<ROWS>(a, r);
+            } while (q.tiles == 0);
+            seg = 0;
+        }
+        u = q.k0;
     }
-    float q[E], o[E], m = -INFINITY, l = 0.f;
+};
+
+// Sets `c` to unit `first` of the request that holds unit c.x of all;
+// returns the number of all units.  One scan of the lengths by the CTA.
+template <int ROWS>
+__device__ int64_t locate(const AttendArgs& a, Cursor<ROWS>& c, int cta, int ctas, int64_t& begin, int64_t& end) {
+    __shared__ int64_t s_part[kWarps], s_hit[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int64_t mine = 0;
+    for (int r = tid; r < a.requests; r += kWarps * 32) mine += units_of(a, request<ROWS>(a, r));
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        q[i] = sili::to_f32(((const T*)a.q)[t * a.qt + h * a.qh + lane * E + i]) * a.scale;
-        o[i] = 0.f;
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s_part[warp] = mine;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all += s_part[w];
+    ctas = (int)min((int64_t)ctas, all);    // no more CTAs than units: every one of them has some
+    if (cta >= ctas) { begin = end = 0; return all; }
+    begin = all * cta / ctas;
+    end = all * (cta + 1) / ctas;
+    int64_t before = 0;
+    for (int base = 0; base < a.requests; base += kWarps * 32) {
+        const int r = base + tid;
+        const int64_t n = r < a.requests ? units_of(a, request<ROWS>(a, r)) : 0;
+        int64_t x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += t;
+        }
+        __syncthreads();
+        if (lane == 31) s_part[warp] = x;
+        __syncthreads();
+        int64_t total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) x += s_part[w];
+            total += s_part[w];
+        }
+        x += before;
+        if (x - n <= begin && begin < x) { s_hit[0] = r; s_hit[1] = begin - (x - n); }
+        before += total;
+        if (begin < before) break;
     }
-    if (r >= 0) {
-        const int64_t len = min((int64_t)max(a.lens[r], 0), (int64_t)a.width * a.page);
-        const int64_t pos = (int64_t)a.lens[r] - 1 - ahead;
-        const int64_t end = min(len, pos + 1), from = a.window ? max(pos - a.window + 1, (int64_t)0) : 0;
-        for (int64_t j = from; j < end; ++j) {
-            const int64_t c = j / a.page;
-            const int pg = a.table[r * a.stride + c];
-            if (pg < 0 || pg >= a.n_pages) continue;
-            float kv[2][E];
+    __syncthreads();
+    c.r = (int)s_hit[0];
+    c.q = request<ROWS>(a, c.r);
+    c.seg = (int)(s_hit[1] / c.q.units);
+    c.u = c.q.k0 + (int)(s_hit[1] % c.q.units);
+    return all;
+}
+
+template <typename T, int E, int NT>
+struct Attend {
+    using L = Layout<E, NT>;
+    static constexpr int kStages = L::kStages;
+    static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kDim = L::kDim, kRows = L::kRows, kSteps = kDim / 16;
+    using Cur = Cursor<kRows>;
+
+    const AttendArgs& a;
+    const int lane, warp, g, t;
+    uint8_t* ring;         // this warp's stages
+    uint32_t ring_at;
+    int* flags;            // per stage: the tile holds keys
+    float* join;
+    uint32_t* qs;          // Q fragments in shared memory (NT > 1)
+
+    // the current segment
+    uint32_t qf[NT > 1 ? 1 : kSteps][kTerms][2];
+    float cf[NT][2];       // logit = S * cf, in powers of two
+    float m[NT][2], l[NT][2], o[kSteps][NT][4];
+    int64_t pos[NT][2], first_pos, last_pos;
+
+    __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, int* all_flags)
+        : a(args), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
+        ring = smem + warp * (kStages * L::kStage);
+        ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+        flags = all_flags + warp * kStages;
+        join = (float*)(smem + L::kRing);
+        qs = (uint32_t*)(smem + L::kRing + L::kJoin);
+    }
+
+    // the key of S's row m (the same permutation in both halves of 8): a thread's four P entries are then keys
+    // t, 4 + t, 8 + t, 12 + t, whose V rows it reads without bank conflicts
+    static __device__ __forceinline__ int key_of(int m) { return (m >> 1) + 4 * (m & 1); }
+
+    // 16-byte chunk c of a key's code row, as stored in a stage
+    static __device__ __forceinline__ int k_chunk(int key, int c) { return E == 8 ? c ^ ((key >> 2) & 1) : c; }
+    static __device__ __forceinline__ int v_chunk(int key, int c) {
+        return E == 8 ? c ^ (2 * (key & 3)) : E == 4 ? c ^ (2 * ((key >> 1) & 1)) : c;
+    }
+
+    __device__ __forceinline__ int page_col(int key0) const {
+        return a.page_shift >= 0 ? key0 >> a.page_shift : key0 / a.page;
+    }
+    __device__ __forceinline__ int fetch_page(const Cur& c) const {
+        const int key0 = c.u * kUnit + warp * 16;
+        return key0 < c.q.len ? __ldg(a.table + c.r * a.stride + page_col(key0)) : -1;
+    }
+
+    // starts the copy of cursor c's tile of page pg into stage s
+    __device__ __forceinline__ void issue(const Cur& c, int pg, int s) {
+        const bool there = pg >= 0 && pg < a.n_pages;
+        if (there) {
+            const int key0 = c.u * kUnit + warp * 16;
+            const int h = c.seg / c.q.tiles, off = key0 - page_col(key0) * a.page;
+            const int64_t kr = sili::kv4_row(pg, 0, h, a.kv_heads, a.page) + off;
+            const int64_t vr = kr + (int64_t)a.kv_heads * a.page;
+            const uint32_t at = ring_at + s * L::kStage;
+            constexpr int kPer = L::kRowBytes / 16;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const int64_t at = sili::kv4_row(pg, w, g, a.kv_heads, a.page) + (j - c * a.page);
-                const uint8_t* p = a.codes + at * (kDim / 2) + lane * (E / 2);
-                const float sc = sili::kv4_scale(a.scales[at * E + lane / (32 / E)]);
+            for (int i = 0; i < 16 * kPer / 32; ++i) {
+                const int n = i * 32 + lane, key = n / kPer, c16 = n % kPer;
+                cp16(at + key * L::kRowBytes + k_chunk(key, c16) * 16, a.codes + kr * L::kRowBytes + n * 16);
+                cp16(at + L::kCodes + key * L::kRowBytes + v_chunk(key, c16) * 16, a.codes + vr * L::kRowBytes + n * 16);
+            }
+            constexpr int kSc = L::kScales / 16;
+            if (lane < 2 * kSc) {
+                const int w = lane >= kSc, n = lane - w * kSc;
+                cp16(at + 2 * L::kCodes + lane * 16, a.scales + (w ? vr : kr) * E + n * 16);
+            }
+        }
+        if (lane == 0) flags[s] = there;
+    }
+
+    __device__ __forceinline__ void begin_segment(const Cur& c) {
+        const int h = c.seg / c.q.tiles, tile = c.seg - h * c.q.tiles, group = a.heads / a.kv_heads;
+        const int rows = c.q.nq * group, row0 = tile * kRows;     // below 2^31: the host has checked tokens * heads
+        first_pos = c.q.pos0 + row0 / group;
+        last_pos = c.q.pos0 + (min(row0 + kRows, rows) - 1) / group;
+        if (NT > 1) __syncthreads();    // the last segment's fragments have been read
 #pragma unroll
-                for (int i = 0; i < E / 2; ++i) {
-                    kv[w][2 * i] = sili::fp4_decode(p[i] & 15u) * sc;
-                    kv[w][2 * i + 1] = sili::fp4_decode(p[i] >> 4) * sc;
+        for (int n = 0; n < NT; ++n) {
+            const int row = row0 + n * 8 + g;
+            const bool real = row < rows;
+            const int64_t tok = c.q.row0 + (real ? row / group : 0);
+            const int head = h * group + (real ? row % group : 0);
+            const T* src = (const T*)a.q + tok * a.qt + head * a.qh + t * (kDim / 4);
+            constexpr int kPart = 8 / sizeof(T) < 4 ? 2 : 4;     // elements of an 8-byte access
+            // NT > 1: warp n % kWarps alone prepares row tile n for all
+            if (NT == 1 || warp == n) {
+                float f = 1.f, x[kDim / 4];
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < kDim / 4; i += kPart) {
+                    sili::Pack<T, kPart> p;
+                    if (real) p = *(const sili::Pack<T, kPart>*)(src + i);
+#pragma unroll
+                    for (int j = 0; j < kPart; ++j) {
+                        x[i + j] = real ? sili::to_f32(p.v[j]) : 0.f;
+                        top = max(top, __float_as_uint(x[i + j]) & 0x7FFFFFFFu);
+                    }
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // the row's largest into [2^14, 2^15): a half holds it, and 38 binary digits below it
+                int e = 0;
+                if (!std::is_same<T, __half>::value && top && top < 0x7F800000u) {
+                    e = 14 - max((int)(top >> 23) - 127, -100);
+                    f = __int_as_float((127 + e) << 23);
+                }
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const float u = x[4 * i + 2 * p] * f, v = x[4 * i + 2 * p + 1] * f;
+                        const uint32_t hi = pack2(u, v);
+                        if (NT == 1) qf[NT > 1 ? 0 : i][0][p] = hi;
+                        else qs[(((n * kSteps + i) * kTerms) * 32 + lane) * 2 + p] = hi;
+                        if (kTerms == 2) {
+                            const uint32_t lo = rest2(u, v, hi);
+                            if (NT == 1) qf[NT > 1 ? 0 : i][kTerms - 1][p] = lo;
+                            else qs[(((n * kSteps + i) * kTerms + kTerms - 1) * 32 + lane) * 2 + p] = lo;
+                        }
+                    }
+                }
+                // undo the scaling; the thread's columns are rows 2t and 2t + 1, held by lanes of g = 2t, 2t + 1
+                const float back = a.scale * kLog2e * __int_as_float((127 - e) << 23);
+                cf[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+                cf[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+                if (NT > 1) {
+                    float* s_cf = (float*)flags - warp * kStages + kWarps * kMaxStages;
+                    if (t == 0) s_cf[n * 8 + g] = back;
                 }
             }
-            float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = fmaf(q[i], kv[0][i], s);
-            s = sili::warp_sum(s);
-            const float mn = fmaxf(m, s), f = m == mn ? 1.f : expf(m - mn), p = expf(s - mn);
-            l = l * f + p;
+            for (int j = 0; j < 2; ++j) {
+                const int col = min(row0 + n * 8 + 2 * t + j, rows - 1);
+                pos[n][j] = c.q.pos0 + col / group;
+                m[n][j] = -INFINITY;
+                l[n][j] = 0.f;
+            }
+        }
+        if (NT > 1) {
+            __syncthreads();
+            const float* s_cf = (const float*)flags - warp * kStages + kWarps * kMaxStages;
 #pragma unroll
-            for (int i = 0; i < E; ++i) o[i] = fmaf(p, kv[1][i], o[i] * f);
-            m = mn;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) cf[n][j] = s_cf[n * 8 + 2 * t + j];
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
+    }
+
+    __device__ __forceinline__ bool sees(int64_t key, int n, int j, int len) const {
+        return key <= pos[n][j] && key < len && (!a.window || key > pos[n][j] - a.window);
+    }
+
+    __device__ __forceinline__ void tile(const Cur& c, int s) {
+        const int key0 = c.u * kUnit + warp * 16, len = c.q.len;
+        if (!flags[s] || key0 > last_pos || (a.window && key0 + 15 <= first_pos - a.window)) return;
+        const uint8_t* st = ring + s * L::kStage;
+        const int ka = key_of(g);
+        float x[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[n][j] = 0.f;
+        {   // S^T = K Q^T
+            constexpr int kWords = kDim / 32;      // words of codes a thread and row
+            uint32_t w[2][kWords];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = ka + 8 * i;
+                const uint8_t* row = st + key * L::kRowBytes;
+                if constexpr (E == 2) {
+                    const uint2 v = *(const uint2*)(row + t * 8);
+                    w[i][0] = v.x; w[i][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < E / 4; ++q) {
+                        const uint4 v = *(const uint4*)(row + k_chunk(key, t * (E / 4) + q) * 16);
+                        w[i][4 * q] = v.x; w[i][4 * q + 1] = v.y; w[i][4 * q + 2] = v.z; w[i][4 * q + 3] = v.w;
+                    }
+                }
+            }
+            const uint8_t* sc = st + 2 * L::kCodes;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                const int grp = E == 2 ? t >> 1 : E == 4 ? t : 2 * t + j / 4;
+                uint32_t f[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t sb = sc[(ka + 8 * i) * E + grp] * 0x00800080u;
+                    sili::kv4_decode4(w[i][j], f[i]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) f[i][q] = mul2(f[i][q], sb);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int q = 0; q < kTerms; ++q) {
+                            uint32_t b0, b1;
+                            if (NT == 1) { b0 = qf[NT > 1 ? 0 : 2 * j + k][q][0]; b1 = qf[NT > 1 ? 0 : 2 * j + k][q][1]; }
+                            else {
+                                const uint2 b = ((const uint2*)qs)[((n * kSteps + 2 * j + k) * kTerms + q) * 32 + lane];
+                                b0 = b.x; b1 = b.y;
+                            }
+                            mma(x[n], f[0][2 * k], f[1][2 * k], f[0][2 * k + 1], f[1][2 * k + 1], b0, b1);
+                        }
+            }
+        }
+        // logits in powers of two, masked
+        const bool inside = key0 + 15 < len && key0 + 15 <= first_pos && (!a.window || key0 > last_pos - a.window);
+        bool above = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[n][j] *= cf[n][j & 1];
+                if (!inside && !sees(key0 + ka + 8 * (j >> 1), n, j & 1, len)) x[n][j] = -INFINITY;
+                above = above || x[n][j] > m[n][j & 1] + kSlack;
+            }
+        if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float top = fmaxf(x[n][j], x[n][j + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float mn = fmaxf(m[n][j], top);
+                    const float f = mn == m[n][j] ? 1.f : ex2(m[n][j] - mn);
+                    m[n][j] = mn;
+                    l[n][j] *= f;
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) { o[i][n][j] *= f; o[i][n][j + 2] *= f; }
+                }
+        }
+        // P^T fragments
+        uint32_t p[NT][kTerms][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float base = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1] - kLift;
+                x[n][j] = ex2(x[n][j] - base);
+                l[n][j & 1] += x[n][j];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t hi = pack2(x[n][2 * i], x[n][2 * i + 1]);
+                if (kTerms == 2) p[n][kTerms - 1][i] = transpose8(rest2(x[n][2 * i], x[n][2 * i + 1], hi));
+                p[n][0][i] = transpose8(hi);
+            }
+        }
+        {   // O^T += V^T P^T
+            constexpr int kWords = kDim / 64;      // words of codes a thread and key
+            const uint8_t* vs = st + L::kCodes;
+            const uint8_t* sc = st + 2 * L::kCodes + L::kScales;
+            const int grp = E == 2 ? g >> 2 : E == 4 ? g >> 1 : g;
+            uint32_t w[4][kWords], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = 4 * i + t;
+                const uint8_t* row = vs + key * L::kRowBytes;
+                if constexpr (E == 2) w[i][0] = *(const uint32_t*)(row + g * 4);
+                else if constexpr (E == 4) {
+                    const uint2 v = *(const uint2*)(row + v_chunk(key, g >> 1) * 16 + (g & 1) * 8);
+                    w[i][0] = v.x; w[i][1] = v.y;
+                } else {
+                    const uint4 v = *(const uint4*)(row + v_chunk(key, g) * 16);
+                    w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+                }
+                b[i] = sc[key * E + grp];
+            }
+            // A scale that is not a number reaches only the rows that see its key: such groups are left out of the
+            // product (0 * NaN would reach every row) and entered by hand.
+            const bool odd = max(max(b[0], b[1]), max(b[2], b[3])) >= 0xF8u;
+            if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = b[i] >= 0xF8u ? 0u : b[i];
+                for (int key = 0; key < 16; ++key) {
+                    if (sc[key * E + grp] < 0xF8u) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            if (sees(key0 + key, n, j, len))
+#pragma unroll
+                                for (int i = 0; i < kSteps; ++i)
+                                    o[i][n][j] = o[i][n][j + 2] = __int_as_float(0x7FC00000);
+                }
+            }
+            const uint32_t s01 = b[0] << 7 | b[1] << 23, s23 = b[2] << 7 | b[3] << 23;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                constexpr uint32_t kLow = 0x0F0F0F0Fu;
+                uint32_t f[4][4];      // keys (t, 4 + t) even / odd elements, then keys (8 + t, 12 + t)
+                sili::kv4_decode4((w[0][j] & kLow) | ((w[1][j] << 4) & ~kLow), f[0]);
+                sili::kv4_decode4(((w[0][j] >> 4) & kLow) | (w[1][j] & ~kLow), f[1]);
+                sili::kv4_decode4((w[2][j] & kLow) | ((w[3][j] << 4) & ~kLow), f[2]);
+                sili::kv4_decode4(((w[2][j] >> 4) & kLow) | (w[3][j] & ~kLow), f[3]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t a0 = mul2(f[0][q], s01), a1 = mul2(f[1][q], s01), a2 = mul2(f[2][q], s23),
+                                   a3 = mul2(f[3][q], s23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < kTerms; ++k) mma(o[4 * j + q][n], a0, a1, a2, a3, p[n][k][0], p[n][k][1]);
+                }
+            }
         }
     }
+
+    __device__ __forceinline__ float* partial(int cta, int slot) const {
+        return (float*)((uint8_t*)a.workspace + kTicketBytes) + (int64_t)(cta * 2 + slot) * kRows * (kDim + 2);
+    }
+
+    // out and lse of one row and four of its values
+    __device__ __forceinline__ void store(const Cur& c, int row, int d, const float (&v)[4], float top, float sum) const {
+        const int h = c.seg / c.q.tiles, group = a.heads / a.kv_heads;
+        const int at = (c.seg - h * c.q.tiles) * kRows + row;
+        if (at >= c.q.nq * group) return;
+        const int64_t id = (int64_t)(c.q.row0 + at / group) * a.heads + h * group + at % group;
+        // sum 0: the row saw nothing; NaN goes through
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        sili::Pack<T, 4> out;
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-        ((T*)a.out)[id * kDim + lane * E + i] = sili::from_f32<T>(l > 0.f ? o[i] / l : (l == 0.f ? 0.f : l));
-    if (lane == 0 && a.lse) a.lse[id] = l == 0.f ? -INFINITY : m + logf(l);
+        for (int i = 0; i < 4; ++i) out.v[i] = sili::from_f32<T>(v[i] * inv);
+        *(sili::Pack<T, 4>*)((T*)a.out + id * kDim + d) = out;
+        if (d == 0 && a.lse) a.lse[id] = sum == 0.f ? -INFINITY : kLn2 * (top - kLift + log2f(sum));
+    }
+
+    // The segment's end in this CTA: joins the warps, then writes the rows, or leaves them to the CTA that comes last.
+    // seg0 and seg1 number the segment's first unit and the one past its last.
+    __device__ __forceinline__ void end_segment(const Cur& c, int64_t seg0, int64_t seg1, int64_t begin, int64_t end,
+                                                int64_t all, int* s_last) {
+        constexpr int kThreads = kWarps * 32, kQuads = kDim / 4;
+        float* jm = join + kWarps * kRows * L::kJoinRow;       // [warp][row] maxima, then sums
+        float* jl = jm + kWarps * kRows;
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float s = l[n][j];
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 8);
+                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                const int row = warp * kRows + n * 8 + 2 * t + j;
+                if (g == 0) { jm[row] = m[n][j]; jl[row] = s; }
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+                    *(float2*)(join + row * L::kJoinRow + g * (kDim / 8) + 2 * i) = make_float2(o[i][n][j], o[i][n][j + 2]);
+            }
+        __syncthreads();
+        const bool whole = seg0 >= begin && seg1 <= end;
+        const int64_t ctas = min((int64_t)gridDim.x, all);
+        const int cta = blockIdx.x;
+        const int lead = whole ? cta : (int)(((seg0 + 1) * ctas - 1) / all);
+        float* part = whole ? nullptr : partial(cta, cta == lead);
+        for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
+            const int row = i / kQuads, d = i % kQuads * 4;
+            float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[w * kRows + row]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float mw = jm[w * kRows + row], f = mw == top ? 1.f : ex2(mw - top);
+                const float4 p = *(const float4*)(join + (w * kRows + row) * L::kJoinRow + d);
+                sum += jl[w * kRows + row] * f;
+                v[0] += p.x * f; v[1] += p.y * f; v[2] += p.z * f; v[3] += p.w * f;
+            }
+            if (whole) store(c, row, d, v, top, sum);
+            else {
+                __stcg((float4*)(part + row * kDim + d), make_float4(v[0], v[1], v[2], v[3]));
+                if (d == 0) { __stcg(part + kRows * kDim + row, top); __stcg(part + kRows * (kDim + 1) + row, sum); }
+            }
+        }
+        if (whole) return;
+        const int last = (int)((seg1 * ctas - 1) / all), n = last - lead + 1;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int* ticket = (int*)a.workspace + lead;
+            const int seen = atomicAdd(ticket, 1);
+            if (seen == n - 1) {
+                *ticket = 0;       // as the next call wants it
+                __threadfence();
+            }
+            *s_last = seen == n - 1;
+        }
+        __syncthreads();
+        if (!*s_last) return;
+        // the weights of the parts, [row][part], in the warps' join space
+        for (int row = warp; row < kRows; row += kWarps) {
+            float top = -INFINITY, sum = 0.f;
+            for (int i = lane; i < n; i += 32)
+                top = fmaxf(top, __ldcg(partial(lead + i, i == 0) + kRows * kDim + row));
+#pragma unroll
+            for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+            for (int i = lane; i < n; i += 32) {
+                const float* p = partial(lead + i, i == 0) + kRows * kDim + row;
+                const float mi = __ldcg(p), f = mi == top ? 1.f : ex2(mi - top);
+                join[row * kMaxCtas + i] = f;
+                sum += __ldcg(p + kRows) * f;
+            }
+#pragma unroll
+            for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            if (lane == 0) { join[kRows * kMaxCtas + row] = top; join[kRows * kMaxCtas + kRows + row] = sum; }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
+            const int row = i / kQuads, d = i % kQuads * 4;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+                const float f = join[row * kMaxCtas + k];
+                const float4 p = __ldcg((const float4*)(partial(lead + k, k == 0) + row * kDim + d));
+                v[0] += p.x * f; v[1] += p.y * f; v[2] += p.z * f; v[3] += p.w * f;
+            }
+            store(c, row, d, v, join[kRows * kMaxCtas + row], join[kRows * kMaxCtas + kRows + row]);
+        }
+    }
+
+    __device__ __forceinline__ void run(Cur c, int64_t begin, int64_t end, int64_t all, int* s_last) {
+        const int64_t n = end - begin;
+        Cur ld = c;
+        int pg = fetch_page(ld);
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) {
+            if (s < n) {
+                const int now = pg;
+                const Cur at = ld;
+                ld.next(a);
+                if (s + 1 < n) pg = fetch_page(ld);
+                issue(at, now, s);
+            }
+            asm volatile("cp.async.commit_group;");
+        }
+        bool fresh = true;
+        int stage = 0;
+        for (int64_t i = 0; i < n; ++i) {
+            if (fresh) begin_segment(c);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
+            __syncwarp();
+            const int64_t ahead = i + kStages - 1;
+            if (ahead < n) {
+                const int now = pg;
+                const Cur at = ld;
+                ld.next(a);
+                if (ahead + 1 < n) pg = fetch_page(ld);
+                issue(at, now, stage == 0 ? kStages - 1 : stage - 1);
+            }
+            asm volatile("cp.async.commit_group;");
+            tile(c, stage);
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            fresh = c.u + 1 == c.q.k0 + c.q.units;
+            if (fresh || i + 1 == n) {
+                const int64_t seg0 = begin + i - (c.u - c.q.k0);
+                end_segment(c, seg0, seg0 + c.q.units, begin, end, all, s_last);
+            }
+            if (i + 1 < n) c.next(a);
+        }
+    }
+};
+
+// rows of q that belong to no request
+template <typename T>
+__device__ void blank_rows(const AttendArgs& a, int dim) {
+    const int64_t from = a.requests ? (a.starts ? min(max((int64_t)a.starts[0], (int64_t)0), a.tokens) : 0) : 0;
+    const int64_t to = a.requests ? (a.starts ? min(max((int64_t)a.starts[a.requests], from), a.tokens)
+                                              : min((int64_t)a.requests, a.tokens)) : 0;
+    const int64_t per = (int64_t)a.heads * dim, skip = to - from, n = (a.tokens - skip) * per;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t x = i < from * per ? i : i + skip * per;
+        ((T*)a.out)[x] = sili::from_f32<T>(0.f);
+        if (a.lse && x % dim == 0) a.lse[x / dim] = -INFINITY;
+    }
+}
+
+template <typename T, int E, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_attend(AttendArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_flags[kWarps * kMaxStages + 8 * 4];   // stages' flags, then the row tiles' logit factors
+    __shared__ int s_last;
+    blank_rows<T>(a, 32 * E);
+    Cursor<8 * NT> c;
+    int64_t begin, end;
+    const int64_t all = locate<8 * NT>(a, c, blockIdx.x, gridDim.x, begin, end);
+    if (begin >= end) return;
+    Attend<T, E, NT> k(a, smem, s_flags);
+    k.run(c, begin, end, all, &s_last);
+}
+
+template <typename T, int E, int NT>
+int launch(const AttendArgs& a, cudaStream_t s) {
+    constexpr int smem = smem_bytes<T, E, NT>();
+    static_assert(8 * NT * (32 * E + 2) <= 32 * 130, "the workspace holds the widest row tile");
+    static_assert(8 * NT * (kMaxCtas + 2) * 4 <= Layout<E, NT>::kJoin, "the parts' weights fit the join space");
+    auto kernel = k_attend<T, E, NT>;
+    // set on every call: the attribute belongs to the current device
+    CKV(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<NT == 1 && E < 8 ? kMaxCtas : kMaxCtas / 2, kWarps * 32, smem, s>>>(a);
+    sili::count_launch();
+    CKV(cudaGetLastError());
+    return SILI_OK;
+}
+
+// Row tiles of 8, 16 or 32 (query, head) rows: the narrowest that holds a
+// request's rows, so that decoding wastes no columns and prompts read the
+// cache least often (registers hold no wider one: 32 rows x 128, 16 x 256).
+template <typename T, int E>
+int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
+    if (rows <= 8) return launch<T, E, 1>(a, s);
+    if (rows <= 16 || E == 8) return launch<T, E, 2>(a, s);
+    return launch<T, E, E == 8 ? 2 : 4>(a, s);
+}
+template <typename T>
+int by_dim(const AttendArgs& a, int dim, int64_t rows, cudaStream_t s) {
+    return dim == 64 ? by_rows<T, 2>(a, rows, s) : dim == 128 ? by_rows<T, 4>(a, rows, s) : by_rows<T, 8>(a, rows, s);
 }
 
 }  // namespace
@@ -113,7 +783,7 @@ extern "C" {
 
 int sili_kv4_attention_workspace(int64_t* bytes) {
     if (!bytes) return bad("kv4_attention_workspace", "null array");
-    *bytes = 0;
+    *bytes = workspace_bytes();
     return SILI_OK;
 }
 
@@ -126,11 +796,12 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
     if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
     if (dim != 64 && dim != 128 && dim != 256) return bad(who, "head dimension must be 64, 128 or 256");
     if (page < 16 || page % 16) return bad(who, "page size must be a multiple of 16");
-    if (tokens < 0 || heads < 1 || kv_heads < 1 || n_pages < 0 || width < 0 || requests < 0 || window < 0 || most_new < 0)
+    if (tokens < 0 || tokens > 0x7fffffffLL || heads < 1 || kv_heads < 1 || n_pages < 0 || width < 0 || requests < 0 || window < 0 || most_new < 0)
         return bad(who, "sizes out of range");
+    if (tokens * heads > 0x7fffff00LL) return bad(who, "sizes out of range");
     if (heads % kv_heads) return bad(who, "the kv heads must divide the query heads");
     if (tokens == 0) return SILI_OK;
-    if (!q || !out || (requests && !lens) || (requests && width && !table) || (n_pages && (!codes || !scales)))
+    if (!q || !out || !workspace || (requests && !lens) || (requests && width && !table) || (n_pages && (!codes || !scales)))
         return bad(who, "null array");
     if (requests && table_stride < width) return bad(who, "table rows overlap");
     if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4) return bad(who, "codes must be 16-byte, scales 4-byte aligned");
@@ -138,25 +809,12 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
     if ((uintptr_t)q % 8 || (uintptr_t)out % 16 || q_token_stride * item % 8 || q_head_stride * item % 8)
         return bad(who, "q rows must be 8-byte aligned");
     AttendArgs a{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
-                 table_stride, width, lens, requests, starts, scale, window, out, lse};
+                 table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
+                 page & (page - 1) ? -1 : __builtin_ctz((unsigned)page)};
     cudaStream_t s = (cudaStream_t)stream;
-    (void)workspace;
-    const int64_t ctas = (tokens * heads + 3) / 4;
-    if (ctas > 0x7fffffffLL) return bad(who, "sizes out of range");
-    auto go = [&](auto kernel) {
-        kernel<<<(unsigned)ctas, 128, 0, s>>>(a);
-        sili::count_launch();
-    };
-    if (dtype == SILI_F32) {
-        if (dim == 64) go(k_attend_simple<float, 2>); else if (dim == 128) go(k_attend_simple<float, 4>); else go(k_attend_simple<float, 8>);
-    } else if (dtype == SILI_F16) {
-        if (dim == 64) go(k_attend_simple<__half, 2>); else if (dim == 128) go(k_attend_simple<__half, 4>); else go(k_attend_simple<__half, 8>);
-    } else {
-        if (dim == 64) go(k_attend_simple<__nv_bfloat16, 2>);
-        else if (dim == 128) go(k_attend_simple<__nv_bfloat16, 4>); else go(k_attend_simple<__nv_bfloat16, 8>);
-    }
-    CKV(cudaGetLastError());
-    return SILI_OK;
+    const int64_t rows = (int64_t)std::max(most_new, 1) * (heads / kv_heads);
+    return dtype == SILI_F32 ? by_dim<float>(a, dim, rows, s)
+         : dtype == SILI_F16 ? by_dim<__half>(a, dim, rows, s) : by_dim<__nv_bfloat16>(a, dim, rows, s);
 }
 
 }  // extern "C"

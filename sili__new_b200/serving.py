@@ -466,10 +466,16 @@ _workspaces: dict = {}
 def _workspace(dev, stream):
     if torch.cuda.is_current_stream_capturing():
         # a graph owns its workspace: it may be replayed on any stream, beside eager calls
-        return torch.zeros(_cuda.kv4_attention_workspace(), dtype=torch.uint8, device=dev)
+        return _new_workspace(dev)
     w = _workspaces.get((dev.index, stream))
     if w is None:
-        w = _workspaces[(dev.index, stream)] = torch.zeros(_cuda.kv4_attention_workspace(), dtype=torch.uint8, device=dev)
+        w = _workspaces[(dev.index, stream)] = _new_workspace(dev)
+    return w
+
+
+def _new_workspace(dev):
+    w = torch.empty(_cuda.kv4_attention_workspace(), dtype=torch.uint8, device=dev)
+    w[:4096].zero_()      # the counters; the rest is written before it is read
     return w
 
 

@@ -94,14 +94,14 @@ def values(codes, scales):
 
 
 def attention(q, codes, scales, table, lens, starts, scale, window, tokens):
-    """(out, lse, spread, logit size) in float64; spread = sum p |v| / sum p,
-    logit size = the largest scale * sum |q k| a row sees (for error bounds)."""
+    """(out, lse, spread, logit size, total) in float64; spread = sum p |v| /
+    sum p, total = sum |v| over the keys seen, logit size = the largest scale * sum |q k| a row sees (for error bounds)."""
     q = q.double().cpu().numpy()
     t, h, d = q.shape
     n_pages, _, hk, page, _ = codes.shape
     codes, scales, table = codes.cpu().numpy(), scales.cpu().numpy(), table.cpu().numpy()
     out, lse = np.zeros((t, h, d)), np.full((t, h), -np.inf)
-    spread, size = np.zeros((t, h, d)), np.zeros((t, h))
+    spread, size, total = np.zeros((t, h, d)), np.zeros((t, h)), np.zeros((t, h, d))
     for r in range(len(lens)):
         n = starts[r + 1] - starts[r]
         length = min(int(lens[r]), table.shape[1] * page)
@@ -130,8 +130,9 @@ def attention(q, codes, scales, table, lens, starts, scale, window, tokens):
                     lse[row, j] = top + math.log(p.sum())
                     out[row, j] = p @ v[seen] / p.sum()
                     spread[row, j] = p @ np.abs(v[seen]) / p.sum()
+                    total[row, j] = np.abs(v[seen]).sum(0)
                     size[row, j] = (np.abs(k[seen]) @ np.abs(q[row, j])).max() * abs(scale)
-    return out, lse, spread, size
+    return out, lse, spread, size, total
 
 
 def random_cache(n_pages, hk, page, d, gen, device="cuda"):

@@ -9,7 +9,8 @@ the output type's half unit (and t half of its smallest subnormal), w the half u
 for 16-bit activations, 2^-21 for fp32, whose probabilities and queries are
 kept in two halves), and e = 2^-20 * (largest scale * sum |q k|) the error of
 a logit (exact products, fp32 sums of at most 256 terms): |out - ref| <= u
-|ref| + t + (w + 4 e + 2^-19) * sum p |v|, |lse - ref| <= 2 e + 2^-19 * (1 +
+|ref| + t + (w + 4 e + 2^-19) * sum p |v| + 2^-33 sum |v| (a half's subnormals: probabilities are at least 2^8 at the
+row's largest, so what a half cannot hold is below 2^-25 / 2^8 of it), |lse - ref| <= 2 e + 2^-19 * (1 +
 |ref|)."""
 import math
 
@@ -322,7 +323,7 @@ def _check_attention(S, case, dtype, window=0, scale=None, decode=False, most_ne
     out, lse = S.cache_attention(q, codes, scales, table, lens,
                                  starts=None if decode else torch.tensor(starts, dtype=torch.int32, device="cuda"),
                                  most_new=most_new, scale=scale, window=window, return_lse=True)
-    ref, ref_lse, spread, size = R.attention(q, codes, scales, table, lens.cpu().numpy(), starts, sc, window, q.shape[0])
+    ref, ref_lse, spread, size, total = R.attention(q, codes, scales, table, lens.cpu().numpy(), starts, sc, window, q.shape[0])
     out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     w = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11
     e = 2.0 ** -20 * size
@@ -330,7 +331,7 @@ def _check_attention(S, case, dtype, window=0, scale=None, decode=False, most_ne
     assert (np.isinf(lse) == empty).all() and (out[empty] == 0).all()
     ok = ~empty
     assert (np.abs(lse - ref_lse)[ok] <= (2 * e + 2.0 ** -19 * (1 + np.abs(ref_lse)))[ok]).all()
-    bound = HALF_UNIT[dtype] * np.abs(ref) + SMALLEST[dtype] + (w + 4 * e[..., None] + 2.0 ** -19) * spread
+    bound = HALF_UNIT[dtype] * np.abs(ref) + SMALLEST[dtype] + (w + 4 * e[..., None] + 2.0 ** -19) * spread + 2.0 ** -33 * total
     worst = (np.abs(out - ref) / np.maximum(bound, 1e-30))[ok].max(initial=0.0)
     assert worst <= 1.0, worst
 
