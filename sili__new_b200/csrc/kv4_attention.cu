@@ -36,7 +36,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 #include "sili_b200.h"
 
 namespace sili {
@@ -53,41 +53,24 @@ namespace {
                                    std::string(#x) + ": " + cudaGetErrorString(e_));                    \
     } while (0)
 
+using sili::AttendArgs;
+using sili::ex2;
+using sili::kLift;
+using sili::kLn2;
+using sili::kLog2e;
+using sili::kSlack;
+using sili::kTicketBytes;
+using sili::mul2;
+using sili::pack2;
+
 int bad(const char* who, const char* what) {
     return sili::set_error(SILI_EINVAL, std::string(who) + ": " + what);
 }
-
-struct AttendArgs {
-    const void* q;
-    int64_t qt, qh;        // q strides of tokens and heads, in elements
-    int64_t tokens;
-    int heads, kv_heads;
-    const uint8_t* codes;
-    const uint8_t* scales;
-    int64_t n_pages;
-    int page;
-    const int* table;
-    int64_t stride;
-    int width;
-    const int* lens;
-    int requests;
-    const int* starts;     // null: request r's one token is row r
-    float scale;
-    int window;
-    void* out;             // [tokens, heads, dim]
-    float* lse;            // [tokens, heads] or null
-    void* workspace;
-    int page_shift;        // log2(page), or -1
-};
 
 constexpr int kWarps = 8;
 constexpr int kUnit = 16 * kWarps;      // keys of a unit
 constexpr int kMaxStages = 4;
 constexpr int kMaxCtas = 2 * 148;       // two CTAs an SM; one for the wider row tiles
-// p = 2^(x - m + 8): room below (a half's subnormals start at 2^-32 of the largest) and above (x may exceed m by 7)
-constexpr float kLift = 8.f, kSlack = 7.f;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kTicketBytes = 4096;
 
 constexpr int64_t workspace_bytes() {
     // two partial results a CTA: rows * (dim + 2) floats
@@ -111,11 +94,6 @@ constexpr int smem_bytes() {
     return L::kRing + L::kJoin + (NT > 1 ? NT * 2 * E * terms * 32 * 8 : 0);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
 }
@@ -129,16 +107,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-    uint32_t c;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-    return c;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
 }
 // what is left of (lo, hi) after rounding to the halves h
 __device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t h) {
@@ -812,6 +780,8 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
                  table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
                  page & (page - 1) ? -1 : __builtin_ctz((unsigned)page)};
     cudaStream_t s = (cudaStream_t)stream;
+    if (starts && sili::kv4_prompt_takes(dtype, dim, tokens, heads, kv_heads, most_new))
+        return sili::kv4_prompt_launch(dtype, dim, a, s);
     const int64_t rows = (int64_t)std::max(most_new, 1) * (heads / kv_heads);
     return dtype == SILI_F32 ? by_dim<float>(a, dim, rows, s)
          : dtype == SILI_F16 ? by_dim<__half>(a, dim, rows, s) : by_dim<__nv_bfloat16>(a, dim, rows, s);

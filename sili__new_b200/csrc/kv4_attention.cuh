@@ -1,0 +1,60 @@
+// What the two attention kernels over the 4-bit cache share.
+#pragma once
+
+#include <string>
+
+#include "kv4.cuh"
+
+namespace sili {
+
+struct AttendArgs {
+    const void* q;
+    int64_t qt, qh;        // q strides of tokens and heads, in elements
+    int64_t tokens;
+    int heads, kv_heads;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    int64_t n_pages;
+    int page;
+    const int* table;
+    int64_t stride;
+    int width;
+    const int* lens;
+    int requests;
+    const int* starts;     // null: request r's one token is row r
+    float scale;
+    int window;
+    void* out;             // [tokens, heads, dim]
+    float* lse;            // [tokens, heads] or null
+    void* workspace;
+    int page_shift;        // log2(page), or -1
+};
+
+// The workspace: a counter a CTA, an error word, then the partial results.
+constexpr int kTicketBytes = 4096;
+constexpr int kErrorWord = kTicketBytes / 4 - 1;
+
+// p = 2^(x - m + 8): room below (a half's subnormals start at 2^-32 of the largest) and above (x may exceed m by 7)
+constexpr float kLift = 8.f, kSlack = 7.f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t c;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Long 16-bit prompts (kv4_prompt.cu): whether this call is one, and the launch.
+bool kv4_prompt_takes(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int64_t most_new);
+int kv4_prompt_launch(int dtype, int dim, const AttendArgs& a, cudaStream_t s);
+
+}  // namespace sili

@@ -1,0 +1,651 @@
+// Attention of long 16-bit prompts over the 4-bit paged cache, on the fifth
+// generation tensor cores (tcgen05, sm_100a).
+//
+// A CTA holds 256 rows (query token x query head of the group) of one kv head
+// as two tiles of 128 and walks the keys 128 at a time:
+//   S_w = Q_w K^T     A: Q in shared memory, B: K, D in tensor memory
+//   P_w = 2^(S_w - m) the softmax warps, row by row in a thread
+//   O_w += P_w V      A: P in tensor memory (over S_w), B: V^T
+// Warps 0-3 and 4-7 are the softmax of tile 0 and 1, so one tile's
+// exponentials run while the other's products do; warps 8-11 turn the next
+// keys' 4-bit K and V into halves in shared memory (K as it lies, V
+// transposed by interleaving the nibbles of two keys), straight from global
+// memory through registers; one thread of warp 12 issues the products.  All
+// operands are K-major with the 128-byte swizzle.  K and V are exact in
+// half; bf16 queries are scaled to halves exactly by a power of two a row;
+// P is rounded once to half (2^-12, below the output's rounding).  The
+// running maximum moves only when a logit exceeds it by 2^7, since O has to
+// be read and written back then.
+//
+// Every wait is bounded: one that gives up sets the workspace's error word,
+// every role leaves its loop, the rows are written as NaN and the tensor
+// memory is freed.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.cuh"
+#include "kv4_attention.cuh"
+#include "sili_b200.h"
+
+namespace sili {
+int set_error(int code, const std::string& msg);
+}
+
+namespace {
+
+using sili::AttendArgs;
+using sili::ex2;
+using sili::kLift;
+using sili::kLn2;
+using sili::kLog2e;
+using sili::kSlack;
+using sili::mul2;
+using sili::pack2;
+
+#define CKP(x)                                                                                          \
+    do {                                                                                                \
+        const cudaError_t e_ = (x);                                                                     \
+        if (e_ != cudaSuccess) return sili::set_error(SILI_ECUDA, std::string(#x) + ": " + cudaGetErrorString(e_)); \
+    } while (0)
+
+constexpr int kM = 128;               // rows of a tile (MMA M)
+constexpr int kTiles = 2;
+constexpr int kKeys = 128;            // keys a step (MMA N of S, K of P V)
+constexpr int kSoftmax = kTiles * 128, kDequant = 128;
+constexpr int kThreads = kSoftmax + kDequant + 32;
+constexpr int kPolls = 1 << 22;       // try_wait polls (each waits a while by itself) before giving up
+
+template <int D>
+struct Smem {
+    alignas(1024) uint8_t q[kTiles][kM * D * 2];
+    alignas(1024) uint8_t k[2][kKeys * D * 2];
+    alignas(1024) uint8_t v[2][kKeys * D * 2];
+    alignas(8) unsigned long long kv_full[2], kv_free[2], s_full[2], p_full[2], drained;
+    uint8_t odd_keys[2][16][8];       // [stage][8 keys][dim / 8 elements]: bits of keys whose V scale is not a number
+    int odd[2];                       // the last step whose stage had any, plus one
+    uint8_t there[2][8];              // [stage][16 keys]: their page exists
+    uint32_t tmem;
+    int dead;
+    int hit[3];                       // the CTA's request, kv head and row tile pair
+};
+
+__device__ __forceinline__ uint32_t addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(unsigned long long* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(addr(b)), "r"(n));
+}
+__device__ __forceinline__ void bar_arrive(unsigned long long* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(addr(b)) : "memory");
+}
+// true when the phase of this parity is complete; false once any role has given up
+__device__ __forceinline__ bool bar_wait(unsigned long long* b, uint32_t parity, int* dead) {
+    const uint32_t a = addr(b);
+    for (int i = 0; i < kPolls; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(a), "r"(parity) : "memory");
+        if (done) return true;
+        if ((i & 255) == 255 && *(volatile int*)dead) return false;
+    }
+    *(volatile int*)dead = 1;
+    return false;
+}
+
+// shared-memory matrix descriptor: K-major, 128-byte swizzle, atoms of 8 rows x 128 bytes 1024 bytes apart
+__device__ __forceinline__ uint64_t desc(const void* p) {
+    return (uint64_t)((addr(p) >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// byte offset of 16-byte chunk c (0..7) of row r in a [rows x 64] half block of that layout
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// kind::f16 instruction descriptor: D f32, A and B f16, both K-major
+__device__ constexpr uint32_t idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(unsigned long long* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(addr(b)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t a, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// What every role knows of the CTA's work.
+struct Work {
+    int r, h, group, rows, row0, len;
+    int64_t pos0;          // position of the request's first query
+    int j0, n[kTiles], last;   // steps [j0, n[w]) of each tile, and of the longer one
+
+    __device__ __forceinline__ int64_t pos_of(int row) const { return pos0 + min(row, rows - 1) / group; }
+};
+
+struct Span {
+    int row0, nq, len, pairs;
+    int64_t pos0;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
+    Span q;
+    const int64_t s0 = min(max((int64_t)a.starts[r], (int64_t)0), a.tokens);
+    const int64_t s1 = min(max((int64_t)a.starts[r + 1], s0), a.tokens);
+    const int all = max(a.lens[r], 0);
+    q.row0 = (int)s0;
+    q.nq = (int)(s1 - s0);
+    q.len = (int)min(min((int64_t)all, (int64_t)a.width * a.page), (int64_t)0x7FFFFF00);
+    q.pos0 = (int64_t)all - q.nq;
+    q.pairs = (q.nq * (a.heads / a.kv_heads) + kTiles * kM - 1) / (kTiles * kM);
+    return q;
+}
+
+// Items are numbered request by request, in each the last rows first (they
+// have the most keys), the kv heads together.  One warp finds item `id`.
+__device__ __forceinline__ bool find_item(const AttendArgs& a, int64_t id, int (&hit)[3]) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int base = 0; base < a.requests; base += 32) {
+        const int r = base + lane;
+        const int pairs = r < a.requests ? span_of(a, r).pairs : 0;
+        const int64_t n = (int64_t)pairs * a.kv_heads;
+        int64_t x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += t;
+        }
+        x += before;
+        const bool mine = x - n <= id && id < x;
+        if (mine) {
+            const int64_t off = id - (x - n);
+            hit[0] = r;
+            hit[1] = (int)(off % a.kv_heads);
+            hit[2] = pairs - 1 - (int)(off / a.kv_heads);
+        }
+        if (__any_sync(0xffffffffu, mine)) return true;
+        before = __shfl_sync(0xffffffffu, x, 31);
+    }
+    return false;
+}
+
+template <typename T, int D>
+struct Prompt {
+    static constexpr int E = D / 32;
+    const AttendArgs& a;
+    Smem<D>& s;
+    Work w;
+
+    __device__ __forceinline__ uint32_t s_col(int t) const { return s.tmem + t * kKeys; }
+    __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + kTiles * kKeys + t * D; }
+
+    // ── warps 8-11: 4-bit keys and values of step j into stage j & 1 ──
+    __device__ __forceinline__ void dequantise() {
+        const int tid = threadIdx.x - kSoftmax, dw = tid >> 5, lane = tid & 31;
+        // K: E lanes a key, 16 bytes (one group of 32) each
+        constexpr int kPer = 32 / E;                // keys of one load instruction
+        const int kq = lane % E, kkey = dw * 32 + lane / E;
+        // V: 8 keys of D/8 elements; lane & 7 numbers the keys, so a store instruction fills whole rows
+        constexpr int kVw = D / 64;                 // words a key
+        const int half = dw & 1, c = lane & 7, db = (dw >> 1) * 4 + (lane >> 3), vkey = half * 64 + c * 8;
+        const int vg = db * (D / 8) / 32;
+        uint4 rk[E];
+        uint32_t sk[E], rv[8][kVw], sv[8];
+        int pk[E], pv;
+        auto page_of = [&](int key) {
+            const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
+            // whole runs of 16 keys (they share a page and a bit of `there`), of which the last may reach past the end
+            return (key & ~15) < w.len ? __ldg(a.table + w.r * a.stride + col) : -1;
+        };
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) pk[i] = page_of(j * kKeys + dw * 32 + i * kPer);
+            pv = page_of(j * kKeys + vkey);
+        };
+        // (first key of the load) -> row of the cache, or -1
+        auto row_of = [&](int pg, int key, int which) -> int64_t {
+            if (pg < 0 || pg >= a.n_pages) return -1;
+            const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
+            return sili::kv4_row(pg, which, w.h, a.kv_heads, a.page) + (key - col * a.page);
+        };
+        uint32_t there = 0;
+        auto load = [&](int j) {
+            there = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int64_t row = row_of(pk[i], j * kKeys + dw * 32 + i * kPer, 0);
+                rk[i] = make_uint4(0, 0, 0, 0);
+                sk[i] = 0;
+                if (row >= 0) {
+                    there |= 1u << i;
+                    rk[i] = __ldg((const uint4*)(a.codes + (row + lane / E) * (D / 2) + kq * 16));
+                    sk[i] = __ldg(a.scales + (row + lane / E) * E + kq);
+                }
+            }
+            const int64_t row = row_of(pv, j * kKeys + vkey, 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sv[i] = 0;
+#pragma unroll
+                for (int q = 0; q < kVw; ++q) rv[i][q] = 0;
+                if (row >= 0) {
+                    const uint8_t* p = a.codes + (row + i) * (D / 2) + db * (D / 16);
+                    if constexpr (kVw == 2) {
+                        const uint2 x = __ldg((const uint2*)p);
+                        rv[i][0] = x.x; rv[i][kVw - 1] = x.y;
+                    } else rv[i][0] = __ldg((const uint32_t*)p);
+                    sv[i] = __ldg(a.scales + (row + i) * E + vg);
+                }
+            }
+        };
+        pages(w.j0);
+        load(w.j0);
+        if (w.j0 + 1 < w.last) pages(w.j0 + 1);
+        for (int j = w.j0; j < w.last; ++j) {
+            const int n = j - w.j0, st = n & 1;
+            if (n >= 2 && !bar_wait(&s.kv_free[st], ((n >> 1) - 1) & 1, &s.dead)) return;
+            // K: rows are keys
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int key = kkey + i * kPer;
+                const uint32_t sc = sk[i] * 0x00800080u;
+                uint8_t* block = s.k[st] + (kq >> 1) * (kKeys * 128);
+                // lanes of the second block go through their four chunks two further on: eight lanes, eight banks' worth
+                const bool far = E == 4 && (kq & 2);
+                const uint32_t wd[4] = {far ? rk[i].z : rk[i].x, far ? rk[i].w : rk[i].y, far ? rk[i].x : rk[i].z,
+                                        far ? rk[i].y : rk[i].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t f[4];
+                    sili::kv4_decode4(wd[q], f);
+                    const int ch = (kq & 1) * 4 + (far ? q ^ 2 : q);
+                    *(uint4*)(block + chunk_at(key, ch)) = make_uint4(mul2(f[0], sc), mul2(f[1], sc), mul2(f[2], sc), mul2(f[3], sc));
+                }
+                if (lane == 0) s.there[st][(dw * 32 + i * kPer) / 16] = there >> i & 1;
+            }
+            // V: rows are elements; scales that are no numbers are left out and noted
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (sv[i] >= 0xF8u) { bits |= 1u << i; sv[i] = 0; }
+            s.odd_keys[st][half * 8 + c][db] = (uint8_t)bits;
+            if (bits) *(volatile int*)&s.odd[st] = j + 1;
+            uint32_t sc[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) sc[p] = sv[2 * p] << 7 | sv[2 * p + 1] << 23;
+            uint8_t* block = s.v[st] + half * (D * 128);
+#pragma unroll
+            for (int q = 0; q < kVw; ++q) {
+                constexpr uint32_t kLow = 0x0F0F0F0Fu;
+                uint32_t even[4][4], odd[4][4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t x = rv[2 * p][q], y = rv[2 * p + 1][q];
+                    sili::kv4_decode4((x & kLow) | ((y << 4) & ~kLow), even[p]);
+                    sili::kv4_decode4(((x >> 4) & kLow) | (y & ~kLow), odd[p]);
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int d = db * (D / 8) + 8 * q + 2 * b;
+                    *(uint4*)(block + chunk_at(d, c)) = make_uint4(mul2(even[0][b], sc[0]), mul2(even[1][b], sc[1]),
+                                                                   mul2(even[2][b], sc[2]), mul2(even[3][b], sc[3]));
+                    *(uint4*)(block + chunk_at(d + 1, c)) = make_uint4(mul2(odd[0][b], sc[0]), mul2(odd[1][b], sc[1]),
+                                                                       mul2(odd[2][b], sc[2]), mul2(odd[3][b], sc[3]));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&s.kv_full[st]);
+            if (j + 1 < w.last) {
+                load(j + 1);
+                if (j + 2 < w.last) pages(j + 2);
+            }
+        }
+    }
+
+    // ── one thread of warp 12: the products ──
+    __device__ __forceinline__ void products() {
+        auto scores = [&](int t, int st) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                mma_ss(s_col(t), desc(s.q[t] + (k >> 2) * (kM * 128)) + 2 * (k & 3),
+                       desc(s.k[st] + (k >> 2) * (kKeys * 128)) + 2 * (k & 3), idesc(kM, kKeys), k > 0);
+            commit(&s.s_full[t]);
+        };
+        if (!bar_wait(&s.kv_full[0], 0, &s.dead)) return;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        for (int t = 0; t < kTiles; ++t)
+            if (w.j0 < w.n[t]) scores(t, 0);
+        for (int j = w.j0; j < w.last; ++j) {
+            const int n = j - w.j0, st = n & 1;
+            for (int t = 0; t < kTiles; ++t) {
+                if (j >= w.n[t]) continue;
+                if (!bar_wait(&s.p_full[t], n & 1, &s.dead)) return;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                    mma_ts(o_col(t), s_col(t) + 8 * k, desc(s.v[st] + (k >> 2) * (D * 128)) + 2 * (k & 3), idesc(kM, D),
+                           n > 0 || k > 0);
+                // the last product of this step: the stage is free when it is done
+                if (t == kTiles - 1 || j >= w.n[t + 1]) commit(&s.kv_free[st]);
+                if (j + 1 < w.n[t]) {
+                    if (!bar_wait(&s.kv_full[st ^ 1], ((n + 1) >> 1) & 1, &s.dead)) return;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    scores(t, st ^ 1);
+                } else {
+                    commit(&s.s_full[t]);      // O is complete
+                }
+            }
+        }
+    }
+
+    // ── warps 0-7: one row a thread ──
+    __device__ __forceinline__ void softmax() {
+        const int t = threadIdx.x >> 7, row = w.row0 + t * kM + (threadIdx.x & 127);
+        const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;     // this warp's quarter of the tensor memory's lanes
+        const int warp_row0 = w.row0 + t * kM + (threadIdx.x & 96);
+        const bool real = row < w.rows;
+        const int64_t q_row = span_row() + (real ? row / w.group : 0);
+        const int head = w.h * w.group + (real ? row % w.group : 0);
+        const int64_t pos = w.pos_of(row), first = w.pos_of(warp_row0), final = w.pos_of(warp_row0 + 31);
+        // Q into shared memory as halves
+        float cf = a.scale * kLog2e;
+        {
+            const T* src = (const T*)a.q + q_row * a.qt + head * a.qh;
+            const int m = threadIdx.x & 127;
+            uint32_t top = 0;
+            float f = 1.f;
+            if (!std::is_same<T, __half>::value && real) {
+                for (int i = 0; i < D; i += 4) {
+                    const sili::Pack<T, 4> p = *(const sili::Pack<T, 4>*)(src + i);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(sili::to_f32(p.v[k])) & 0x7FFFFFFFu);
+                }
+                if (top && top < 0x7F800000u) {
+                    const int e = 14 - max((int)(top >> 23) - 127, -100);
+                    f = __int_as_float((127 + e) << 23);
+                    cf *= __int_as_float((127 - e) << 23);
+                }
+            }
+#pragma unroll 4
+            for (int i = 0; i < D; i += 8) {
+                uint4 o = make_uint4(0, 0, 0, 0);
+                if (real) {
+                    const sili::Pack<T, 4> p = *(const sili::Pack<T, 4>*)(src + i), q = *(const sili::Pack<T, 4>*)(src + i + 4);
+                    o = make_uint4(pack2(sili::to_f32(p.v[0]) * f, sili::to_f32(p.v[1]) * f),
+                                   pack2(sili::to_f32(p.v[2]) * f, sili::to_f32(p.v[3]) * f),
+                                   pack2(sili::to_f32(q.v[0]) * f, sili::to_f32(q.v[1]) * f),
+                                   pack2(sili::to_f32(q.v[2]) * f, sili::to_f32(q.v[3]) * f));
+                }
+                *(uint4*)(s.q[t] + (i >> 6) * (kM * 128) + chunk_at(m, (i & 63) >> 3)) = o;
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();       // Q is there: the products may begin
+        float base = -INFINITY, l = 0.f;       // base: the running maximum - lift
+        uint32_t poisoned = 0;                 // groups of 32 elements in which the row saw a NaN
+        bool ok = true;
+        for (int j = w.j0; j < w.n[t] && ok; ++j) {
+            const int n = j - w.j0, st = n & 1, key0 = j * kKeys;
+            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], n & 1, &s.dead));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            // keys [lo, hi) of the step are the row's; pages that are not there, 16 keys a bit
+            uint32_t gone = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) gone |= (s.there[st][i] ? 0u : 1u) << i;
+            const bool inside = !gone && key0 + kKeys - 1 <= first && key0 + kKeys <= w.len && (!a.window || key0 > final - a.window);
+            const int hi = (int)min((int64_t)kKeys, min(pos + 1, (int64_t)w.len) - key0);
+            const int lo = a.window ? (int)max((int64_t)0, pos - a.window + 1 - key0) : 0;
+            auto mask = [&](float (&x)[32], int c) {
+                if (inside) return;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int key = 32 * c + i;
+                    if (key < lo || key >= hi || (gone >> (key / 16) & 1)) x[i] = -INFINITY;
+                }
+            };
+            float x[32], top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_ld32(s_col(t) + lanes + 32 * c, x);
+                if (cf < 0.f)      // a negative scale: the largest logit is the smallest product
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = -x[i];
+                mask(x, c);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(x[i], x[i + 1]));
+            }
+            top *= fabsf(cf);
+            // (cf 0 and nothing seen: 0 * -inf; NaN compares false)
+            if (__any_sync(0xffffffffu, top - kLift > base + kSlack)) {
+                const float fresh = fmaxf(base, top - kLift);
+                const float f = fresh == base ? 1.f : ex2(base - fresh);
+                base = fresh;
+                l *= f;
+                if (n > 0)
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t r[16];
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                            : "r"(o_col(t) + lanes + 16 * c));
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                        tmem_st16(o_col(t) + lanes + 16 * c, r);
+                    }
+            }
+            const float shift = base == -INFINITY ? 0.f : base;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_ld32(s_col(t) + lanes + 32 * c, x);
+                mask(x, c);
+                uint32_t p[16];
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float u = ex2(fmaf(x[i], cf, -shift)), v = ex2(fmaf(x[i + 1], cf, -shift));
+                    if (!inside && cf <= 0.f) {        // -inf times a scale that is not positive
+                        u = x[i] == -INFINITY ? 0.f : u;
+                        v = x[i + 1] == -INFINITY ? 0.f : v;
+                    }
+                    sum0 += u; sum1 += v;
+                    p[i / 2] = pack2(u, v);
+                }
+                l += sum0 + sum1;
+                tmem_st16(s_col(t) + lanes + 16 * c, p);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            if (*(volatile int*)&s.odd[st] == j + 1) {
+                for (int key = max(lo, 0); key < hi; ++key) {
+                    if (gone >> (key / 16) & 1) continue;
+                    for (int g = 0; g < E; ++g)
+                        if (s.odd_keys[st][key >> 3][g * (8 / E)] >> (key & 7) & 1) poisoned |= 1u << g;
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            bar_arrive(&s.p_full[t]);
+        }
+        const int steps = w.n[t] - w.j0;
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], steps & 1, &s.dead));
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        // l 0: the row saw nothing
+        float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t id = q_row * a.heads + head;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            float x[32];
+            __syncwarp();
+            if (steps > 0) tmem_ld32(o_col(t) + lanes + 32 * c, x);
+            else
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = 0.f;
+            const bool bad = !ok || (poisoned >> c & 1);
+            if (real)
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    sili::Pack<T, 8> o;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) o.v[k] = sili::from_f32<T>(bad ? __int_as_float(0x7FC00000) : x[i + k] * inv);
+                    *(sili::Pack<T, 8>*)((T*)a.out + id * D + 32 * c + i) = o;
+                }
+        }
+        if (real && a.lse) a.lse[id] = !ok ? __int_as_float(0x7FC00000) : l == 0.f ? -INFINITY : kLn2 * (base + log2f(l));
+    }
+
+    int first_row;
+    __device__ __forceinline__ int64_t span_row() const { return first_row; }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) k_prompt(AttendArgs a) {
+    extern __shared__ uint8_t raw[];
+    Smem<D>& s = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5;
+    // rows of q that belong to no request
+    {
+        const int64_t from = a.requests ? min(max((int64_t)a.starts[0], (int64_t)0), a.tokens) : 0;
+        const int64_t to = a.requests ? min(max((int64_t)a.starts[a.requests], from), a.tokens) : 0;
+        const int64_t per = (int64_t)a.heads * D, n = (a.tokens - (to - from)) * per;
+        for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+            const int64_t x = i < from * per ? i : i + (to - from) * per;
+            ((T*)a.out)[x] = sili::from_f32<T>(0.f);
+            if (a.lse && x % D == 0) a.lse[x / D] = -INFINITY;
+        }
+    }
+    if (warp == 0) {
+        int hit[3] = {-1, 0, 0};
+        const bool found = find_item(a, blockIdx.x, hit);
+        if (!found && threadIdx.x == 0) s.hit[0] = -1;
+        if (hit[0] >= 0) { s.hit[0] = hit[0]; s.hit[1] = hit[1]; s.hit[2] = hit[2]; }
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&s.kv_full[i], kDequant);
+            bar_init(&s.kv_free[i], 1);
+            bar_init(&s.s_full[i], 1);
+            bar_init(&s.p_full[i], 128);
+            s.odd[i] = 0;
+        }
+        bar_init(&s.drained, 1);
+        s.dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    if (s.hit[0] < 0) return;
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(addr(&s.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const Span q = span_of(a, s.hit[0]);
+    Prompt<T, D> k{a, s};
+    Work& w = k.w;
+    w.r = s.hit[0];
+    w.h = s.hit[1];
+    w.group = a.heads / a.kv_heads;
+    w.rows = q.nq * w.group;
+    w.row0 = s.hit[2] * (kTiles * kM);
+    w.len = q.len;
+    w.pos0 = q.pos0;
+    k.first_row = q.row0;
+    w.j0 = a.window ? (int)(max((int64_t)0, w.pos_of(w.row0) - a.window + 1) / kKeys) : 0;
+    w.last = w.j0;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        w.n[t] = w.j0;
+        if (w.row0 + t * kM < w.rows) {
+            const int64_t hi = min((int64_t)w.len, w.pos_of(w.row0 + t * kM + kM - 1) + 1);
+            w.n[t] = max(w.j0, (int)((hi + kKeys - 1) / kKeys));
+        }
+        w.last = max(w.last, w.n[t]);
+    }
+    if (warp < kSoftmax / 32) {
+        k.softmax();
+    } else {
+        __syncthreads();       // Q is there
+        if (w.last > w.j0) {
+            if (warp < (kSoftmax + kDequant) / 32) k.dequantise();
+            else if ((threadIdx.x & 31) == 0) {
+                k.products();
+                // what was begun is waited for (bounded): the tensor memory is freed next
+                if (*(volatile int*)&s.dead) {
+                    atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
+                    int quiet = 0;
+                    commit(&s.drained);
+                    bar_wait(&s.drained, 0, &quiet);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(512));
+}
+
+template <typename T, int D>
+int launch(const AttendArgs& a, cudaStream_t s) {
+    constexpr int smem = (int)sizeof(Smem<D>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    auto kernel = k_prompt<T, D>;
+    CKP(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // no more items than every request's rows rounded up; CTAs past the last leave at once
+    const int64_t rows = a.tokens * (a.heads / a.kv_heads);
+    const int64_t items = (rows / (kTiles * kM) + a.requests + 1) * a.kv_heads;
+    if (items > 0x7fffffffLL) return sili::set_error(SILI_EINVAL, "kv4_attention: sizes out of range");
+    kernel<<<(unsigned)items, kThreads, smem, s>>>(a);
+    sili::count_launch();
+    CKP(cudaGetLastError());
+    return SILI_OK;
+}
+
+}  // namespace
+
+namespace sili {
+
+// From about half the SMs' worth of full row pairs on; below, the split over
+// keys of the other kernel fills the card better.
+bool kv4_prompt_takes(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int64_t most_new) {
+    const int64_t group = heads / kv_heads;
+    return dtype != SILI_F32 && (dim == 64 || dim == 128) && most_new * group >= 128 &&
+           tokens * group / (kTiles * kM) * kv_heads >= 74;
+}
+int kv4_prompt_launch(int dtype, int dim, const AttendArgs& a, cudaStream_t s) {
+    if (dtype == SILI_F16) return dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+    return dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace sili

@@ -357,6 +357,43 @@ def test_attention_prompt(S, dtype, lens, new, h, hk, dim, page, window):
     _check_attention(S, case, dtype, window=window, most_new=1)     # a wrong hint changes nothing
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,new,h,hk,dim,page,window", [
+    ([700, 130, 20], [500, 100, 20], 32, 8, 128, 16, 0), ([641, 0, 300], [641, 0, 300], 28, 4, 64, 48, 0),
+    ([900, 257], [500, 130], 32, 8, 128, 64, 70), ([260, 5, 400], [255, 5, 360], 32, 1, 128, 128, 0),
+    ([300, 310], [300, 300], 40, 40, 64, 16, 129)])
+def test_attention_long_prompt(S, dtype, lens, new, h, hk, dim, page, window):
+    """Enough 16-bit rows for the tensor-memory kernel; odd groups, ragged ends, windows, queries before the keys."""
+    case = _attend_case(lens, new, h, hk, dim, page, dtype, sum(lens) + window, extra_rows=3)
+    assert case[0].shape[0] * h >= 74 * 256
+    _check_attention(S, case, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_long_prompt_edges(S, dtype):
+    """Requests with fewer keys than queries, missing pages, NaN in K and V of single keys, large and negative scales."""
+    case = _attend_case([300, 420, 200], [330, 300, 7], 32, 8, 128, 16, dtype, 21, scale_q=4.0)
+    q, codes, scales, table, lens, starts = case
+    table[1, 3], table[1, 20] = -1, 1 << 29
+    _check_attention(S, case, dtype)
+    _check_attention(S, case, dtype, scale=-0.05)
+    _check_attention(S, case, dtype, scale=0.0)
+    starts32 = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    clean = S.cache_attention(q, codes, scales, table, lens, starts=starts32)
+    # V of request 1's key 250, kv head 3, values 64..95: seen by queries at positions >= 250 (row 330 + 130 on)
+    scales[table[1, 15].long(), 1, 3, 10, 2] = 0xFF
+    got = S.cache_attention(q, codes, scales, table, lens, starts=starts32)
+    bad = torch.isnan(got)
+    want = torch.zeros_like(bad)
+    want[330 + 130:630, 12:16, 64:96] = True
+    assert torch.equal(bad, want) and torch.equal(got[~bad], clean[~bad])
+    # K of the same key: its readers' rows are NaN as a whole, no other row changes
+    scales[table[1, 15].long(), 0, 3, 10, 0] = 0xFF
+    got = S.cache_attention(q, codes, scales, table, lens, starts=starts32)
+    want[330 + 130:630, 12:16] = True
+    assert torch.equal(torch.isnan(got), want) and torch.equal(got[~want], clean[~want])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_window_decode(S, dtype):
     case = _attend_case([900, 30, 64, 1], [1] * 4, 8, 2, 128, 16, dtype, 11)
