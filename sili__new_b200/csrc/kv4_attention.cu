@@ -704,7 +704,7 @@ __device__ void blank_rows(const AttendArgs& a, int dim) {
 }
 
 template <typename T, int E, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_attend(AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_attend(const __grid_constant__ AttendArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_flags[kWarps * kMaxStages + 8 * 4];   // stages' flags, then the row tiles' logit factors
     __shared__ int s_last;

@@ -119,19 +119,24 @@ __device__ __forceinline__ void commit(unsigned long long* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(addr(b)) : "memory");
 }
 
+// 32 columns of this warp's lanes; the registers are not to be touched before tmem_wait has taken them through
 __device__ __forceinline__ void tmem_ld32(uint32_t a, float (&v)[32]) {
-    uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(a));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+          "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+          "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+          "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+          "+f"(v[31])::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
     asm volatile(
@@ -365,6 +370,23 @@ struct Prompt {
         }
     }
 
+    // O's row times f
+    __device__ __forceinline__ void rescale(int t, uint32_t lanes, float f) {
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+            uint32_t r[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                "tcgen05.wait::ld.sync.aligned;"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                : "r"(o_col(t) + lanes + 16 * c) : "memory");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+            tmem_st16(o_col(t) + lanes + 16 * c, r);
+        }
+    }
+
     // ── warps 0-7: one row a thread ──
     __device__ __forceinline__ void softmax() {
         const int t = threadIdx.x >> 7, row = w.row0 + t * kM + (threadIdx.x & 127);
@@ -375,12 +397,13 @@ struct Prompt {
         const int head = w.h * w.group + (real ? row % w.group : 0);
         const int64_t pos = w.pos_of(row), first = w.pos_of(warp_row0), final = w.pos_of(warp_row0 + 31);
         // Q into shared memory as halves
-        float cf = a.scale * kLog2e;
+        // (with the scale's sign, so that the logits' factor is never negative)
+        float cf = fabsf(a.scale) * kLog2e;
         {
             const T* src = (const T*)a.q + q_row * a.qt + head * a.qh;
             const int m = threadIdx.x & 127;
             uint32_t top = 0;
-            float f = 1.f;
+            float f = a.scale < 0.f ? -1.f : 1.f;
             if (!std::is_same<T, __half>::value && real) {
                 for (int i = 0; i < D; i += 4) {
                     const sili::Pack<T, 4> p = *(const sili::Pack<T, 4>*)(src + i);
@@ -389,7 +412,7 @@ struct Prompt {
                 }
                 if (top && top < 0x7F800000u) {
                     const int e = 14 - max((int)(top >> 23) - 127, -100);
-                    f = __int_as_float((127 + e) << 23);
+                    f *= __int_as_float((127 + e) << 23);
                     cf *= __int_as_float((127 - e) << 23);
                 }
             }
@@ -423,67 +446,67 @@ struct Prompt {
             const bool inside = !gone && key0 + kKeys - 1 <= first && key0 + kKeys <= w.len && (!a.window || key0 > final - a.window);
             const int hi = (int)min((int64_t)kKeys, min(pos + 1, (int64_t)w.len) - key0);
             const int lo = a.window ? (int)max((int64_t)0, pos - a.window + 1 - key0) : 0;
-            auto mask = [&](float (&x)[32], int c) {
-                if (inside) return;
+            auto step = [&](auto masked) {
+                auto mask = [&](float (&y)[32], int c) {
+                    if constexpr (decltype(masked)::value) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int key = 32 * c + i;
-                    if (key < lo || key >= hi || (gone >> (key / 16) & 1)) x[i] = -INFINITY;
+                        for (int i = 0; i < 32; ++i) {
+                            const int key = 32 * c + i;
+                            if (key < lo || key >= hi || (gone >> (key / 16) & 1)) y[i] = -INFINITY;
+                        }
+                    }
+                };
+                // two passes over S, the next 32 columns on their way while the current ones are worked on
+                float x[2][32], top = -INFINITY;
+                tmem_ld32(s_col(t) + lanes, x[0]);
+                tmem_wait(x[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float(&y)[32] = x[c & 1];
+                    tmem_ld32(s_col(t) + lanes + 32 * ((c + 1) & 3), x[~c & 1]);
+                    mask(y, c);
+                    float m0 = fmaxf(y[0], y[1]), m1 = fmaxf(y[2], y[3]);
+#pragma unroll
+                    for (int i = 4; i < 32; i += 4) {
+                        m0 = fmaxf(m0, fmaxf(y[i], y[i + 1]));
+                        m1 = fmaxf(m1, fmaxf(y[i + 2], y[i + 3]));
+                    }
+                    top = fmaxf(top, fmaxf(m0, m1));
+                    tmem_wait(x[~c & 1]);
+                }
+                if (top != -INFINITY) top *= cf;
+                if (__any_sync(0xffffffffu, top - kLift > base + kSlack)) {
+                    const float fresh = fmaxf(base, top - kLift);
+                    const float f = fresh == base ? 1.f : ex2(base - fresh);
+                    base = fresh;
+                    l *= f;
+                    if (n > 0) rescale(t, lanes, f);
+                }
+                const float shift = base == -INFINITY ? 0.f : base;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float(&y)[32] = x[c & 1];      // x[0] already holds the first columns
+                    if (c < 3) tmem_ld32(s_col(t) + lanes + 32 * (c + 1), x[~c & 1]);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], cf, -shift);
+                    mask(y, c);
+                    uint32_t p[16];
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float u = ex2(y[i]), v = ex2(y[i + 1]);
+                        sum0 += u; sum1 += v;
+                        p[i / 2] = pack2(u, v);
+                    }
+                    l += sum0 + sum1;
+                    // P takes the place of columns that have been read
+                    if (c < 3) tmem_wait(x[~c & 1]);
+                    tmem_st16(s_col(t) + lanes + 16 * c, p);
                 }
             };
-            float x[32], top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_ld32(s_col(t) + lanes + 32 * c, x);
-                if (cf < 0.f)      // a negative scale: the largest logit is the smallest product
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = -x[i];
-                mask(x, c);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(x[i], x[i + 1]));
-            }
-            top *= fabsf(cf);
-            // (cf 0 and nothing seen: 0 * -inf; NaN compares false)
-            if (__any_sync(0xffffffffu, top - kLift > base + kSlack)) {
-                const float fresh = fmaxf(base, top - kLift);
-                const float f = fresh == base ? 1.f : ex2(base - fresh);
-                base = fresh;
-                l *= f;
-                if (n > 0)
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t r[16];
-                        asm volatile(
-                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                            : "r"(o_col(t) + lanes + 16 * c));
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-                        tmem_st16(o_col(t) + lanes + 16 * c, r);
-                    }
-            }
-            const float shift = base == -INFINITY ? 0.f : base;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_ld32(s_col(t) + lanes + 32 * c, x);
-                mask(x, c);
-                uint32_t p[16];
-                float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float u = ex2(fmaf(x[i], cf, -shift)), v = ex2(fmaf(x[i + 1], cf, -shift));
-                    if (!inside && cf <= 0.f) {        // -inf times a scale that is not positive
-                        u = x[i] == -INFINITY ? 0.f : u;
-                        v = x[i + 1] == -INFINITY ? 0.f : v;
-                    }
-                    sum0 += u; sum1 += v;
-                    p[i / 2] = pack2(u, v);
-                }
-                l += sum0 + sum1;
-                tmem_st16(s_col(t) + lanes + 16 * c, p);
-            }
+            // two copies of the step: the masks' arithmetic must not run in the steps without any
+            if (inside) step(std::false_type{});
+            else step(std::true_type{});
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (*(volatile int*)&s.odd[st] == j + 1) {
                 for (int key = max(lo, 0); key < hi; ++key) {
@@ -505,8 +528,10 @@ struct Prompt {
         for (int c = 0; c < D / 32; ++c) {
             float x[32];
             __syncwarp();
-            if (steps > 0) tmem_ld32(o_col(t) + lanes + 32 * c, x);
-            else
+            if (steps > 0) {
+                tmem_ld32(o_col(t) + lanes + 32 * c, x);
+                tmem_wait(x);
+            } else
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] = 0.f;
             const bool bad = !ok || (poisoned >> c & 1);
@@ -527,7 +552,7 @@ struct Prompt {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) k_prompt(AttendArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ AttendArgs a) {
     extern __shared__ uint8_t raw[];
     Smem<D>& s = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5;
