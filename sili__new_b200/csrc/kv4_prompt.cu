@@ -10,7 +10,7 @@
 // exponentials run while the other's products do; warps 8-11 turn the next
 // keys' 4-bit K and V into halves in shared memory (K as it lies, V
 // transposed by interleaving the nibbles of two keys), straight from global
-// memory through registers; one thread of warp 12 issues the products.  All
+// memory through registers; one thread of warp 16 issues the products.  All
 // operands are K-major with the 128-byte swizzle.  K and V are exact in
 // half; bf16 queries are scaled to halves exactly by a power of two a row;
 // P is rounded once to half (2^-12, below the output's rounding).  The
@@ -55,8 +55,12 @@ using sili::pack2;
 constexpr int kM = 128;               // rows of a tile (MMA M)
 constexpr int kTiles = 2;
 constexpr int kKeys = 128;            // keys a step (MMA N of S, K of P V)
-constexpr int kSoftmax = kTiles * 128, kDequant = 128;
-constexpr int kThreads = kSoftmax + kDequant + 32;
+constexpr int kSoftmax = kTiles * 128, kDequant = 256;
+constexpr int kThreads = kSoftmax + kDequant + 128;     // whole warpgroups: each sets its share of the registers
+// registers a thread after the split; together what the launch holds: 96 * 640
+constexpr int kRegsSoftmax = 136, kRegsDequant = 80, kRegsRest = 48;
+static_assert(kSoftmax * kRegsSoftmax + kDequant * kRegsDequant + 128 * kRegsRest <= 96 * kThreads, "register split");
+constexpr int kMmaWarp = (kSoftmax + kDequant) / 32;
 constexpr int kPolls = 1 << 22;       // try_wait polls (each waits a while by itself) before giving up
 
 template <int D>
@@ -65,9 +69,9 @@ struct Smem {
     alignas(1024) uint8_t k[2][kKeys * D * 2];
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     alignas(8) unsigned long long kv_full[2], kv_free[2], s_full[2], p_full[2], drained;
-    uint8_t odd_keys[2][16][8];       // [stage][8 keys][dim / 8 elements]: bits of keys whose V scale is not a number
+    uint8_t odd_keys[2][16][4];       // [stage][8 keys][group]: bits of keys whose V scale is not a number
     int odd[2];                       // the last step whose stage had any, plus one
-    uint8_t there[2][8];              // [stage][16 keys]: their page exists
+    alignas(8) uint8_t there[2][8];   // [stage][16 keys]: their page exists
     uint32_t tmem;
     int dead;
     int hit[3];                       // the CTA's request, kv head and row tile pair
@@ -97,46 +101,51 @@ __device__ __forceinline__ bool bar_wait(unsigned long long* b, uint32_t parity,
     return false;
 }
 
-// shared-memory matrix descriptor: K-major, 128-byte swizzle, atoms of 8 rows x 128 bytes 1024 bytes apart
-__device__ __forceinline__ uint64_t desc(const void* p) {
-    return (uint64_t)((addr(p) >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// shared-memory matrix descriptor: K-major, 128-byte swizzle, atoms of 8 rows x 128 bytes 1024 bytes apart.  Only the
+// low word (start address / 16, leading offset 1) differs between operands: the issuing thread adds to that alone.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(const void* p) { return ((addr(p) >> 4) & 0x3FFFu) | (1u << 16); }
 // byte offset of 16-byte chunk c (0..7) of row r in a [rows x 64] half block of that layout
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
 // kind::f16 instruction descriptor: D f32, A and B f16, both K-major
 __device__ constexpr uint32_t idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+// D += A B (ACC) or D = A B; A in shared memory or (ts) in tensor memory
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id),
+                 "n"(kDescHigh), "n"(ACC ? 1 : 0));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "mov.b64 y, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id),
+                 "n"(kDescHigh), "r"((uint32_t)acc));
 }
 __device__ __forceinline__ void commit(unsigned long long* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(addr(b)) : "memory");
 }
 
-// 32 columns of this warp's lanes; the registers are not to be touched before tmem_wait has taken them through
-__device__ __forceinline__ void tmem_ld32(uint32_t a, float (&v)[32]) {
+// 16 columns of this warp's lanes; the registers are not to be touched before tmem_wait has taken them through
+__device__ __forceinline__ void tmem_ld16(uint32_t a, float (&v)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
-          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
-          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
-          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(a));
 }
-__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
+__device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-          "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
-          "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
-          "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
-          "+f"(v[31])::"memory");
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t c;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
     asm volatile(
@@ -211,162 +220,167 @@ struct Prompt {
     __device__ __forceinline__ uint32_t s_col(int t) const { return s.tmem + t * kKeys; }
     __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + kTiles * kKeys + t * D; }
 
-    // ── warps 8-11: 4-bit keys and values of step j into stage j & 1 ──
+    // ── warps 8-15: 4-bit keys and values of step j into stage j & 1 ──
     __device__ __forceinline__ void dequantise() {
         const int tid = threadIdx.x - kSoftmax, dw = tid >> 5, lane = tid & 31;
-        // K: E lanes a key, 16 bytes (one group of 32) each
-        constexpr int kPer = 32 / E;                // keys of one load instruction
-        const int kq = lane % E, kkey = dw * 32 + lane / E;
-        // V: 8 keys of D/8 elements; lane & 7 numbers the keys, so a store instruction fills whole rows
-        constexpr int kVw = D / 64;                 // words a key
+        // K: 16 keys a warp, E lanes a key, 16 bytes (one group of 32) each
+        constexpr int kPer = 32 / E, kLoads = 16 / kPer;       // keys of one load instruction, loads
+        const int kq = lane % E, kkey = dw * 16;
+        // V: 8 keys x 8 elements a thread; lane & 7 numbers the keys, so a store instruction fills whole rows
         const int half = dw & 1, c = lane & 7, db = (dw >> 1) * 4 + (lane >> 3), vkey = half * 64 + c * 8;
-        const int vg = db * (D / 8) / 32;
-        uint4 rk[E];
-        uint32_t sk[E], rv[8][kVw], sv[8];
-        int pk[E], pv;
+        const bool has_v = db < D / 8;
+        const int vg = db >> 2;
+        uint4 rk[kLoads];
+        uint32_t sk[kLoads], rv[8], sv[8];
+        int pk, pv, next_pk, next_pv;
+        auto col_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page; };
         auto page_of = [&](int key) {
-            const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
             // whole runs of 16 keys (they share a page and a bit of `there`), of which the last may reach past the end
-            return (key & ~15) < w.len ? __ldg(a.table + w.r * a.stride + col) : -1;
+            return (key & ~15) < w.len ? __ldg(a.table + w.r * a.stride + col_of(key)) : -1;
         };
         auto pages = [&](int j) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) pk[i] = page_of(j * kKeys + dw * 32 + i * kPer);
-            pv = page_of(j * kKeys + vkey);
+            next_pk = page_of(j * kKeys + kkey);
+            next_pv = page_of(j * kKeys + vkey);
         };
-        // (first key of the load) -> row of the cache, or -1
-        auto row_of = [&](int pg, int key, int which) -> int64_t {
-            if (pg < 0 || pg >= a.n_pages) return -1;
-            const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
-            return sili::kv4_row(pg, which, w.h, a.kv_heads, a.page) + (key - col * a.page);
+        auto row_of = [&](int pg, int key, int which) {
+            return sili::kv4_row(pg, which, w.h, a.kv_heads, a.page) + (key - col_of(key) * a.page);
         };
-        uint32_t there = 0;
-        auto load = [&](int j) {
-            there = 0;
+        auto load_k = [&](int j) {
+            const bool there = pk >= 0 && pk < a.n_pages;
+            const int64_t row = there ? row_of(pk, j * kKeys + kkey, 0) + lane / E : 0;
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const int64_t row = row_of(pk[i], j * kKeys + dw * 32 + i * kPer, 0);
+            for (int i = 0; i < kLoads; ++i) {
                 rk[i] = make_uint4(0, 0, 0, 0);
                 sk[i] = 0;
-                if (row >= 0) {
-                    there |= 1u << i;
-                    rk[i] = __ldg((const uint4*)(a.codes + (row + lane / E) * (D / 2) + kq * 16));
-                    sk[i] = __ldg(a.scales + (row + lane / E) * E + kq);
+                if (there) {
+                    rk[i] = __ldg((const uint4*)(a.codes + (row + i * kPer) * (D / 2) + kq * 16));
+                    sk[i] = __ldg(a.scales + (row + i * kPer) * E + kq);
                 }
             }
-            const int64_t row = row_of(pv, j * kKeys + vkey, 1);
+            return there;
+        };
+        auto load_v = [&](int j) {
+            const bool there = has_v && pv >= 0 && pv < a.n_pages;
+            const int64_t row = there ? row_of(pv, j * kKeys + vkey, 1) : 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sv[i] = 0;
-#pragma unroll
-                for (int q = 0; q < kVw; ++q) rv[i][q] = 0;
-                if (row >= 0) {
-                    const uint8_t* p = a.codes + (row + i) * (D / 2) + db * (D / 16);
-                    if constexpr (kVw == 2) {
-                        const uint2 x = __ldg((const uint2*)p);
-                        rv[i][0] = x.x; rv[i][kVw - 1] = x.y;
-                    } else rv[i][0] = __ldg((const uint32_t*)p);
+                rv[i] = sv[i] = 0;
+                if (there) {
+                    rv[i] = __ldg((const uint32_t*)(a.codes + (row + i) * (D / 2) + db * 4));
                     sv[i] = __ldg(a.scales + (row + i) * E + vg);
                 }
             }
         };
         pages(w.j0);
-        load(w.j0);
+        pk = next_pk; pv = next_pv;
+        bool there = load_k(w.j0);
+        load_v(w.j0);
         if (w.j0 + 1 < w.last) pages(w.j0 + 1);
         for (int j = w.j0; j < w.last; ++j) {
             const int n = j - w.j0, st = n & 1;
+            const bool more = j + 1 < w.last;
             if (n >= 2 && !bar_wait(&s.kv_free[st], ((n >> 1) - 1) & 1, &s.dead)) return;
             // K: rows are keys
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const int key = kkey + i * kPer;
-                const uint32_t sc = sk[i] * 0x00800080u;
+            if (lane == 0) s.there[st][dw] = there;
+            {
                 uint8_t* block = s.k[st] + (kq >> 1) * (kKeys * 128);
                 // lanes of the second block go through their four chunks two further on: eight lanes, eight banks' worth
                 const bool far = E == 4 && (kq & 2);
-                const uint32_t wd[4] = {far ? rk[i].z : rk[i].x, far ? rk[i].w : rk[i].y, far ? rk[i].x : rk[i].z,
-                                        far ? rk[i].y : rk[i].w};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t f[4];
-                    sili::kv4_decode4(wd[q], f);
-                    const int ch = (kq & 1) * 4 + (far ? q ^ 2 : q);
-                    *(uint4*)(block + chunk_at(key, ch)) = make_uint4(mul2(f[0], sc), mul2(f[1], sc), mul2(f[2], sc), mul2(f[3], sc));
+                for (int i = 0; i < kLoads; ++i) {
+                    const int key = kkey + lane / E + i * kPer;
+                    const uint32_t sc = sk[i] * 0x00800080u;
+                    const uint32_t wd[4] = {far ? rk[i].z : rk[i].x, far ? rk[i].w : rk[i].y, far ? rk[i].x : rk[i].z,
+                                            far ? rk[i].y : rk[i].w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t f[4];
+                        sili::kv4_decode4(wd[q], f);
+                        const int ch = (kq & 1) * 4 + (far ? q ^ 2 : q);
+                        *(uint4*)(block + chunk_at(key, ch)) =
+                            make_uint4(mul2(f[0], sc), mul2(f[1], sc), mul2(f[2], sc), mul2(f[3], sc));
+                    }
                 }
-                if (lane == 0) s.there[st][(dw * 32 + i * kPer) / 16] = there >> i & 1;
+            }
+            if (more) {
+                pk = next_pk;
+                there = load_k(j + 1);
             }
             // V: rows are elements; scales that are no numbers are left out and noted
-            uint32_t bits = 0;
+            if (has_v) {
+                uint32_t bits = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (sv[i] >= 0xF8u) { bits |= 1u << i; sv[i] = 0; }
-            s.odd_keys[st][half * 8 + c][db] = (uint8_t)bits;
-            if (bits) *(volatile int*)&s.odd[st] = j + 1;
-            uint32_t sc[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) sc[p] = sv[2 * p] << 7 | sv[2 * p + 1] << 23;
-            uint8_t* block = s.v[st] + half * (D * 128);
-#pragma unroll
-            for (int q = 0; q < kVw; ++q) {
+                for (int i = 0; i < 8; ++i)
+                    if (sv[i] >= 0xF8u) { bits |= 1u << i; sv[i] = 0; }
+                if ((db & 3) == 0) s.odd_keys[st][half * 8 + c][vg] = (uint8_t)bits;
+                if (bits) *(volatile int*)&s.odd[st] = j + 1;
                 constexpr uint32_t kLow = 0x0F0F0F0Fu;
                 uint32_t even[4][4], odd[4][4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const uint32_t x = rv[2 * p][q], y = rv[2 * p + 1][q];
+                    const uint32_t x = rv[2 * p], y = rv[2 * p + 1], sc = sv[2 * p] << 7 | sv[2 * p + 1] << 23;
                     sili::kv4_decode4((x & kLow) | ((y << 4) & ~kLow), even[p]);
                     sili::kv4_decode4(((x >> 4) & kLow) | (y & ~kLow), odd[p]);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) { even[p][b] = mul2(even[p][b], sc); odd[p][b] = mul2(odd[p][b], sc); }
                 }
+                uint8_t* block = s.v[st] + half * (D * 128);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const int d = db * (D / 8) + 8 * q + 2 * b;
-                    *(uint4*)(block + chunk_at(d, c)) = make_uint4(mul2(even[0][b], sc[0]), mul2(even[1][b], sc[1]),
-                                                                   mul2(even[2][b], sc[2]), mul2(even[3][b], sc[3]));
-                    *(uint4*)(block + chunk_at(d + 1, c)) = make_uint4(mul2(odd[0][b], sc[0]), mul2(odd[1][b], sc[1]),
-                                                                       mul2(odd[2][b], sc[2]), mul2(odd[3][b], sc[3]));
+                    const int d = db * 8 + 2 * b;
+                    *(uint4*)(block + chunk_at(d, c)) = make_uint4(even[0][b], even[1][b], even[2][b], even[3][b]);
+                    *(uint4*)(block + chunk_at(d + 1, c)) = make_uint4(odd[0][b], odd[1][b], odd[2][b], odd[3][b]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             bar_arrive(&s.kv_full[st]);
-            if (j + 1 < w.last) {
-                load(j + 1);
+            if (more) {
+                pv = next_pv;
+                load_v(j + 1);
                 if (j + 2 < w.last) pages(j + 2);
             }
         }
     }
 
-    // ── one thread of warp 12: the products ──
+    // ── one thread of warp 16: the products ──
+    // One thread's instructions are the chain that every product waits for, so it computes nothing per product but an
+    // addition to a descriptor's low word.
     __device__ __forceinline__ void products() {
-        auto scores = [&](int t, int st) {
+        const uint32_t q0 = desc_low(s.q[0]), k0 = desc_low(s.k[0]), v0 = desc_low(s.v[0]);
+        constexpr uint32_t kTileQ = kM * D * 2 / 16, kStage = kKeys * D * 2 / 16;
+        const int n0 = w.n[0] - w.j0, n1 = w.n[1] - w.j0, steps = w.last - w.j0;
+        auto scores = [&](uint32_t q, uint32_t d, unsigned long long* done, int st) {
+            const uint32_t k = k0 + st * kStage;
+            mma_ss<false>(d, q, k, idesc(kM, kKeys));
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                mma_ss(s_col(t), desc(s.q[t] + (k >> 2) * (kM * 128)) + 2 * (k & 3),
-                       desc(s.k[st] + (k >> 2) * (kKeys * 128)) + 2 * (k & 3), idesc(kM, kKeys), k > 0);
-            commit(&s.s_full[t]);
+            for (int i = 1; i < D / 16; ++i)
+                mma_ss<true>(d, q + (i >> 2) * (kM * 8) + 2 * (i & 3), k + (i >> 2) * (kKeys * 8) + 2 * (i & 3), idesc(kM, kKeys));
+            commit(done);
+        };
+        auto tile = [&](auto which, int n, int mine) {      // false: a wait gave up
+            constexpr int t = decltype(which)::value;
+            const int st = n & 1;
+            if (!bar_wait(&s.p_full[t], n & 1, &s.dead)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            const uint32_t v = v0 + st * kStage, p = s_col(t), o = o_col(t);
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i)
+                mma_ts(o, p + 8 * i, v + (i >> 2) * (D * 8) + 2 * (i & 3), idesc(kM, D), i > 0 || n > 0);
+            // the last product of this step: the stage is free when it is done
+            if (t == 1 || n >= n1) commit(&s.kv_free[st]);
+            if (n + 1 == mine) { commit(&s.s_full[t]); return true; }       // O is complete
+            if (!bar_wait(&s.kv_full[st ^ 1], ((n + 1) >> 1) & 1, &s.dead)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            scores(q0 + t * kTileQ, s_col(t), &s.s_full[t], st ^ 1);
+            return true;
         };
         if (!bar_wait(&s.kv_full[0], 0, &s.dead)) return;
         asm volatile("tcgen05.fence::after_thread_sync;");
-        for (int t = 0; t < kTiles; ++t)
-            if (w.j0 < w.n[t]) scores(t, 0);
-        for (int j = w.j0; j < w.last; ++j) {
-            const int n = j - w.j0, st = n & 1;
-            for (int t = 0; t < kTiles; ++t) {
-                if (j >= w.n[t]) continue;
-                if (!bar_wait(&s.p_full[t], n & 1, &s.dead)) return;
-                asm volatile("tcgen05.fence::after_thread_sync;");
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(o_col(t), s_col(t) + 8 * k, desc(s.v[st] + (k >> 2) * (D * 128)) + 2 * (k & 3), idesc(kM, D),
-                           n > 0 || k > 0);
-                // the last product of this step: the stage is free when it is done
-                if (t == kTiles - 1 || j >= w.n[t + 1]) commit(&s.kv_free[st]);
-                if (j + 1 < w.n[t]) {
-                    if (!bar_wait(&s.kv_full[st ^ 1], ((n + 1) >> 1) & 1, &s.dead)) return;
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    scores(t, st ^ 1);
-                } else {
-                    commit(&s.s_full[t]);      // O is complete
-                }
-            }
+        if (n0 > 0) scores(q0, s_col(0), &s.s_full[0], 0);
+        if (n1 > 0) scores(q0 + kTileQ, s_col(1), &s.s_full[1], 0);
+        for (int n = 0; n < steps; ++n) {
+            if (n < n0 && !tile(std::integral_constant<int, 0>{}, n, n0)) return;
+            if (n < n1 && !tile(std::integral_constant<int, 1>{}, n, n1)) return;
         }
     }
 
@@ -374,15 +388,12 @@ struct Prompt {
     __device__ __forceinline__ void rescale(int t, uint32_t lanes, float f) {
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
+            float x[16];
+            tmem_ld16(o_col(t) + lanes + 16 * c, x);
+            tmem_wait(x);
             uint32_t r[16];
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-                "tcgen05.wait::ld.sync.aligned;"
-                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                : "r"(o_col(t) + lanes + 16 * c) : "memory");
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(x[i] * f);
             tmem_st16(o_col(t) + lanes + 16 * c, r);
         }
     }
@@ -395,7 +406,11 @@ struct Prompt {
         const bool real = row < w.rows;
         const int64_t q_row = span_row() + (real ? row / w.group : 0);
         const int head = w.h * w.group + (real ? row % w.group : 0);
-        const int64_t pos = w.pos_of(row), first = w.pos_of(warp_row0), final = w.pos_of(warp_row0 + 31);
+        // the row sees keys [from, to); every row of the warp sees those in [all_from, all_to)
+        const int64_t pos = w.pos_of(row);
+        const int to = (int)min(pos + 1, (int64_t)w.len), from = a.window ? (int)max(pos - a.window + 1, (int64_t)0) : 0;
+        const int all_to = (int)min(w.pos_of(warp_row0) + 1, (int64_t)w.len);
+        const int all_from = a.window ? (int)max(w.pos_of(warp_row0 + 31) - a.window + 1, (int64_t)0) : 0;
         // Q into shared memory as halves
         // (with the scale's sign, so that the logits' factor is never negative)
         float cf = fabsf(a.scale) * kLog2e;
@@ -439,80 +454,117 @@ struct Prompt {
             ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], n & 1, &s.dead));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            // keys [lo, hi) of the step are the row's; pages that are not there, 16 keys a bit
-            uint32_t gone = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) gone |= (s.there[st][i] ? 0u : 1u) << i;
-            const bool inside = !gone && key0 + kKeys - 1 <= first && key0 + kKeys <= w.len && (!a.window || key0 > final - a.window);
-            const int hi = (int)min((int64_t)kKeys, min(pos + 1, (int64_t)w.len) - key0);
-            const int lo = a.window ? (int)max((int64_t)0, pos - a.window + 1 - key0) : 0;
+            // keys [lo, hi) of the step are the row's; pages that are not there, a byte per 16 keys
+            const uint64_t there = *(const volatile uint64_t*)s.there[st];
+            const bool inside = there == 0x0101010101010101ull && key0 + kKeys <= all_to && key0 >= all_from;
+            const int hi = to - key0, lo = from - key0;
             auto step = [&](auto masked) {
-                auto mask = [&](float (&y)[32], int c) {
-                    if constexpr (decltype(masked)::value) {
+                auto mask = [&](float (&y)[16], int chunk) {
+                    if constexpr (!decltype(masked)::value) return;
+                    const bool here = there >> (8 * chunk) & 1;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = 32 * c + i;
-                            if (key < lo || key >= hi || (gone >> (key / 16) & 1)) y[i] = -INFINITY;
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = 16 * chunk + i;
+                        if (key < lo || key >= hi || !here) y[i] = -INFINITY;
+                    }
+                };
+                // The running maximum is that of the keys before, so P follows from S in one pass, 64 keys at a time (the
+                // next 16 columns on their way while the current ones are worked on).  A row whose P passes 2^15 first
+                // sends its warp through the maximum of these keys, whose S is there until P is stored; the maximum
+                // moves by whole powers of two, so what is held under the old one is rescaled exactly.
+                float x[2][16];
+                auto raise = [&](int half) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");    // O and P as last stored
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                        tmem_ld16(s_col(t) + lanes + 16 * c, x[0]);
+                        tmem_wait(x[0]);
+                        mask(x[0], c);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(x[0][i], x[0][i + 1]));
+                    }
+                    if (top != -INFINITY) top = top * cf - kLift;
+                    float f = 1.f;
+                    if (base == -INFINITY) {
+                        base = top;
+                    } else if (top > base) {
+                        const float up = ceilf(top - base);       // inf where a logit is: NaN from there on
+                        base += up;
+                        f = up < 127.f ? __int_as_float((127 - (int)up) << 23) : 0.f;
+                    }
+                    l *= f;
+                    if (n > 0) rescale(t, lanes, f);
+                    if (half) {       // the first 64 keys' P
+                        const uint32_t f2 = pack2(f, f);
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            tmem_ld16(s_col(t) + lanes + 16 * c, x[0]);
+                            tmem_wait(x[0]);
+                            uint32_t q[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) q[i] = mul2(__float_as_uint(x[0][i]), f2);
+                            tmem_st16(s_col(t) + lanes + 16 * c, q);
                         }
                     }
                 };
-                // two passes over S, the next 32 columns on their way while the current ones are worked on
-                float x[2][32], top = -INFINITY;
-                tmem_ld32(s_col(t) + lanes, x[0]);
-                tmem_wait(x[0]);
+                // (loops kept rolled: the roles share the instruction cache)
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    bool high = __any_sync(0xffffffffu, base == -INFINITY);
+                    uint32_t p[2][16];
+                    float sum;
+#pragma unroll 1
+                    for (;;) {
+                        if (high) {
+                            const float before = base;
+                            raise(half);
+                            high = __any_sync(0xffffffffu, base > before);
+                        }
+                        const float shift = base == -INFINITY ? 0.f : base;
+                        float sum0 = 0.f, sum1 = 0.f;
+                        uint32_t most = 0, more = 0;
+                        tmem_ld16(s_col(t) + lanes + 64 * half, x[0]);
+                        tmem_wait(x[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float(&y)[32] = x[c & 1];
-                    tmem_ld32(s_col(t) + lanes + 32 * ((c + 1) & 3), x[~c & 1]);
-                    mask(y, c);
-                    float m0 = fmaxf(y[0], y[1]), m1 = fmaxf(y[2], y[3]);
+                        for (int c = 0; c < 4; ++c) {
+                            float(&y)[16] = x[c & 1];
+                            if (c < 3) tmem_ld16(s_col(t) + lanes + 64 * half + 16 * (c + 1), x[~c & 1]);
 #pragma unroll
-                    for (int i = 4; i < 32; i += 4) {
-                        m0 = fmaxf(m0, fmaxf(y[i], y[i + 1]));
-                        m1 = fmaxf(m1, fmaxf(y[i + 2], y[i + 3]));
+                            for (int i = 0; i < 16; ++i) y[i] = fmaf(y[i], cf, -shift);
+                            mask(y, 4 * half + c);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float u = ex2(y[i]), v = ex2(y[i + 1]);
+                                sum0 += u; sum1 += v;
+                                const uint32_t h = pack2(u, v);
+                                p[c / 2][8 * (c & 1) + i / 2] = h;
+                                if (i & 2) most = max2(most, h); else more = max2(more, h);
+                            }
+                            if (c < 3) tmem_wait(x[~c & 1]);
+                        }
+                        sum = sum0 + sum1;
+                        most = max2(most, more);
+                        // 2^15 as a half is 0x7800 (NaN is passed over by max2)
+                        const bool over = __any_sync(0xffffffffu, (most & 0xFFFFu) > 0x7800u || (most >> 16) > 0x7800u);
+                        // once raised, only a row without a finite maximum is still over
+                        if (!over || high) break;
+                        high = true;
                     }
-                    top = fmaxf(top, fmaxf(m0, m1));
-                    tmem_wait(x[~c & 1]);
-                }
-                if (top != -INFINITY) top *= cf;
-                if (__any_sync(0xffffffffu, top - kLift > base + kSlack)) {
-                    const float fresh = fmaxf(base, top - kLift);
-                    const float f = fresh == base ? 1.f : ex2(base - fresh);
-                    base = fresh;
-                    l *= f;
-                    if (n > 0) rescale(t, lanes, f);
-                }
-                const float shift = base == -INFINITY ? 0.f : base;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float(&y)[32] = x[c & 1];      // x[0] already holds the first columns
-                    if (c < 3) tmem_ld32(s_col(t) + lanes + 32 * (c + 1), x[~c & 1]);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], cf, -shift);
-                    mask(y, c);
-                    uint32_t p[16];
-                    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float u = ex2(y[i]), v = ex2(y[i + 1]);
-                        sum0 += u; sum1 += v;
-                        p[i / 2] = pack2(u, v);
-                    }
-                    l += sum0 + sum1;
-                    // P takes the place of columns that have been read
-                    if (c < 3) tmem_wait(x[~c & 1]);
-                    tmem_st16(s_col(t) + lanes + 16 * c, p);
+                    l += sum;
+                    tmem_st16(s_col(t) + lanes + 32 * half, p[0]);
+                    tmem_st16(s_col(t) + lanes + 32 * half + 16, p[1]);
                 }
             };
-            // two copies of the step: the masks' arithmetic must not run in the steps without any
+            // two copies: the masks' arithmetic must not run in the steps without any
             if (inside) step(std::false_type{});
             else step(std::true_type{});
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (*(volatile int*)&s.odd[st] == j + 1) {
-                for (int key = max(lo, 0); key < hi; ++key) {
-                    if (gone >> (key / 16) & 1) continue;
+                for (int key = max(lo, 0); key < min(hi, kKeys); ++key) {
+                    if (!(there >> (8 * (key / 16)) & 1)) continue;
                     for (int g = 0; g < E; ++g)
-                        if (s.odd_keys[st][key >> 3][g * (8 / E)] >> (key & 7) & 1) poisoned |= 1u << g;
+                        if (s.odd_keys[st][key >> 3][g] >> (key & 7) & 1) poisoned |= 1u << g;
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
@@ -525,23 +577,23 @@ struct Prompt {
         float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t id = q_row * a.heads + head;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-            float x[32];
+        for (int c = 0; c < D / 16; ++c) {
+            float x[16];
             __syncwarp();
             if (steps > 0) {
-                tmem_ld32(o_col(t) + lanes + 32 * c, x);
+                tmem_ld16(o_col(t) + lanes + 16 * c, x);
                 tmem_wait(x);
             } else
 #pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = 0.f;
-            const bool bad = !ok || (poisoned >> c & 1);
+                for (int i = 0; i < 16; ++i) x[i] = 0.f;
+            const bool bad = !ok || (poisoned >> (c / 2) & 1);
             if (real)
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
+                for (int i = 0; i < 16; i += 8) {
                     sili::Pack<T, 8> o;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) o.v[k] = sili::from_f32<T>(bad ? __int_as_float(0x7FC00000) : x[i + k] * inv);
-                    *(sili::Pack<T, 8>*)((T*)a.out + id * D + 32 * c + i) = o;
+                    *(sili::Pack<T, 8>*)((T*)a.out + id * D + 16 * c + i) = o;
                 }
         }
         if (real && a.lse) a.lse[id] = !ok ? __int_as_float(0x7FC00000) : l == 0.f ? -INFINITY : kLn2 * (base + log2f(l));
@@ -588,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     }
     __syncthreads();
     if (s.hit[0] < 0) return;
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(addr(&s.tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -618,27 +670,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         w.last = max(w.last, w.n[t]);
     }
     if (warp < kSoftmax / 32) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         k.softmax();
-    } else {
+    } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDequant));
         __syncthreads();       // Q is there
-        if (w.last > w.j0) {
-            if (warp < (kSoftmax + kDequant) / 32) k.dequantise();
-            else if ((threadIdx.x & 31) == 0) {
-                k.products();
-                // what was begun is waited for (bounded): the tensor memory is freed next
-                if (*(volatile int*)&s.dead) {
-                    atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
-                    int quiet = 0;
-                    commit(&s.drained);
-                    bar_wait(&s.drained, 0, &quiet);
-                }
+        if (w.last > w.j0) k.dequantise();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+        __syncthreads();       // Q is there
+        if (w.last > w.j0 && threadIdx.x == kMmaWarp * 32) {
+            k.products();
+            // what was begun is waited for (bounded): the tensor memory is freed next
+            if (*(volatile int*)&s.dead) {
+                atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
+                int quiet = 0;
+                commit(&s.drained);
+                bar_wait(&s.drained, 0, &quiet);
             }
-            __syncwarp();
         }
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(512));
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(512));
 }
 
 template <typename T, int D>
