@@ -61,7 +61,8 @@ constexpr int kThreads = kSoftmax + kDequant + 128;     // whole warpgroups: eac
 constexpr int kRegsSoftmax = 136, kRegsDequant = 80, kRegsRest = 48;
 static_assert(kSoftmax * kRegsSoftmax + kDequant * kRegsDequant + 128 * kRegsRest <= 96 * kThreads, "register split");
 constexpr int kMmaWarp = (kSoftmax + kDequant) / 32;
-constexpr int kPolls = 1 << 22;       // try_wait polls (each waits a while by itself) before giving up
+constexpr int kPolls = 4096;          // polls of a wait, each asleep for up to kNap ns, before it gives up
+constexpr uint32_t kNap = 1000000;
 
 template <int D>
 struct Smem {
@@ -91,11 +92,11 @@ __device__ __forceinline__ bool bar_wait(unsigned long long* b, uint32_t parity,
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(a), "r"(parity) : "memory");
+            : "=r"(done) : "r"(a), "r"(parity), "r"(kNap) : "memory");
         if (done) return true;
-        if ((i & 255) == 255 && *(volatile int*)dead) return false;
+        if (*(volatile int*)dead) return false;
     }
     *(volatile int*)dead = 1;
     return false;
@@ -141,11 +142,6 @@ __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
                    "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
-}
-__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
-    uint32_t c;
-    asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-    return c;
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
     asm volatile(
@@ -469,7 +465,7 @@ struct Prompt {
                     }
                 };
                 // The running maximum is that of the keys before, so P follows from S in one pass, 64 keys at a time (the
-                // next 16 columns on their way while the current ones are worked on).  A row whose P passes 2^15 first
+                // next 16 columns on their way while the current ones are worked on).  A row whose P passes a half's range first
                 // sends its warp through the maximum of these keys, whose S is there until P is stored; the maximum
                 // moves by whole powers of two, so what is held under the old one is rescaled exactly.
                 float x[2][16];
@@ -523,7 +519,6 @@ struct Prompt {
                         }
                         const float shift = base == -INFINITY ? 0.f : base;
                         float sum0 = 0.f, sum1 = 0.f;
-                        uint32_t most = 0, more = 0;
                         tmem_ld16(s_col(t) + lanes + 64 * half, x[0]);
                         tmem_wait(x[0]);
 #pragma unroll
@@ -537,16 +532,13 @@ struct Prompt {
                             for (int i = 0; i < 16; i += 2) {
                                 const float u = ex2(y[i]), v = ex2(y[i + 1]);
                                 sum0 += u; sum1 += v;
-                                const uint32_t h = pack2(u, v);
-                                p[c / 2][8 * (c & 1) + i / 2] = h;
-                                if (i & 2) most = max2(most, h); else more = max2(more, h);
+                                p[c / 2][8 * (c & 1) + i / 2] = pack2(u, v);
                             }
                             if (c < 3) tmem_wait(x[~c & 1]);
                         }
                         sum = sum0 + sum1;
-                        most = max2(most, more);
-                        // 2^15 as a half is 0x7800 (NaN is passed over by max2)
-                        const bool over = __any_sync(0xffffffffu, (most & 0xFFFFu) > 0x7800u || (most >> 16) > 0x7800u);
+                        // a sum that a half holds has no summand that it does not
+                        const bool over = __any_sync(0xffffffffu, sum > 65504.f);
                         // once raised, only a row without a finite maximum is still over
                         if (!over || high) break;
                         high = true;
