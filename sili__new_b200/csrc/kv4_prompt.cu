@@ -10,7 +10,7 @@
 // exponentials run while the other's products do; warps 8-11 turn the next
 // keys' 4-bit K and V into halves in shared memory (K as it lies, V
 // transposed by interleaving the nibbles of two keys), straight from global
-// memory through registers; one thread of warp 16 issues the products.  All
+// memory through registers; a thread of warps 16 and 17 each issues a tile's products.  All
 // operands are K-major with the 128-byte swizzle.  K and V are exact in
 // half; bf16 queries are scaled to halves exactly by a power of two a row;
 // P is rounded once to half (2^-12, below the output's rounding).  The
@@ -54,7 +54,8 @@ using sili::pack2;
 
 constexpr int kM = 128;               // rows of a tile (MMA M)
 constexpr int kTiles = 2;
-constexpr int kKeys = 128;            // keys a step (MMA N of S, K of P V)
+constexpr int kKeys = 128;            // keys a stage of shared memory
+constexpr int kSub = 64;              // keys a step of a tile (MMA N of S, K of P V)
 constexpr int kSoftmax = kTiles * 128, kDequant = 256;
 constexpr int kThreads = kSoftmax + kDequant + 128;     // whole warpgroups: each sets its share of the registers
 // registers a thread after the split; together what the launch holds: 96 * 640
@@ -69,7 +70,8 @@ struct Smem {
     alignas(1024) uint8_t q[kTiles][kM * D * 2];
     alignas(1024) uint8_t k[2][kKeys * D * 2];
     alignas(1024) uint8_t v[2][kKeys * D * 2];
-    alignas(8) unsigned long long kv_full[2], kv_free[2], s_full[2], p_full[2], drained;
+    alignas(8) unsigned long long kv_full[2], kv_free[2];                                  // by stage
+    unsigned long long s_full[2], s_free[2], p_full[2], p_free[2], drained[2];  // by tile
     uint8_t odd_keys[2][16][4];       // [stage][8 keys][group]: bits of keys whose V scale is not a number
     int odd[2];                       // the last step whose stage had any, plus one
     alignas(8) uint8_t there[2][8];   // [stage][16 keys]: their page exists
@@ -141,7 +143,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t a, float (&v)[16]) {
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 ::"memory");
+}
+__device__ __forceinline__ void tmem_wait(float (&v)[64]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                   "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]),
+                   "+f"(v[32]), "+f"(v[33]), "+f"(v[34]), "+f"(v[35]), "+f"(v[36]), "+f"(v[37]), "+f"(v[38]), "+f"(v[39]),
+                   "+f"(v[40]), "+f"(v[41]), "+f"(v[42]), "+f"(v[43]), "+f"(v[44]), "+f"(v[45]), "+f"(v[46]), "+f"(v[47]),
+                   "+f"(v[48]), "+f"(v[49]), "+f"(v[50]), "+f"(v[51]), "+f"(v[52]), "+f"(v[53]), "+f"(v[54]), "+f"(v[55]),
+                   "+f"(v[56]), "+f"(v[57]), "+f"(v[58]), "+f"(v[59]), "+f"(v[60]), "+f"(v[61]), "+f"(v[62]), "+f"(v[63])
+                 ::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
     asm volatile(
@@ -155,7 +170,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
 struct Work {
     int r, h, group, rows, row0, len;
     int64_t pos0;          // position of the request's first query
-    int j0, n[kTiles], last;   // steps [j0, n[w]) of each tile, and of the longer one
+    int j0, last;              // stages [j0, last) of keys
+    int n[kTiles];             // each tile's steps, from stage j0 on
 
     __device__ __forceinline__ int64_t pos_of(int row) const { return pos0 + min(row, rows - 1) / group; }
 };
@@ -213,8 +229,10 @@ struct Prompt {
     Smem<D>& s;
     Work w;
 
-    __device__ __forceinline__ uint32_t s_col(int t) const { return s.tmem + t * kKeys; }
-    __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + kTiles * kKeys + t * D; }
+    // tensor memory: S (64 columns a tile), P (32), O (dim)
+    __device__ __forceinline__ uint32_t s_col(int t) const { return s.tmem + t * kSub; }
+    __device__ __forceinline__ uint32_t p_col(int t) const { return s.tmem + kTiles * kSub + t * (kSub / 2); }
+    __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + kTiles * kSub * 3 / 2 + t * D; }
 
     // ── warps 8-15: 4-bit keys and values of step j into stage j & 1 ──
     __device__ __forceinline__ void dequantise() {
@@ -338,45 +356,45 @@ struct Prompt {
         }
     }
 
-    // ── one thread of warp 16: the products ──
-    // One thread's instructions are the chain that every product waits for, so it computes nothing per product but an
-    // addition to a descriptor's low word.
-    __device__ __forceinline__ void products() {
-        const uint32_t q0 = desc_low(s.q[0]), k0 = desc_low(s.k[0]), v0 = desc_low(s.v[0]);
-        constexpr uint32_t kTileQ = kM * D * 2 / 16, kStage = kKeys * D * 2 / 16;
-        const int n0 = w.n[0] - w.j0, n1 = w.n[1] - w.j0, steps = w.last - w.j0;
-        auto scores = [&](uint32_t q, uint32_t d, unsigned long long* done, int st) {
-            const uint32_t k = k0 + st * kStage;
-            mma_ss<false>(d, q, k, idesc(kM, kKeys));
+    // ── one thread of warps 16 and 17 each: the products of tile t ──
+    // (a thread a tile: neither waits behind the other's products being queued).  The thread's instructions are the chain
+    // that its tile waits for, so it computes nothing per product but an addition to a descriptor's low word.
+    __device__ __forceinline__ void products(int t) {
+        constexpr uint32_t kStage = kKeys * D * 2 / 16;
+        const uint32_t q = desc_low(s.q[t]), k0 = desc_low(s.k[0]), v0 = desc_low(s.v[0]), d = s_col(t), p = p_col(t), o = o_col(t);
+        const int mine = w.n[t], stages = w.last - w.j0;
+        auto scores = [&](int i) {      // step i: the keys' rows 64 (i & 1) on of stage (i >> 1) & 1
+            const uint32_t k = k0 + (i >> 1 & 1) * kStage + (i & 1) * (kSub * 8);
+            mma_ss<false>(d, q, k, idesc(kM, kSub));
 #pragma unroll
-            for (int i = 1; i < D / 16; ++i)
-                mma_ss<true>(d, q + (i >> 2) * (kM * 8) + 2 * (i & 3), k + (i >> 2) * (kKeys * 8) + 2 * (i & 3), idesc(kM, kKeys));
-            commit(done);
+            for (int c = 1; c < D / 16; ++c)
+                mma_ss<true>(d, q + (c >> 2) * (kM * 8) + 2 * (c & 3), k + (c >> 2) * (kKeys * 8) + 2 * (c & 3), idesc(kM, kSub));
+            commit(&s.s_full[t]);
         };
-        auto tile = [&](auto which, int n, int mine) {      // false: a wait gave up
-            constexpr int t = decltype(which)::value;
-            const int st = n & 1;
-            if (!bar_wait(&s.p_full[t], n & 1, &s.dead)) return false;
+        if (mine > 0) {
+            if (!bar_wait(&s.kv_full[0], 0, &s.dead)) return;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            const uint32_t v = v0 + st * kStage, p = s_col(t), o = o_col(t);
+            scores(0);
+        }
+        for (int i = 0; i < mine; ++i) {
+            if (i + 1 < mine) {
+                if (((i + 1) & 1) == 0 && !bar_wait(&s.kv_full[(i + 1) >> 1 & 1], (i + 1) >> 2 & 1, &s.dead)) return;
+                if (!bar_wait(&s.s_free[t], i & 1, &s.dead)) return;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                scores(i + 1);
+            }
+            if (!bar_wait(&s.p_full[t], i & 1, &s.dead)) return;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            const uint32_t v = v0 + (i >> 1 & 1) * kStage + (i & 1) * (D * 8);
 #pragma unroll
-            for (int i = 0; i < kKeys / 16; ++i)
-                mma_ts(o, p + 8 * i, v + (i >> 2) * (D * 8) + 2 * (i & 3), idesc(kM, D), i > 0 || n > 0);
-            // the last product of this step: the stage is free when it is done
-            if (t == 1 || n >= n1) commit(&s.kv_free[st]);
-            if (n + 1 == mine) { commit(&s.s_full[t]); return true; }       // O is complete
-            if (!bar_wait(&s.kv_full[st ^ 1], ((n + 1) >> 1) & 1, &s.dead)) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            scores(q0 + t * kTileQ, s_col(t), &s.s_full[t], st ^ 1);
-            return true;
-        };
-        if (!bar_wait(&s.kv_full[0], 0, &s.dead)) return;
-        asm volatile("tcgen05.fence::after_thread_sync;");
-        if (n0 > 0) scores(q0, s_col(0), &s.s_full[0], 0);
-        if (n1 > 0) scores(q0 + kTileQ, s_col(1), &s.s_full[1], 0);
-        for (int n = 0; n < steps; ++n) {
-            if (n < n0 && !tile(std::integral_constant<int, 0>{}, n, n0)) return;
-            if (n < n1 && !tile(std::integral_constant<int, 1>{}, n, n1)) return;
+            for (int c = 0; c < kSub / 16; ++c) mma_ts(o, p + 8 * c, v + 2 * c, idesc(kM, D), c > 0 || i > 0);
+            commit(&s.p_free[t]);
+            if ((i & 1) || i + 1 == mine) commit(&s.kv_free[i >> 1 & 1]);
+        }
+        // the other tile's stages: this one is done with them as soon as they are filled
+        for (int n = (mine + 1) >> 1; n < stages; ++n) {
+            if (!bar_wait(&s.kv_full[n & 1], (n >> 1) & 1, &s.dead)) return;
+            bar_arrive(&s.kv_free[n & 1]);
         }
     }
 
@@ -440,130 +458,79 @@ struct Prompt {
                 *(uint4*)(s.q[t] + (i >> 6) * (kM * 128) + chunk_at(m, (i & 63) >> 3)) = o;
             }
         }
+        cf = fmaxf(cf, 0x1p-126f);      // not 0, which would undo a mask's -inf
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();       // Q is there: the products may begin
         float base = -INFINITY, l = 0.f;       // base: the running maximum - lift
         uint32_t poisoned = 0;                 // groups of 32 elements in which the row saw a NaN
         bool ok = true;
-        for (int j = w.j0; j < w.n[t] && ok; ++j) {
-            const int n = j - w.j0, st = n & 1, key0 = j * kKeys;
-            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], n & 1, &s.dead));
+        for (int i = 0; i < w.n[t]; ++i) {
+            const int j = w.j0 + (i >> 1), st = i >> 1 & 1, half = i & 1, key0 = j * kKeys + half * kSub;
+            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], i & 1, &s.dead));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
+            float x[kSub];
+#pragma unroll
+            for (int c = 0; c < kSub; c += 16) tmem_ld16(s_col(t) + lanes + c, reinterpret_cast<float(&)[16]>(x[c]));
+            tmem_wait(x);
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            bar_arrive(&s.s_free[t]);          // the next scores may come while these are worked on
             // keys [lo, hi) of the step are the row's; pages that are not there, a byte per 16 keys
-            const uint64_t there = *(const volatile uint64_t*)s.there[st];
-            const bool inside = there == 0x0101010101010101ull && key0 + kKeys <= all_to && key0 >= all_from;
+            const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
             const int hi = to - key0, lo = from - key0;
-            auto step = [&](auto masked) {
-                auto mask = [&](float (&y)[16], int chunk) {
-                    if constexpr (!decltype(masked)::value) return;
-                    const bool here = there >> (8 * chunk) & 1;
+            if (there != 0x01010101u || key0 + kSub > all_to || key0 < all_from) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = 16 * chunk + i;
-                        if (key < lo || key >= hi || !here) y[i] = -INFINITY;
-                    }
-                };
-                // The running maximum is that of the keys before, so P follows from S in one pass, 64 keys at a time (the
-                // next 16 columns on their way while the current ones are worked on).  A row whose P passes a half's range first
-                // sends its warp through the maximum of these keys, whose S is there until P is stored; the maximum
-                // moves by whole powers of two, so what is held under the old one is rescaled exactly.
-                float x[2][16];
-                auto raise = [&](int half) {
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");    // O and P as last stored
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 4 * half; c < 4 * half + 4; ++c) {
-                        tmem_ld16(s_col(t) + lanes + 16 * c, x[0]);
-                        tmem_wait(x[0]);
-                        mask(x[0], c);
+                for (int k = 0; k < kSub; ++k)
+                    if (k < lo || k >= hi || !(there >> (k / 16 * 8) & 1)) x[k] = -INFINITY;
+            }
+            float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(x[0][i], x[0][i + 1]));
-                    }
-                    if (top != -INFINITY) top = top * cf - kLift;
-                    float f = 1.f;
-                    if (base == -INFINITY) {
-                        base = top;
-                    } else if (top > base) {
-                        const float up = ceilf(top - base);       // inf where a logit is: NaN from there on
-                        base += up;
-                        f = up < 127.f ? __int_as_float((127 - (int)up) << 23) : 0.f;
-                    }
-                    l *= f;
-                    if (n > 0) rescale(t, lanes, f);
-                    if (half) {       // the first 64 keys' P
-                        const uint32_t f2 = pack2(f, f);
-#pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            tmem_ld16(s_col(t) + lanes + 16 * c, x[0]);
-                            tmem_wait(x[0]);
-                            uint32_t q[16];
+            for (int k = 4; k < kSub; k += 4) {
+                top = fmaxf(top, fmaxf(x[k], x[k + 1]));
+                top1 = fmaxf(top1, fmaxf(x[k + 2], x[k + 3]));
+            }
+            top = fmaxf(top, top1);
+            if (top != -INFINITY) top = top * cf - kLift;
+            // O and P as the last product left them
+            if (i > 0) {
+                ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+            }
+            if (__any_sync(0xffffffffu, top > base + kSlack)) {       // (NaN compares false)
+                const float fresh = fmaxf(base, top);
+                const float f = fresh == base ? 1.f : ex2(base - fresh);
+                base = fresh;
+                l *= f;
+                if (i > 0) rescale(t, lanes, f);
+            }
+            const float shift = base == -INFINITY ? 0.f : base;
+            float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) q[i] = mul2(__float_as_uint(x[0][i]), f2);
-                            tmem_st16(s_col(t) + lanes + 16 * c, q);
-                        }
-                    }
-                };
-                // (loops kept rolled: the roles share the instruction cache)
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    bool high = __any_sync(0xffffffffu, base == -INFINITY);
-                    uint32_t p[2][16];
-                    float sum;
-#pragma unroll 1
-                    for (;;) {
-                        if (high) {
-                            const float before = base;
-                            raise(half);
-                            high = __any_sync(0xffffffffu, base > before);
-                        }
-                        const float shift = base == -INFINITY ? 0.f : base;
-                        float sum0 = 0.f, sum1 = 0.f;
-                        tmem_ld16(s_col(t) + lanes + 64 * half, x[0]);
-                        tmem_wait(x[0]);
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float(&y)[16] = x[c & 1];
-                            if (c < 3) tmem_ld16(s_col(t) + lanes + 64 * half + 16 * (c + 1), x[~c & 1]);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = fmaf(y[i], cf, -shift);
-                            mask(y, 4 * half + c);
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float u = ex2(y[i]), v = ex2(y[i + 1]);
-                                sum0 += u; sum1 += v;
-                                p[c / 2][8 * (c & 1) + i / 2] = pack2(u, v);
-                            }
-                            if (c < 3) tmem_wait(x[~c & 1]);
-                        }
-                        sum = sum0 + sum1;
-                        // a sum that a half holds has no summand that it does not
-                        const bool over = __any_sync(0xffffffffu, sum > 65504.f);
-                        // once raised, only a row without a finite maximum is still over
-                        if (!over || high) break;
-                        high = true;
-                    }
-                    l += sum;
-                    tmem_st16(s_col(t) + lanes + 32 * half, p[0]);
-                    tmem_st16(s_col(t) + lanes + 32 * half + 16, p[1]);
+                for (int k = 0; k < 32; k += 2) {
+                    const float u = ex2(fmaf(x[32 * c + k], cf, -shift)), v = ex2(fmaf(x[32 * c + k + 1], cf, -shift));
+                    sum0 += u; sum1 += v;
+                    p[k / 2] = pack2(u, v);
                 }
-            };
-            // two copies: the masks' arithmetic must not run in the steps without any
-            if (inside) step(std::false_type{});
-            else step(std::true_type{});
+                tmem_st16(p_col(t) + lanes + 16 * c, p);
+            }
+            l += sum0 + sum1;
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (*(volatile int*)&s.odd[st] == j + 1) {
-                for (int key = max(lo, 0); key < min(hi, kKeys); ++key) {
-                    if (!(there >> (8 * (key / 16)) & 1)) continue;
+                for (int k = max(lo, 0); k < min(hi, kSub); ++k) {
+                    if (!(there >> (k / 16 * 8) & 1)) continue;
                     for (int g = 0; g < E; ++g)
-                        if (s.odd_keys[st][key >> 3][g] >> (key & 7) & 1) poisoned |= 1u << g;
+                        if (s.odd_keys[st][(half * kSub + k) >> 3][g] >> (k & 7) & 1) poisoned |= 1u << g;
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
             bar_arrive(&s.p_full[t]);
         }
-        const int steps = w.n[t] - w.j0;
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], steps & 1, &s.dead));
+        const int steps = w.n[t];
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (steps - 1) & 1, &s.dead));
         asm volatile("tcgen05.fence::after_thread_sync;");
         // l 0: the row saw nothing
         float inv = l == 0.f ? 0.f : 1.f / l;
@@ -620,12 +587,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(&s.kv_full[i], kDequant);
-            bar_init(&s.kv_free[i], 1);
+            bar_init(&s.kv_free[i], kTiles);
             bar_init(&s.s_full[i], 1);
+            bar_init(&s.drained[i], 1);
+            bar_init(&s.s_free[i], 128);
             bar_init(&s.p_full[i], 128);
+            bar_init(&s.p_free[i], 1);
             s.odd[i] = 0;
         }
-        bar_init(&s.drained, 1);
         s.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -654,12 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     w.last = w.j0;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-        w.n[t] = w.j0;
+        w.n[t] = 0;
         if (w.row0 + t * kM < w.rows) {
-            const int64_t hi = min((int64_t)w.len, w.pos_of(w.row0 + t * kM + kM - 1) + 1);
-            w.n[t] = max(w.j0, (int)((hi + kKeys - 1) / kKeys));
+            const int64_t hi = min((int64_t)w.len, w.pos_of(w.row0 + t * kM + kM - 1) + 1) - (int64_t)w.j0 * kKeys;
+            w.n[t] = max(0, (int)((hi + kSub - 1) / kSub));
         }
-        w.last = max(w.last, w.n[t]);
+        w.last = max(w.last, w.j0 + (w.n[t] + 1) / 2);
     }
     if (warp < kSoftmax / 32) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -671,14 +640,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
         __syncthreads();       // Q is there
-        if (w.last > w.j0 && threadIdx.x == kMmaWarp * 32) {
-            k.products();
+        const int t = warp - kMmaWarp;
+        if (w.last > w.j0 && t < kTiles && (threadIdx.x & 31) == 0) {
+            k.products(t);
             // what was begun is waited for (bounded): the tensor memory is freed next
             if (*(volatile int*)&s.dead) {
                 atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
                 int quiet = 0;
-                commit(&s.drained);
-                bar_wait(&s.drained, 0, &quiet);
+                commit(&s.drained[t]);
+                bar_wait(&s.drained[t], 0, &quiet);
             }
         }
         __syncwarp();
