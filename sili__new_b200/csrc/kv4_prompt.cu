@@ -42,7 +42,6 @@ using sili::ex2;
 using sili::kLift;
 using sili::kLn2;
 using sili::kLog2e;
-using sili::kSlack;
 using sili::mul2;
 using sili::pack2;
 
@@ -59,7 +58,7 @@ constexpr int kSub = 64;              // keys a step of a tile (MMA N of S, K of
 constexpr int kSoftmax = kTiles * 128, kDequant = 256;
 constexpr int kThreads = kSoftmax + kDequant + 128;     // whole warpgroups: each sets its share of the registers
 // registers a thread after the split; together what the launch holds: 96 * 640
-constexpr int kRegsSoftmax = 136, kRegsDequant = 80, kRegsRest = 48;
+constexpr int kRegsSoftmax = 144, kRegsDequant = 72, kRegsRest = 48;
 static_assert(kSoftmax * kRegsSoftmax + kDequant * kRegsDequant + 128 * kRegsRest <= 96 * kThreads, "register split");
 constexpr int kMmaWarp = (kSoftmax + kDequant) / 32;
 constexpr int kPolls = 4096;          // polls of a wait, each asleep for up to kNap ns, before it gives up
@@ -71,7 +70,9 @@ struct Smem {
     alignas(1024) uint8_t k[2][kKeys * D * 2];
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     alignas(8) unsigned long long kv_full[2], kv_free[2];                                  // by stage
-    unsigned long long s_full[2], s_free[2], p_full[2], p_free[2], drained[2];  // by tile
+    unsigned long long s_full[2], s_free[2], p_free[2], o_full[2], drained[2];   // by tile
+    // by tile and the step's parity: a warp may be a step ahead of its tile's others, and must not count for their step
+    unsigned long long p_full[2][2];
     uint8_t odd_keys[2][16][4];       // [stage][8 keys][group]: bits of keys whose V scale is not a number
     int odd[2];                       // the last step whose stage had any, plus one
     alignas(8) uint8_t there[2][8];   // [stage][16 keys]: their page exists
@@ -229,10 +230,10 @@ struct Prompt {
     Smem<D>& s;
     Work w;
 
-    // tensor memory: S (64 columns a tile), P (32), O (dim)
+    // tensor memory: S (64 columns a tile), P (two of 32), O (dim)
     __device__ __forceinline__ uint32_t s_col(int t) const { return s.tmem + t * kSub; }
-    __device__ __forceinline__ uint32_t p_col(int t) const { return s.tmem + kTiles * kSub + t * (kSub / 2); }
-    __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + kTiles * kSub * 3 / 2 + t * D; }
+    __device__ __forceinline__ uint32_t p_col(int t) const { return s.tmem + kTiles * kSub + t * kSub; }
+    __device__ __forceinline__ uint32_t o_col(int t) const { return s.tmem + 2 * kTiles * kSub + t * D; }
 
     // ── warps 8-15: 4-bit keys and values of step j into stage j & 1 ──
     __device__ __forceinline__ void dequantise() {
@@ -383,12 +384,13 @@ struct Prompt {
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 scores(i + 1);
             }
-            if (!bar_wait(&s.p_full[t], i & 1, &s.dead)) return;
+            if (!bar_wait(&s.p_full[t][i & 1], (i >> 1) & 1, &s.dead)) return;
             asm volatile("tcgen05.fence::after_thread_sync;");
             const uint32_t v = v0 + (i >> 1 & 1) * kStage + (i & 1) * (D * 8);
 #pragma unroll
-            for (int c = 0; c < kSub / 16; ++c) mma_ts(o, p + 8 * c, v + 2 * c, idesc(kM, D), c > 0 || i > 0);
+            for (int c = 0; c < kSub / 16; ++c) mma_ts(o, p + (i & 1) * (kSub / 2) + 8 * c, v + 2 * c, idesc(kM, D), c > 0 || i > 0);
             commit(&s.p_free[t]);
+            if (i + 1 == mine) commit(&s.o_full[t]);
             if ((i & 1) || i + 1 == mine) commit(&s.kv_free[i >> 1 & 1]);
         }
         // the other tile's stages: this one is done with them as soon as they are filled
@@ -483,41 +485,46 @@ struct Prompt {
                 for (int k = 0; k < kSub; ++k)
                     if (k < lo || k >= hi || !(there >> (k / 16 * 8) & 1)) x[k] = -INFINITY;
             }
-            float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
+            // The running maximum is that of the keys before, so P follows at once; a row whose P passes a half's range
+            // (a sum that a half holds has no summand that it does not) sends its warp through these keys' maximum
+            // and once more through P.  P's buffer was last read by the product two steps ago, which was queued before
+            // these scores; O waits for the last product.
+            bool high = __any_sync(0xffffffffu, base == -INFINITY);
+            uint32_t p[2][16];
+            float sum;
+            for (bool again = true; again;) {
+                if (high) {
+                    float top = -INFINITY;
 #pragma unroll
-            for (int k = 4; k < kSub; k += 4) {
-                top = fmaxf(top, fmaxf(x[k], x[k + 1]));
-                top1 = fmaxf(top1, fmaxf(x[k + 2], x[k + 3]));
-            }
-            top = fmaxf(top, top1);
-            if (top != -INFINITY) top = top * cf - kLift;
-            // O and P as the last product left them
-            if (i > 0) {
-                ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead));
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;");
-            }
-            if (__any_sync(0xffffffffu, top > base + kSlack)) {       // (NaN compares false)
-                const float fresh = fmaxf(base, top);
-                const float f = fresh == base ? 1.f : ex2(base - fresh);
-                base = fresh;
-                l *= f;
-                if (i > 0) rescale(t, lanes, f);
-            }
-            const float shift = base == -INFINITY ? 0.f : base;
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t p[16];
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    const float u = ex2(fmaf(x[32 * c + k], cf, -shift)), v = ex2(fmaf(x[32 * c + k + 1], cf, -shift));
-                    sum0 += u; sum1 += v;
-                    p[k / 2] = pack2(u, v);
+                    for (int k = 0; k < kSub; k += 2) top = fmaxf(top, fmaxf(x[k], x[k + 1]));
+                    if (top != -INFINITY) top = top * cf - kLift;
+                    const float fresh = fmaxf(base, top);
+                    const float f = fresh == base ? 1.f : ex2(base - fresh);
+                    base = fresh;
+                    l *= f;
+                    if (i > 0) {
+                        ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;");
+                        rescale(t, lanes, f);
+                    }
                 }
-                tmem_st16(p_col(t) + lanes + 16 * c, p);
+                const float shift = base == -INFINITY ? 0.f : base;
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int k = 0; k < kSub; k += 2) {
+                    const float u = ex2(fmaf(x[k], cf, -shift)), v = ex2(fmaf(x[k + 1], cf, -shift));
+                    sum0 += u; sum1 += v;
+                    p[k / 32][k / 2 % 16] = pack2(u, v);
+                }
+                sum = sum0 + sum1;
+                again = !high && __any_sync(0xffffffffu, sum > 65504.f);
+                high = true;
             }
-            l += sum0 + sum1;
+            if (!ok) break;
+            tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2), p[0]);
+            tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2) + 16, p[1]);
+            l += sum;
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (*(volatile int*)&s.odd[st] == j + 1) {
                 for (int k = max(lo, 0); k < min(hi, kSub); ++k) {
@@ -527,10 +534,11 @@ struct Prompt {
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
-            bar_arrive(&s.p_full[t]);
+            bar_arrive(&s.p_full[t][i & 1]);
         }
         const int steps = w.n[t];
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (steps - 1) & 1, &s.dead));
+        // (a barrier of its own: p_free may be one or two phases behind here, which a parity does not tell apart)
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], 0, &s.dead));
         asm volatile("tcgen05.fence::after_thread_sync;");
         // l 0: the row saw nothing
         float inv = l == 0.f ? 0.f : 1.f / l;
@@ -589,9 +597,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             bar_init(&s.kv_full[i], kDequant);
             bar_init(&s.kv_free[i], kTiles);
             bar_init(&s.s_full[i], 1);
+            bar_init(&s.o_full[i], 1);
             bar_init(&s.drained[i], 1);
             bar_init(&s.s_free[i], 128);
-            bar_init(&s.p_full[i], 128);
+            bar_init(&s.p_full[i][0], 128);
+            bar_init(&s.p_full[i][1], 128);
             bar_init(&s.p_free[i], 1);
             s.odd[i] = 0;
         }
