@@ -254,12 +254,10 @@ struct Attend {
         return E == 8 ? c ^ (2 * (key & 3)) : E == 4 ? c ^ (2 * ((key >> 1) & 1)) : c;
     }
 
-    __device__ __forceinline__ int page_col(int key0) const {
-        return a.page_shift >= 0 ? key0 >> a.page_shift : key0 / a.page;
-    }
     __device__ __forceinline__ int fetch_page(const Cur& c) const {
         const int key0 = c.u * kUnit + warp * 16;
-        return key0 < c.q.len ? __ldg(a.table + c.r * a.stride + page_col(key0)) : -1;
+        int off;
+        return key0 < c.q.len ? __ldg(a.table + c.r * a.stride + a.column(key0, off)) : -1;
     }
 
     // starts the copy of cursor c's tile of page pg into stage s
@@ -267,7 +265,9 @@ struct Attend {
         const bool there = pg >= 0 && pg < a.n_pages;
         if (there) {
             const int key0 = c.u * kUnit + warp * 16;
-            const int h = c.seg / c.q.tiles, off = key0 - page_col(key0) * a.page;
+            const int h = c.seg / c.q.tiles;
+            int off;
+            a.column(key0, off);
             const int64_t kr = sili::kv4_row(pg, 0, h, a.kv_heads, a.page) + off;
             const int64_t vr = kr + (int64_t)a.kv_heads * a.page;
             const uint32_t at = ring_at + s * L::kStage;
@@ -772,13 +772,13 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
     if (!q || !out || !workspace || (requests && !lens) || (requests && width && !table) || (n_pages && (!codes || !scales)))
         return bad(who, "null array");
     if (requests && table_stride < width) return bad(who, "table rows overlap");
-    if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4) return bad(who, "codes must be 16-byte, scales 4-byte aligned");
+    if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return bad(who, "codes and scales must be 16-byte aligned");
     const int64_t item = dtype == SILI_F32 ? 4 : 2;
     if ((uintptr_t)q % 8 || (uintptr_t)out % 16 || q_token_stride * item % 8 || q_head_stride * item % 8)
         return bad(who, "q rows must be 8-byte aligned");
     AttendArgs a{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
                  table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
-                 page & (page - 1) ? -1 : __builtin_ctz((unsigned)page)};
+                 (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16))};
     cudaStream_t s = (cudaStream_t)stream;
     if (starts && sili::kv4_prompt_takes(dtype, dim, tokens, heads, kv_heads, most_new))
         return sili::kv4_prompt_launch(dtype, dim, a, s);

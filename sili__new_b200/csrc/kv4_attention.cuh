@@ -27,7 +27,19 @@ struct AttendArgs {
     void* out;             // [tokens, heads, dim]
     float* lse;            // [tokens, heads] or null
     void* workspace;
-    int page_shift;        // log2(page), or -1
+    uint32_t page16;       // page / 16
+    uint32_t page_magic;   // ceil(2^32 / page16); 0 where page16 is 1
+
+    // the table column of a key and the key's place in its page: one high product in place of a division, corrected by
+    // one where the product is one too large (magic exceeds 2^32 / page16 by less than one)
+    __device__ __forceinline__ int column(int key, int& off) const {
+        const uint32_t run = (uint32_t)key >> 4;
+        uint32_t col = page_magic ? __umulhi(run, page_magic) : run;
+        int left = (int)(run - col * page16);
+        if (left < 0) { --col; left += (int)page16; }
+        off = left * 16 + (key & 15);
+        return (int)col;
+    }
 };
 
 // The workspace: a counter a CTA, an error word, then the partial results.

@@ -245,45 +245,62 @@ struct Prompt {
         const int half = dw & 1, c = lane & 7, db = (dw >> 1) * 4 + (lane >> 3), vkey = half * 64 + c * 8;
         const bool has_v = db < D / 8;
         const int vg = db >> 2;
-        uint4 rk[kLoads];
-        uint32_t sk[kLoads], rv[8], sv[8];
+        uint4 rk[kLoads], sv[E / 2];
+        uint32_t sk[kLoads], rv[8];
         int pk, pv, next_pk, next_pv;
-        auto col_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page; };
         auto page_of = [&](int key) {
             // whole runs of 16 keys (they share a page and a bit of `there`), of which the last may reach past the end
-            return (key & ~15) < w.len ? __ldg(a.table + w.r * a.stride + col_of(key)) : -1;
+            int off;
+            return (key & ~15) < w.len ? __ldg(a.table + w.r * a.stride + a.column(key, off)) : -1;
         };
         auto pages = [&](int j) {
             next_pk = page_of(j * kKeys + kkey);
             next_pv = page_of(j * kKeys + vkey);
         };
-        auto row_of = [&](int pg, int key, int which) {
-            return sili::kv4_row(pg, which, w.h, a.kv_heads, a.page) + (key - col_of(key) * a.page);
+        const int64_t head_rows = (int64_t)w.h * a.page, v_rows = (int64_t)a.kv_heads * a.page;
+        auto row_of = [&](int pg, int key) {
+            int off;
+            a.column(key, off);
+            return (int64_t)pg * (2 * v_rows) + head_rows + off;
         };
+        // (what a missing page leaves in K is masked in S; its V scales are zeroed, for 0 * NaN is none)
         auto load_k = [&](int j) {
             const bool there = pk >= 0 && pk < a.n_pages;
-            const int64_t row = there ? row_of(pk, j * kKeys + kkey, 0) + lane / E : 0;
+            if (there) {
+                const int64_t row = row_of(pk, j * kKeys + kkey) + lane / E;
+                const uint8_t* codes = a.codes + row * (D / 2) + kq * 16;
+                const uint8_t* scales = a.scales + row * E + kq;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                rk[i] = make_uint4(0, 0, 0, 0);
-                sk[i] = 0;
-                if (there) {
-                    rk[i] = __ldg((const uint4*)(a.codes + (row + i * kPer) * (D / 2) + kq * 16));
-                    sk[i] = __ldg(a.scales + (row + i * kPer) * E + kq);
+                for (int i = 0; i < kLoads; ++i) {
+                    rk[i] = __ldg((const uint4*)(codes + i * kPer * (D / 2)));
+                    sk[i] = __ldg(scales + i * kPer * E);
                 }
             }
             return there;
         };
         auto load_v = [&](int j) {
-            const bool there = has_v && pv >= 0 && pv < a.n_pages;
-            const int64_t row = there ? row_of(pv, j * kKeys + vkey, 1) : 0;
+            if (has_v && pv >= 0 && pv < a.n_pages) {
+                const int64_t row = row_of(pv, j * kKeys + vkey) + v_rows;
+                const uint8_t* codes = a.codes + row * (D / 2) + db * 4;
+                const uint8_t* scales = a.scales + row * E;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                rv[i] = sv[i] = 0;
-                if (there) {
-                    rv[i] = __ldg((const uint32_t*)(a.codes + (row + i) * (D / 2) + db * 4));
-                    sv[i] = __ldg(a.scales + (row + i) * E + vg);
-                }
+                for (int i = 0; i < 8; ++i) rv[i] = __ldg((const uint32_t*)(codes + i * (D / 2)));
+#pragma unroll
+                for (int i = 0; i < E / 2; ++i) sv[i] = __ldg((const uint4*)(scales + 16 * i));
+            } else {
+#pragma unroll
+                for (int i = 0; i < E / 2; ++i) sv[i] = make_uint4(0, 0, 0, 0);
+            }
+        };
+        // the scales of keys 2p and 2p + 1 as bytes 0 and 2
+        const uint32_t pick = E == 4 ? (uint32_t)(vg | (4 + vg) << 8) : (uint32_t)(vg | (2 + vg) << 8);      // selector nibbles 0 and 2
+        auto pair_of = [&](int p) {
+            if constexpr (E == 4) {
+                const uint4 v = sv[p >> 1 & (E / 2 - 1)];
+                return __byte_perm(p & 1 ? v.z : v.x, p & 1 ? v.w : v.y, pick) & 0x00FF00FFu;
+            } else {
+                const uint32_t v = p == 0 ? sv[0].x : p == 1 ? sv[0].y : p == 2 ? sv[0].z : sv[0].w;
+                return __byte_perm(v, 0, pick) & 0x00FF00FFu;
             }
         };
         pages(w.j0);
@@ -323,17 +340,26 @@ struct Prompt {
             }
             // V: rows are elements; scales that are no numbers are left out and noted
             if (has_v) {
-                uint32_t bits = 0;
+                uint32_t pairs[4], odd_any = 0, bits = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (sv[i] >= 0xF8u) { bits |= 1u << i; sv[i] = 0; }
+                for (int p = 0; p < 4; ++p) {
+                    pairs[p] = pair_of(p);
+                    odd_any |= pairs[p] + 0x00080008u;      // carries into bit 8 of a byte of at least 0xF8
+                }
+                if (odd_any & 0x01000100u) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        if ((pairs[p] & 0xFFu) >= 0xF8u) { bits |= 1u << (2 * p); pairs[p] &= 0xFFFF0000u; }
+                        if ((pairs[p] >> 16) >= 0xF8u) { bits |= 2u << (2 * p); pairs[p] &= 0xFFFFu; }
+                    }
+                    *(volatile int*)&s.odd[st] = j + 1;
+                }
                 if ((db & 3) == 0) s.odd_keys[st][half * 8 + c][vg] = (uint8_t)bits;
-                if (bits) *(volatile int*)&s.odd[st] = j + 1;
                 constexpr uint32_t kLow = 0x0F0F0F0Fu;
                 uint32_t even[4][4], odd[4][4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const uint32_t x = rv[2 * p], y = rv[2 * p + 1], sc = sv[2 * p] << 7 | sv[2 * p + 1] << 23;
+                    const uint32_t x = rv[2 * p], y = rv[2 * p + 1], sc = pairs[p] << 7;
                     sili::kv4_decode4((x & kLow) | ((y << 4) & ~kLow), even[p]);
                     sili::kv4_decode4(((x >> 4) & kLow) | (y & ~kLow), odd[p]);
 #pragma unroll
