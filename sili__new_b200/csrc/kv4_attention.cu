@@ -70,6 +70,7 @@ int bad(const char* who, const char* what) {
 constexpr int kWarps = 8;
 constexpr int kUnit = 16 * kWarps;      // keys of a unit
 constexpr int kMaxStages = 4;
+constexpr float kNoMaximum = -3e38f;    // below every finite logit, and finite: a masked key's -inf over it is -inf
 constexpr int kMaxCtas = 2 * 148;       // two CTAs an SM; one for the wider row tiles
 
 constexpr int64_t workspace_bytes() {
@@ -144,26 +145,38 @@ __device__ __forceinline__ int64_t units_of(const AttendArgs& a, const Req& q) {
     return (int64_t)q.units * q.tiles * a.kv_heads;
 }
 
-// A position in the numbered units: request, segment (kv head, row tile) and unit of keys.
+// A position in the numbered units: request, kv head, row tile and unit of
+// keys, with what the copies need of them.
 template <int ROWS>
 struct Cursor {
     Req q;
-    int r, seg, u;
+    int r, h, tile, u;
+    const int* pages;      // the request's row of the table
+    int64_t head_rows;     // token rows of the kv head before this one, in a page
+
+    __device__ __forceinline__ void enter(const AttendArgs& a) {
+        pages = a.table + r * a.stride;
+        head_rows = (int64_t)h * a.page;
+    }
     __device__ __forceinline__ void next(const AttendArgs& a) {
         if (++u < q.k0 + q.units) return;
-        if (++seg == q.tiles * a.kv_heads) {
+        u = q.k0;
+        if (++tile < q.tiles) return;
+        tile = 0;
+        if (++h == a.kv_heads) {
+            h = 0;
             do {
                 if (++r >= a.requests) return;      // past the last unit; never read there
                 q = request<ROWS>(a, r);
             } while (q.tiles == 0);
-            seg = 0;
+            u = q.k0;
         }
-        u = q.k0;
+        enter(a);
     }
 };
 
-// Sets `c` to unit `first` of the request that holds unit c.x of all;
-// returns the number of all units.  One scan of the lengths by the CTA.
+// The CTA's run [begin, end) of the units, `c` set to its first; returns the
+// number of all units.  One scan of the lengths by the CTA.
 template <int ROWS>
 __device__ int64_t locate(const AttendArgs& a, Cursor<ROWS>& c, int cta, int ctas, int64_t& begin, int64_t& end) {
     __shared__ int64_t s_part[kWarps], s_hit[2];
@@ -208,8 +221,11 @@ __device__ int64_t locate(const AttendArgs& a, Cursor<ROWS>& c, int cta, int cta
     __syncthreads();
     c.r = (int)s_hit[0];
     c.q = request<ROWS>(a, c.r);
-    c.seg = (int)(s_hit[1] / c.q.units);
-    c.u = c.q.k0 + (int)(s_hit[1] % c.q.units);
+    const int64_t seg = s_hit[1] / c.q.units;
+    c.u = c.q.k0 + (int)(s_hit[1] - seg * c.q.units);
+    c.h = (int)(seg / c.q.tiles);
+    c.tile = (int)(seg - (int64_t)c.h * c.q.tiles);
+    c.enter(a);
     return all;
 }
 
@@ -232,8 +248,10 @@ struct Attend {
     // the current segment
     uint32_t qf[NT > 1 ? 1 : kSteps][kTerms][2];
     float cf[NT][2];       // logit = S * cf, in powers of two
-    float m[NT][2], l[NT][2], o[kSteps][NT][4];
-    int64_t pos[NT][2], first_pos, last_pos;
+    float base[NT][2];     // the running maximum - lift
+    float l[NT][2], o[kSteps][NT][4];
+    int to[NT][2], from[NT][2];        // the columns' keys [from, to)
+    int any_from, any_to, all_from, all_to;   // keys that any of the rows sees, that every row sees
 
     __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, int* all_flags)
         : a(args), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
@@ -257,19 +275,17 @@ struct Attend {
     __device__ __forceinline__ int fetch_page(const Cur& c) const {
         const int key0 = c.u * kUnit + warp * 16;
         int off;
-        return key0 < c.q.len ? __ldg(a.table + c.r * a.stride + a.column(key0, off)) : -1;
+        return key0 < c.q.len ? __ldg(c.pages + a.column(key0, off)) : -1;
     }
 
     // starts the copy of cursor c's tile of page pg into stage s
     __device__ __forceinline__ void issue(const Cur& c, int pg, int s) {
         const bool there = pg >= 0 && pg < a.n_pages;
         if (there) {
-            const int key0 = c.u * kUnit + warp * 16;
-            const int h = c.seg / c.q.tiles;
             int off;
-            a.column(key0, off);
-            const int64_t kr = sili::kv4_row(pg, 0, h, a.kv_heads, a.page) + off;
-            const int64_t vr = kr + (int64_t)a.kv_heads * a.page;
+            a.column(c.u * kUnit + warp * 16, off);
+            const int64_t half = (int64_t)a.kv_heads * a.page;      // token rows of K, and of V, in a page
+            const int64_t kr = pg * (2 * half) + c.head_rows + off, vr = kr + half;
             const uint32_t at = ring_at + s * L::kStage;
             constexpr int kPer = L::kRowBytes / 16;
 #pragma unroll
@@ -288,10 +304,15 @@ struct Attend {
     }
 
     __device__ __forceinline__ void begin_segment(const Cur& c) {
-        const int h = c.seg / c.q.tiles, tile = c.seg - h * c.q.tiles, group = a.heads / a.kv_heads;
-        const int rows = c.q.nq * group, row0 = tile * kRows;     // below 2^31: the host has checked tokens * heads
-        first_pos = c.q.pos0 + row0 / group;
-        last_pos = c.q.pos0 + (min(row0 + kRows, rows) - 1) / group;
+        const int h = c.h, group = a.heads / a.kv_heads;
+        const int rows = c.q.nq * group, row0 = c.tile * kRows;     // below 2^31: the host has checked tokens * heads
+        auto span = [&](int row, int& from_, int& to_) {
+            const int64_t pos = c.q.pos0 + row / group;
+            to_ = (int)min(pos + 1, (int64_t)c.q.len);
+            from_ = a.window ? (int)max(pos - a.window + 1, (int64_t)0) : 0;
+        };
+        span(row0, any_from, all_to);
+        span(min(row0 + kRows, rows) - 1, all_from, any_to);
         if (NT > 1) __syncthreads();    // the last segment's fragments have been read
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -319,10 +340,12 @@ struct Attend {
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // the row's largest into [2^14, 2^15): a half holds it, and 38 binary digits below it
                 int e = 0;
+                const float sign = a.scale < 0.f ? -1.f : 1.f;
                 if (!std::is_same<T, __half>::value && top && top < 0x7F800000u) {
                     e = 14 - max((int)(top >> 23) - 127, -100);
                     f = __int_as_float((127 + e) << 23);
                 }
+                f *= sign;
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
@@ -338,8 +361,8 @@ struct Attend {
                         }
                     }
                 }
-                // undo the scaling; the thread's columns are rows 2t and 2t + 1, held by lanes of g = 2t, 2t + 1
-                const float back = a.scale * kLog2e * __int_as_float((127 - e) << 23);
+                // undo the scaling (the scale's sign is in q; not 0, which would undo a mask's -inf); the thread's columns are rows 2t and 2t + 1, held by lanes of g = 2t, 2t + 1
+                const float back = fmaxf(fabsf(a.scale) * kLog2e * __int_as_float((127 - e) << 23), 0x1p-126f);
                 cf[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
                 cf[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
                 if (NT > 1) {
@@ -349,9 +372,8 @@ struct Attend {
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int col = min(row0 + n * 8 + 2 * t + j, rows - 1);
-                pos[n][j] = c.q.pos0 + col / group;
-                m[n][j] = -INFINITY;
+                span(min(row0 + n * 8 + 2 * t + j, rows - 1), from[n][j], to[n][j]);
+                base[n][j] = kNoMaximum;
                 l[n][j] = 0.f;
             }
         }
@@ -371,13 +393,32 @@ struct Attend {
                 for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
     }
 
-    __device__ __forceinline__ bool sees(int64_t key, int n, int j, int len) const {
-        return key <= pos[n][j] && key < len && (!a.window || key > pos[n][j] - a.window);
+    __device__ __forceinline__ bool sees(int key, int n, int j) const { return key < to[n][j] && key >= from[n][j]; }
+
+    // Moves the columns' maxima to those of these keys' products x where they are larger; e: the exponents over them.
+    __device__ __forceinline__ void raise(const float (&x)[NT][4], float (&e)[NT][4]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float top = fmaxf(x[n][j], x[n][j + 2]) * cf[n][j];
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float fresh = fmaxf(base[n][j], top - kLift);
+                const float f = fresh == base[n][j] ? 1.f : ex2(base[n][j] - fresh);
+                base[n][j] = fresh;
+                l[n][j] *= f;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) { o[i][n][j] *= f; o[i][n][j + 2] *= f; }
+                e[n][j] = fmaf(x[n][j], cf[n][j], -fresh);
+                e[n][j + 2] = fmaf(x[n][j + 2], cf[n][j], -fresh);
+            }
     }
 
     __device__ __forceinline__ void tile(const Cur& c, int s) {
-        const int key0 = c.u * kUnit + warp * 16, len = c.q.len;
-        if (!flags[s] || key0 > last_pos || (a.window && key0 + 15 <= first_pos - a.window)) return;
+        const int key0 = c.u * kUnit + warp * 16;
+        if (!flags[s] || key0 >= any_to || key0 + 16 <= any_from) return;
         const uint8_t* st = ring + s * L::kStage;
         const int ka = key_of(g);
         float x[NT][4];
@@ -431,42 +472,31 @@ struct Attend {
                         }
             }
         }
-        // logits in powers of two, masked
-        const bool inside = key0 + 15 < len && key0 + 15 <= first_pos && (!a.window || key0 > last_pos - a.window);
+        // exponents over the running maximum
+        float e[NT][4];
+        if (!(key0 + 16 <= all_to && key0 >= all_from)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!sees(key0 + ka + 8 * (j >> 1), n, j & 1)) x[n][j] = -INFINITY;
+        }
         bool above = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[n][j] *= cf[n][j & 1];
-                if (!inside && !sees(key0 + ka + 8 * (j >> 1), n, j & 1, len)) x[n][j] = -INFINITY;
-                above = above || x[n][j] > m[n][j & 1] + kSlack;
+                e[n][j] = fmaf(x[n][j], cf[n][j & 1], -base[n][j & 1]);
+                above = above || e[n][j] > kLift + kSlack;
             }
-        if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float top = fmaxf(x[n][j], x[n][j + 2]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float mn = fmaxf(m[n][j], top);
-                    const float f = mn == m[n][j] ? 1.f : ex2(m[n][j] - mn);
-                    m[n][j] = mn;
-                    l[n][j] *= f;
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) { o[i][n][j] *= f; o[i][n][j + 2] *= f; }
-                }
-        }
+        if (__any_sync(0xffffffffu, above)) raise(x, e);
         // P^T fragments
         uint32_t p[NT][kTerms][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float base = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1] - kLift;
-                x[n][j] = ex2(x[n][j] - base);
+                x[n][j] = ex2(e[n][j]);
                 l[n][j & 1] += x[n][j];
             }
 #pragma unroll
@@ -508,7 +538,7 @@ struct Attend {
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
-                            if (sees(key0 + key, n, j, len))
+                            if (sees(key0 + key, n, j))
 #pragma unroll
                                 for (int i = 0; i < kSteps; ++i)
                                     o[i][n][j] = o[i][n][j + 2] = __int_as_float(0x7FC00000);
@@ -542,8 +572,8 @@ struct Attend {
 
     // out and lse of one row and four of its values
     __device__ __forceinline__ void store(const Cur& c, int row, int d, const float (&v)[4], float top, float sum) const {
-        const int h = c.seg / c.q.tiles, group = a.heads / a.kv_heads;
-        const int at = (c.seg - h * c.q.tiles) * kRows + row;
+        const int h = c.h, group = a.heads / a.kv_heads;
+        const int at = c.tile * kRows + row;
         if (at >= c.q.nq * group) return;
         const int64_t id = (int64_t)(c.q.row0 + at / group) * a.heads + h * group + at % group;
         // sum 0: the row saw nothing; NaN goes through
@@ -552,7 +582,7 @@ struct Attend {
 #pragma unroll
         for (int i = 0; i < 4; ++i) out.v[i] = sili::from_f32<T>(v[i] * inv);
         *(sili::Pack<T, 4>*)((T*)a.out + id * kDim + d) = out;
-        if (d == 0 && a.lse) a.lse[id] = sum == 0.f ? -INFINITY : kLn2 * (top - kLift + log2f(sum));
+        if (d == 0 && a.lse) a.lse[id] = sum == 0.f ? -INFINITY : kLn2 * (top + log2f(sum));
     }
 
     // The segment's end in this CTA: joins the warps, then writes the rows, or leaves them to the CTA that comes last.
@@ -572,7 +602,7 @@ struct Attend {
                 s += __shfl_xor_sync(0xffffffffu, s, 8);
                 s += __shfl_xor_sync(0xffffffffu, s, 16);
                 const int row = warp * kRows + n * 8 + 2 * t + j;
-                if (g == 0) { jm[row] = m[n][j]; jl[row] = s; }
+                if (g == 0) { jm[row] = base[n][j]; jl[row] = s; }
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i)
                     *(float2*)(join + row * L::kJoinRow + g * (kDim / 8) + 2 * i) = make_float2(o[i][n][j], o[i][n][j + 2]);
@@ -585,7 +615,7 @@ struct Attend {
         float* part = whole ? nullptr : partial(cta, cta == lead);
         for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
             const int row = i / kQuads, d = i % kQuads * 4;
-            float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            float top = kNoMaximum, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[w * kRows + row]);
 #pragma unroll
@@ -618,7 +648,7 @@ struct Attend {
         if (!*s_last) return;
         // the weights of the parts, [row][part], in the warps' join space
         for (int row = warp; row < kRows; row += kWarps) {
-            float top = -INFINITY, sum = 0.f;
+            float top = kNoMaximum, sum = 0.f;
             for (int i = lane; i < n; i += 32)
                 top = fmaxf(top, __ldcg(partial(lead + i, i == 0) + kRows * kDim + row));
 #pragma unroll
@@ -648,7 +678,7 @@ struct Attend {
     }
 
     __device__ __forceinline__ void run(Cur c, int64_t begin, int64_t end, int64_t all, int* s_last) {
-        const int64_t n = end - begin;
+        const int n = (int)(end - begin);
         Cur ld = c;
         int pg = fetch_page(ld);
 #pragma unroll
@@ -664,11 +694,11 @@ struct Attend {
         }
         bool fresh = true;
         int stage = 0;
-        for (int64_t i = 0; i < n; ++i) {
+        for (int i = 0; i < n; ++i) {
             if (fresh) begin_segment(c);
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
             __syncwarp();
-            const int64_t ahead = i + kStages - 1;
+            const int ahead = i + kStages - 1;
             if (ahead < n) {
                 const int now = pg;
                 const Cur at = ld;
