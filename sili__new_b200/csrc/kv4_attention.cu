@@ -145,33 +145,27 @@ __device__ __forceinline__ int64_t units_of(const AttendArgs& a, const Req& q) {
     return (int64_t)q.units * q.tiles * a.kv_heads;
 }
 
-// A position in the numbered units: request, kv head, row tile and unit of
-// keys, with what the copies need of them.
+// A position in the numbered units: request, kv head, row tile (a segment)
+// and unit of keys.
 template <int ROWS>
 struct Cursor {
     Req q;
     int r, h, tile, u;
-    const int* pages;      // the request's row of the table
-    int64_t head_rows;     // token rows of the kv head before this one, in a page
 
-    __device__ __forceinline__ void enter(const AttendArgs& a) {
-        pages = a.table + r * a.stride;
-        head_rows = (int64_t)h * a.page;
-    }
-    __device__ __forceinline__ void next(const AttendArgs& a) {
-        if (++u < q.k0 + q.units) return;
-        u = q.k0;
-        if (++tile < q.tiles) return;
-        tile = 0;
-        if (++h == a.kv_heads) {
-            h = 0;
-            do {
-                if (++r >= a.requests) return;      // past the last unit; never read there
-                q = request<ROWS>(a, r);
-            } while (q.tiles == 0);
-            u = q.k0;
+    __device__ __forceinline__ int left() const { return q.k0 + q.units - u; }    // units of the segment from u on
+    // the first unit of the next segment (past the last one: never looked at)
+    __device__ __forceinline__ void next_segment(const AttendArgs& a) {
+        if (++tile == q.tiles) {
+            tile = 0;
+            if (++h == a.kv_heads) {
+                h = 0;
+                do {
+                    if (++r >= a.requests) return;
+                    q = request<ROWS>(a, r);
+                } while (q.tiles == 0);
+            }
         }
-        enter(a);
+        u = q.k0;
     }
 };
 
@@ -225,7 +219,6 @@ __device__ int64_t locate(const AttendArgs& a, Cursor<ROWS>& c, int cta, int cta
     c.u = c.q.k0 + (int)(s_hit[1] - seg * c.q.units);
     c.h = (int)(seg / c.q.tiles);
     c.tile = (int)(seg - (int64_t)c.h * c.q.tiles);
-    c.enter(a);
     return all;
 }
 
@@ -272,32 +265,59 @@ struct Attend {
         return E == 8 ? c ^ (2 * (key & 3)) : E == 4 ? c ^ (2 * ((key >> 1) & 1)) : c;
     }
 
-    __device__ __forceinline__ int fetch_page(const Cur& c) const {
-        const int key0 = c.u * kUnit + warp * 16;
-        int off;
-        return key0 < c.q.len ? __ldg(c.pages + a.column(key0, off)) : -1;
+    // What the copies of this warp's tiles need, a tile ahead of them: within a segment a step is an addition to `key0`.
+    struct Loader {
+        Cur c;
+        int key0, left, len;     // the next tile's first key, the segment's tiles from there on, the request's keys
+        int page, off;           // its page (-1: none) and place in it
+        const int* pages;        // the request's row of the table
+        const uint8_t *codes, *scales;   // the kv head's first K row of page 0, and this lane's 16 bytes
+    };
+    __device__ __forceinline__ void look(Loader& d) const {
+        d.page = -1;
+        if (d.key0 < d.len) d.page = __ldg(d.pages + a.column(d.key0, d.off));
+    }
+    __device__ __forceinline__ void enter(Loader& d) const {
+        d.key0 = d.c.u * kUnit + warp * 16;
+        d.left = d.c.left();
+        d.len = d.c.q.len;
+        d.pages = a.table + d.c.r * a.stride;
+        const int64_t rows = (int64_t)d.c.h * a.page;
+        d.codes = a.codes + rows * L::kRowBytes + lane * 16;
+        d.scales = a.scales + rows * E + (lane % (L::kScales / 16)) * 16;
+    }
+    __device__ __forceinline__ void step(Loader& d, bool more) const {
+        d.key0 += kUnit;
+        if (--d.left == 0 && more) {
+            d.c.next_segment(a);
+            enter(d);
+        }
+        if (more) look(d);
     }
 
-    // starts the copy of cursor c's tile of page pg into stage s
-    __device__ __forceinline__ void issue(const Cur& c, int pg, int s) {
-        const bool there = pg >= 0 && pg < a.n_pages;
+    // starts the copy of the loader's tile into stage s
+    __device__ __forceinline__ void issue(const Loader& d, int s) {
+        const bool there = (unsigned)d.page < (unsigned)a.n_pages;
         if (there) {
-            int off;
-            a.column(c.u * kUnit + warp * 16, off);
-            const int64_t half = (int64_t)a.kv_heads * a.page;      // token rows of K, and of V, in a page
-            const int64_t kr = pg * (2 * half) + c.head_rows + off, vr = kr + half;
+            // (the host has checked that a page's bytes fit 31 bits)
+            const uint32_t half = (uint32_t)a.kv_heads * a.page;     // token rows of K, and of V, in a page
+            const uint8_t* k = d.codes + (uint64_t)(uint32_t)d.page * (2 * half * L::kRowBytes) + d.off * L::kRowBytes;
+            const uint8_t* v = k + half * L::kRowBytes;
             const uint32_t at = ring_at + s * L::kStage;
-            constexpr int kPer = L::kRowBytes / 16;
+            constexpr int kPer = L::kRowBytes / 16, kStep = 32 / kPer;     // lanes a key, keys of one copy instruction
+            const int key = lane / kPer, c16 = lane % kPer;
+            // the chunks' swizzles go by key bits that a step of kStep keys leaves alone
+            static_assert(E == 8 || kStep % 4 == 0, "swizzle");
 #pragma unroll
-            for (int i = 0; i < 16 * kPer / 32; ++i) {
-                const int n = i * 32 + lane, key = n / kPer, c16 = n % kPer;
-                cp16(at + key * L::kRowBytes + k_chunk(key, c16) * 16, a.codes + kr * L::kRowBytes + n * 16);
-                cp16(at + L::kCodes + key * L::kRowBytes + v_chunk(key, c16) * 16, a.codes + vr * L::kRowBytes + n * 16);
+            for (int i = 0; i < 16 / kStep; ++i) {
+                const int kk = E == 8 ? key + i * kStep : key;
+                cp16(at + (key + i * kStep) * L::kRowBytes + k_chunk(kk, c16) * 16, k + i * 512);
+                cp16(at + L::kCodes + (key + i * kStep) * L::kRowBytes + v_chunk(kk, c16) * 16, v + i * 512);
             }
             constexpr int kSc = L::kScales / 16;
             if (lane < 2 * kSc) {
-                const int w = lane >= kSc, n = lane - w * kSc;
-                cp16(at + 2 * L::kCodes + lane * 16, a.scales + (w ? vr : kr) * E + n * 16);
+                const uint8_t* p = d.scales + (uint64_t)(uint32_t)d.page * (2 * half * E) + d.off * E;
+                cp16(at + 2 * L::kCodes + lane * 16, lane >= kSc ? p + half * E : p);
             }
         }
         if (lane == 0) flags[s] = there;
@@ -416,8 +436,7 @@ struct Attend {
             }
     }
 
-    __device__ __forceinline__ void tile(const Cur& c, int s) {
-        const int key0 = c.u * kUnit + warp * 16;
+    __device__ __forceinline__ void tile(int key0, int s) {
         if (!flags[s] || key0 >= any_to || key0 + 16 <= any_from) return;
         const uint8_t* st = ring + s * L::kStage;
         const int ka = key_of(g);
@@ -679,42 +698,40 @@ struct Attend {
 
     __device__ __forceinline__ void run(Cur c, int64_t begin, int64_t end, int64_t all, int* s_last) {
         const int n = (int)(end - begin);
-        Cur ld = c;
-        int pg = fetch_page(ld);
-#pragma unroll
+        Loader d;
+        d.c = c;
+        enter(d);
+        look(d);
+#pragma unroll 1
         for (int s = 0; s < kStages - 1; ++s) {
             if (s < n) {
-                const int now = pg;
-                const Cur at = ld;
-                ld.next(a);
-                if (s + 1 < n) pg = fetch_page(ld);
-                issue(at, now, s);
+                issue(d, s);
+                step(d, s + 1 < n);
             }
             asm volatile("cp.async.commit_group;");
         }
-        bool fresh = true;
-        int stage = 0;
-        for (int i = 0; i < n; ++i) {
-            if (fresh) begin_segment(c);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
-            __syncwarp();
-            const int ahead = i + kStages - 1;
-            if (ahead < n) {
-                const int now = pg;
-                const Cur at = ld;
-                ld.next(a);
-                if (ahead + 1 < n) pg = fetch_page(ld);
-                issue(at, now, stage == 0 ? kStages - 1 : stage - 1);
+        int stage = 0, done = 0;
+        while (done < n) {
+            begin_segment(c);
+            const int here = min(c.left(), n - done);
+            int key0 = c.u * kUnit + warp * 16;
+#pragma unroll 1
+            for (int i = 0; i < here; ++i, key0 += kUnit) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
+                __syncwarp();
+                const int ahead = done + i + kStages - 1;
+                if (ahead < n) {
+                    issue(d, stage == 0 ? kStages - 1 : stage - 1);
+                    step(d, ahead + 1 < n);
+                }
+                asm volatile("cp.async.commit_group;");
+                tile(key0, stage);
+                stage = stage + 1 == kStages ? 0 : stage + 1;
             }
-            asm volatile("cp.async.commit_group;");
-            tile(c, stage);
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            fresh = c.u + 1 == c.q.k0 + c.q.units;
-            if (fresh || i + 1 == n) {
-                const int64_t seg0 = begin + i - (c.u - c.q.k0);
-                end_segment(c, seg0, seg0 + c.q.units, begin, end, all, s_last);
-            }
-            if (i + 1 < n) c.next(a);
+            const int64_t seg0 = begin + done - (c.u - c.q.k0);
+            end_segment(c, seg0, seg0 + c.q.units, begin, end, all, s_last);
+            done += here;
+            if (done < n) c.next_segment(a);
         }
     }
 };
@@ -796,6 +813,7 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
     if (page < 16 || page % 16) return bad(who, "page size must be a multiple of 16");
     if (tokens < 0 || tokens > 0x7fffffffLL || heads < 1 || kv_heads < 1 || n_pages < 0 || width < 0 || requests < 0 || window < 0 || most_new < 0)
         return bad(who, "sizes out of range");
+    if ((int64_t)kv_heads * page * dim > 0x7fffffffLL || n_pages > 0x7fffffffLL) return bad(who, "sizes out of range");
     if (tokens * heads > 0x7fffff00LL) return bad(who, "sizes out of range");
     if (heads % kv_heads) return bad(who, "the kv heads must divide the query heads");
     if (tokens == 0) return SILI_OK;
