@@ -56,11 +56,13 @@ struct Kv4Thresholds {
 #pragma unroll
         for (int i = 0; i < 7; ++i) t[i] = s > 0.f ? f[i] * s : __int_as_float(0x7FC00000);
     }
+    // three comparisons: which half of the codes, which quarter, which one
     __device__ __forceinline__ uint32_t code(float x) const {
         const float a = fabsf(x);
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 7; ++i) m += a >= t[i] ? 1u : 0u;
+        const bool b2 = a >= t[3];
+        const bool b1 = a >= (b2 ? t[5] : t[1]);
+        const bool b0 = a >= (b1 ? (b2 ? t[6] : t[2]) : (b2 ? t[4] : t[0]));
+        const uint32_t m = (b2 ? 4u : 0u) + (b1 ? 2u : 0u) + (b0 ? 1u : 0u);
         return m && x < 0.f ? m + 8u : m;
     }
 };

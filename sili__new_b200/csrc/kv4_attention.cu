@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -770,8 +771,8 @@ int launch(const AttendArgs& a, cudaStream_t s) {
     static_assert(8 * NT * (32 * E + 2) <= 32 * 130, "the workspace holds the widest row tile");
     static_assert(8 * NT * (kMaxCtas + 2) * 4 <= Layout<E, NT>::kJoin, "the parts' weights fit the join space");
     auto kernel = k_attend<T, E, NT>;
-    // set on every call: the attribute belongs to the current device
-    CKV(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> set{0};
+    CKV(sili::allow_smem(kernel, smem, set));
     kernel<<<NT == 1 && E < 8 ? kMaxCtas : kMaxCtas / 2, kWarps * 32, smem, s>>>(a);
     sili::count_launch();
     CKV(cudaGetLastError());

@@ -1,6 +1,7 @@
 // What the two attention kernels over the 4-bit cache share.
 #pragma once
 
+#include <atomic>
 #include <string>
 
 #include "kv4.cuh"
@@ -65,6 +66,20 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; `set` remembers the devices (a bit each)
+// on which it has, which the attribute belongs to.
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& set) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit && (set.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 // Long 16-bit prompts (kv4_prompt.cu): whether this call is one, and the launch.
 bool kv4_prompt_takes(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int64_t most_new);
 int kv4_prompt_launch(int dtype, int dim, const AttendArgs& a, cudaStream_t s);

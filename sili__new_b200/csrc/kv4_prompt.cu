@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -699,7 +700,8 @@ int launch(const AttendArgs& a, cudaStream_t s) {
     constexpr int smem = (int)sizeof(Smem<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto kernel = k_prompt<T, D>;
-    CKP(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> set{0};
+    CKP(sili::allow_smem(kernel, smem, set));
     // no more items than every request's rows rounded up; CTAs past the last leave at once
     const int64_t rows = a.tokens * (a.heads / a.kv_heads);
     const int64_t items = (rows / (kTiles * kM) + a.requests + 1) * a.kv_heads;

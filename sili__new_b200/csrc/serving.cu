@@ -420,97 +420,116 @@ struct AppendArgs {
     const int64_t* slots;
 };
 
-// A warp per head row, E = dim / 32 consecutive elements a lane, so a group
-// of 32 is 32 / E lanes: its maximum is log2(32 / E) shuffles and its codes
-// leave as E / 2 bytes a lane, 32 / E lanes together.  In half layout the
+// Eight consecutive elements a lane, dim / 8 lanes a head row (1, 2 or 4 rows
+// a warp), so a group of 32 is four lanes: its maximum is two shuffles and its
+// codes leave as four bytes a lane, whole rows together.  In half layout the
 // rotation's partner element is rot/2 away, the same element of another lane
 // (rot % 16 == 0), and comes by shuffle.  A CTA's warps share one token and
 // walk its q, k and v rows with the token's cosines in registers.
-template <typename T, int E>
-__global__ void __launch_bounds__(256) k_kv4_append(AppendArgs a) {
-    using P = Pack<T, E>;
-    constexpr int kDim = 32 * E, kLanes = 32 / E;
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ AppendArgs a) {
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes;     // lanes a row, rows a warp
+    constexpr int kWord = sizeof(T) == 2 ? 4 : 8;          // 32-bit words of a lane's elements
     const RotaryArgs& r = a.r;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes;
     const int64_t t = blockIdx.x;
     const int nq = r.heads[0], nk = r.heads[1], rows = nq + 2 * nk;
-    const int half = r.rot / 2, e = lane * E;
+    const int half = r.rot / 2, e = sub * 8;
     const bool turns = e < r.rot;
     const int64_t pos = r.rot ? load_position(r.positions, r.pos64, t) : 0;
     const bool pad = pos < 0, past = r.rot && pos >= r.n_positions;
     const float blank = pad ? 0.f : __int_as_float(0x7FC00000);
-    float c[E], s[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) { c[i] = 1.f; s[i] = 0.f; }
+    float c[8], s[8];
     if (turns && !pad && !past) {
+        if (r.interleaved) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int j = r.interleaved ? (e + i) / 2 : (e < half ? e + i : e + i - half);
-            c[i] = __ldg(r.cos + pos * half + j);
-            s[i] = __ldg(r.sin + pos * half + j);
+            for (int i = 0; i < 8; ++i) {
+                c[i] = __ldg(r.cos + pos * half + e / 2 + i / 2);
+                s[i] = __ldg(r.sin + pos * half + e / 2 + i / 2);
+            }
+        } else {
+            // the second half's sine with the sign that its sum takes
+            const int j = e < half ? e : e - half;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = __ldg(r.cos + pos * half + j + i);
+                s[i] = __ldg(r.sin + pos * half + j + i);
+                s[i] = e < half ? -s[i] : s[i];
+            }
         }
     }
-    const int partner = (e < half ? e + half : e - half) / E & 31;
+    const int partner = (lane - sub) + ((e < half ? e + half : e - half) / 8 & (kLanes - 1));
     const int64_t slot = a.slots[t];
     const bool stored = slot >= 0 && slot < a.n_slots;
     const int64_t pg = stored ? slot / a.page : 0;
-    const int off = stored ? (int)(slot - pg * a.page) : 0;
+    const int64_t row_at = pg * (2 * (int64_t)nk * a.page) + (slot - pg * a.page);     // K's row of kv head 0
+    const T* const src0 = (const T*)r.x[0] + t * r.xt[0] + e;
+    const T* const src1 = (const T*)r.x[1] + t * r.xt[1] + e;
+    const T* const src2 = (const T*)a.v + t * a.vt + e;
 #pragma unroll 2
-    for (int row = blockIdx.y * 8 + warp; row < rows; row += 8 * gridDim.y) {
+    for (int row0 = (blockIdx.y * 8 + warp) * kRows; row0 < rows; row0 += 8 * kRows * gridDim.y) {
+        const int row = row0 + lane / kLanes;
         const int w = row < nq ? 0 : row < nq + nk ? 1 : 2;
-        if (w && !stored) continue;
         const int h = w == 0 ? row : w == 1 ? row - nq : row - nq - nk;
-        const T* src = w == 0 ? (const T*)r.x[0] + t * r.xt[0] + h * r.xh[0]
-                     : w == 1 ? (const T*)r.x[1] + t * r.xt[1] + h * r.xh[1] : (const T*)a.v + t * a.vt + h * a.vh;
-        const P p = *(const P*)(src + e);
-        float x[E];
+        const bool active = row < rows && (w == 0 || stored);
+        union { uint32_t u[kWord]; Pack<T, 8> p; uint4 v[kWord / 4]; } in;
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = sili::to_f32(p.v[i]);
-        if (w < 2 && r.rot) {
+        for (int i = 0; i < kWord / 4; ++i) in.v[i] = make_uint4(0, 0, 0, 0);
+        if (active) {
+            const T* src = w == 0 ? src0 + h * r.xh[0] : w == 1 ? src1 + h * r.xh[1] : src2 + h * a.vh;
+#pragma unroll
+            for (int i = 0; i < kWord / 4; ++i) in.v[i] = __ldg((const uint4*)src + i);
+        }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = sili::to_f32(in.p.v[i]);
+        if (r.rot) {
             if (r.interleaved) {
-                if (turns)
+                if (turns && w < 2) {
 #pragma unroll
-                    for (int i = 0; i < E; i += 2) {
+                    for (int i = 0; i < 8; i += 2) {
                         const float f = x[i], g = x[i + 1];
                         x[i] = __fsub_rn(__fmul_rn(f, c[i]), __fmul_rn(g, s[i]));
                         x[i + 1] = __fadd_rn(__fmul_rn(g, c[i]), __fmul_rn(f, s[i]));
                     }
+                }
             } else {
+                union { uint32_t u[kWord]; Pack<T, 8> p; } other;
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const float g = __shfl_sync(0xffffffffu, x[i], partner);
-                    if (turns)
-                        x[i] = e < half ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(g, s[i]))
-                                        : __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(g, s[i]));
+                for (int i = 0; i < kWord; ++i) other.u[i] = __shfl_sync(0xffffffffu, in.u[i], partner);
+                if (turns && w < 2) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(sili::to_f32(other.p.v[i]), s[i]));
                 }
             }
-            if (pad || past)
+            if ((pad || past) && w < 2) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[i] = blank;
+                for (int i = 0; i < 8; ++i) x[i] = blank;
+            }
         }
         if (w == 0) {
-            P o;
+            Pack<T, 8> o;
 #pragma unroll
-            for (int i = 0; i < E; ++i) o.v[i] = sili::from_f32<T>(x[i]);
-            *(P*)((T*)r.y[0] + t * r.yt[0] + h * r.yh[0] + e) = o;
-            continue;
+            for (int i = 0; i < 8; ++i) o.v[i] = sili::from_f32<T>(x[i]);
+            if (active) *(Pack<T, 8>*)((T*)r.y[0] + t * r.yt[0] + h * r.yh[0] + e) = o;
         }
+        if (row0 + kRows <= nq) continue;      // q rows only: nothing to quantise (the same for the whole warp)
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const uint32_t b = sili::kv4_scale_byte(m);
         const sili::Kv4Thresholds th(sili::kv4_scale(b));
         uint32_t packed = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) packed |= th.code(x[i]) << (4 * i);
-        const int64_t at = sili::kv4_row(pg, w - 1, h, nk, a.page) + off;
-        uint8_t* dst = a.codes + at * (kDim / 2) + lane * (E / 2);
-        if constexpr (E == 2) *dst = (uint8_t)packed;
-        else if constexpr (E == 4) *(uint16_t*)dst = (uint16_t)packed;
-        else *(uint32_t*)dst = packed;
-        if (lane % kLanes == 0) a.scales[at * E + lane / kLanes] = (uint8_t)b;
+        for (int i = 0; i < 8; ++i) packed |= th.code(x[i]) << (4 * i);
+        if (active && w) {
+            const int64_t at = row_at + ((int64_t)(w - 1) * nk + h) * a.page;
+            *(uint32_t*)(a.codes + at * (D / 2) + sub * 4) = packed;
+            if (sub % 4 == 0) a.scales[at * (D / 32) + sub / 4] = (uint8_t)b;
+        }
     }
 }
 
@@ -680,32 +699,34 @@ int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_
     if (q_heads && !rot) return bad(who, "q is only taken along to be rotated");
     if (tokens == 0) return SILI_OK;
     if (!k || !v || !slots || (q_heads && (!q || !q_out)) || (n_pages && (!codes || !scales))) return bad(who, "null array");
-    const int64_t item = dtype == SILI_F32 ? 4 : 2, e = dim / 32;
+    const int64_t item = dtype == SILI_F32 ? 4 : 2;
     auto aligned = [&](const void* p, int64_t ts, int64_t hs) {
-        return (uintptr_t)p % (e * item) == 0 && ts % e == 0 && hs % e == 0;
+        return (uintptr_t)p % 16 == 0 && ts * item % 16 == 0 && hs * item % 16 == 0;
     };
     if (!aligned(k, k_token_stride, k_head_stride) || !aligned(v, v_token_stride, v_head_stride) ||
         (q_heads && (!aligned(q, q_token_stride, q_head_stride) || !aligned(q_out, qo_token_stride, qo_head_stride))))
-        return bad(who, "rows must start on a multiple of dim / 32 elements");
+        return bad(who, "rows must start on 16 bytes");
     if ((uintptr_t)codes % 16) return bad(who, "codes must be 16-byte aligned");
     AppendArgs a{{{q, k}, {q_out, nullptr}, {q_token_stride, k_token_stride}, {q_head_stride, k_head_stride},
                   {qo_token_stride, 0}, {qo_head_stride, 0}, {q_heads, kv_heads}, tokens, dim, rot, cos, sin, n_positions,
                   positions, pos64, interleaved, 1.f},
                  v, v_token_stride, v_head_stride, codes, scales, n_pages * page, page, slots};
     cudaStream_t s = (cudaStream_t)stream;
-    const int passes = (q_heads + 2 * kv_heads + 7) / 8;
+    const int per = 8 * (256 / dim);       // rows a pass of a CTA
+    const int passes = (q_heads + 2 * kv_heads + per - 1) / per;
     const dim3 grid((unsigned)tokens, (unsigned)std::max<int64_t>(1, std::min<int64_t>(passes, 592 / tokens)));
     auto go = [&](auto kernel) {
         kernel<<<grid, 256, 0, s>>>(a);
         sili::count_launch();
     };
     if (dtype == SILI_F32) {
-        if (dim == 64) go(k_kv4_append<float, 2>); else if (dim == 128) go(k_kv4_append<float, 4>); else go(k_kv4_append<float, 8>);
+        if (dim == 64) go(k_kv4_append<float, 64>); else if (dim == 128) go(k_kv4_append<float, 128>); else go(k_kv4_append<float, 256>);
     } else if (dtype == SILI_F16) {
-        if (dim == 64) go(k_kv4_append<__half, 2>); else if (dim == 128) go(k_kv4_append<__half, 4>); else go(k_kv4_append<__half, 8>);
+        if (dim == 64) go(k_kv4_append<__half, 64>);
+        else if (dim == 128) go(k_kv4_append<__half, 128>); else go(k_kv4_append<__half, 256>);
     } else {
-        if (dim == 64) go(k_kv4_append<__nv_bfloat16, 2>);
-        else if (dim == 128) go(k_kv4_append<__nv_bfloat16, 4>); else go(k_kv4_append<__nv_bfloat16, 8>);
+        if (dim == 64) go(k_kv4_append<__nv_bfloat16, 64>);
+        else if (dim == 128) go(k_kv4_append<__nv_bfloat16, 128>); else go(k_kv4_append<__nv_bfloat16, 256>);
     }
     CKS(cudaGetLastError());
     return SILI_OK;

@@ -41,19 +41,18 @@ def _dtype_code(t, who):
     return code
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream     # torch.cuda.current_stream(dev).cuda_stream, without the objects
+_I32, _I64, _U8, _F32 = torch.int32, torch.int64, torch.uint8, torch.float32
+
+
 def _on_device(who, dev, *arrays):
-    """Every array on one CUDA device, which becomes the current one."""
+    """The current stream's handle of the CUDA device that every array is on."""
     if dev.type != "cuda":
         raise ValueError(f"{who}: arrays must be CUDA tensors")
     for a in arrays:
         if a is not None and a.device != dev:
             raise ValueError(f"{who}: arrays are on different devices")
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-def _on(dev):
-    """Context that makes `dev` the current device (nothing to do where it is already)."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _raw_stream(dev.index)
 
 
 class _Here:
@@ -67,17 +66,26 @@ class _Here:
 _HERE = _Here()
 
 
+def _on(dev):
+    """Context that makes `dev` the current device (nothing to do where it is already)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
 def _contiguous(who, name, t, dtype, shape=None):
+    if t.dtype is dtype and (shape is None or t.shape == shape) and t.is_contiguous():
+        return
     if t.dtype != dtype:
         raise ValueError(f"{who}: {name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be contiguous")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{who}: {name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{who}: {name} must be {list(shape)}, got {list(t.shape)}")
 
 
 def _heads(who, name, t, tokens=None, dim=None, dtype=None):
     """[tokens, heads, dim] with the last axis contiguous; any other strides."""
+    if t.dim() == 3 and t.stride(2) == 1 and (tokens is None or t.shape[0] == tokens) and \
+            (dim is None or t.shape[2] == dim) and (dtype is None or t.dtype is dtype):
+        return
     if t.dim() != 3:
         raise ValueError(f"{who}: {name} must be [tokens, heads, dim], got {list(t.shape)}")
     if t.stride(2) != 1 and t.shape[2] > 1:
@@ -148,17 +156,18 @@ def page_tables(cached, fresh, table, ring, pool, page: int, max_tokens: int) ->
     s = _on_device(who, dev, fresh, table, ring, pool)
     with _on(dev):
         # one allocation a type: int64 slots, pool, status; int32 positions, starts, lens (and the scan of large batches)
-        wide = torch.empty(max_tokens + 5, dtype=torch.int64, device=dev)
-        small = torch.empty(max_tokens + 2 * n + 1 + (n + 1 if n > 4096 else 0), dtype=torch.int32, device=dev)
-        slots, pool_out, status = wide[:max_tokens], wide[max_tokens:max_tokens + 2], wide[max_tokens + 2:]
-        positions = small[:max_tokens]
-        starts = small[max_tokens:max_tokens + n + 1]
-        lens = small[max_tokens + n + 1:max_tokens + 2 * n + 1]
-        scratch = small[max_tokens + 2 * n + 1:]
+        extra = n + 1 if n > 4096 else 0
+        wide = torch.empty(max_tokens + 5, dtype=_I64, device=dev)
+        small = torch.empty(max_tokens + 2 * n + 1 + extra, dtype=_I32, device=dev)
+        at8, at4 = wide.data_ptr(), small.data_ptr()
+        at_starts = at4 + 4 * max_tokens
+        at_lens = at_starts + 4 * (n + 1)
         _cuda.page_tables_ptr(cached.data_ptr(), fresh.data_ptr(), n, table.data_ptr(), _row_stride(table), table.shape[1],
-                              ring.data_ptr(), ring.numel(), pool.data_ptr(), page, max_tokens, starts.data_ptr(),
-                              lens.data_ptr(), slots.data_ptr(), positions.data_ptr(), pool_out.data_ptr(),
-                              status.data_ptr(), scratch.data_ptr() if n > 4096 else 0, s)
+                              ring.data_ptr(), ring.numel(), pool.data_ptr(), page, max_tokens, at_starts, at_lens, at8,
+                              at4, at8 + 8 * max_tokens, at8 + 8 * (max_tokens + 2), at_lens + 4 * n if extra else 0, s)
+        slots, pool_out, status = wide.split_with_sizes((max_tokens, 2, 3))
+        positions, starts, lens, *_ = small.split_with_sizes((max_tokens, n + 1, n, extra) if extra else
+                                                             (max_tokens, n + 1, n))
     return PageTables(starts, lens, slots, positions, pool_out, status)
 
 
@@ -255,7 +264,7 @@ def rotary_table(n_positions: int, rotary_dim: int, base: float = 10000.0, scali
         cos = torch.empty(n_positions, rotary_dim // 2, dtype=torch.float32, device=dev)
         sin = torch.empty_like(cos)
         _cuda.rotary_table_ptr(inv, n_positions, gain, cos.data_ptr(), sin.data_ptr(),
-                               torch.cuda.current_stream(dev).cuda_stream)
+                               _raw_stream(dev.index))
     return cos, sin
 
 
@@ -464,7 +473,7 @@ _workspaces: dict = {}
 
 
 def _workspace(dev, stream):
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         # a graph owns its workspace: it may be replayed on any stream, beside eager calls
         return _new_workspace(dev)
     w = _workspaces.get((dev.index, stream))
