@@ -420,6 +420,20 @@ struct AppendArgs {
     const int64_t* slots;
 };
 
+// page and place of a slot; in 32 bits where the cache has no more slots
+__device__ __forceinline__ int64_t split_slot(int64_t slot, int64_t n_slots, int page, int& off) {
+    if (n_slots <= 0x7fffffff) {
+        const uint32_t pg = (uint32_t)slot / (uint32_t)page;
+        off = (int)((uint32_t)slot - pg * (uint32_t)page);
+        return pg;
+    }
+    const int64_t pg = slot / page;
+    off = (int)(slot - pg * page);
+    return pg;
+}
+
+constexpr int kAppendThreads = 128;
+
 // Eight consecutive elements a lane, dim / 8 lanes a head row (1, 2 or 4 rows
 // a warp), so a group of 32 is four lanes: its maximum is two shuffles and its
 // codes leave as four bytes a lane, whole rows together.  In half layout the
@@ -427,8 +441,9 @@ struct AppendArgs {
 // (rot % 16 == 0), and comes by shuffle.  A CTA's warps share one token and
 // walk its q, k and v rows with the token's cosines in registers.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_constant__ AppendArgs a) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes;     // lanes a row, rows a warp
+    constexpr int kWarps = kAppendThreads / 32;
     constexpr int kWord = sizeof(T) == 2 ? 4 : 8;          // 32-bit words of a lane's elements
     const RotaryArgs& r = a.r;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes;
@@ -442,32 +457,34 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ Appe
     float c[8], s[8];
     if (turns && !pad && !past) {
         if (r.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                c[i] = __ldg(r.cos + pos * half + e / 2 + i / 2);
-                s[i] = __ldg(r.sin + pos * half + e / 2 + i / 2);
-            }
+            const float4 u = __ldg((const float4*)(r.cos + pos * half + e / 2));
+            const float4 v = __ldg((const float4*)(r.sin + pos * half + e / 2));
+            c[0] = c[1] = u.x; c[2] = c[3] = u.y; c[4] = c[5] = u.z; c[6] = c[7] = u.w;
+            s[0] = s[1] = v.x; s[2] = s[3] = v.y; s[4] = s[5] = v.z; s[6] = s[7] = v.w;
         } else {
             // the second half's sine with the sign that its sum takes
             const int j = e < half ? e : e - half;
+            const float sign = e < half ? -1.f : 1.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                c[i] = __ldg(r.cos + pos * half + j + i);
-                s[i] = __ldg(r.sin + pos * half + j + i);
-                s[i] = e < half ? -s[i] : s[i];
+            for (int i = 0; i < 2; ++i) {
+                const float4 u = __ldg((const float4*)(r.cos + pos * half + j) + i);
+                const float4 v = __ldg((const float4*)(r.sin + pos * half + j) + i);
+                c[4 * i] = u.x; c[4 * i + 1] = u.y; c[4 * i + 2] = u.z; c[4 * i + 3] = u.w;
+                s[4 * i] = sign * v.x; s[4 * i + 1] = sign * v.y; s[4 * i + 2] = sign * v.z; s[4 * i + 3] = sign * v.w;
             }
         }
     }
     const int partner = (lane - sub) + ((e < half ? e + half : e - half) / 8 & (kLanes - 1));
     const int64_t slot = a.slots[t];
     const bool stored = slot >= 0 && slot < a.n_slots;
-    const int64_t pg = stored ? slot / a.page : 0;
-    const int64_t row_at = pg * (2 * (int64_t)nk * a.page) + (slot - pg * a.page);     // K's row of kv head 0
+    int off;
+    const int64_t pg = split_slot(stored ? slot : 0, a.n_slots, a.page, off);
+    const int64_t row_at = pg * (2 * (int64_t)nk * a.page) + off;     // K's row of kv head 0
     const T* const src0 = (const T*)r.x[0] + t * r.xt[0] + e;
     const T* const src1 = (const T*)r.x[1] + t * r.xt[1] + e;
     const T* const src2 = (const T*)a.v + t * a.vt + e;
 #pragma unroll 2
-    for (int row0 = (blockIdx.y * 8 + warp) * kRows; row0 < rows; row0 += 8 * kRows * gridDim.y) {
+    for (int row0 = (blockIdx.y * kWarps + warp) * kRows; row0 < rows; row0 += kWarps * kRows * gridDim.y) {
         const int row = row0 + lane / kLanes;
         const int w = row < nq ? 0 : row < nq + nk ? 1 : 2;
         const int h = w == 0 ? row : w == 1 ? row - nq : row - nq - nk;
@@ -544,36 +561,44 @@ struct ReadArgs {
     void* v;
 };
 
-// 8 elements (4 bytes of codes) a thread: one 16- or 32-byte write each.  A
-// CTA takes whole tokens, so a token's units divide by 32-bit shifts only.
+// 8 elements (4 bytes of codes) of K and of V a thread: one 16- or 32-byte
+// write each.  A CTA takes whole tokens, so a token's units divide by 32-bit
+// shifts only.
 template <typename T>
 __global__ void __launch_bounds__(256) k_kv4_read(ReadArgs a, int dim, int tokens_per_cta) {
-    const int per = dim / 8, all = 2 * a.kv_heads * per;
+    const int per = dim / 8, all = a.kv_heads * per;
     const int64_t t = (int64_t)blockIdx.x * tokens_per_cta + threadIdx.x / (unsigned)all;
     if (threadIdx.x >= (unsigned)(all * tokens_per_cta) || t >= a.tokens) return;
     const int64_t slot = a.slots[t];
     const bool stored = slot >= 0 && slot < a.n_slots;
-    const int64_t pg = stored ? slot / a.page : 0;
-    const int off = (int)(slot - pg * a.page);
+    int off;
+    const int64_t pg = split_slot(stored ? slot : 0, a.n_slots, a.page, off);
+    const int64_t half = (int64_t)a.kv_heads * a.page, row0 = pg * (2 * half) + off;
     for (int u = threadIdx.x % (unsigned)all; u < all; u += 256) {
-        const int unit = u % per, row = u / per, w = row >= a.kv_heads, h = w ? row - a.kv_heads : row;
-        Pack<T, 8> o;
+        const int h = u / per, unit = u - h * per;
+        const int64_t at = row0 + (int64_t)h * a.page, to = (t * a.kv_heads + h) * dim + unit * 8;
+        uint32_t code[2] = {0, 0}, sc[2] = {0, 0};
         if (stored) {
-            const int64_t at = sili::kv4_row(pg, w, h, a.kv_heads, a.page) + off;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                code[w] = __ldg((const uint32_t*)(a.codes + (at + w * half) * (dim / 2) + unit * 4));
+                sc[w] = __ldg(a.scales + (at + w * half) * (dim / 32) + unit / 4);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
             uint32_t f[4];
-            sili::kv4_decode4(*(const uint32_t*)(a.codes + at * (dim / 2) + unit * 4), f);
-            const float sc = sili::kv4_scale(a.scales[at * (dim / 32) + unit / 4]);
+            sili::kv4_decode4(code[w], f);
+            const float scale = sili::kv4_scale(sc[w]);
+            Pack<T, 8> o;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const float2 v2 = sili::half2_bits_to_float2(f[q]);
-                o.v[2 * q] = sili::from_f32<T>(v2.x * sc);
-                o.v[2 * q + 1] = sili::from_f32<T>(v2.y * sc);
+                o.v[2 * q] = sili::from_f32<T>(v2.x * scale);
+                o.v[2 * q + 1] = sili::from_f32<T>(v2.y * scale);
             }
-        } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) o.v[q] = sili::from_f32<T>(0.f);
+            *(Pack<T, 8>*)((T*)(w ? a.v : a.k) + to) = o;
         }
-        *(Pack<T, 8>*)((T*)(w ? a.v : a.k) + (t * a.kv_heads + h) * dim + unit * 8) = o;
     }
 }
 
@@ -691,6 +716,7 @@ int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_
         const int rc = check_rotary(who, dtype, tokens, dim, rot, positions, cos, sin, n_positions);
         if (rc) return rc;
         if (rot % 16) return bad(who, "the rotated part must be a multiple of 16");
+        if ((uintptr_t)cos % 16 || (uintptr_t)sin % 16) return bad(who, "the table must be 16-byte aligned");
     }
     if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
     if (dim != 64 && dim != 128 && dim != 256) return bad(who, "head dimension must be 64, 128 or 256");
@@ -712,11 +738,11 @@ int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_
                   positions, pos64, interleaved, 1.f},
                  v, v_token_stride, v_head_stride, codes, scales, n_pages * page, page, slots};
     cudaStream_t s = (cudaStream_t)stream;
-    const int per = 8 * (256 / dim);       // rows a pass of a CTA
+    const int per = kAppendThreads / 32 * (256 / dim);       // rows a pass of a CTA
     const int passes = (q_heads + 2 * kv_heads + per - 1) / per;
     const dim3 grid((unsigned)tokens, (unsigned)std::max<int64_t>(1, std::min<int64_t>(passes, 592 / tokens)));
     auto go = [&](auto kernel) {
-        kernel<<<grid, 256, 0, s>>>(a);
+        kernel<<<grid, kAppendThreads, 0, s>>>(a);
         sili::count_launch();
     };
     if (dtype == SILI_F32) {
@@ -742,7 +768,7 @@ int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_
     if (!slots || !k_out || !v_out || (n_pages && (!codes || !scales))) return bad(who, "null array");
     if ((uintptr_t)k_out % 32 || (uintptr_t)v_out % 32 || (uintptr_t)codes % 16) return bad(who, "outputs must be 32-byte, codes 16-byte aligned");
     ReadArgs a{codes, scales, n_pages * page, page, kv_heads, slots, tokens, k_out, v_out};
-    const int tpc = std::max(1, 256 / (2 * kv_heads * (dim / 8)));
+    const int tpc = std::max(1, 256 / (kv_heads * (dim / 8)));
     if ((tokens + tpc - 1) / tpc > 0x7fffffffLL) return bad(who, "sizes out of range");
     const unsigned grid = (unsigned)((tokens + tpc - 1) / tpc);
     cudaStream_t s = (cudaStream_t)stream;
