@@ -195,31 +195,43 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
     return q;
 }
 
-// Items are numbered request by request, in each the last rows first (they
-// have the most keys), the kv heads together.  One warp finds item `id`.
+// Items (a kv head's pair of row tiles) are numbered by level, and a request's
+// last rows, which have the most keys, are its level 0: the long items start
+// first and the short ones fill the card's last round.  Within a level the
+// requests that reach it follow one another, their kv heads together.  One
+// warp finds item `id`: the level by bisection of the items before it,
+// kv heads * sum over requests of min(pairs, level).
 __device__ __forceinline__ bool find_item(const AttendArgs& a, int64_t id, int (&hit)[3]) {
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;
-    for (int base = 0; base < a.requests; base += 32) {
-        const int r = base + lane;
-        const int pairs = r < a.requests ? span_of(a, r).pairs : 0;
-        const int64_t n = (int64_t)pairs * a.kv_heads;
-        int64_t x = n;
+    const int64_t want = id / a.kv_heads;       // among pairs
+    auto before = [&](int level) {
+        int64_t n = 0;
+        for (int r = lane; r < a.requests; r += 32) n += min(span_of(a, r).pairs, level);
+        return sili::warp_sum(n);
+    };
+    int most = 0;
+    for (int r = lane; r < a.requests; r += 32) most = max(most, span_of(a, r).pairs);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += t;
+    for (int o = 16; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (want >= before(most)) return false;
+    int lo = 0, hi = most;                      // before(lo) <= want < before(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before(mid) <= want) lo = mid; else hi = mid;
+    }
+    int64_t rank = want - before(lo);           // among the requests that reach level lo
+    for (int base = 0; base < a.requests; base += 32) {
+        const int r = base + lane, pairs = r < a.requests ? span_of(a, r).pairs : 0;
+        const unsigned reach = __ballot_sync(0xffffffffu, pairs > lo);
+        if (rank < __popc(reach)) {
+            if ((reach >> lane & 1) && __popc(reach & ((1u << lane) - 1u)) == (int)rank) {
+                hit[0] = r;
+                hit[1] = (int)(id % a.kv_heads);
+                hit[2] = pairs - 1 - lo;
+            }
+            return true;
         }
-        x += before;
-        const bool mine = x - n <= id && id < x;
-        if (mine) {
-            const int64_t off = id - (x - n);
-            hit[0] = r;
-            hit[1] = (int)(off % a.kv_heads);
-            hit[2] = pairs - 1 - (int)(off / a.kv_heads);
-        }
-        if (__any_sync(0xffffffffu, mine)) return true;
-        before = __shfl_sync(0xffffffffu, x, 31);
+        rank -= __popc(reach);
     }
     return false;
 }
@@ -458,33 +470,39 @@ struct Prompt {
         // (with the scale's sign, so that the logits' factor is never negative)
         float cf = fabsf(a.scale) * kLog2e;
         {
+            // the whole row at once: its loads are in flight together
             const T* src = (const T*)a.q + q_row * a.qt + head * a.qh;
             const int m = threadIdx.x & 127;
-            uint32_t top = 0;
-            float f = a.scale < 0.f ? -1.f : 1.f;
-            if (!std::is_same<T, __half>::value && real) {
-                for (int i = 0; i < D; i += 4) {
-                    const sili::Pack<T, 4> p = *(const sili::Pack<T, 4>*)(src + i);
+            sili::Pack<T, 4> row4[D / 4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(sili::to_f32(p.v[k])) & 0x7FFFFFFFu);
-                }
+            for (int i = 0; i < D / 4; ++i) {
+                if (real) row4[i] = *(const sili::Pack<T, 4>*)(src + 4 * i);
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) row4[i].v[k] = sili::from_f32<T>(0.f);
+            }
+            float f = a.scale < 0.f ? -1.f : 1.f;
+            if (!std::is_same<T, __half>::value) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < D / 4; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(sili::to_f32(row4[i].v[k])) & 0x7FFFFFFFu);
                 if (top && top < 0x7F800000u) {
                     const int e = 14 - max((int)(top >> 23) - 127, -100);
                     f *= __int_as_float((127 + e) << 23);
                     cf *= __int_as_float((127 - e) << 23);
                 }
             }
-#pragma unroll 4
+#pragma unroll
             for (int i = 0; i < D; i += 8) {
-                uint4 o = make_uint4(0, 0, 0, 0);
-                if (real) {
-                    const sili::Pack<T, 4> p = *(const sili::Pack<T, 4>*)(src + i), q = *(const sili::Pack<T, 4>*)(src + i + 4);
-                    o = make_uint4(pack2(sili::to_f32(p.v[0]) * f, sili::to_f32(p.v[1]) * f),
-                                   pack2(sili::to_f32(p.v[2]) * f, sili::to_f32(p.v[3]) * f),
-                                   pack2(sili::to_f32(q.v[0]) * f, sili::to_f32(q.v[1]) * f),
-                                   pack2(sili::to_f32(q.v[2]) * f, sili::to_f32(q.v[3]) * f));
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const sili::Pack<T, 4>& p = row4[i / 4 + k / 2];
+                    o[k] = pack2(sili::to_f32(p.v[2 * (k & 1)]) * f, sili::to_f32(p.v[2 * (k & 1) + 1]) * f);
                 }
-                *(uint4*)(s.q[t] + (i >> 6) * (kM * 128) + chunk_at(m, (i & 63) >> 3)) = o;
+                *(uint4*)(s.q[t] + (i >> 6) * (kM * 128) + chunk_at(m, (i & 63) >> 3)) = make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
         cf = fmaxf(cf, 0x1p-126f);      // not 0, which would undo a mask's -inf
