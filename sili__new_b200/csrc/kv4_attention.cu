@@ -89,11 +89,18 @@ struct Layout {
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kJoin = kWarps * kRows * (kJoinRow + 2) * 4;
 };
+// The Q fragments lie in shared memory where the registers are needed: wide
+// row tiles, and fp32's two terms beside a second CTA (128 registers a thread:
+// in registers they spill, 160 against 133 us on the fp32 decode batch).
+template <typename T, int E, int NT>
+constexpr bool q_shared() {
+    return NT > 1 || (sizeof(T) == 4 && E < 8);
+}
 template <typename T, int E, int NT>
 constexpr int smem_bytes() {
     using L = Layout<E, NT>;
     constexpr int terms = sizeof(T) == 4 ? 2 : 1;
-    return L::kRing + L::kJoin + (NT > 1 ? NT * 2 * E * terms * 32 * 8 : 0);
+    return L::kRing + L::kJoin + (q_shared<T, E, NT>() ? NT * 2 * E * terms * 32 * 8 : 0);
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -229,6 +236,7 @@ struct Attend {
     static constexpr int kStages = L::kStages;
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
     static constexpr int kDim = L::kDim, kRows = L::kRows, kSteps = kDim / 16;
+    static constexpr bool kShared = q_shared<T, E, NT>();
     using Cur = Cursor<kRows>;
 
     const AttendArgs& a;
@@ -237,10 +245,10 @@ struct Attend {
     uint32_t ring_at;
     int* flags;            // per stage: the tile holds keys
     float* join;
-    uint32_t* qs;          // Q fragments in shared memory (NT > 1)
+    uint32_t* qs;          // Q fragments in shared memory (kShared)
 
     // the current segment
-    uint32_t qf[NT > 1 ? 1 : kSteps][kTerms][2];
+    uint32_t qf[kShared ? 1 : kSteps][kTerms][2];
     float cf[NT][2];       // logit = S * cf, in powers of two
     float base[NT][2];     // the running maximum - lift
     float l[NT][2], o[kSteps][NT][4];
@@ -334,7 +342,7 @@ struct Attend {
         };
         span(row0, any_from, all_to);
         span(min(row0 + kRows, rows) - 1, all_from, any_to);
-        if (NT > 1) __syncthreads();    // the last segment's fragments have been read
+        if (kShared) __syncthreads();    // the last segment's fragments have been read
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int row = row0 + n * 8 + g;
@@ -343,8 +351,8 @@ struct Attend {
             const int head = h * group + (real ? row % group : 0);
             const T* src = (const T*)a.q + tok * a.qt + head * a.qh + t * (kDim / 4);
             constexpr int kPart = 8 / sizeof(T) < 4 ? 2 : 4;     // elements of an 8-byte access
-            // NT > 1: warp n % kWarps alone prepares row tile n for all
-            if (NT == 1 || warp == n) {
+            // shared: warp n alone prepares row tile n for all
+            if (!kShared || warp == n) {
                 float f = 1.f, x[kDim / 4];
                 uint32_t top = 0;
 #pragma unroll
@@ -373,11 +381,11 @@ struct Attend {
                     for (int p = 0; p < 2; ++p) {
                         const float u = x[4 * i + 2 * p] * f, v = x[4 * i + 2 * p + 1] * f;
                         const uint32_t hi = pack2(u, v);
-                        if (NT == 1) qf[NT > 1 ? 0 : i][0][p] = hi;
+                        if (!kShared) qf[kShared ? 0 : i][0][p] = hi;
                         else qs[(((n * kSteps + i) * kTerms) * 32 + lane) * 2 + p] = hi;
                         if (kTerms == 2) {
                             const uint32_t lo = rest2(u, v, hi);
-                            if (NT == 1) qf[NT > 1 ? 0 : i][kTerms - 1][p] = lo;
+                            if (!kShared) qf[kShared ? 0 : i][kTerms - 1][p] = lo;
                             else qs[(((n * kSteps + i) * kTerms + kTerms - 1) * 32 + lane) * 2 + p] = lo;
                         }
                     }
@@ -386,7 +394,7 @@ struct Attend {
                 const float back = fmaxf(fabsf(a.scale) * kLog2e * __int_as_float((127 - e) << 23), 0x1p-126f);
                 cf[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
                 cf[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-                if (NT > 1) {
+                if (kShared) {
                     float* s_cf = (float*)flags - warp * kStages + kWarps * kMaxStages;
                     if (t == 0) s_cf[n * 8 + g] = back;
                 }
@@ -398,7 +406,7 @@ struct Attend {
                 l[n][j] = 0.f;
             }
         }
-        if (NT > 1) {
+        if (kShared) {
             __syncthreads();
             const float* s_cf = (const float*)flags - warp * kStages + kWarps * kMaxStages;
 #pragma unroll
@@ -483,7 +491,7 @@ struct Attend {
 #pragma unroll
                         for (int q = 0; q < kTerms; ++q) {
                             uint32_t b0, b1;
-                            if (NT == 1) { b0 = qf[NT > 1 ? 0 : 2 * j + k][q][0]; b1 = qf[NT > 1 ? 0 : 2 * j + k][q][1]; }
+                            if (!kShared) { b0 = qf[kShared ? 0 : 2 * j + k][q][0]; b1 = qf[kShared ? 0 : 2 * j + k][q][1]; }
                             else {
                                 const uint2 b = ((const uint2*)qs)[((n * kSteps + 2 * j + k) * kTerms + q) * 32 + lane];
                                 b0 = b.x; b1 = b.y;
