@@ -510,6 +510,10 @@ int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_
  * once before its first call, and left as a call leaves it; calls that may run at the same time need
  * one each.  page: a multiple of 16. */
 int sili_kv4_attention_workspace(int64_t* bytes);
+/* SILI_ETIMEOUT when a bounded device-side wait of a call that used this
+ * workspace gave up since the last look (its rows are NaN), else SILI_OK;
+ * waits for the stream. */
+int sili_kv4_attention_status(void* workspace, void* stream);
 int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
                        int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads,
                        const int* table, int64_t table_stride, int width, const int* lens, int requests,

@@ -805,6 +805,17 @@ int by_dim(const AttendArgs& a, int dim, int64_t rows, cudaStream_t s) {
 
 extern "C" {
 
+int sili_kv4_attention_status(void* workspace, void* stream) {
+    if (!workspace) return bad("kv4_attention_status", "null workspace");
+    unsigned word = 0, *at = (unsigned*)workspace + sili::kErrorWord;
+    cudaStream_t s = (cudaStream_t)stream;
+    CKV(cudaMemcpyAsync(&word, at, sizeof word, cudaMemcpyDeviceToHost, s));
+    CKV(cudaStreamSynchronize(s));
+    if (!word) return SILI_OK;
+    CKV(cudaMemsetAsync(at, 0, sizeof word, s));
+    return sili::set_error(SILI_ETIMEOUT, "kv4_attention: a device-side wait gave up; the rows it served are NaN");
+}
+
 int sili_kv4_attention_workspace(int64_t* bytes) {
     if (!bytes) return bad("kv4_attention_workspace", "null array");
     *bytes = workspace_bytes();

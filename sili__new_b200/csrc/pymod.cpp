@@ -826,6 +826,9 @@ PYBIND11_MODULE(_cuda, m) {
         check(sili_kv4_read(dtype, (const uint8_t*)codes, (const uint8_t*)scales, n_pages, page, kv_heads, dim,
                             (const int64_t*)slots, tokens, (void*)k, (void*)v, (void*)stream));
     });
+    m.def("kv4_attention_status_ptr", [](uintptr_t workspace, uintptr_t stream) {
+        check(sili_kv4_attention_status((void*)workspace, (void*)stream));
+    });
     m.def("kv4_attention_workspace", []() {
         int64_t n = 0;
         check(sili_kv4_attention_workspace(&n));

@@ -47,7 +47,9 @@ int bad(const char* who, const char* what) {
 // (binary search), stands at cached[r] + i - starts[r], and the page of
 // column c is table[r][c] where c was there before, else
 // ring[(taken + first[r] + c - have[r]) mod size].  No lookup reads what the
-// launch writes, so CTAs need no order among themselves.
+// launch writes, so CTAs need no order among themselves.  The data is little
+// (0.9 MB for 1531 requests and 68k tokens): a call is its launch and a few L2
+// latencies, 19 us with the host's side at 64 and at 1531 requests alike.
 struct TableArgs {
     const int* cached;
     const int* fresh;
@@ -311,9 +313,12 @@ __device__ __forceinline__ int64_t load_position(const void* p, int pos64, int64
 // V elements an access.  One unit of a head row is V pairs (half layout: V
 // elements at i and V at i + rot/2), V/2 pairs (interleaved: V adjacent
 // elements) or V elements that pass through; a thread keeps its unit and so
-// its cosines while it walks the heads.
+// its cosines while it walks the heads.  Bound by HBM: each value is read and
+// written once.  8191 tokens of 32 + 8 heads x 128 in fp32, forward and
+// gradient: 148 us, 4.6 TB/s; few tokens are spread over several CTAs each, a
+// call of 64 tokens is its launch (19 us with the host's side).
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_rotary(RotaryArgs a, int units, int rot_units, int rows) {
+__global__ void __launch_bounds__(V == 1 ? 1024 : 256) k_rotary(RotaryArgs a, int units, int rot_units, int rows) {
     using P = Pack<T, V>;
     const int u = threadIdx.x % units, row = threadIdx.x / units;
     if (row >= rows) return;
@@ -439,7 +444,10 @@ constexpr int kAppendThreads = 128;
 // codes leave as four bytes a lane, whole rows together.  In half layout the
 // rotation's partner element is rot/2 away, the same element of another lane
 // (rot % 16 == 0), and comes by shuffle.  A CTA's warps share one token and
-// walk its q, k and v rows with the token's cosines in registers.
+// walk its q, k and v rows with the token's cosines in registers.  Bound by
+// instructions (the codes: three comparisons a value) before HBM: 16384
+// tokens of 32 + 2 x 8 heads x 128 in bf16 take 132 us, 2.6 TB/s, and the
+// read-back below 24 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_constant__ AppendArgs a) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes;     // lanes a row, rows a warp

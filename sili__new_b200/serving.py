@@ -404,9 +404,10 @@ def _check_slots(who, slots, tokens):
 def cache_append(k, v, codes, scales, slots, cos=None, sin=None, positions=None, layout: str = "half", q=None,
                  q_out=None):
     """Writes k, v [tokens, kv heads, dim] into the cache at ``slots`` (int64;
-    a slot outside the cache, such as a padding token's -1, is passed over),
-    in one launch with the rotation of k, and of ``q`` when given, by
-    ``positions`` (see ``rotary``; the rotated part a multiple of 16).
+    a slot outside the cache, such as a padding token's -1, is passed over;
+    no two tokens may share one), in one launch with the rotation of k, and of
+    ``q`` when given, by ``positions`` (see ``rotary``; the rotated part a
+    multiple of 16).  Head rows start on 16 bytes (any strides otherwise).
     Returns the rotated q (None without q)."""
     who = "cache_append"
     n_pages, hk, page, dim = _check_cache(who, codes, scales)
@@ -488,6 +489,17 @@ def _new_workspace(dev):
     return w
 
 
+def check_attention(device=None):
+    """Raises RuntimeError if a device-side wait of an eager ``cache_attention``
+    on the current stream gave up since the last check (its rows are NaN).
+    Waits for the stream; a captured call's rows tell by themselves."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    w = _workspaces.get((dev.index, _raw_stream(dev.index)))
+    if w is not None:
+        with _on(dev):
+            _cuda.kv4_attention_status_ptr(w.data_ptr(), _raw_stream(dev.index))
+
+
 def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, scale=None, window: int = 0, out=None,
                     return_lse: bool = False):
     """Causal attention of q [tokens, heads, dim] over the 4-bit cache.
@@ -525,6 +537,7 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
             most_new = tokens
     if window < 0:
         raise ValueError(f"{who}: window must not be negative")
+    window, most_new = min(window, 0x7FFFFFFF), min(most_new, 0x7FFFFFFF)
     dev = q.device
     s = _on_device(who, dev, codes, scales, table, lens, starts, out)
     with _on(dev):

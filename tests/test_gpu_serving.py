@@ -543,3 +543,35 @@ def test_refusals(S):
     with pytest.raises(ValueError):
         _cuda.kv4_attention_ptr(0, x.data_ptr(), 128, 64, 2, 2, 96, c.codes.data_ptr(), c.scales.data_ptr(), 2, 16, 2,
                                 table.data_ptr(), 2, 2, lens.data_ptr(), 2, 0, 1, 1.0, 0, x.data_ptr(), 0, 0, 0)
+
+
+def test_served_block_example(S):
+    """The example's prompts, decoding, release and reuse over folded sparse projections (fp32 throughout)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_folded_attention.py")
+    spec = importlib.util.spec_from_file_location("serve_folded_attention", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    block, worst = mod.main(["--check", "--decode", "8"])
+    assert block.lens.tolist() == [37 + 9, 30 + 4, 0, 64 + 9]
+    held = block.table[block.table >= 0].tolist()
+    assert len(held) == len(set(held)) == sum(-(-n // 16) for n in block.lens.tolist())
+    assert worst <= 2e-6        # fp32: a few units of 2^-24 in logits of size ~10 and in the sums
+
+
+def test_rotary_wide_heads_off_alignment(S):
+    """More pairs than a CTA of the aligned path has threads."""
+    g = _gen(30)
+    cos, sin = S.rotary_table(9, 1000)
+    x = torch.randn(3, 2 * 1024 + 1, generator=g, device="cuda")[:, 1:].view(3, 2, 1024)
+    pos = torch.tensor([0, 3, 8], device="cuda")
+    for layout in ("half", "interleaved"):
+        got = S.rotary(x, None, cos, sin, pos, layout=layout)[0]
+        assert torch.equal(got, S.rotary(x.contiguous(), None, cos, sin, pos, layout=layout)[0])
+    with pytest.raises(ValueError):
+        S.rotary(torch.zeros(3, 1, 1026, device="cuda"), None, cos, sin, pos)
+
+
+def test_check_attention_is_quiet(S):
+    S.check_attention()
