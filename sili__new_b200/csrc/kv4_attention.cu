@@ -484,20 +484,26 @@ struct Attend {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) f[i][q] = mul2(f[i][q], sb);
                 }
+                // (fp32: two steps at a time, small terms first, added outside the matrix unit, which cuts: see below)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int n = 0; n < NT; ++n) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int q = kTerms - 1; q >= 0; --q)
 #pragma unroll
-                        for (int q = 0; q < kTerms; ++q) {
+                        for (int k = 0; k < 2; ++k) {
                             uint32_t b0, b1;
                             if (!kShared) { b0 = qf[kShared ? 0 : 2 * j + k][q][0]; b1 = qf[kShared ? 0 : 2 * j + k][q][1]; }
                             else {
                                 const uint2 b = ((const uint2*)qs)[((n * kSteps + 2 * j + k) * kTerms + q) * 32 + lane];
                                 b0 = b.x; b1 = b.y;
                             }
-                            mma(x[n], f[0][2 * k], f[1][2 * k], f[0][2 * k + 1], f[1][2 * k + 1], b0, b1);
+                            mma(kTerms == 1 ? x[n] : sum, f[0][2 * k], f[1][2 * k], f[0][2 * k + 1], f[1][2 * k + 1], b0, b1);
                         }
+                    if (kTerms == 2)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[n][k] += sum[k];
+                }
             }
         }
         // exponents over the running maximum
@@ -587,8 +593,17 @@ struct Attend {
                                    a3 = mul2(f[3][q], s23);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
+                        if (kTerms == 1) {
+                            mma(o[4 * j + q][n], a0, a1, a2, a3, p[n][0][0], p[n][0][1]);
+                        } else {
+                            // The matrix unit cuts what it adds to its accumulator, always towards zero: over a few
+                            // hundred tiles that is 3e-6 of O.  So fp32's tiles are added outside, rounded.
+                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma(sum, a0, a1, a2, a3, p[n][kTerms - 1][0], p[n][kTerms - 1][1]);
+                            mma(sum, a0, a1, a2, a3, p[n][0][0], p[n][0][1]);
 #pragma unroll
-                        for (int k = 0; k < kTerms; ++k) mma(o[4 * j + q][n], a0, a1, a2, a3, p[n][k][0], p[n][k][1]);
+                            for (int k = 0; k < 4; ++k) o[4 * j + q][n][k] += sum[k];
+                        }
                 }
             }
         }
