@@ -6,7 +6,9 @@ and the policy siblings ``SparseLinearLayerNoScale`` /
 ``SparseLinearLayerNoScaleDeterministic`` / ``SparseLinearLayerResync`` /
 ``SparseLinearLayerResyncDeterministic``, with the same method surface, plus the module functions ``dense_to_csr``,
 ``dense_to_top_k_csr``, ``fp4_quantize_array``, ``seed_fp4_stochastic_rng``,
-``csr_union`` and the banded / sparse attention functions.
+``csr_union`` and the banded / sparse attention functions.  Serving a folded
+stack (page tables, rotary positions, the 4-bit cache and its attention) is in
+``sili__new_b200.serving``, imported by itself (it needs torch).
 All compute runs in ``libsili_b200.so`` (CUDA kernels behind the C ABI of
 ``include/sili_b200.h``); there is no CPU path.  Importing fails loudly when
 the extension has not been built (``python -m sili__new_b200.build``).

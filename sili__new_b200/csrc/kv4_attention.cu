@@ -28,6 +28,15 @@
 // not depend on which that is.  Warps take 16 keys each (within one page) and
 // keep a ring of cp.async stages; the page of the next tile is fetched one
 // step ahead.
+//
+// What bounds it, 96 requests of 2k-16k keys, 32 heads over 8, dim 128, bf16
+// (0.96 GB, 146 us at the card's copy rate): 279 us, 3.4 TB/s.  A warp's 16
+// keys x 136 bytes take about 425 instructions, 266 of them the tile's own
+// (64 conversions at half rate, 64 scalings, 16 products, the softmax); the
+// schedulers issue two of three cycles with 16 warps an SM, which registers
+// (128 a thread) and the ring (104 KB a CTA) allow.  With 8 warps an SM and a
+// longer ring it took 389 us; with bulk copies by one lane in place of
+// cp.async by all, 355 against 325 at the time.
 #include <cuda_runtime.h>
 
 #include <algorithm>
