@@ -456,9 +456,30 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
     const RotaryArgs& r = a.r;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes;
     const int64_t t = blockIdx.x;
-    const int nq = r.heads[0], nk = r.heads[1], rows = nq + 2 * nk;
+    const int nq = r.heads[0], nk = r.heads[1];
     const int half = r.rot / 2, e = sub * 8;
     const bool turns = e < r.rot;
+    const T* const qs = (const T*)r.x[0] + t * r.xt[0] + e;
+    T* const qo = (T*)r.y[0] + t * r.yt[0] + e;
+    const T* const ks = (const T*)r.x[1] + t * r.xt[1] + e;
+    const T* const vs = (const T*)a.v + t * a.vt + e;
+    const int first = (blockIdx.y * kWarps + warp) * kRows + lane / kLanes, step = kWarps * kRows * gridDim.y;
+    using In = union { uint32_t u[kWord]; Pack<T, 8> p; uint4 v[kWord / 4]; };
+    auto fetch = [&](const T* src, bool active) {
+        In in;
+#pragma unroll
+        for (int i = 0; i < kWord / 4; ++i) in.v[i] = active ? __ldg((const uint4*)src + i) : make_uint4(0, 0, 0, 0);
+        return in;
+    };
+    constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;     // q rows whose loads are in flight together
+    In batch[kBatch];
+    auto fetch_q = [&](int h0) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) batch[k] = fetch(qs + (h0 + k * step) * r.xh[0], h0 + k * step < nq);
+    };
+    // before the position and the table's row, which wait for one another
+    fetch_q(first);
+    const int64_t slot = a.slots[t];
     const int64_t pos = r.rot ? load_position(r.positions, r.pos64, t) : 0;
     const bool pad = pos < 0, past = r.rot && pos >= r.n_positions;
     const float blank = pad ? 0.f : __int_as_float(0x7FC00000);
@@ -483,63 +504,60 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
         }
     }
     const int partner = (lane - sub) + ((e < half ? e + half : e - half) / 8 & (kLanes - 1));
-    const int64_t slot = a.slots[t];
     const bool stored = slot >= 0 && slot < a.n_slots;
     int off;
     const int64_t pg = split_slot(stored ? slot : 0, a.n_slots, a.page, off);
     const int64_t row_at = pg * (2 * (int64_t)nk * a.page) + off;     // K's row of kv head 0
-    const T* const src0 = (const T*)r.x[0] + t * r.xt[0] + e;
-    const T* const src1 = (const T*)r.x[1] + t * r.xt[1] + e;
-    const T* const src2 = (const T*)a.v + t * a.vt + e;
-#pragma unroll 2
-    for (int row0 = (blockIdx.y * kWarps + warp) * kRows; row0 < rows; row0 += kWarps * kRows * gridDim.y) {
-        const int row = row0 + lane / kLanes;
-        const int w = row < nq ? 0 : row < nq + nk ? 1 : 2;
-        const int h = w == 0 ? row : w == 1 ? row - nq : row - nq - nk;
-        const bool active = row < rows && (w == 0 || stored);
-        union { uint32_t u[kWord]; Pack<T, 8> p; uint4 v[kWord / 4]; } in;
-#pragma unroll
-        for (int i = 0; i < kWord / 4; ++i) in.v[i] = make_uint4(0, 0, 0, 0);
-        if (active) {
-            const T* src = w == 0 ? src0 + h * r.xh[0] : w == 1 ? src1 + h * r.xh[1] : src2 + h * a.vh;
-#pragma unroll
-            for (int i = 0; i < kWord / 4; ++i) in.v[i] = __ldg((const uint4*)src + i);
-        }
-        float x[8];
+    // the row's eight values, turned where `turn` says so (every lane of the warp comes here together)
+    auto turned = [&](const In& in, bool turn, float (&x)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = sili::to_f32(in.p.v[i]);
-        if (r.rot) {
-            if (r.interleaved) {
-                if (turns && w < 2) {
+        if (!r.rot) return;
+        if (r.interleaved) {
+            if (turns && turn) {
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const float f = x[i], g = x[i + 1];
-                        x[i] = __fsub_rn(__fmul_rn(f, c[i]), __fmul_rn(g, s[i]));
-                        x[i + 1] = __fadd_rn(__fmul_rn(g, c[i]), __fmul_rn(f, s[i]));
-                    }
-                }
-            } else {
-                union { uint32_t u[kWord]; Pack<T, 8> p; } other;
-#pragma unroll
-                for (int i = 0; i < kWord; ++i) other.u[i] = __shfl_sync(0xffffffffu, in.u[i], partner);
-                if (turns && w < 2) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(sili::to_f32(other.p.v[i]), s[i]));
+                for (int i = 0; i < 8; i += 2) {
+                    const float f = x[i], g = x[i + 1];
+                    x[i] = __fsub_rn(__fmul_rn(f, c[i]), __fmul_rn(g, s[i]));
+                    x[i + 1] = __fadd_rn(__fmul_rn(g, c[i]), __fmul_rn(f, s[i]));
                 }
             }
-            if ((pad || past) && w < 2) {
+        } else {
+            In other;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = blank;
+            for (int i = 0; i < kWord; ++i) other.u[i] = __shfl_sync(0xffffffffu, in.u[i], partner);
+            if (turns && turn) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(sili::to_f32(other.p.v[i]), s[i]));
             }
         }
-        if (w == 0) {
+        if ((pad || past) && turn) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = blank;
+        }
+    };
+    float x[8];
+    for (int h0 = first; h0 - lane / kLanes < nq;) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int h = h0 + k * step;
+            if (h - lane / kLanes >= nq) break;        // (the same for the whole warp)
+            turned(batch[k], true, x);
             Pack<T, 8> o;
 #pragma unroll
             for (int i = 0; i < 8; ++i) o.v[i] = sili::from_f32<T>(x[i]);
-            if (active) *(Pack<T, 8>*)((T*)r.y[0] + t * r.yt[0] + h * r.yh[0] + e) = o;
+            if (h < nq) *(Pack<T, 8>*)(qo + h * r.yh[0]) = o;
         }
-        if (row0 + kRows <= nq) continue;      // q rows only: nothing to quantise (the same for the whole warp)
+        h0 += kBatch * step;
+        if (h0 - lane / kLanes < nq) fetch_q(h0);
+    }
+    if (!stored) return;
+#pragma unroll 2
+    for (int row = first; row - lane / kLanes < 2 * nk; row += step) {      // K's rows, then V's
+        const bool is_v = row >= nk, active = row < 2 * nk;
+        const int h = is_v ? row - nk : row;
+        turned(fetch(is_v ? vs + h * a.vh : ks + h * r.xh[1], active), !is_v, x);
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
@@ -550,8 +568,8 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
         uint32_t packed = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) packed |= th.code(x[i]) << (4 * i);
-        if (active && w) {
-            const int64_t at = row_at + ((int64_t)(w - 1) * nk + h) * a.page;
+        if (active) {
+            const int64_t at = row_at + (int64_t)row * a.page;       // V's rows follow K's nk heads
             *(uint32_t*)(a.codes + at * (D / 2) + sub * 4) = packed;
             if (sub % 4 == 0) a.scales[at * (D / 32) + sub / 4] = (uint8_t)b;
         }
@@ -747,7 +765,7 @@ int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_
                  v, v_token_stride, v_head_stride, codes, scales, n_pages * page, page, slots};
     cudaStream_t s = (cudaStream_t)stream;
     const int per = kAppendThreads / 32 * (256 / dim);       // rows a pass of a CTA
-    const int passes = (q_heads + 2 * kv_heads + per - 1) / per;
+    const int passes = (std::max(q_heads, 2 * kv_heads) + per - 1) / per;
     const dim3 grid((unsigned)tokens, (unsigned)std::max<int64_t>(1, std::min<int64_t>(passes, 592 / tokens)));
     auto go = [&](auto kernel) {
         kernel<<<grid, kAppendThreads, 0, s>>>(a);
