@@ -315,10 +315,13 @@ __device__ __forceinline__ int64_t load_position(const void* p, int pos64, int64
 // elements) or V elements that pass through; a thread keeps its unit and so
 // its cosines while it walks the heads.  Bound by HBM: each value is read and
 // written once.  8191 tokens of 32 + 8 heads x 128 in fp32, forward and
-// gradient: 148 us, 4.6 TB/s; few tokens are spread over several CTAs each, a
+// gradient: 131 us, 5.1 TB/s (whole heads turned, 16001 tokens: 6.1 TB/s; in
+// bf16 4.2).  The fp32 form is held to 32 registers: with 8 CTAs an SM in
+// place of 5 it took 131 us for 148; the 16-bit one keeps its registers (80
+// us against 113 with 8).  Few tokens are spread over several CTAs each, a
 // call of 64 tokens is its launch (19 us with the host's side).
 template <typename T, int V>
-__global__ void __launch_bounds__(V == 1 ? 1024 : 256) k_rotary(RotaryArgs a, int units, int rot_units, int rows) {
+__global__ void __launch_bounds__(V == 1 ? 1024 : 256, V == 1 || sizeof(T) == 2 ? 1 : 8) k_rotary(RotaryArgs a, int units, int rot_units, int rows) {
     using P = Pack<T, V>;
     const int u = threadIdx.x % units, row = threadIdx.x / units;
     if (row >= rows) return;
@@ -380,10 +383,10 @@ void launch_rotary(const RotaryArgs& a, cudaStream_t s) {
     const int rot_units = a.interleaved ? (V > 1 ? a.rot / V : a.rot / 2) : a.rot / 2 / V;
     const int units = rot_units + (a.dim - a.rot) / V;
     const int heads = a.heads[0] + a.heads[1];
-    const int rows = std::max(1, std::min(heads, 256 / units));
-    const int threads = (rows * units + 31) / 32 * 32;
+    // as many heads side by side as 256 threads hold, evened out over the passes that all heads then take
+    const int fit = std::max(1, std::min(heads, 256 / units)), passes = (heads + fit - 1) / fit;
+    const int rows = (heads + passes - 1) / passes, threads = (rows * units + 31) / 32 * 32;
     // few tokens: more CTAs a token, so that every SM has some (one head a thread at the extreme)
-    const int passes = (heads + rows - 1) / rows;
     const int split = (int)std::max<int64_t>(1, std::min<int64_t>(passes, 592 / std::max<int64_t>(a.tokens, 1)));
     k_rotary<T, V><<<dim3((unsigned)a.tokens, split), threads, 0, s>>>(a, units, rot_units, rows);
     sili::count_launch();
@@ -446,10 +449,10 @@ constexpr int kAppendThreads = 128;
 // (rot % 16 == 0), and comes by shuffle.  A CTA's warps share one token and
 // walk its q, k and v rows with the token's cosines in registers.  Bound by
 // instructions (the codes: three comparisons a value) before HBM: 16384
-// tokens of 32 + 2 x 8 heads x 128 in bf16 take 132 us, 2.6 TB/s, and the
-// read-back below 24 us.
+// tokens of 32 + 2 x 8 heads x 128 in bf16 take 111 us (8 CTAs an SM: 64
+// registers; 127 us with 5), 3.1 TB/s, and the read-back below 24 us.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 8) k_kv4_append(const __grid_constant__ AppendArgs a) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes;     // lanes a row, rows a warp
     constexpr int kWarps = kAppendThreads / 32;
     constexpr int kWord = sizeof(T) == 2 ? 4 : 8;          // 32-bit words of a lane's elements

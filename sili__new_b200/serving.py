@@ -47,12 +47,15 @@ _I32, _I64, _U8, _F32 = torch.int32, torch.int64, torch.uint8, torch.float32
 
 def _on_device(who, dev, *arrays):
     """The current stream's handle of the CUDA device that every array is on."""
+    at = dev.index
+    for a in arrays:
+        if a is not None and (a.get_device() != at or not a.is_cuda):
+            if not a.is_cuda or dev.type != "cuda":
+                raise ValueError(f"{who}: arrays must be CUDA tensors")
+            raise ValueError(f"{who}: arrays are on different devices")
     if dev.type != "cuda":
         raise ValueError(f"{who}: arrays must be CUDA tensors")
-    for a in arrays:
-        if a is not None and a.device != dev:
-            raise ValueError(f"{who}: arrays are on different devices")
-    return _raw_stream(dev.index)
+    return _raw_stream(at)
 
 
 class _Here:
@@ -68,7 +71,7 @@ _HERE = _Here()
 
 def _on(dev):
     """Context that makes `dev` the current device (nothing to do where it is already)."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _contiguous(who, name, t, dtype, shape=None):
@@ -269,16 +272,20 @@ def rotary_table(n_positions: int, rotary_dim: int, base: float = 10000.0, scali
 
 
 def _check_table(who, cos, sin, positions, tokens, dim):
-    if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] < 1:
-        raise ValueError(f"{who}: cos must be [positions, rotary_dim / 2], got {list(cos.shape)}")
-    _contiguous(who, "cos", cos, torch.float32)
-    _contiguous(who, "sin", sin, torch.float32, tuple(cos.shape))
-    if 2 * cos.shape[1] > dim:
-        raise ValueError(f"{who}: the table turns {2 * cos.shape[1]} elements, the head has {dim}")
-    if positions.dtype not in (torch.int32, torch.int64):
+    shape = cos.shape
+    if len(shape) == 2 and shape[0] >= 1 and 2 <= 2 * shape[1] <= dim and cos.dtype is _F32 and sin.dtype is _F32 and \
+            sin.shape == shape and cos.is_contiguous() and sin.is_contiguous() and \
+            positions.dtype in (_I32, _I64) and positions.shape == (tokens,) and positions.is_contiguous():
+        return
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"{who}: cos must be [positions, rotary_dim / 2], got {list(shape)}")
+    _contiguous(who, "cos", cos, _F32)
+    _contiguous(who, "sin", sin, _F32, tuple(shape))
+    if 2 * shape[1] > dim:
+        raise ValueError(f"{who}: the table turns {2 * shape[1]} elements, the head has {dim}")
+    if positions.dtype not in (_I32, _I64):
         raise ValueError(f"{who}: positions must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) != (tokens,) or not positions.is_contiguous():
-        raise ValueError(f"{who}: positions must be a contiguous [{tokens}], got {list(positions.shape)}")
+    raise ValueError(f"{who}: positions must be a contiguous [{tokens}], got {list(positions.shape)}")
 
 
 def _interleaved(who, layout):
@@ -387,12 +394,19 @@ class KVCache4:
 
 
 def _check_cache(who, codes, scales):
-    if codes.dim() != 5 or codes.shape[1] != 2 or 2 * codes.shape[4] not in HEAD_DIMS:
+    shape = codes.shape
+    if len(shape) == 5:
+        n_pages, two, hk, page, half = shape
+        if two == 2 and 2 * half in HEAD_DIMS and codes.dtype is _U8 and scales.dtype is _U8 and \
+                scales.shape == (n_pages, 2, hk, page, half // (GROUP // 2)) and codes.is_contiguous() and \
+                scales.is_contiguous():
+            return n_pages, hk, page, 2 * half
+    if len(shape) != 5 or shape[1] != 2 or 2 * shape[4] not in HEAD_DIMS:
         raise ValueError(f"{who}: codes must be [pages, 2, kv heads, page, dim / 2] with dim in {HEAD_DIMS}, "
-                         f"got {list(codes.shape)}")
-    _contiguous(who, "codes", codes, torch.uint8)
-    _contiguous(who, "scales", scales, torch.uint8, (*codes.shape[:4], codes.shape[4] // (GROUP // 2)))
-    return codes.shape[0], codes.shape[2], codes.shape[3], 2 * codes.shape[4]
+                         f"got {list(shape)}")
+    _contiguous(who, "codes", codes, _U8)
+    _contiguous(who, "scales", scales, _U8, (*shape[:4], shape[4] // (GROUP // 2)))
+    return shape[0], shape[2], shape[3], 2 * shape[4]
 
 
 def _check_slots(who, slots, tokens):
