@@ -30,7 +30,7 @@
 // step ahead.
 //
 // What bounds it, 96 requests of 2k-16k keys, 32 heads over 8, dim 128, bf16
-// (0.96 GB, 146 us at the card's copy rate): 279 us, 3.4 TB/s.  A warp's 16
+// (0.96 GB, 146 us at the card's copy rate): 276 us, 3.5 TB/s.  A warp's 16
 // keys x 136 bytes take about 425 instructions, 266 of them the tile's own
 // (64 conversions at half rate, 64 scalings, 16 products, the softmax); the
 // schedulers issue two of three cycles with 16 warps an SM, which registers

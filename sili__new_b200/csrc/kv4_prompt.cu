@@ -18,8 +18,8 @@
 // be read and written back then.
 //
 // What bounds it, 3 chunks of about 2000 tokens over 4.7k-6.6k keys, 32 heads
-// over 8, dim 128, bf16 (464 GFLOP, 281 us at the card's matrix rate): 702 us,
-// 660 TFLOP/s.  No unit is full (tensor pipe 32 %, exponentials 33 %, issue
+// over 8, dim 128, bf16 (464 GFLOP, 281 us at the card's matrix rate): 693 us,
+// 670 TFLOP/s.  No unit is full (tensor pipe 32 %, exponentials 33 %, issue
 // 50 %; leaving out half the P V products changes nothing, all
 // dequantisation 7 %): a step is the softmax warps' chain of about 2600
 // clocks for 64 keys (scores' barrier, tensor-memory load, maximum,

@@ -523,7 +523,7 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
     request r's queries are rows starts[r] .. starts[r + 1), at its last
     positions; without it row r is request r's one query.  ``most_new``: the
     largest number of queries of a request, if the host knows it (it picks the
-    kernel, not the result).  ``window`` > 0: only the last so many keys.
+    kernel, not the result; without it the mean is taken).  ``window`` > 0: only the last so many keys.
     ``scale``: 1 / sqrt(dim) by default.  Grouped queries: query head h reads
     kv head h // (heads / kv heads).  Rows that see nothing (no keys, or past
     the last request's) are zeros, their lse -inf.  Returns ``out`` [tokens,
@@ -548,7 +548,7 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
     else:
         _contiguous(who, "starts", starts, torch.int32, (requests + 1,))
         if most_new is None:
-            most_new = tokens
+            most_new = -(-tokens // max(requests, 1))
     if window < 0:
         raise ValueError(f"{who}: window must not be negative")
     window, most_new = min(window, 0x7FFFFFFF), min(most_new, 0x7FFFFFFF)
