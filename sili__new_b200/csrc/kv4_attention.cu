@@ -252,7 +252,9 @@ struct Attend {
     const int lane, warp, g, t;
     uint8_t* ring;         // this warp's stages
     uint32_t ring_at;
-    int* flags;            // per stage: the tile holds keys
+    uint32_t held = 0;     // a bit a stage: its tile holds keys
+    float* s_cf;           // the row tiles' logit factors (q_shared)
+    int step_pages, step_off;   // a unit of keys in table entries and rows
     float* join;
     uint32_t* qs;          // Q fragments in shared memory (kShared)
 
@@ -264,11 +266,13 @@ struct Attend {
     int to[NT][2], from[NT][2];        // the columns' keys [from, to)
     int any_from, any_to, all_from, all_to;   // keys that any of the rows sees, that every row sees
 
-    __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, int* all_flags)
+    __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, float* factors)
         : a(args), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
         ring = smem + warp * (kStages * L::kStage);
         ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-        flags = all_flags + warp * kStages;
+        s_cf = factors;
+        step_pages = kUnit / a.page;
+        step_off = kUnit - step_pages * a.page;
         join = (float*)(smem + L::kRing);
         qs = (uint32_t*)(smem + L::kRing + L::kJoin);
     }
@@ -288,24 +292,26 @@ struct Attend {
         Cur c;
         int key0, left, len;     // the next tile's first key, the segment's tiles from there on, the request's keys
         int page, off;           // its page (-1: none) and place in it
-        const int* pages;        // the request's row of the table
+        const int* entry;        // its entry in the table
         const uint8_t *codes, *scales;   // the kv head's first K row of page 0, and this lane's 16 bytes
     };
     __device__ __forceinline__ void look(Loader& d) const {
-        d.page = -1;
-        if (d.key0 < d.len) d.page = __ldg(d.pages + a.column(d.key0, d.off));
+        d.page = d.key0 < d.len ? __ldg(d.entry) : -1;
     }
     __device__ __forceinline__ void enter(Loader& d) const {
         d.key0 = d.c.u * kUnit + warp * 16;
         d.left = d.c.left();
         d.len = d.c.q.len;
-        d.pages = a.table + d.c.r * a.stride;
+        d.entry = a.table + d.c.r * a.stride + a.column(d.key0, d.off);
         const int64_t rows = (int64_t)d.c.h * a.page;
         d.codes = a.codes + rows * L::kRowBytes + lane * 16;
         d.scales = a.scales + rows * E + (lane % (L::kScales / 16)) * 16;
     }
     __device__ __forceinline__ void step(Loader& d, bool more) const {
         d.key0 += kUnit;
+        d.entry += step_pages;
+        d.off += step_off;
+        if (d.off >= a.page) { d.off -= a.page; ++d.entry; }
         if (--d.left == 0 && more) {
             d.c.next_segment(a);
             enter(d);
@@ -318,7 +324,7 @@ struct Attend {
         const bool there = (unsigned)d.page < (unsigned)a.n_pages;
         if (there) {
             // (the host has checked that a page's bytes fit 31 bits)
-            const uint32_t half = (uint32_t)a.kv_heads * a.page;     // token rows of K, and of V, in a page
+            const uint32_t half = a.half_rows;
             const uint8_t* k = d.codes + (uint64_t)(uint32_t)d.page * (2 * half * L::kRowBytes) + d.off * L::kRowBytes;
             const uint8_t* v = k + half * L::kRowBytes;
             const uint32_t at = ring_at + s * L::kStage;
@@ -338,7 +344,7 @@ struct Attend {
                 cp16(at + 2 * L::kCodes + lane * 16, lane >= kSc ? p + half * E : p);
             }
         }
-        if (lane == 0) flags[s] = there;
+        held = there ? held | 1u << s : held & ~(1u << s);
     }
 
     __device__ __forceinline__ void begin_segment(const Cur& c) {
@@ -404,7 +410,6 @@ struct Attend {
                 cf[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
                 cf[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
                 if (kShared) {
-                    float* s_cf = (float*)flags - warp * kStages + kWarps * kMaxStages;
                     if (t == 0) s_cf[n * 8 + g] = back;
                 }
             }
@@ -417,7 +422,6 @@ struct Attend {
         }
         if (kShared) {
             __syncthreads();
-            const float* s_cf = (const float*)flags - warp * kStages + kWarps * kMaxStages;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -455,7 +459,7 @@ struct Attend {
     }
 
     __device__ __forceinline__ void tile(int key0, int s) {
-        if (!flags[s] || key0 >= any_to || key0 + 16 <= any_from) return;
+        if (!(held >> s & 1) || key0 >= any_to || key0 + 16 <= any_from) return;
         const uint8_t* st = ring + s * L::kStage;
         const int ka = key_of(g);
         float x[NT][4];
@@ -786,14 +790,14 @@ __device__ void blank_rows(const AttendArgs& a, int dim) {
 template <typename T, int E, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_attend(const __grid_constant__ AttendArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_flags[kWarps * kMaxStages + 8 * 4];   // stages' flags, then the row tiles' logit factors
+    __shared__ float s_factors[8 * 4];
     __shared__ int s_last;
     blank_rows<T>(a, 32 * E);
     Cursor<8 * NT> c;
     int64_t begin, end;
     const int64_t all = locate<8 * NT>(a, c, blockIdx.x, gridDim.x, begin, end);
     if (begin >= end) return;
-    Attend<T, E, NT> k(a, smem, s_flags);
+    Attend<T, E, NT> k(a, smem, s_factors);
     k.run(c, begin, end, all, &s_last);
 }
 
@@ -870,7 +874,8 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
         return bad(who, "q rows must be 8-byte aligned");
     AttendArgs a{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
                  table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
-                 (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16))};
+                 (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16)),
+                 (uint32_t)(kv_heads * page)};
     cudaStream_t s = (cudaStream_t)stream;
     if (starts && sili::kv4_prompt_takes(dtype, dim, tokens, heads, kv_heads, most_new))
         return sili::kv4_prompt_launch(dtype, dim, a, s);
