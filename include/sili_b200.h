@@ -484,7 +484,8 @@ int sili_rotary(int dtype, const void* q, int64_t q_token_stride, int64_t q_head
  *
  * append: K (rotated first when rot > 0, rot a multiple of 16) and V of each
  * token into its slot; slots outside [0, n_pages * page) are passed over; two
- * tokens must not share one.  With q_heads > 0, q_out gets the rotated q. */
+ * tokens must not share one.  With q_heads > 0, q_out (which may be q) gets the
+ * rotated q. */
 int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
                     int64_t qo_token_stride, int64_t qo_head_stride, int q_heads, const void* k, int64_t k_token_stride,
                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int kv_heads,

@@ -30,13 +30,15 @@
 // step ahead.
 //
 // What bounds it, 96 requests of 2k-16k keys, 32 heads over 8, dim 128, bf16
-// (0.96 GB, 146 us at the card's copy rate): 276 us, 3.5 TB/s.  A warp's 16
-// keys x 136 bytes take about 425 instructions, 266 of them the tile's own
+// (0.96 GB, 146 us at the card's copy rate): 271 us, 3.5 TB/s.  A warp's 16
+// keys x 136 bytes take about 400 instructions, 266 of them the tile's own
 // (64 conversions at half rate, 64 scalings, 16 products, the softmax); the
 // schedulers issue two of three cycles with 16 warps an SM, which registers
 // (128 a thread) and the ring (104 KB a CTA) allow.  With 8 warps an SM and a
 // longer ring it took 389 us; with bulk copies by one lane in place of
-// cp.async by all, 355 against 325 at the time.
+// cp.async by all, 355 against 325 at the time.  A few short requests (4, up
+// to 700 keys) are a chain of latencies, 15 us: lengths, query, page, keys, the
+// join of the parts (with at least 4 units a CTA in place of 1: 18 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kAppendThreads, 8) k_kv4_append(const __grid_c
     auto fetch = [&](const T* src, bool active) {
         In in;
 #pragma unroll
-        for (int i = 0; i < kWord / 4; ++i) in.v[i] = active ? __ldg((const uint4*)src + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kWord / 4; ++i) in.v[i] = active ? ((const uint4*)src)[i] : make_uint4(0, 0, 0, 0);
         return in;
     };
     constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;     // q rows whose loads are in flight together

@@ -332,7 +332,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, positions, layout):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.layout, ctx.has_k = layout, k is not None
+        ctx.layout = layout
         return _turn("rotary", q, k, cos, sin, positions, layout, False, None, None)
 
     @staticmethod
@@ -422,7 +422,7 @@ def cache_append(k, v, codes, scales, slots, cos=None, sin=None, positions=None,
     no two tokens may share one), in one launch with the rotation of k, and of
     ``q`` when given, by ``positions`` (see ``rotary``; the rotated part a
     multiple of 16).  Head rows start on 16 bytes (any strides otherwise).
-    Returns the rotated q (None without q)."""
+    Returns the rotated q (None without q; ``q_out`` may be q itself)."""
     who = "cache_append"
     n_pages, hk, page, dim = _check_cache(who, codes, scales)
     code = _dtype_code(k, who)

@@ -575,3 +575,24 @@ def test_rotary_wide_heads_off_alignment(S):
 
 def test_check_attention_is_quiet(S):
     S.check_attention()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_turns_q_in_place(S, dtype):
+    g = _gen(31)
+    cos, sin = S.rotary_table(64, 128)
+    pos = torch.randint(0, 64, (50,), generator=g, device="cuda")
+    q = torch.randn(50, 41, 128, generator=g, device="cuda").to(dtype)
+    k = torch.randn(50, 3, 128, generator=g, device="cuda").to(dtype)
+    c = S.KVCache4(4, 16, 3, 128)
+    slots = torch.arange(50, device="cuda")
+    want = S.cache_append(k, k, c.codes, c.scales, slots, cos=cos, sin=sin, positions=pos, q=q)
+    assert S.cache_append(k, k, c.codes, c.scales, slots, cos=cos, sin=sin, positions=pos, q=q, q_out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_attention_without_a_hint(S):
+    """most_new left out: the mean number of queries picks the kernel, the result stays."""
+    case = _attend_case([300, 40, 77], [40, 1, 1], 8, 2, 128, 16, torch.bfloat16, 32)
+    _check_attention(S, case, torch.bfloat16)
+    _check_attention(S, case, torch.bfloat16, most_new=40)
