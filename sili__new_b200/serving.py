@@ -507,7 +507,9 @@ def check_attention(device=None):
     """Raises RuntimeError if a device-side wait of an eager ``cache_attention``
     on the current stream gave up since the last check (its rows are NaN).
     Waits for the stream; a captured call's rows tell by themselves."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    dev = torch.device("cuda" if device is None else device)
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
     w = _workspaces.get((dev.index, _raw_stream(dev.index)))
     if w is not None:
         with _on(dev):
