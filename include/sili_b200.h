@@ -499,7 +499,8 @@ int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_
 /* Causal attention over the cache.  Request r's lens[r] tokens lie in the
  * pages table[r][0..]; its queries are the rows starts[r] .. starts[r + 1) of
  * q [tokens, heads, dim] and stand at its last positions (starts NULL: one
- * query a request, row r).  Query head h reads kv head h / (heads /
+ * query a request, row r); rows past `tokens`, as a step has them that brings
+ * more tokens than it has rows, are left out and move no other row.  Query head h reads kv head h / (heads /
  * kv_heads).  A query sees the keys up to its own position, with window > 0
  * only the last `window` of them; keys of a page that is not there (an entry
  * outside [0, n_pages)) are not seen.  out [tokens, heads, dim] =

@@ -146,13 +146,14 @@ __device__ __forceinline__ Req request(const AttendArgs& a, int r) {
     Req q;
     int64_t s0 = r, s1 = r + 1;
     if (a.starts) { s0 = a.starts[r]; s1 = a.starts[r + 1]; }
+    const int64_t past = s1;     // may lie beyond the rows of q: those that are there keep their positions
     s0 = min(max(s0, (int64_t)0), a.tokens);
     s1 = min(max(s1, s0), a.tokens);
     q.row0 = (int)s0;
     q.nq = (int)(s1 - s0);
     const int all = max(a.lens[r], 0);
     q.len = (int)min(min((int64_t)all, (int64_t)a.width * a.page), (int64_t)0x7FFFFF00);
-    q.pos0 = (int64_t)all - q.nq;
+    q.pos0 = all - (past - s0);
     const int64_t from = a.window ? max(q.pos0 - a.window + 1, (int64_t)0) : 0;
     q.k0 = (int)(from / kUnit);
     q.units = max((q.len + kUnit - 1) / kUnit - q.k0, 1);

@@ -196,12 +196,12 @@ struct Span {
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
     Span q;
     const int64_t s0 = min(max((int64_t)a.starts[r], (int64_t)0), a.tokens);
-    const int64_t s1 = min(max((int64_t)a.starts[r + 1], s0), a.tokens);
+    const int64_t past = a.starts[r + 1], s1 = min(max(past, s0), a.tokens);     // (rows that q lacks keep their positions)
     const int all = max(a.lens[r], 0);
     q.row0 = (int)s0;
     q.nq = (int)(s1 - s0);
     q.len = (int)min(min((int64_t)all, (int64_t)a.width * a.page), (int64_t)0x7FFFFF00);
-    q.pos0 = (int64_t)all - q.nq;
+    q.pos0 = all - (past - s0);
     q.pairs = (q.nq * (a.heads / a.kv_heads) + kTiles * kM - 1) / (kTiles * kM);
     return q;
 }

@@ -523,7 +523,8 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
     ``table`` int32 [requests, width] and ``lens`` int32 [requests] (cached
     plus new tokens) from ``page_tables``.  ``starts`` int32 [requests + 1]:
     request r's queries are rows starts[r] .. starts[r + 1), at its last
-    positions; without it row r is request r's one query.  ``most_new``: the
+    positions (rows that q does not have, beyond ``max_tokens``, are left out);
+    without it row r is request r's one query.  ``most_new``: the
     largest number of queries of a request, if the host knows it (it picks the
     kernel, not the result; without it the mean is taken).  ``window`` > 0: only the last so many keys.
     ``scale``: 1 / sqrt(dim) by default.  Grouped queries: query head h reads
