@@ -516,6 +516,12 @@ int sili_kv4_attention_workspace(int64_t* bytes);
  * workspace gave up since the last look (its rows are NaN), else SILI_OK;
  * waits for the stream. */
 int sili_kv4_attention_status(void* workspace, void* stream);
+/* How often such a wait looks, asleep for up to a millisecond each time,
+ * before it gives up: at most 4096 (which a negative number stands for, and
+ * which holds at first); output_polls for the last wait of a row tile, the one
+ * for its output.  0 gives up without a look.  For the calls of the process
+ * that follow; captured calls keep theirs. */
+int sili_kv4_attention_wait_limit(int polls, int output_polls);
 int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
                        int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads,
                        const int* table, int64_t table_stride, int width, const int* lens, int requests,

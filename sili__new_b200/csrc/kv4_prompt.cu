@@ -74,6 +74,7 @@ constexpr int kRegsSoftmax = 144, kRegsDequant = 72, kRegsRest = 48;
 static_assert(kSoftmax * kRegsSoftmax + kDequant * kRegsDequant + 128 * kRegsRest <= 96 * kThreads, "register split");
 constexpr int kMmaWarp = (kSoftmax + kDequant) / 32;
 constexpr int kPolls = 4096;          // polls of a wait, each asleep for up to kNap ns, before it gives up
+std::atomic<int> g_polls{kPolls}, g_output_polls{kPolls};     // sili_kv4_attention_wait_limit
 constexpr uint32_t kNap = 1000000;
 
 template <int D>
@@ -101,9 +102,9 @@ __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(addr(b)) : "memory");
 }
 // true when the phase of this parity is complete; false once any role has given up
-__device__ __forceinline__ bool bar_wait(unsigned long long* b, uint32_t parity, int* dead) {
+__device__ __forceinline__ bool bar_wait(unsigned long long* b, uint32_t parity, int* dead, int polls) {
     const uint32_t a = addr(b);
-    for (int i = 0; i < kPolls; ++i) {
+    for (int i = 0; i < polls; ++i) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -336,7 +337,7 @@ struct Prompt {
         for (int j = w.j0; j < w.last; ++j) {
             const int n = j - w.j0, st = n & 1;
             const bool more = j + 1 < w.last;
-            if (n >= 2 && !bar_wait(&s.kv_free[st], ((n >> 1) - 1) & 1, &s.dead)) return;
+            if (n >= 2 && !bar_wait(&s.kv_free[st], ((n >> 1) - 1) & 1, &s.dead, a.polls)) return;
             // K: rows are keys
             if (lane == 0) s.there[st][dw] = there;
             {
@@ -424,18 +425,18 @@ struct Prompt {
             commit(&s.s_full[t]);
         };
         if (mine > 0) {
-            if (!bar_wait(&s.kv_full[0], 0, &s.dead)) return;
+            if (!bar_wait(&s.kv_full[0], 0, &s.dead, a.polls)) return;
             asm volatile("tcgen05.fence::after_thread_sync;");
             scores(0);
         }
         for (int i = 0; i < mine; ++i) {
             if (i + 1 < mine) {
-                if (((i + 1) & 1) == 0 && !bar_wait(&s.kv_full[(i + 1) >> 1 & 1], (i + 1) >> 2 & 1, &s.dead)) return;
-                if (!bar_wait(&s.s_free[t], i & 1, &s.dead)) return;
+                if (((i + 1) & 1) == 0 && !bar_wait(&s.kv_full[(i + 1) >> 1 & 1], (i + 1) >> 2 & 1, &s.dead, a.polls)) return;
+                if (!bar_wait(&s.s_free[t], i & 1, &s.dead, a.polls)) return;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 scores(i + 1);
             }
-            if (!bar_wait(&s.p_full[t][i & 1], (i >> 1) & 1, &s.dead)) return;
+            if (!bar_wait(&s.p_full[t][i & 1], (i >> 1) & 1, &s.dead, a.polls)) return;
             asm volatile("tcgen05.fence::after_thread_sync;");
             const uint32_t v = v0 + (i >> 1 & 1) * kStage + (i & 1) * (D * 8);
 #pragma unroll
@@ -446,7 +447,7 @@ struct Prompt {
         }
         // the other tile's stages: this one is done with them as soon as they are filled
         for (int n = (mine + 1) >> 1; n < stages; ++n) {
-            if (!bar_wait(&s.kv_full[n & 1], (n >> 1) & 1, &s.dead)) return;
+            if (!bar_wait(&s.kv_full[n & 1], (n >> 1) & 1, &s.dead, a.polls)) return;
             bar_arrive(&s.kv_free[n & 1]);
         }
     }
@@ -525,7 +526,7 @@ struct Prompt {
         bool ok = true;
         for (int i = 0; i < w.n[t]; ++i) {
             const int j = w.j0 + (i >> 1), st = i >> 1 & 1, half = i & 1, key0 = j * kKeys + half * kSub;
-            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], i & 1, &s.dead));
+            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], i & 1, &s.dead, a.polls));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
             float x[kSub];
@@ -559,7 +560,7 @@ struct Prompt {
                 base = fresh;
                 l *= f;
                 if (i > 0) {
-                    ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead));
+                    ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead, a.polls));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     rescale(t, lanes, f);
@@ -591,7 +592,7 @@ struct Prompt {
         }
         const int steps = w.n[t];
         // (a barrier of its own: p_free may be one or two phases behind here, which a parity does not tell apart)
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], 0, &s.dead));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], 0, &s.dead, a.output_polls));
         asm volatile("tcgen05.fence::after_thread_sync;");
         // l 0: the row saw nothing
         float inv = l == 0.f ? 0.f : 1.f / l;
@@ -704,20 +705,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
         __syncthreads();       // Q is there
         const int t = warp - kMmaWarp;
-        if (w.last > w.j0 && t < kTiles && (threadIdx.x & 31) == 0) {
-            k.products(t);
-            // what was begun is waited for (bounded): the tensor memory is freed next
-            if (*(volatile int*)&s.dead) {
-                atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
-                int quiet = 0;
-                commit(&s.drained[t]);
-                bar_wait(&s.drained[t], 0, &quiet);
-            }
-        }
+        if (w.last > w.j0 && t < kTiles && (threadIdx.x & 31) == 0) k.products(t);
         __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
+    if (*(volatile int*)&s.dead) {     // (every role has left its loop: it is the same for all threads)
+        // Whichever role gave up: the products that a thread has queued may still run, so that thread waits for them
+        // (bounded) before the tensor memory is freed and the shared memory with it.
+        const int t = warp - kMmaWarp;
+        if (t >= 0 && t < kTiles && (threadIdx.x & 31) == 0) {
+            atomicOr((unsigned*)a.workspace + sili::kErrorWord, 1u);
+            int quiet = 0;
+            commit(&s.drained[t]);
+            bar_wait(&s.drained[t], 0, &quiet, kPolls);
+        }
+        __syncthreads();
+    }
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(512));
 }
 
@@ -749,9 +753,18 @@ bool kv4_prompt_takes(int dtype, int dim, int64_t tokens, int heads, int kv_head
     return dtype != SILI_F32 && (dim == 64 || dim == 128) && most_new * group >= 128 &&
            tokens * group / (kTiles * kM) * kv_heads >= 74;
 }
-int kv4_prompt_launch(int dtype, int dim, const AttendArgs& a, cudaStream_t s) {
+int kv4_prompt_launch(int dtype, int dim, const AttendArgs& args, cudaStream_t s) {
+    AttendArgs a = args;
+    a.polls = g_polls.load(std::memory_order_relaxed);
+    a.output_polls = g_output_polls.load(std::memory_order_relaxed);
     if (dtype == SILI_F16) return dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
     return dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
 }
 
 }  // namespace sili
+
+extern "C" int sili_kv4_attention_wait_limit(int polls, int output_polls) {
+    g_polls.store(polls < 0 ? kPolls : std::min(polls, kPolls), std::memory_order_relaxed);
+    g_output_polls.store(output_polls < 0 ? kPolls : std::min(output_polls, kPolls), std::memory_order_relaxed);
+    return SILI_OK;
+}

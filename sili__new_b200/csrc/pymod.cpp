@@ -829,6 +829,9 @@ PYBIND11_MODULE(_cuda, m) {
     m.def("kv4_attention_status_ptr", [](uintptr_t workspace, uintptr_t stream) {
         check(sili_kv4_attention_status((void*)workspace, (void*)stream));
     });
+    m.def("kv4_attention_wait_limit", [](int polls, int output_polls) {
+        check(sili_kv4_attention_wait_limit(polls, output_polls));
+    }, py::arg("polls") = -1, py::arg("output_polls") = -1);
     m.def("kv4_attention_workspace", []() {
         int64_t n = 0;
         check(sili_kv4_attention_workspace(&n));
