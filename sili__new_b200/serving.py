@@ -26,6 +26,7 @@ from typing import NamedTuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _cuda
 
@@ -329,24 +330,51 @@ def _turn(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out):
 
 
 class _Rotary(torch.autograd.Function):
+    """The turn is linear: its gradient is the turn back, its tangent the same turn, each differentiable in its turn."""
+
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, layout):
+    def forward(q, k, cos, sin, positions, layout, inverse):
+        return _turn("rotary", q, k, cos, sin, positions, layout, inverse, None, None)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, cos, sin, positions, ctx.layout, ctx.inverse = inputs
         ctx.save_for_backward(cos, sin, positions)
-        ctx.layout = layout
-        return _turn("rotary", q, k, cos, sin, positions, layout, False, None, None)
+        ctx.save_for_forward(cos, sin, positions)
+
+    @staticmethod
+    def _of_both(ctx, inverse, dq, dk):
+        """(dq, dk) turned; either may be None."""
+        cos, sin, positions = ctx.saved_tensors
+        grads = [None, None]
+        parts = [(i, g if g.stride(-1) == 1 else g.contiguous()) for i, g in enumerate((dq, dk)) if g is not None]
+        if parts:
+            out = _Rotary.apply(parts[0][1], parts[1][1] if len(parts) > 1 else None, cos, sin, positions, ctx.layout,
+                                inverse)
+            for (i, _), g in zip(parts, out):
+                grads[i] = g
+        return grads
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        if dq is None and dk is None:
-            return None, None, None, None, None, None
-        grads = [None, None]
-        parts = [(i, g if g.stride(-1) == 1 else g.contiguous()) for i, g in enumerate((dq, dk)) if g is not None]
-        out = _turn("rotary", parts[0][1], parts[1][1] if len(parts) > 1 else None, cos, sin, positions, ctx.layout,
-                    True, None, None)
-        for (i, _), g in zip(parts, out):
-            grads[i] = g
-        return grads[0], grads[1], None, None, None, None
+        return (*_Rotary._of_both(ctx, not ctx.inverse, dq, dk), None, None, None, None, None)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return tuple(_Rotary._of_both(ctx, ctx.inverse, tq, tk))
+
+
+def _is_dual(t):
+    return t is not None and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _rotary(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or \
+            forward_ad._current_level >= 0 and (_is_dual(q) or _is_dual(k)):
+        if q_out is not None or k_out is not None:
+            raise ValueError(f"{who}: an output array and a gradient exclude each other")
+        return _Rotary.apply(q, k, cos, sin, positions, layout, inverse)
+    return _turn(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out)
 
 
 def rotary(q, k, cos, sin, positions, layout: str = "half", q_out=None, k_out=None):
@@ -356,19 +384,15 @@ def rotary(q, k, cos, sin, positions, layout: str = "half", q_out=None, k_out=No
     (i, i + half) or adjacent ones.  ``cos`` / ``sin`` from ``rotary_table``;
     ``positions`` int32 or int64 [tokens]: a negative one (padding) gives
     zeros, one past the table NaN.  ``q_out`` / ``k_out`` may be the inputs
-    (in place).  Differentiable in q and k when no output is given.  Returns
-    (q', k')."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        if q_out is not None or k_out is not None:
-            raise ValueError("rotary: an output array and a gradient exclude each other")
-        return _Rotary.apply(q, k, cos, sin, positions, layout)
-    return _turn("rotary", q, k, cos, sin, positions, layout, False, q_out, k_out)
+    (in place).  Differentiable in q and k to any order, in reverse and forward
+    mode, when no output is given; not in the table.  Returns (q', k')."""
+    return _rotary("rotary", q, k, cos, sin, positions, layout, False, q_out, k_out)
 
 
 def rotary_backward(dq, dk, cos, sin, positions, layout: str = "half", q_out=None, k_out=None):
     """The gradient of ``rotary``: (dq, dk) of its outputs -> of its inputs
-    (the turn back by the same angles)."""
-    return _turn("rotary_backward", dq, dk, cos, sin, positions, layout, True, q_out, k_out)
+    (the turn back by the same angles); differentiable as ``rotary`` is."""
+    return _rotary("rotary_backward", dq, dk, cos, sin, positions, layout, True, q_out, k_out)
 
 
 # ── the 4-bit cache ──────────────────────────────────────────────────────────
