@@ -12,7 +12,9 @@ projections are this library's sparse layers goes::
 Everything stays on the device: no call reads a length back to the host, so a
 step can be captured in a CUDA graph.  All work is enqueued on torch's current
 stream of the arrays' device; arrays made on another stream are ordered by the
-caller, as for any torch operation.  fp32, fp16 and bf16 activations.
+caller, as for any torch operation.  fp32, fp16 and bf16 activations.  Rotary
+is differentiable; the cache's calls are not, and refuse inputs that ask for a
+gradient.
 
 The cache's format (``KVCache4``): groups of 32 values along the head share
 one scale byte (the upper byte below the sign of a half, amax / 6 rounded to
@@ -100,6 +102,20 @@ def _heads(who, name, t, tokens=None, dim=None, dtype=None):
         raise ValueError(f"{who}: {name} has head dimension {t.shape[2]}, expected {dim}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
+
+
+def _is_dual(t):
+    return t is not None and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _no_gradient(who, *arrays):
+    """Refuses inputs whose gradient or tangent the call would drop."""
+    if torch.is_grad_enabled():
+        for a in arrays:
+            if a is not None and a.requires_grad:
+                raise ValueError(f"{who}: has no gradient: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0 and any(_is_dual(a) for a in arrays):
+        raise ValueError(f"{who}: has no gradient: its inputs must not carry a tangent")
 
 
 # ── page tables ──────────────────────────────────────────────────────────────
@@ -364,10 +380,6 @@ class _Rotary(torch.autograd.Function):
         return tuple(_Rotary._of_both(ctx, ctx.inverse, tq, tk))
 
 
-def _is_dual(t):
-    return t is not None and forward_ad.unpack_dual(t).tangent is not None
-
-
 def _rotary(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out):
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or \
             forward_ad._current_level >= 0 and (_is_dual(q) or _is_dual(k)):
@@ -473,6 +485,7 @@ def cache_append(k, v, codes, scales, slots, cos=None, sin=None, positions=None,
             if q_out.shape != q.shape:
                 raise ValueError(f"{who}: q_out must have q's shape")
     inter = _interleaved(who, layout)
+    _no_gradient(who, k, v, q)
     dev = k.device
     s = _on_device(who, dev, v, codes, scales, slots, cos, sin, positions, q, q_out)
     with _on(dev):
@@ -579,6 +592,7 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
     if window < 0:
         raise ValueError(f"{who}: window must not be negative")
     window, most_new = min(window, 0x7FFFFFFF), min(most_new, 0x7FFFFFFF)
+    _no_gradient(who, q)
     dev = q.device
     s = _on_device(who, dev, codes, scales, table, lens, starts, out)
     with _on(dev):

@@ -1,0 +1,36 @@
+"""What the serving calls refuse before they look for a device (no GPU)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from sili__new_b200 import serving as S
+
+
+@pytest.fixture
+def calls():
+    """Each call by the name of the input that takes part in it, as a function of that input."""
+    x = torch.zeros(2, 2, 64)
+    cos, pos = torch.zeros(4, 16), torch.zeros(2, dtype=torch.int32)
+    codes, scales = torch.zeros(2, 2, 2, 16, 32, dtype=torch.uint8), torch.zeros(2, 2, 2, 16, 2, dtype=torch.uint8)
+    slots = torch.zeros(2, dtype=torch.int64)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    turn = dict(cos=cos, sin=cos, positions=pos)
+    return x, {"append k": lambda a: S.cache_append(a, x, codes, scales, slots),
+               "append v": lambda a: S.cache_append(x, a, codes, scales, slots),
+               "append q": lambda a: S.cache_append(x, x, codes, scales, slots, q=a, **turn),
+               "attention q": lambda a: S.cache_attention(a, codes, scales, table, lens)}
+
+
+@pytest.mark.parametrize("which", ["append k", "append v", "append q", "attention q"])
+def test_a_gradient_that_would_be_lost_is_refused(calls, which):
+    x, by_name = calls
+    call = by_name[which]
+    with pytest.raises(ValueError, match="no gradient"):
+        call(x.clone().requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
+        call(forward_ad.make_dual(x, torch.ones_like(x)))
+    # not asked for: the call goes on (to the next refusal here)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        call(x.clone().requires_grad_())
+    with pytest.raises(ValueError, match="CUDA"):
+        call(x)
