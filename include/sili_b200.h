@@ -485,7 +485,7 @@ int sili_rotary(int dtype, const void* q, int64_t q_token_stride, int64_t q_head
  * append: K (rotated first when rot > 0, rot a multiple of 16) and V of each
  * token into its slot; slots outside [0, n_pages * page) are passed over; two
  * tokens must not share one.  With q_heads > 0, q_out (which may be q) gets the
- * rotated q. */
+ * rotated q.  Head rows start on 16 bytes. */
 int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
                     int64_t qo_token_stride, int64_t qo_head_stride, int q_heads, const void* k, int64_t k_token_stride,
                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int kv_heads,
@@ -505,7 +505,7 @@ int sili_kv4_read(int dtype, const uint8_t* codes, const uint8_t* scales, int64_
  * only the last `window` of them; keys of a page that is not there (an entry
  * outside [0, n_pages)) are not seen.  out [tokens, heads, dim] =
  * softmax(scale q k) v, rounded once; lse [tokens, heads] (may be NULL) the
- * natural log of the softmax's sum.  A row that sees nothing, or belongs to
+ * natural log of the softmax's sum.  q's rows start on 8 bytes, out on 16.  A row that sees nothing, or belongs to
  * no request, gives zeros and -inf.  most_new: the largest number of queries
  * of a request, as the host knows it; it chooses the kernel, not the result.
  * workspace: sili_kv4_attention_workspace bytes, the first 4096 of them zeroed

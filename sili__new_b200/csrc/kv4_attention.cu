@@ -873,8 +873,10 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
     if (requests && table_stride < width) return bad(who, "table rows overlap");
     if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return bad(who, "codes and scales must be 16-byte aligned");
     const int64_t item = dtype == SILI_F32 ? 4 : 2;
-    if ((uintptr_t)q % 8 || (uintptr_t)out % 16 || q_token_stride * item % 8 || q_head_stride * item % 8)
+    // (the stride of a single token or head is never used, and may be anything)
+    if ((uintptr_t)q % 8 || (tokens > 1 && q_token_stride * item % 8) || (heads > 1 && q_head_stride * item % 8))
         return bad(who, "q rows must be 8-byte aligned");
+    if ((uintptr_t)out % 16) return bad(who, "out must be 16-byte aligned");
     AttendArgs a{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
                  table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
                  (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16)),

@@ -755,11 +755,13 @@ int sili_kv4_append(int dtype, const void* q, int64_t q_token_stride, int64_t q_
     if (tokens == 0) return SILI_OK;
     if (!k || !v || !slots || (q_heads && (!q || !q_out)) || (n_pages && (!codes || !scales))) return bad(who, "null array");
     const int64_t item = dtype == SILI_F32 ? 4 : 2;
-    auto aligned = [&](const void* p, int64_t ts, int64_t hs) {
-        return (uintptr_t)p % 16 == 0 && ts * item % 16 == 0 && hs * item % 16 == 0;
+    // (the stride of a single token or head is never used, and may be anything)
+    auto aligned = [&](const void* p, int64_t ts, int64_t hs, int heads) {
+        return (uintptr_t)p % 16 == 0 && (tokens == 1 || ts * item % 16 == 0) && (heads == 1 || hs * item % 16 == 0);
     };
-    if (!aligned(k, k_token_stride, k_head_stride) || !aligned(v, v_token_stride, v_head_stride) ||
-        (q_heads && (!aligned(q, q_token_stride, q_head_stride) || !aligned(q_out, qo_token_stride, qo_head_stride))))
+    if (!aligned(k, k_token_stride, k_head_stride, kv_heads) || !aligned(v, v_token_stride, v_head_stride, kv_heads) ||
+        (q_heads && (!aligned(q, q_token_stride, q_head_stride, q_heads) ||
+                     !aligned(q_out, qo_token_stride, qo_head_stride, q_heads))))
         return bad(who, "rows must start on 16 bytes");
     if ((uintptr_t)codes % 16) return bad(who, "codes must be 16-byte aligned");
     AppendArgs a{{{q, k}, {q_out, nullptr}, {q_token_stride, k_token_stride}, {q_head_stride, k_head_stride},

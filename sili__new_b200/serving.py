@@ -555,7 +555,8 @@ def check_attention(device=None):
 
 def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, scale=None, window: int = 0, out=None,
                     return_lse: bool = False):
-    """Causal attention of q [tokens, heads, dim] over the 4-bit cache.
+    """Causal attention of q [tokens, heads, dim] (rows start on 8 bytes, any
+    strides otherwise) over the 4-bit cache.
 
     ``table`` int32 [requests, width] and ``lens`` int32 [requests] (cached
     plus new tokens) from ``page_tables``.  ``starts`` int32 [requests + 1]:
