@@ -104,6 +104,17 @@ def _heads(who, name, t, tokens=None, dim=None, dtype=None):
         raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
 
 
+def _apart(who, name, t):
+    """Refuses an output [tokens, heads, dim] whose rows may share elements."""
+    (tokens, heads, dim), (st, sh, _) = t.shape, t.stride()
+    if (heads < 2 or sh >= dim) and (tokens < 2 or st >= (sh * (heads - 1) if heads > 1 else 0) + dim):
+        return
+    if (tokens < 2 or st >= dim) and (heads < 2 or sh >= (st * (tokens - 1) if tokens > 1 else 0) + dim):
+        return
+    if t.numel():
+        raise ValueError(f"{who}: {name}'s rows may share elements (strides {list(t.stride())})")
+
+
 def _is_dual(t):
     return t is not None and forward_ad.unpack_dual(t).tangent is not None
 
@@ -320,12 +331,13 @@ def _turn(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out):
     _check_table(who, cos, sin, positions, tokens, dim)
     inter = _interleaved(who, layout)
     dev = q.device
-    s = _on_device(who, dev, k, cos, sin, positions, q_out, k_out)
     for name, x, o in (("q_out", q, q_out), ("k_out", k, k_out)):
         if o is not None:
             _heads(who, name, o, tokens, dim, q.dtype)
             if x is None or o.shape != x.shape:
                 raise ValueError(f"{who}: {name} must have its input's shape")
+            _apart(who, name, o)
+    s = _on_device(who, dev, k, cos, sin, positions, q_out, k_out)
     with _on(dev):
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
@@ -396,8 +408,9 @@ def rotary(q, k, cos, sin, positions, layout: str = "half", q_out=None, k_out=No
     (i, i + half) or adjacent ones.  ``cos`` / ``sin`` from ``rotary_table``;
     ``positions`` int32 or int64 [tokens]: a negative one (padding) gives
     zeros, one past the table NaN.  ``q_out`` / ``k_out`` may be the inputs
-    (in place).  Differentiable in q and k to any order, in reverse and forward
-    mode, when no output is given; not in the table.  Returns (q', k')."""
+    (in place), and share no elements otherwise.  Differentiable in q and k to
+    any order, in reverse and forward mode, when no output is given; not in
+    the table.  Returns (q', k')."""
     return _rotary("rotary", q, k, cos, sin, positions, layout, False, q_out, k_out)
 
 
@@ -484,6 +497,7 @@ def cache_append(k, v, codes, scales, slots, cos=None, sin=None, positions=None,
             _heads(who, "q_out", q_out, tokens, dim, k.dtype)
             if q_out.shape != q.shape:
                 raise ValueError(f"{who}: q_out must have q's shape")
+            _apart(who, "q_out", q_out)
     inter = _interleaved(who, layout)
     _no_gradient(who, k, v, q)
     dev = k.device

@@ -34,3 +34,25 @@ def test_a_gradient_that_would_be_lost_is_refused(calls, which):
         call(x.clone().requires_grad_())
     with pytest.raises(ValueError, match="CUDA"):
         call(x)
+
+
+def test_outputs_whose_rows_share_elements_are_refused():
+    """Several rows would be written to one place, in no order."""
+    x, cos, pos = torch.zeros(4, 3, 64), torch.zeros(4, 16), torch.zeros(4, dtype=torch.int32)
+    codes, scales = torch.zeros(2, 2, 3, 16, 32, dtype=torch.uint8), torch.zeros(2, 2, 3, 16, 2, dtype=torch.uint8)
+    slots = torch.zeros(4, dtype=torch.int64)
+    turn = dict(cos=cos, sin=cos, positions=pos)
+    flat = torch.zeros(4096)
+    for strides in ((0, 64, 1), (192, 0, 1), (192, 32, 1), (64, 128, 1), (100, 64, 1), (64, 64, 1)):
+        out = flat.as_strided(x.shape, strides)
+        for call in (lambda o: S.rotary(x, None, cos, cos, pos, q_out=o), lambda o: S.rotary(x, x, cos, cos, pos, k_out=o),
+                     lambda o: S.rotary_backward(x, x, cos, cos, pos, k_out=o),
+                     lambda o: S.cache_append(x, x, codes, scales, slots, q=x, q_out=o, **turn)):
+            with pytest.raises(ValueError, match="share elements"):
+                call(out)
+    # rows apart from one another, tokens or heads outermost, and axes of length one: on to the next refusal
+    for shape, strides in ((x.shape, (192, 64, 1)), (x.shape, (300, 70, 1)), (x.shape, (64, 256, 1)), (x.shape, (65, 700, 1)),
+                           ((1, 3, 64), (0, 64, 1)), ((4, 1, 64), (64, 0, 1)), ((4, 1, 64), (64, 1, 1)), ((0, 3, 64), (0, 0, 1))):
+        y, p = torch.zeros(shape), pos[:shape[0]]
+        with pytest.raises(ValueError, match="CUDA"):
+            S.rotary(y, None, cos, cos, p, q_out=flat.as_strided(shape, strides))
