@@ -522,6 +522,9 @@ int sili_kv4_attention_status(void* workspace, void* stream);
  * for its output.  0 gives up without a look.  For the calls of the process
  * that follow; captured calls keep theirs. */
 int sili_kv4_attention_wait_limit(int polls, int output_polls);
+/* Whether a call with `starts` of these sizes runs in the kernel of long 16-bit
+ * prompts (1) or in the one that splits every request over its keys (0). */
+int sili_kv4_attention_long_prompt(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int most_new, int* yes);
 int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
                        int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads,
                        const int* table, int64_t table_stride, int width, const int* lens, int requests,

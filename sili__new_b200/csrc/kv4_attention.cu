@@ -853,6 +853,15 @@ int sili_kv4_attention_workspace(int64_t* bytes) {
     return SILI_OK;
 }
 
+int sili_kv4_attention_long_prompt(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int most_new, int* yes) {
+    const char* who = "kv4_attention_long_prompt";
+    if (!yes) return bad(who, "null array");
+    if (tokens < 0 || tokens > 0x7fffffffLL || heads < 1 || kv_heads < 1 || heads % kv_heads || most_new < 0)
+        return bad(who, "sizes out of range");
+    *yes = sili::kv4_prompt_takes(dtype, dim, tokens, heads, kv_heads, most_new);
+    return SILI_OK;
+}
+
 int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
                        int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads,
                        const int* table, int64_t table_stride, int width, const int* lens, int requests,

@@ -832,6 +832,11 @@ PYBIND11_MODULE(_cuda, m) {
     m.def("kv4_attention_wait_limit", [](int polls, int output_polls) {
         check(sili_kv4_attention_wait_limit(polls, output_polls));
     }, py::arg("polls") = -1, py::arg("output_polls") = -1);
+    m.def("kv4_attention_long_prompt", [](int dtype, int dim, int64_t tokens, int heads, int kv_heads, int most_new) {
+        int yes = 0;
+        check(sili_kv4_attention_long_prompt(dtype, dim, tokens, heads, kv_heads, most_new, &yes));
+        return yes != 0;
+    });
     m.def("kv4_attention_workspace", []() {
         int64_t n = 0;
         check(sili_kv4_attention_workspace(&n));
