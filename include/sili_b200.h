@@ -442,9 +442,11 @@ int sili_banded_attention_backward(const float* q, const float* k, const float* 
  * page size + offset) and positions, -1 beyond the last token up to
  * max_tokens; pool_out; status = {pages that lacked, tokens beyond
  * max_tokens, pages beyond the table's width}.  A page that lacks is entered
- * as -1 and its tokens' slots are -1; entries and tokens that lacked can be
- * asked for again with the same lengths.  Running a call again with the same
- * inputs writes the same values.  scratch: n + 1 ints, needed above 4096
+ * as -1 and its tokens' slots are -1.  Running a call again with the same
+ * inputs writes the same values, and a step that lacked pages can be asked for
+ * again with the lengths and the pool of before it, once sili_release_pages
+ * has given pages back by those; with pool_out the pages that it did get would
+ * be taken a second time.  scratch: n + 1 ints, needed above 4096
  * requests only.  Fewer than 2^31 new tokens. */
 int sili_page_tables(const int* cached, const int* fresh, int n_requests, int* table, int64_t table_stride, int width,
                      const int* ring, int ring_size, const int64_t* pool, int page, int64_t max_tokens, int* starts,

@@ -175,7 +175,10 @@ def page_tables(cached, fresh, table, ring, pool, page: int, max_tokens: int) ->
     from ``ring`` in request order (``pool`` = pages taken, given); -1 where
     the ring runs out, and the tokens of such a page have slot -1.  Nothing is
     read back: look at ``status`` when it suits.  The same inputs again write
-    the same values, so pass the returned ``pool`` on to the next step."""
+    the same values, so pass the returned ``pool`` on to the next step.  A step
+    that lacked pages is asked for again with the lengths and the ``pool`` of
+    before it, after ``release_pages`` with those (its returned pool counts the
+    pages that it did get as held)."""
     who = "page_tables"
     n = cached.numel()
     dev = cached.device
