@@ -85,9 +85,10 @@ constexpr int kMaxStages = 4;
 constexpr float kNoMaximum = -3e38f;    // below every finite logit, and finite: a masked key's -inf over it is -inf
 constexpr int kMaxCtas = 2 * 148;       // two CTAs an SM; one for the wider row tiles
 
+static_assert(kMaxCtas <= sili::kSlotWord, "the counters end before the slots' bits");
 constexpr int64_t workspace_bytes() {
     // two partial results a CTA: rows * (dim + 2) floats
-    return kTicketBytes + (int64_t)kMaxCtas * 2 * 32 * 130 * 4;
+    return kTicketBytes + std::max((int64_t)kMaxCtas * 2 * 32 * 130 * 4, sili::kSlotBytes);
 }
 
 template <int E, int NT>

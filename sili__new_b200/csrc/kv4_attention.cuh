@@ -45,9 +45,14 @@ struct AttendArgs {
     }
 };
 
-// The workspace: a counter a CTA, an error word, then the partial results.
+// The workspace: a counter a CTA, the taken slots' bits, an error word; then the partial results of the one kernel, or
+// the other's slots.
 constexpr int kTicketBytes = 4096;
 constexpr int kErrorWord = kTicketBytes / 4 - 1;
+// A slot: the sums of a CTA's 256 rows that have left tensor memory (kv4_prompt.cu), and the maxima they stand over.  As
+// many as CTAs can be resident, one an SM.
+constexpr int kSlotWord = 512, kSlotWords = 5, kSlotRows = 256, kSlotDim = 128;
+constexpr int64_t kSlotFloats = kSlotRows * (kSlotDim + 1), kSlotBytes = kSlotWords * 32 * kSlotFloats * 4;
 
 // p = 2^(x - m + 8): room below (a half's subnormals start at 2^-32 of the largest) and above (x may exceed m by 7)
 constexpr float kLift = 8.f, kSlack = 7.f;

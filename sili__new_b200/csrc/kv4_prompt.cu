@@ -73,6 +73,13 @@ constexpr int kThreads = kSoftmax + kDequant + 128;     // whole warpgroups: eac
 constexpr int kRegsSoftmax = 144, kRegsDequant = 72, kRegsRest = 48;
 static_assert(kSoftmax * kRegsSoftmax + kDequant * kRegsDequant + 128 * kRegsRest <= 96 * kThreads, "register split");
 constexpr int kMmaWarp = (kSoftmax + kDequant) / 32;
+// Steps after which a row tile's O leaves tensor memory.  The matrix unit cuts what it adds to an accumulator towards
+// zero: with V of one sign the output was short by 6e-9 a key, 1.6e-3 over 262144 keys.  So long rows' sums are added
+// outside, rounded, in a slot of the workspace: every 16384 keys in fp16, 65536 in bf16, which leaves a fifth of the
+// output's half unit (1e-4, 4e-4).  1184 queries of 32 heads over 8, dim 128, over 262144 keys: 11.9 ms in bf16, 12.1 in
+// fp16, 11.5 with the sums left where they were; up to 16384 keys the same.
+template <typename T>
+constexpr int kAside = std::is_same<T, __half>::value ? 256 : 1024;
 constexpr int kPolls = 4096;          // polls of a wait, each asleep for up to kNap ns, before it gives up
 std::atomic<int> g_polls{kPolls}, g_output_polls{kPolls};     // sili_kv4_attention_wait_limit
 constexpr uint32_t kNap = 1000000;
@@ -92,6 +99,7 @@ struct Smem {
     uint32_t tmem;
     int dead;
     int hit[3];                       // the CTA's request, kv head and row tile pair
+    int slot;                         // of the workspace, for rows of more than kAside steps; -1: none
 };
 
 __device__ __forceinline__ uint32_t addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -416,6 +424,7 @@ struct Prompt {
         constexpr uint32_t kStage = kKeys * D * 2 / 16;
         const uint32_t q = desc_low(s.q[t]), k0 = desc_low(s.k[0]), v0 = desc_low(s.v[0]), d = s_col(t), p = p_col(t), o = o_col(t);
         const int mine = w.n[t], stages = w.last - w.j0;
+        const int over = s.slot >= 0 ? kAside<T> - 1 : 0x7FFFFFFF;      // O starts anew at steps that have none of these bits
         auto scores = [&](int i) {      // step i: the keys' rows 64 (i & 1) on of stage (i >> 1) & 1
             const uint32_t k = k0 + (i >> 1 & 1) * kStage + (i & 1) * (kSub * 8);
             mma_ss<false>(d, q, k, idesc(kM, kSub));
@@ -440,9 +449,9 @@ struct Prompt {
             asm volatile("tcgen05.fence::after_thread_sync;");
             const uint32_t v = v0 + (i >> 1 & 1) * kStage + (i & 1) * (D * 8);
 #pragma unroll
-            for (int c = 0; c < kSub / 16; ++c) mma_ts(o, p + (i & 1) * (kSub / 2) + 8 * c, v + 2 * c, idesc(kM, D), c > 0 || i > 0);
+            for (int c = 0; c < kSub / 16; ++c) mma_ts(o, p + (i & 1) * (kSub / 2) + 8 * c, v + 2 * c, idesc(kM, D), c > 0 || (i & over));
             commit(&s.p_free[t]);
-            if (i + 1 == mine) commit(&s.o_full[t]);
+            if (i + 1 == mine || ((i + 1) & over) == 0) commit(&s.o_full[t]);
             if ((i & 1) || i + 1 == mine) commit(&s.kv_free[i >> 1 & 1]);
         }
         // the other tile's stages: this one is done with them as soon as they are filled
@@ -464,6 +473,68 @@ struct Prompt {
             for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(x[i] * f);
             tmem_st16(o_col(t) + lanes + 16 * c, r);
         }
+    }
+
+    // this thread's part of the CTA's slot: 16 of its row's sums at a time, and the maximum they stand over
+    __device__ __forceinline__ float4* aside(int t, int c) const {
+        float* at = (float*)((uint8_t*)a.workspace + sili::kTicketBytes) + s.slot * sili::kSlotFloats;
+        return (float4*)(at + ((t * (D / 16) + c) * kM + (threadIdx.x & 127)) * 16);
+    }
+    __device__ __forceinline__ float* aside_base() const {
+        return (float*)((uint8_t*)a.workspace + sili::kTicketBytes) + (s.slot + 1) * sili::kSlotFloats - kSoftmax + threadIdx.x;
+    }
+    // x += the row's 16 sums of chunk c, taken from the maximum they stand over by f
+    __device__ __forceinline__ void add_aside(int t, int c, float f, float (&x)[16]) const {
+        const float4* at = aside(t, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = __ldcg(at + i);
+            x[4 * i] = fmaf(v.x, f, x[4 * i]);
+            x[4 * i + 1] = fmaf(v.y, f, x[4 * i + 1]);
+            x[4 * i + 2] = fmaf(v.z, f, x[4 * i + 2]);
+            x[4 * i + 3] = fmaf(v.w, f, x[4 * i + 3]);
+        }
+    }
+    __device__ __forceinline__ float aside_factor(float base) const {
+        const float was = __ldcg(aside_base());
+        return was == base ? 1.f : ex2(was - base);      // (both -inf: nothing seen yet)
+    }
+    // O's row joins its sum in the slot; the next product overwrites O
+    __device__ __forceinline__ void set_aside(int t, uint32_t lanes, float base, bool first) const {
+        const float f = first ? 0.f : aside_factor(base);
+        // 64 columns at a time, their loads in flight together
+#pragma unroll 1
+        for (int c = 0; c < D / 16; c += 4) {
+            float x[64];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tmem_ld16(o_col(t) + lanes + 16 * (c + k), reinterpret_cast<float(&)[16]>(x[16 * k]));
+            tmem_wait(x);
+            if (!first)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) add_aside(t, c + k, f, reinterpret_cast<float(&)[16]>(x[16 * k]));
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                __stcg(aside(t, c + i / 4) + i % 4, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+        }
+        __stcg(aside_base(), base);
+    }
+
+    // A slot for a CTA with rows of more than kAside steps.  There are more slots than CTAs can be resident, so one of
+    // them is free; none found within the bound (never seen): the CTA goes on without.
+    __device__ __forceinline__ int take_slot() const {
+        if (max(w.n[0], w.n[1]) <= kAside<T>) return -1;
+        uint32_t* bits = (uint32_t*)a.workspace + sili::kSlotWord;
+        for (int i = 0; i < 64 * sili::kSlotWords; ++i) {
+            const int word = (blockIdx.x + i) % sili::kSlotWords;
+            for (uint32_t left = ~*(volatile uint32_t*)(bits + word); left; left &= left - 1) {
+                const uint32_t bit = left & (0u - left);
+                if (!(atomicOr(bits + word, bit) & bit)) {
+                    __threadfence();
+                    return word * 32 + __ffs(bit) - 1;
+                }
+            }
+        }
+        return -1;
     }
 
     // ── warps 0-7: one row a thread ──
@@ -519,83 +590,96 @@ struct Prompt {
             }
         }
         cf = fmaxf(cf, 0x1p-126f);      // not 0, which would undo a mask's -inf
+        if (threadIdx.x == 0) s.slot = take_slot();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();       // Q is there: the products may begin
         float base = -INFINITY, l = 0.f;       // base: the running maximum - lift
         uint32_t poisoned = 0;                 // groups of 32 elements in which the row saw a NaN
         bool ok = true;
-        for (int i = 0; i < w.n[t]; ++i) {
-            const int j = w.j0 + (i >> 1), st = i >> 1 & 1, half = i & 1, key0 = j * kKeys + half * kSub;
-            ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], i & 1, &s.dead, a.polls));
+        const int steps = w.n[t], block = s.slot >= 0 ? kAside<T> : steps;
+        int i = 0, filled = 0;                 // filled: how often O has been whole, once a block
+        for (int end = min(block, steps); i < steps; end = min(end + block, steps)) {
+            if (i > 0) {
+                ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], filled & 1, &s.dead, a.polls));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                set_aside(t, lanes, base, filled++ == 0);
+            }
+            for (; i < end; ++i) {
+                const int j = w.j0 + (i >> 1), st = i >> 1 & 1, half = i & 1, key0 = j * kKeys + half * kSub;
+                ok = __all_sync(0xffffffffu, bar_wait(&s.s_full[t], i & 1, &s.dead, a.polls));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                float x[kSub];
+#pragma unroll
+                for (int c = 0; c < kSub; c += 16) tmem_ld16(s_col(t) + lanes + c, reinterpret_cast<float(&)[16]>(x[c]));
+                tmem_wait(x);
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                bar_arrive(&s.s_free[t]);          // the next scores may come while these are worked on
+                // keys [lo, hi) of the step are the row's; pages that are not there, a byte per 16 keys
+                const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
+                const int hi = to - key0, lo = from - key0;
+                if (there != 0x01010101u || key0 + kSub > all_to || key0 < all_from) {
+#pragma unroll
+                    for (int k = 0; k < kSub; ++k)
+                        if (k < lo || k >= hi || !(there >> (k / 16 * 8) & 1)) x[k] = -INFINITY;
+                }
+                // The running maximum moves when a logit exceeds it by 2^7: P stays within a half, and O is seldom read and
+                // written back.  (The maximum comes first although the sum of P would tell as well: P then takes the place
+                // of S in the registers, and the exponentials have room to overlap: 1225 against 1700 clocks.)
+                float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
+#pragma unroll
+                for (int k = 4; k < kSub; k += 4) {
+                    top = fmaxf(top, fmaxf(x[k], x[k + 1]));
+                    top1 = fmaxf(top1, fmaxf(x[k + 2], x[k + 3]));
+                }
+                top = fmaxf(top, top1);
+                if (top != -INFINITY) top = top * cf - kLift;
+                if (__any_sync(0xffffffffu, top > base + kSlack)) {       // (NaN compares false)
+                    const float fresh = fmaxf(base, top);
+                    const float f = fresh == base ? 1.f : ex2(base - fresh);
+                    base = fresh;
+                    l *= f;
+                    if (i > 0) {
+                        ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead, a.polls));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;");
+                        rescale(t, lanes, f);     // (for nothing where O has just been set aside)
+                    }
+                }
+                const float shift = base == -INFINITY ? 0.f : base;
+                // P's buffer was last read by the product two steps ago, which was queued before these scores
+                uint32_t p[2][16];
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int k = 0; k < kSub; k += 2) {
+                    const float u = ex2(fmaf(x[k], cf, -shift)), v = ex2(fmaf(x[k + 1], cf, -shift));
+                    sum0 += u; sum1 += v;
+                    p[k / 32][k / 2 % 16] = pack2(u, v);
+                }
+                tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2), p[0]);
+                tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2) + 16, p[1]);
+                l += sum0 + sum1;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                if (*(volatile int*)&s.odd[st] == j + 1) {
+                    for (int k = max(lo, 0); k < min(hi, kSub); ++k) {
+                        if (!(there >> (k / 16 * 8) & 1)) continue;
+                        for (int g = 0; g < E; ++g)
+                            if (s.odd_keys[st][(half * kSub + k) >> 3][g] >> (k & 7) & 1) poisoned |= 1u << g;
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                bar_arrive(&s.p_full[t][i & 1]);
+            }
             if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            float x[kSub];
-#pragma unroll
-            for (int c = 0; c < kSub; c += 16) tmem_ld16(s_col(t) + lanes + c, reinterpret_cast<float(&)[16]>(x[c]));
-            tmem_wait(x);
-            asm volatile("tcgen05.fence::before_thread_sync;");
-            bar_arrive(&s.s_free[t]);          // the next scores may come while these are worked on
-            // keys [lo, hi) of the step are the row's; pages that are not there, a byte per 16 keys
-            const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
-            const int hi = to - key0, lo = from - key0;
-            if (there != 0x01010101u || key0 + kSub > all_to || key0 < all_from) {
-#pragma unroll
-                for (int k = 0; k < kSub; ++k)
-                    if (k < lo || k >= hi || !(there >> (k / 16 * 8) & 1)) x[k] = -INFINITY;
-            }
-            // The running maximum moves when a logit exceeds it by 2^7: P stays within a half, and O is seldom read and
-            // written back.  (The maximum comes first although the sum of P would tell as well: P then takes the place
-            // of S in the registers, and the exponentials have room to overlap: 1225 against 1700 clocks.)
-            float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
-#pragma unroll
-            for (int k = 4; k < kSub; k += 4) {
-                top = fmaxf(top, fmaxf(x[k], x[k + 1]));
-                top1 = fmaxf(top1, fmaxf(x[k + 2], x[k + 3]));
-            }
-            top = fmaxf(top, top1);
-            if (top != -INFINITY) top = top * cf - kLift;
-            if (__any_sync(0xffffffffu, top > base + kSlack)) {       // (NaN compares false)
-                const float fresh = fmaxf(base, top);
-                const float f = fresh == base ? 1.f : ex2(base - fresh);
-                base = fresh;
-                l *= f;
-                if (i > 0) {
-                    ok = __all_sync(0xffffffffu, bar_wait(&s.p_free[t], (i - 1) & 1, &s.dead, a.polls));
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    rescale(t, lanes, f);
-                }
-            }
-            const float shift = base == -INFINITY ? 0.f : base;
-            // P's buffer was last read by the product two steps ago, which was queued before these scores
-            uint32_t p[2][16];
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int k = 0; k < kSub; k += 2) {
-                const float u = ex2(fmaf(x[k], cf, -shift)), v = ex2(fmaf(x[k + 1], cf, -shift));
-                sum0 += u; sum1 += v;
-                p[k / 32][k / 2 % 16] = pack2(u, v);
-            }
-            tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2), p[0]);
-            tmem_st16(p_col(t) + lanes + (i & 1) * (kSub / 2) + 16, p[1]);
-            l += sum0 + sum1;
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            if (*(volatile int*)&s.odd[st] == j + 1) {
-                for (int k = max(lo, 0); k < min(hi, kSub); ++k) {
-                    if (!(there >> (k / 16 * 8) & 1)) continue;
-                    for (int g = 0; g < E; ++g)
-                        if (s.odd_keys[st][(half * kSub + k) >> 3][g] >> (k & 7) & 1) poisoned |= 1u << g;
-                }
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;");
-            bar_arrive(&s.p_full[t][i & 1]);
         }
-        const int steps = w.n[t];
         // (a barrier of its own: p_free may be one or two phases behind here, which a parity does not tell apart)
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], 0, &s.dead, a.output_polls));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, bar_wait(&s.o_full[t], filled & 1, &s.dead, a.output_polls));
         asm volatile("tcgen05.fence::after_thread_sync;");
         // l 0: the row saw nothing
         float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool more = filled > 0 && ok;
+        const float f = more ? aside_factor(base) : 0.f;
         const int64_t id = q_row * a.heads + head;
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
@@ -604,6 +688,7 @@ struct Prompt {
             if (steps > 0) {
                 tmem_ld16(o_col(t) + lanes + 16 * c, x);
                 tmem_wait(x);
+                if (more) add_aside(t, c, f, x);
             } else
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -722,6 +807,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         }
         __syncthreads();
     }
+    if (threadIdx.x == 0 && s.slot >= 0) {
+        __threadfence();       // the next owner's sums come after this one's
+        atomicAnd((uint32_t*)a.workspace + sili::kSlotWord + s.slot / 32, ~(1u << s.slot % 32));
+    }
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(512));
 }
 
@@ -729,6 +818,7 @@ template <typename T, int D>
 int launch(const AttendArgs& a, cudaStream_t s) {
     constexpr int smem = (int)sizeof(Smem<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    static_assert(kSoftmax == sili::kSlotRows && D <= sili::kSlotDim, "a slot holds a CTA's rows");
     auto kernel = k_prompt<T, D>;
     static std::atomic<uint64_t> set{0};
     CKP(sili::allow_smem(kernel, smem, set));
