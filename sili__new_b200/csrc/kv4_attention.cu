@@ -82,13 +82,18 @@ int bad(const char* who, const char* what) {
 constexpr int kWarps = 8;
 constexpr int kUnit = 16 * kWarps;      // keys of a unit
 constexpr int kMaxStages = 4;
+// Units of a segment that a warp's 16-bit sums take in at most.  The matrix unit cuts what it adds to an accumulator
+// towards zero, 7e-8 a product where V has one sign: 5.8e-4, more than fp16's half unit, after the 8192 products of a
+// warp whose CTA walked 1048576 keys.  So a longer run is walked in pieces, whose sums are added in the workspace, rounded
+// (7e-5 is left).  In the loop itself the same cost 13 % of a decode batch, by its registers.
+constexpr int kPiece = 1024;
 constexpr float kNoMaximum = -3e38f;    // below every finite logit, and finite: a masked key's -inf over it is -inf
 constexpr int kMaxCtas = 2 * 148;       // two CTAs an SM; one for the wider row tiles
 
 static_assert(kMaxCtas <= sili::kSlotWord, "the counters end before the slots' bits");
 constexpr int64_t workspace_bytes() {
-    // two partial results a CTA: rows * (dim + 2) floats
-    return kTicketBytes + std::max((int64_t)kMaxCtas * 2 * 32 * 130 * 4, sili::kSlotBytes);
+    // two partial results a CTA: rows * (dim + 4) floats
+    return kTicketBytes + std::max((int64_t)kMaxCtas * 2 * 32 * 132 * 4, sili::kSlotBytes);
 }
 
 template <int E, int NT>
@@ -626,8 +631,10 @@ struct Attend {
         }
     }
 
+    // a part of a segment: [row][dim] sums, then the rows' maxima and the sums of their probabilities; those twice, so that
+    // the pieces of a run write the one while the other is read
     __device__ __forceinline__ float* partial(int cta, int slot) const {
-        return (float*)((uint8_t*)a.workspace + kTicketBytes) + (int64_t)(cta * 2 + slot) * kRows * (kDim + 2);
+        return (float*)((uint8_t*)a.workspace + kTicketBytes) + (int64_t)(cta * 2 + slot) * kRows * (kDim + 4);
     }
 
     // out and lse of one row and four of its values
@@ -646,9 +653,10 @@ struct Attend {
     }
 
     // The segment's end in this CTA: joins the warps, then writes the rows, or leaves them to the CTA that comes last.
-    // seg0 and seg1 number the segment's first unit and the one past its last.
+    // seg0 and seg1 number the segment's first unit and the one past its last.  Of a run in pieces, the first ones (`left`
+    // pieces follow) only leave their sums, and the others (`again`) add those before to theirs.
     __device__ __forceinline__ void end_segment(const Cur& c, int64_t seg0, int64_t seg1, int64_t begin, int64_t end,
-                                                int64_t all, int* s_last) {
+                                                int64_t all, int* s_last, bool again, int left) {
         constexpr int kThreads = kWarps * 32, kQuads = kDim / 4;
         float* jm = join + kWarps * kRows * L::kJoinRow;       // [warp][row] maxima, then sums
         float* jl = jm + kWarps * kRows;
@@ -672,7 +680,9 @@ struct Attend {
         const int64_t ctas = min((int64_t)gridDim.x, all);
         const int cta = blockIdx.x;
         const int lead = whole ? cta : (int)(((seg0 + 1) * ctas - 1) / all);
-        float* part = whole ? nullptr : partial(cta, cta == lead);
+        // (a whole segment's pieces use the place of the segment that this CTA begins last)
+        float* part = partial(cta, cta == lead);
+        float* tops = part + kRows * (kDim + 2 * (left & 1));
         for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
             const int row = i / kQuads, d = i % kQuads * 4;
             float top = kNoMaximum, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -685,13 +695,23 @@ struct Attend {
                 sum += jl[w * kRows + row] * f;
                 v[0] += p.x * f; v[1] += p.y * f; v[2] += p.z * f; v[3] += p.w * f;
             }
-            if (whole) store(c, row, d, v, top, sum);
+            if (kTerms == 1 && again) {
+                const float* before = part + kRows * (kDim + 2 * (~left & 1));
+                const float was = __ldcg(before + row), most = fmaxf(was, top);
+                const float f = was == most ? 1.f : ex2(was - most), h = top == most ? 1.f : ex2(top - most);
+                const float4 p = __ldcg((const float4*)(part + row * kDim + d));
+                sum = fmaf(sum, h, __ldcg(before + kRows + row) * f);
+                v[0] = fmaf(v[0], h, p.x * f); v[1] = fmaf(v[1], h, p.y * f);
+                v[2] = fmaf(v[2], h, p.z * f); v[3] = fmaf(v[3], h, p.w * f);
+                top = most;
+            }
+            if (whole && !left) store(c, row, d, v, top, sum);
             else {
                 __stcg((float4*)(part + row * kDim + d), make_float4(v[0], v[1], v[2], v[3]));
-                if (d == 0) { __stcg(part + kRows * kDim + row, top); __stcg(part + kRows * (kDim + 1) + row, sum); }
+                if (d == 0) { __stcg(tops + row, top); __stcg(tops + kRows + row, sum); }
             }
         }
-        if (whole) return;
+        if (whole || left) return;
         const int last = (int)((seg1 * ctas - 1) / all), n = last - lead + 1;
         __threadfence();
         __syncthreads();
@@ -752,9 +772,10 @@ struct Attend {
             asm volatile("cp.async.commit_group;");
         }
         int stage = 0, done = 0;
+        bool again = false;      // the segment's last piece lies behind
         while (done < n) {
             begin_segment(c);
-            const int here = min(c.left(), n - done);
+            const int rest = min(c.left(), n - done), here = kTerms == 1 ? min(rest, kPiece) : rest;
             int key0 = c.u * kUnit + warp * 16;
 #pragma unroll 1
             for (int i = 0; i < here; ++i, key0 += kUnit) {
@@ -770,9 +791,12 @@ struct Attend {
                 stage = stage + 1 == kStages ? 0 : stage + 1;
             }
             const int64_t seg0 = begin + done - (c.u - c.q.k0);
-            end_segment(c, seg0, seg0 + c.q.units, begin, end, all, s_last);
+            end_segment(c, seg0, seg0 + c.q.units, begin, end, all, s_last, kTerms == 1 && again,
+                        kTerms == 1 ? (rest - here + kPiece - 1) / kPiece : 0);
             done += here;
-            if (done < n) c.next_segment(a);
+            again = here < rest;
+            if (again) c.u += here;
+            if (!again && done < n) c.next_segment(a);
         }
     }
 };
@@ -808,7 +832,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_atten
 template <typename T, int E, int NT>
 int launch(const AttendArgs& a, cudaStream_t s) {
     constexpr int smem = smem_bytes<T, E, NT>();
-    static_assert(8 * NT * (32 * E + 2) <= 32 * 130, "the workspace holds the widest row tile");
+    static_assert(8 * NT * (32 * E + 4) <= 32 * 132, "the workspace holds the widest row tile");
     static_assert(8 * NT * (kMaxCtas + 2) * 4 <= Layout<E, NT>::kJoin, "the parts' weights fit the join space");
     auto kernel = k_attend<T, E, NT>;
     static std::atomic<uint64_t> set{0};

@@ -74,3 +74,55 @@ def test_long_prompt_sums_move_with_the_maximum():
         bound = 2.0 ** -11 * np.abs(ref) + 2.0 ** -25 + (2.0 ** -11 + 4 * e[..., None] + 2.0 ** -19) * spread + 2.0 ** -33 * total
         assert (np.abs(out[row].double().cpu().numpy() - ref[0]) <= bound[0]).all()
         assert (np.abs(lse[row].double().cpu().numpy() - ref_lse[0]) <= 2 * e[0] + 2.0 ** -19 * (1 + np.abs(ref_lse[0]))).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("requests,h,hk,d", [(300, 1, 1, 128), (310, 12, 1, 64), (160, 20, 1, 128), (160, 4, 1, 256)])
+def test_long_decode_sums_hold(dtype, requests, h, hk, d):
+    """More segments than CTAs, of more keys than a warp's sums take in at once (the requests share their pages)."""
+    from sili__new_b200 import serving as S
+    keys = 1000001 if d == 128 and h == 1 else 300001
+    codes, scales, want = _one_v(keys, hk, d, keys + h)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = torch.arange(codes.shape[0], dtype=torch.int32, device="cuda").repeat(requests, 1)
+    lens = torch.full((requests,), keys, dtype=torch.int32, device="cuda")
+    lens[5], lens[77] = 0, 200000
+    q = (torch.randn(requests, h, d, generator=g, device="cuda") * 0.3).to(dtype)
+    out, lse = S.cache_attention(q, codes, scales, table, lens, return_lse=True)
+    assert torch.equal(out, S.cache_attention(q, codes, scales, table, lens))
+    assert (out[5] == 0).all() and torch.isinf(lse[5]).all()
+    there = torch.arange(requests, device="cuda") != 5
+    off = out.double()[there].view(-1, hk, h // hk, d) / want[None, :, None] - 1
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[dtype]
+    w = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11
+    assert float(off.abs().max()) <= u + w + 2.0 ** -19
+    assert abs(float(off.mean())) <= 2.0 ** -12
+    # a request by itself is split over all CTAs, in other parts
+    for r in (0, 77, requests - 1):
+        one, one_lse = S.cache_attention(q[r:r + 1], codes, scales, table[r:r + 1], lens[r:r + 1], return_lse=True)
+        assert float((one_lse - lse[r:r + 1]).abs().max()) <= 2.0 ** -18 * (1 + float(one_lse.abs().max()))
+        assert float((one - out[r:r + 1]).abs().max()) <= (2 * u + 2.0 ** -19) * float(want.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("h,d", [(1, 64), (9, 128)])
+def test_long_decode_sums_move_with_the_maximum(dtype, h, d):
+    from sili__new_b200 import serving as S
+    keys, requests, page = 290000, 300, 80
+    g = torch.Generator(device="cuda").manual_seed(4)
+    codes, scales = R.random_cache(-(-keys // page), 1, page, d, g)
+    codes[:, 0] = 0x22
+    at = torch.arange(codes.shape[0], device="cuda")[:, None] * page + torch.arange(page, device="cuda")
+    grow = 60 + 2 * ((at % 150000) // 3000)                # K: from 2^-7.4 up to 28, twice
+    scales[:, 0] = grow[:, None, :, None].to(torch.uint8)
+    table = torch.arange(codes.shape[0], dtype=torch.int32, device="cuda").repeat(requests, 1)
+    lens = torch.full((requests,), keys, dtype=torch.int32, device="cuda")
+    q = torch.randn(requests, h, d, generator=g, device="cuda").to(dtype)
+    out, lse = S.cache_attention(q, codes, scales, table, lens, return_lse=True)
+    for r in (0, 150, requests - 1):
+        ref, ref_lse, spread, size, total = R.attention(q[r:r + 1], codes, scales, table[r:r + 1], [keys], [0, 1], d ** -0.5, 0, 1)
+        e = 2.0 ** -20 * size
+        u, w, least = (2.0 ** -24, 2.0 ** -21, 2.0 ** -150) if dtype == torch.float32 else (2.0 ** -11, 2.0 ** -11, 2.0 ** -25)
+        bound = u * np.abs(ref) + least + (w + 4 * e[..., None] + 2.0 ** -19) * spread + 2.0 ** -33 * total
+        assert (np.abs(out[r].double().cpu().numpy() - ref[0]) <= bound[0]).all()
+        assert (np.abs(lse[r].double().cpu().numpy() - ref_lse[0]) <= 2 * e[0] + 2.0 ** -19 * (1 + np.abs(ref_lse[0]))).all()
