@@ -124,7 +124,7 @@ def _no_gradient(who, *arrays):
     if torch.is_grad_enabled():
         for a in arrays:
             if a is not None and a.requires_grad:
-                raise ValueError(f"{who}: has no gradient: call it under torch.no_grad() or detach its inputs")
+                raise ValueError(f"{who}: has no gradient: call it under torch.no_grad() or with detached inputs")
     if forward_ad._current_level >= 0 and any(_is_dual(a) for a in arrays):
         raise ValueError(f"{who}: has no gradient: its inputs must not carry a tangent")
 
@@ -396,6 +396,7 @@ class _Rotary(torch.autograd.Function):
 
 
 def _rotary(who, q, k, cos, sin, positions, layout, inverse, q_out, k_out):
+    _no_gradient(f"{who}'s table", cos, sin)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or \
             forward_ad._current_level >= 0 and (_is_dual(q) or _is_dual(k)):
         if q_out is not None or k_out is not None:
@@ -413,7 +414,7 @@ def rotary(q, k, cos, sin, positions, layout: str = "half", q_out=None, k_out=No
     zeros, one past the table NaN.  ``q_out`` / ``k_out`` may be the inputs
     (in place), and share no elements otherwise.  Differentiable in q and k to
     any order, in reverse and forward mode, when no output is given; not in
-    the table.  Returns (q', k')."""
+    the table, which must not ask for a gradient.  Returns (q', k')."""
     return _rotary("rotary", q, k, cos, sin, positions, layout, False, q_out, k_out)
 
 
@@ -502,7 +503,7 @@ def cache_append(k, v, codes, scales, slots, cos=None, sin=None, positions=None,
                 raise ValueError(f"{who}: q_out must have q's shape")
             _apart(who, "q_out", q_out)
     inter = _interleaved(who, layout)
-    _no_gradient(who, k, v, q)
+    _no_gradient(who, k, v, q, cos, sin)
     dev = k.device
     s = _on_device(who, dev, v, codes, scales, slots, cos, sin, positions, q, q_out)
     with _on(dev):

@@ -56,3 +56,18 @@ def test_outputs_whose_rows_share_elements_are_refused():
         y, p = torch.zeros(shape), pos[:shape[0]]
         with pytest.raises(ValueError, match="CUDA"):
             S.rotary(y, None, cos, cos, p, q_out=flat.as_strided(shape, strides))
+
+
+def test_a_table_that_asks_for_a_gradient_is_refused():
+    x, cos, pos = torch.zeros(2, 2, 64), torch.zeros(4, 16), torch.zeros(2, dtype=torch.int32)
+    codes, scales = torch.zeros(2, 2, 2, 16, 32, dtype=torch.uint8), torch.zeros(2, 2, 2, 16, 2, dtype=torch.uint8)
+    slots = torch.zeros(2, dtype=torch.int64)
+    learned = cos.clone().requires_grad_()
+    for c, s in ((learned, cos), (cos, learned)):
+        for call in (lambda: S.rotary(x, None, c, s, pos), lambda: S.rotary(x.clone().requires_grad_(), x, c, s, pos),
+                     lambda: S.rotary_backward(x, None, c, s, pos),
+                     lambda: S.cache_append(x, x, codes, scales, slots, cos=c, sin=s, positions=pos)):
+            with pytest.raises(ValueError, match="no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+                call()
