@@ -14,9 +14,13 @@
 // the conversion (4 logic operations for 16 values).
 //
 // fp32 queries and probabilities are split into two halves (hi + lo, 22 bits,
-// after scaling a row by a power of two), 16-bit queries are exact in one;
-// probabilities are then rounded to one half (relative 2^-12, below the
-// output's own rounding).  Sums, maxima and outputs are fp32.  The running
+// after scaling a row by a power of two).  16-bit queries are one half: fp16 as
+// they are, bf16 scaled likewise, exact down to 2^-31 of a row's largest and
+// within 2^-39 of it below.  Their probabilities are rounded to one half, by at
+// most 2^-11 of themselves (their sum is taken before): the output's own half
+// unit in fp16 for few keys, less over many, where the errors average; a second
+// half would double the products.  Sums, maxima and outputs are fp32; 16-bit
+// sums lie in the matrix unit's accumulators, which it cuts (see kPiece).  The running
 // maximum is moved only when a logit exceeds it by 2^7 (p <= 2^15 is still a
 // half): a warp vote in place of a reduction per tile.
 //

@@ -2,24 +2,31 @@
 // generation tensor cores (tcgen05, sm_100a).
 //
 // A CTA holds 256 rows (query token x query head of the group) of one kv head
-// as two tiles of 128 and walks the keys 128 at a time:
+// as two tiles of 128.  Keys come into shared memory 128 at a time, and a tile
+// takes 64 of them a step:
 //   S_w = Q_w K^T     A: Q in shared memory, B: K, D in tensor memory
 //   P_w = 2^(S_w - m) the softmax warps, row by row in a thread
-//   O_w += P_w V      A: P in tensor memory (over S_w), B: V^T
+//   O_w += P_w V      A: P in tensor memory (beside S_w, twice), B: V^T
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1, so one tile's
-// exponentials run while the other's products do; warps 8-11 turn the next
+// exponentials run while the other's products do; warps 8-15 turn the next
 // keys' 4-bit K and V into halves in shared memory (K as it lies, V
 // transposed by interleaving the nibbles of two keys), straight from global
 // memory through registers; a thread of warps 16 and 17 each issues a tile's products.  All
-// operands are K-major with the 128-byte swizzle.  K and V are exact in
-// half; bf16 queries are scaled to halves exactly by a power of two a row;
-// P is rounded once to half (2^-12, below the output's rounding).  The
-// running maximum moves only when a logit exceeds it by 2^7, since O has to
-// be read and written back then.
+// operands are K-major with the 128-byte swizzle.
+//
+// Roundings.  K and V are exact in half.  fp16 queries stay as they are; bf16
+// ones are scaled by a power of two a row, their largest into [2^14, 2^15):
+// exact down to 2^-31 of it, and within 2^-39 of it below that.  P is rounded
+// once to half, by at most 2^-11 of itself (its sum is taken before): in fp16
+// that is the output's own half unit for a row of few keys, and averages out
+// over many (2.3e-4 against 2.1e-4 with P in fp32, on 262143 keys); a second
+// half for the rest would double the P V products.  The running maximum moves
+// only when a logit exceeds it by 2^7, since O has to be read and written back
+// then.  What the matrix unit cuts off O: see kAside.
 //
 // What bounds it, 3 chunks of about 2000 tokens over 4.7k-6.6k keys, 32 heads
-// over 8, dim 128, bf16 (464 GFLOP, 281 us at the card's matrix rate): 693 us,
-// 670 TFLOP/s.  No unit is full (tensor pipe 32 %, exponentials 33 %, issue
+// over 8, dim 128, bf16 (464 GFLOP, 281 us at the card's matrix rate): 698 us,
+// 665 TFLOP/s.  No unit is full (tensor pipe 32 %, exponentials 33 %, issue
 // 50 %; leaving out half the P V products changes nothing, all
 // dequantisation 7 %): a step is the softmax warps' chain of about 2600
 // clocks for 64 keys (scores' barrier, tensor-memory load, maximum,
@@ -836,8 +843,18 @@ int launch(const AttendArgs& a, cudaStream_t s) {
 
 namespace sili {
 
-// From about half the SMs' worth of full row pairs on; below, the split over
-// keys of the other kernel fills the card better.
+// Full row pairs from which on this kernel is taken: half the SMs' worth, where it is ahead at every size measured.  us
+// of one request in bf16, this kernel | the other, which splits the keys:
+//   32 heads over 8 x 128,  1024 keys: 48 pairs 47 |  74, 72: 47 |  94, 128:  47 |  149
+//                           4096 keys: 32 117 | 117, 48 118 | 162, 72 118 | 229, 128 119 | 389
+//                          16384 keys: 24 399 | 275, 32 399 | 354, 48 398 | 518, 72 399 | 762
+//   32 over 4 x 64,         4096 keys: 32 104 |  78, 48 104 | 105, 72 104 | 145
+//                          16384 keys: 48 362 | 312, 64 361 | 406, 72 360 | 453
+//   14 over 14 x 64,       16384 keys: 42 354 | 276, 70 359 | 439
+// They cross between 20 pairs (1024 keys) and 60 (dim 64 over 16384), so calls between there and 74 pairs take up to
+// twice the time that this kernel would.  The rule looks at all rows of a batch: a request with one query beside a long
+// prompt is walked here by one CTA a kv head, however long it is (262143 keys beside 2048 queries: 5.8 ms; in two calls
+// 0.18 + 0.09).
 bool kv4_prompt_takes(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int64_t most_new) {
     const int64_t group = heads / kv_heads;
     return dtype != SILI_F32 && (dim == 64 || dim == 128) && most_new * group >= 128 &&

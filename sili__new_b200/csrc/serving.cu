@@ -313,10 +313,11 @@ __device__ __forceinline__ int64_t load_position(const void* p, int pos64, int64
 // V elements an access.  One unit of a head row is V pairs (half layout: V
 // elements at i and V at i + rot/2), V/2 pairs (interleaved: V adjacent
 // elements) or V elements that pass through; a thread keeps its unit and so
-// its cosines while it walks the heads.  Bound by HBM: each value is read and
-// written once.  8191 tokens of 32 + 8 heads x 128 in fp32, forward and
-// gradient: 131 us, 5.1 TB/s (whole heads turned, 16001 tokens: 6.1 TB/s; in
-// bf16 4.2).  The fp32 form is held to 32 registers: with 8 CTAs an SM in
+// its cosines while it walks the heads.  Each value is read and written once.
+// 8191 tokens of 32 + 8 heads x 128 in fp32, forward and gradient: 131 us,
+// 5.1 TB/s, bound by HBM (whole heads turned, 16001 tokens: 6.1 TB/s).  In
+// bf16 4.2 TB/s, not HBM's bound: y may be x, so a thread's next loads wait
+// behind its stores.  The fp32 form is held to 32 registers: with 8 CTAs an SM in
 // place of 5 it took 131 us for 148; the 16-bit one keeps its registers (80
 // us against 113 with 8).  Few tokens are spread over several CTAs each, a
 // call of 64 tokens is its launch (19 us with the host's side).
