@@ -483,10 +483,9 @@ def run(state):
         if op == "adjust":
             return {"logits": serving.adjust_logits(s["logits"], **rules)}
         return {"token": serving.pick_tokens(s["logits"], **rules)}
-    a = serving.accept_drafts(s["drafted"], s["parents"], s["picked"], s["starts"], s["lens"])
-    serving.keep_drafts(s["caches"], s["table"], s["starts"], s["lens"], a.path)
-    pool = serving.trim_pages(s["lens"], a.lens, s["table"], s["ring"], s["pool"], s["page"])
-    return {"path": a.path, "kept": a.kept, "token": a.token, "lens": a.lens, "ring": s["ring"], "pool": pool,
+    a = serving.settle_drafts(s["drafted"], s["parents"], s["picked"], s["starts"], s["lens"], s["table"], s["caches"],
+                              s["ring"], s["pool"])
+    return {"path": a.path, "kept": a.kept, "token": a.token, "lens": a.lens, "ring": s["ring"], "pool": a.pool,
             "codes": [c for c, _ in s["caches"]], "scales": [b for _, b in s["caches"]]}
 
 
