@@ -533,6 +533,90 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
                        const int* starts, int most_new, float scale, int window, void* out, float* lse, void* workspace,
                        void* stream);
 
+/* ── serving: drafted tokens ──────────────────────────────────────────────
+ * A step that verifies drafted tokens: request r's are the rows starts[r] ..
+ * starts[r + 1) of the step's arrays, a row's parent before it; they have been
+ * appended to the cache behind the request's committed tokens, in the rows'
+ * order, and lens counts them.  Rows past `tokens` are left out.  Device
+ * arrays only, as above. */
+
+/* The plan of a step's trees.  parents[row]: the parent's place among the
+ * request's rows, -1 for a row that follows the committed tokens; a row whose
+ * parent is neither -1 nor an earlier row is none, and so are its descendants.
+ * masks [tokens, words]: bit j of a row's words is set where the row sees the
+ * request's row j, its ancestors and itself (with window > 0 the nearest
+ * `window` of them); positions[row] = committed + its depth.  Rows that are
+ * none, of no request, or past the masks' 64 * words bits: mask 0, position
+ * -1.  words: 1 to 4. */
+int sili_draft_tree(const int* parents, const int* starts, const int* lens, int requests, int64_t tokens, int words,
+                    int window, int64_t* masks, int* positions, void* stream);
+/* sili_kv4_attention for such a step: row i of a request sees the committed
+ * keys, with window > 0 only the last window - (bits of its mask) of them, and
+ * the request's drafted keys whose bits its mask has.  A row without a bit sees
+ * nothing.  masks [tokens, words], words 1 to 4. */
+int sili_kv4_tree_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                            int heads, int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page,
+                            int kv_heads, const int* table, int64_t table_stride, int width, const int* lens, int requests,
+                            const int* starts, const int64_t* masks, int words, int most_new, float scale, int window,
+                            void* out, float* lse, void* workspace, void* stream);
+
+/* What is done to a row's logits x of token v before a token is taken, in
+ * fp32, each operation rounded:
+ *   seen in the request's history, or on the row's path: x > 0 ? x / repetition : x * repetition
+ *   c > 0 times in the history behind the prompt and on the path: x - frequency * c - presence
+ *   + the bias of v;  / temperature, where that is above 0;  -inf where v is not allowed.
+ * Any part may be NULL.  Without starts row r is request r's one row; rows of
+ * no request are left as they are. */
+typedef struct sili_logit_rules {
+    const int* starts;             /* [requests + 1] or NULL */
+    const int* history;            /* [requests, history_width], rows history_stride apart; tokens outside the vocabulary are passed over */
+    int64_t history_stride;
+    int history_width;
+    const int* history_lens;       /* [requests] */
+    const int* prompt_lens;        /* [requests]: so many of them are the prompt's; NULL: none */
+    const int* drafted;            /* [rows]: the rows' own tokens; a row's path is those that its mask names */
+    const int64_t* masks;          /* [rows, words] */
+    int words;
+    const float* repetition;       /* [requests] each */
+    const float* presence;
+    const float* frequency;
+    const float* temperature;
+    const int* bias_tokens;        /* [requests, biases]; tokens outside the vocabulary stand for none, one that is listed again adds up */
+    const float* bias_values;
+    int biases;
+    const uint32_t* allowed;       /* [rows, allowed_stride]: bit v % 32 of word v / 32 */
+    int64_t allowed_stride;
+} sili_logit_rules;
+/* out [rows, vocab] (may be the logits) in the logits' type, rounded once.
+ * Rows lie `stride` elements apart. */
+int sili_adjust_logits(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
+                       const sili_logit_rules* rules, void* out, int64_t out_stride, void* stream);
+/* token[row]: the lowest of the tokens whose value by the rules is the largest
+ * (in fp32; the first NaN where there is one), -1 where none is above -inf or
+ * the row is no request's.  No logits are written.  scratch:
+ * sili_pick_tokens_scratch bytes. */
+int sili_pick_tokens_scratch(int64_t rows, int vocab, int64_t* bytes);
+int sili_pick_tokens(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
+                     const sili_logit_rules* rules, int* token, void* scratch, void* stream);
+
+/* The end of such a step.  From a request's row 0 (whose parent must be -1)
+ * on, the first row whose parent is the current one and whose drafted token is
+ * the current one's pick (int, or int64 with picked64; negative: none) follows
+ * it.  path[starts[r] + j]: the j-th of the kept[r] accepted rows, -1 after
+ * them and in rows of no request; token[r]: the last one's pick, -1 where
+ * nothing was kept; lens_out = committed + kept.  The accepted rows' keys and
+ * values move to the places behind the committed tokens in each of the
+ * n_caches caches (host arrays of device pointers; all of one shape and under
+ * one table).  Pages that lens took and lens_out does not go back to the ring
+ * in request order; the table keeps their entries, which nothing reads past a
+ * request's length.  But for the caches, the same inputs write the same values
+ * again. */
+int sili_settle_drafts(const int* drafted, const int* parents, const void* picked, int picked64, const int* starts,
+                       const int* lens, int requests, int64_t tokens, int* path, int* kept, int* token, int* lens_out,
+                       const int* table, int64_t table_stride, int width, int* ring, int ring_size, const int64_t* pool,
+                       int64_t* pool_out, int n_caches, void* const* codes, void* const* scales, int64_t n_pages, int page,
+                       int kv_heads, int dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -252,7 +252,9 @@ __device__ int64_t locate(const AttendArgs& a, Cursor<ROWS>& c, int cta, int cta
     return all;
 }
 
-template <typename T, int E, int NT>
+// TREE: the queries are drafted tokens.  A row sees the keys up to q.pos0 (the committed ones) as its window leaves them,
+// and of the request's own, which follow, those that its mask names.
+template <typename T, int E, int NT, bool TREE>
 struct Attend {
     using L = Layout<E, NT>;
     static constexpr int kStages = L::kStages;
@@ -278,6 +280,7 @@ struct Attend {
     float l[NT][2], o[kSteps][NT][4];
     int to[NT][2], from[NT][2];        // the columns' keys [from, to)
     int any_from, any_to, all_from, all_to;   // keys that any of the rows sees, that every row sees
+    int own, token[TREE ? NT : 1][2];         // TREE: the first drafted key, the columns' rows of q
 
     __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, float* factors)
         : a(args), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
@@ -364,12 +367,22 @@ struct Attend {
         const int h = c.h, group = a.heads / a.kv_heads;
         const int rows = c.q.nq * group, row0 = c.tile * kRows;     // below 2^31: the host has checked tokens * heads
         auto span = [&](int row, int& from_, int& to_) {
-            const int64_t pos = c.q.pos0 + row / group;
-            to_ = (int)min(pos + 1, (int64_t)c.q.len);
-            from_ = a.window ? (int)max(pos - a.window + 1, (int64_t)0) : 0;
+            if constexpr (TREE) {
+                int some = 0;
+                for (int i = 0; i < a.words; ++i)
+                    some += __popcll((unsigned long long)a.masks[(int64_t)(c.q.row0 + row / group) * a.words + i]);
+                to_ = some ? (int)min(max(c.q.pos0, (int64_t)0), (int64_t)c.q.len) : 0;
+                from_ = a.window ? (int)min(max(c.q.pos0 + some - a.window, (int64_t)0), (int64_t)0x7FFFFFFF) : 0;
+            } else {
+                const int64_t pos = c.q.pos0 + row / group;
+                to_ = (int)min(pos + 1, (int64_t)c.q.len);
+                from_ = a.window ? (int)max(pos - a.window + 1, (int64_t)0) : 0;
+            }
         };
-        span(row0, any_from, all_to);
-        span(min(row0 + kRows, rows) - 1, all_from, any_to);
+        if constexpr (!TREE) {
+            span(row0, any_from, all_to);
+            span(min(row0 + kRows, rows) - 1, all_from, any_to);
+        }
         if (kShared) __syncthreads();    // the last segment's fragments have been read
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -428,9 +441,32 @@ struct Attend {
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                span(min(row0 + n * 8 + 2 * t + j, rows - 1), from[n][j], to[n][j]);
+                const int row = min(row0 + n * 8 + 2 * t + j, rows - 1);
+                span(row, from[n][j], to[n][j]);
+                if constexpr (TREE) token[n][j] = c.q.row0 + row / group;
                 base[n][j] = kNoMaximum;
                 l[n][j] = 0.f;
+            }
+        }
+        if constexpr (TREE) {
+            own = (int)min(max(c.q.pos0, (int64_t)-0x7FFFFFFF), (int64_t)0x7FFFFFFF);
+            any_to = c.q.len;
+            all_to = 0x7FFFFFFF;
+            all_from = 0;
+            any_from = max(own, 0);       // (a row that sees a committed key sees the last of them, as far as a window goes)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    all_to = min(all_to, to[n][j]);
+                    all_from = max(all_from, from[n][j]);
+                    any_from = min(any_from, from[n][j]);
+                }
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                all_to = min(all_to, __shfl_xor_sync(0xffffffffu, all_to, o));
+                all_from = max(all_from, __shfl_xor_sync(0xffffffffu, all_from, o));
+                any_from = min(any_from, __shfl_xor_sync(0xffffffffu, any_from, o));
             }
         }
         if (kShared) {
@@ -448,7 +484,16 @@ struct Attend {
                 for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
     }
 
-    __device__ __forceinline__ bool sees(int key, int n, int j) const { return key < to[n][j] && key >= from[n][j]; }
+    __device__ __forceinline__ bool sees(int key, int n, int j) const {
+        if constexpr (TREE) {
+            if (key >= own) {
+                const uint32_t d = (uint32_t)key - (uint32_t)own;
+                return key < any_to && d < 64u * a.words &&
+                       (a.masks[(int64_t)token[n][j] * a.words + (d >> 6)] >> (d & 63) & 1);
+            }
+        }
+        return key < to[n][j] && key >= from[n][j];
+    }
 
     // Moves the columns' maxima to those of these keys' products x where they are larger; e: the exponents over them.
     __device__ __forceinline__ void raise(const float (&x)[NT][4], float (&e)[NT][4]) {
@@ -819,7 +864,7 @@ __device__ void blank_rows(const AttendArgs& a, int dim) {
     }
 }
 
-template <typename T, int E, int NT>
+template <typename T, int E, int NT, bool TREE>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_attend(const __grid_constant__ AttendArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_factors[8 * 4];
@@ -829,16 +874,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_atten
     int64_t begin, end;
     const int64_t all = locate<8 * NT>(a, c, blockIdx.x, gridDim.x, begin, end);
     if (begin >= end) return;
-    Attend<T, E, NT> k(a, smem, s_factors);
+    Attend<T, E, NT, TREE> k(a, smem, s_factors);
     k.run(c, begin, end, all, &s_last);
 }
 
-template <typename T, int E, int NT>
+template <typename T, int E, int NT, bool TREE>
 int launch(const AttendArgs& a, cudaStream_t s) {
     constexpr int smem = smem_bytes<T, E, NT>();
     static_assert(8 * NT * (32 * E + 4) <= 32 * 132, "the workspace holds the widest row tile");
     static_assert(8 * NT * (kMaxCtas + 2) * 4 <= Layout<E, NT>::kJoin, "the parts' weights fit the join space");
-    auto kernel = k_attend<T, E, NT>;
+    auto kernel = k_attend<T, E, NT, TREE>;
     static std::atomic<uint64_t> set{0};
     CKV(sili::allow_smem(kernel, smem, set));
     kernel<<<NT == 1 && E < 8 ? kMaxCtas : kMaxCtas / 2, kWarps * 32, smem, s>>>(a);
@@ -850,15 +895,51 @@ int launch(const AttendArgs& a, cudaStream_t s) {
 // Row tiles of 8, 16 or 32 (query, head) rows: the narrowest that holds a
 // request's rows, so that decoding wastes no columns and prompts read the
 // cache least often (registers hold no wider one: 32 rows x 128, 16 x 256).
-template <typename T, int E>
+template <typename T, int E, bool TREE>
 int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
-    if (rows <= 8) return launch<T, E, 1>(a, s);
-    if (rows <= 16 || E == 8) return launch<T, E, 2>(a, s);
-    return launch<T, E, E == 8 ? 2 : 4>(a, s);
+    if (rows <= 8) return launch<T, E, 1, TREE>(a, s);
+    if (rows <= 16 || E == 8) return launch<T, E, 2, TREE>(a, s);
+    return launch<T, E, E == 8 ? 2 : 4, TREE>(a, s);
 }
-template <typename T>
+template <typename T, bool TREE>
 int by_dim(const AttendArgs& a, int dim, int64_t rows, cudaStream_t s) {
-    return dim == 64 ? by_rows<T, 2>(a, rows, s) : dim == 128 ? by_rows<T, 4>(a, rows, s) : by_rows<T, 8>(a, rows, s);
+    return dim == 64 ? by_rows<T, 2, TREE>(a, rows, s) : dim == 128 ? by_rows<T, 4, TREE>(a, rows, s)
+                                                                    : by_rows<T, 8, TREE>(a, rows, s);
+}
+template <bool TREE>
+int by_type(int dtype, const AttendArgs& a, int dim, int64_t rows, cudaStream_t s) {
+    return dtype == SILI_F32 ? by_dim<float, TREE>(a, dim, rows, s)
+         : dtype == SILI_F16 ? by_dim<__half, TREE>(a, dim, rows, s) : by_dim<__nv_bfloat16, TREE>(a, dim, rows, s);
+}
+
+// What the two entries check, and the arguments that they pass on.
+int prepare(const char* who, int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int heads,
+            int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page, int kv_heads, const int* table,
+            int64_t table_stride, int width, const int* lens, int requests, const int* starts, int most_new, float scale,
+            int window, void* out, float* lse, void* workspace, AttendArgs& a) {
+    if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
+    if (dim != 64 && dim != 128 && dim != 256) return bad(who, "head dimension must be 64, 128 or 256");
+    if (page < 16 || page % 16) return bad(who, "page size must be a multiple of 16");
+    if (tokens < 0 || tokens > 0x7fffffffLL || heads < 1 || kv_heads < 1 || n_pages < 0 || width < 0 || requests < 0 || window < 0 || most_new < 0)
+        return bad(who, "sizes out of range");
+    if ((int64_t)kv_heads * page * dim > 0x7fffffffLL || n_pages > 0x7fffffffLL) return bad(who, "sizes out of range");
+    if (tokens * heads > 0x7fffff00LL) return bad(who, "sizes out of range");
+    if (heads % kv_heads) return bad(who, "the kv heads must divide the query heads");
+    if (tokens == 0) return SILI_OK;
+    if (!q || !out || !workspace || (requests && !lens) || (requests && width && !table) || (n_pages && (!codes || !scales)))
+        return bad(who, "null array");
+    if (requests && table_stride < width) return bad(who, "table rows overlap");
+    if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return bad(who, "codes and scales must be 16-byte aligned");
+    const int64_t item = dtype == SILI_F32 ? 4 : 2;
+    // (the stride of a single token or head is never used, and may be anything)
+    if ((uintptr_t)q % 8 || (tokens > 1 && q_token_stride * item % 8) || (heads > 1 && q_head_stride * item % 8))
+        return bad(who, "q rows must be 8-byte aligned");
+    if ((uintptr_t)out % 16) return bad(who, "out must be 16-byte aligned");
+    a = AttendArgs{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
+                   table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
+                   (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16)),
+                   (uint32_t)(kv_heads * page)};
+    return SILI_OK;
 }
 
 }  // namespace
@@ -896,35 +977,35 @@ int sili_kv4_attention(int dtype, const void* q, int64_t q_token_stride, int64_t
                        const int* table, int64_t table_stride, int width, const int* lens, int requests,
                        const int* starts, int most_new, float scale, int window, void* out, float* lse, void* workspace,
                        void* stream) {
-    const char* who = "kv4_attention";
-    if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
-    if (dim != 64 && dim != 128 && dim != 256) return bad(who, "head dimension must be 64, 128 or 256");
-    if (page < 16 || page % 16) return bad(who, "page size must be a multiple of 16");
-    if (tokens < 0 || tokens > 0x7fffffffLL || heads < 1 || kv_heads < 1 || n_pages < 0 || width < 0 || requests < 0 || window < 0 || most_new < 0)
-        return bad(who, "sizes out of range");
-    if ((int64_t)kv_heads * page * dim > 0x7fffffffLL || n_pages > 0x7fffffffLL) return bad(who, "sizes out of range");
-    if (tokens * heads > 0x7fffff00LL) return bad(who, "sizes out of range");
-    if (heads % kv_heads) return bad(who, "the kv heads must divide the query heads");
+    AttendArgs a{};
+    if (const int e = prepare("kv4_attention", dtype, q, q_token_stride, q_head_stride, tokens, heads, dim, codes, scales,
+                              n_pages, page, kv_heads, table, table_stride, width, lens, requests, starts, most_new, scale,
+                              window, out, lse, workspace, a))
+        return e;
     if (tokens == 0) return SILI_OK;
-    if (!q || !out || !workspace || (requests && !lens) || (requests && width && !table) || (n_pages && (!codes || !scales)))
-        return bad(who, "null array");
-    if (requests && table_stride < width) return bad(who, "table rows overlap");
-    if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return bad(who, "codes and scales must be 16-byte aligned");
-    const int64_t item = dtype == SILI_F32 ? 4 : 2;
-    // (the stride of a single token or head is never used, and may be anything)
-    if ((uintptr_t)q % 8 || (tokens > 1 && q_token_stride * item % 8) || (heads > 1 && q_head_stride * item % 8))
-        return bad(who, "q rows must be 8-byte aligned");
-    if ((uintptr_t)out % 16) return bad(who, "out must be 16-byte aligned");
-    AttendArgs a{q, q_token_stride, q_head_stride, tokens, heads, kv_heads, codes, scales, n_pages, page, table,
-                 table_stride, width, lens, requests, starts, scale, window, out, lse, workspace,
-                 (uint32_t)page / 16, page == 16 ? 0u : (uint32_t)((0x100000000ull + page / 16 - 1) / (page / 16)),
-                 (uint32_t)(kv_heads * page)};
     cudaStream_t s = (cudaStream_t)stream;
     if (starts && sili::kv4_prompt_takes(dtype, dim, tokens, heads, kv_heads, most_new))
         return sili::kv4_prompt_launch(dtype, dim, a, s);
-    const int64_t rows = (int64_t)std::max(most_new, 1) * (heads / kv_heads);
-    return dtype == SILI_F32 ? by_dim<float>(a, dim, rows, s)
-         : dtype == SILI_F16 ? by_dim<__half>(a, dim, rows, s) : by_dim<__nv_bfloat16>(a, dim, rows, s);
+    return by_type<false>(dtype, a, dim, (int64_t)std::max(most_new, 1) * (heads / kv_heads), s);
+}
+
+int sili_kv4_tree_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                            int heads, int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page,
+                            int kv_heads, const int* table, int64_t table_stride, int width, const int* lens, int requests,
+                            const int* starts, const int64_t* masks, int words, int most_new, float scale, int window,
+                            void* out, float* lse, void* workspace, void* stream) {
+    const char* who = "kv4_tree_attention";
+    AttendArgs a{};
+    if (const int e = prepare(who, dtype, q, q_token_stride, q_head_stride, tokens, heads, dim, codes, scales, n_pages, page,
+                              kv_heads, table, table_stride, width, lens, requests, starts, most_new, scale, window, out,
+                              lse, workspace, a))
+        return e;
+    if (words < 1 || words > 4) return bad(who, "masks must have 1 to 4 words a row");
+    if (tokens == 0) return SILI_OK;
+    if (!masks || (requests && !starts)) return bad(who, "null array");
+    a.masks = masks;
+    a.words = words;
+    return by_type<true>(dtype, a, dim, (int64_t)std::max(most_new, 1) * (heads / kv_heads), (cudaStream_t)stream);
 }
 
 }  // extern "C"

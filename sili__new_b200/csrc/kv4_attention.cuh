@@ -32,6 +32,8 @@ struct AttendArgs {
     uint32_t page_magic;   // ceil(2^32 / page16); 0 where page16 is 1
     uint32_t half_rows;    // token rows of K, and of V, in a page: kv_heads * page
     int polls, output_polls;   // of a wait before it gives up, and of a row tile's last one (kv4_prompt.cu sets them)
+    const int64_t* masks;      // [tokens, words]: the drafted keys that a row sees; null where there are no drafts
+    int words;
 
     // the table column of a key and the key's place in its page: one high product in place of a division, corrected by
     // one where the product is one too large (magic exceeds 2^32 / page16 by less than one)

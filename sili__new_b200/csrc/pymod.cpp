@@ -852,6 +852,60 @@ PYBIND11_MODULE(_cuda, m) {
                                  (const int*)lens, requests, (const int*)starts, most_new, scale, window, (void*)out,
                                  (float*)lse, (void*)workspace, (void*)stream));
     });
+    m.def("draft_tree_ptr", [](uintptr_t parents, uintptr_t starts, uintptr_t lens, int requests, int64_t tokens, int words,
+                               int window, uintptr_t masks, uintptr_t positions, uintptr_t stream) {
+        check(sili_draft_tree((const int*)parents, (const int*)starts, (const int*)lens, requests, tokens, words, window,
+                              (int64_t*)masks, (int*)positions, (void*)stream));
+    });
+    m.def("kv4_tree_attention_ptr", [](int dtype, uintptr_t q, int64_t qt, int64_t qh, int64_t tokens, int heads, int dim,
+                                       uintptr_t codes, uintptr_t scales, int64_t n_pages, int page, int kv_heads,
+                                       uintptr_t table, int64_t stride, int width, uintptr_t lens, int requests,
+                                       uintptr_t starts, uintptr_t masks, int words, int most_new, float scale, int window,
+                                       uintptr_t out, uintptr_t lse, uintptr_t workspace, uintptr_t stream) {
+        check(sili_kv4_tree_attention(dtype, (const void*)q, qt, qh, tokens, heads, dim, (const uint8_t*)codes,
+                                      (const uint8_t*)scales, n_pages, page, kv_heads, (const int*)table, stride, width,
+                                      (const int*)lens, requests, (const int*)starts, (const int64_t*)masks, words,
+                                      most_new, scale, window, (void*)out, (float*)lse, (void*)workspace, (void*)stream));
+    });
+    py::class_<sili_logit_rules>(m, "LogitRules").def(py::init([](
+            uintptr_t starts, uintptr_t history, int64_t history_stride, int history_width, uintptr_t history_lens,
+            uintptr_t prompt_lens, uintptr_t drafted, uintptr_t masks, int words, uintptr_t repetition, uintptr_t presence,
+            uintptr_t frequency, uintptr_t temperature, uintptr_t bias_tokens, uintptr_t bias_values, int biases,
+            uintptr_t allowed, int64_t allowed_stride) {
+        return sili_logit_rules{(const int*)starts, (const int*)history, history_stride, history_width,
+                                (const int*)history_lens, (const int*)prompt_lens, (const int*)drafted,
+                                (const int64_t*)masks, words, (const float*)repetition, (const float*)presence,
+                                (const float*)frequency, (const float*)temperature, (const int*)bias_tokens,
+                                (const float*)bias_values, biases, (const uint32_t*)allowed, allowed_stride};
+    }));
+    m.def("adjust_logits_ptr", [](int dtype, uintptr_t logits, int64_t stride, int64_t rows, int vocab, int requests,
+                                  const sili_logit_rules& rules, uintptr_t out, int64_t out_stride, uintptr_t stream) {
+        check(sili_adjust_logits(dtype, (const void*)logits, stride, rows, vocab, requests, &rules, (void*)out, out_stride,
+                                 (void*)stream));
+    });
+    m.def("pick_tokens_scratch", [](int64_t rows, int vocab) {
+        int64_t n = 0;
+        check(sili_pick_tokens_scratch(rows, vocab, &n));
+        return n;
+    });
+    m.def("pick_tokens_ptr", [](int dtype, uintptr_t logits, int64_t stride, int64_t rows, int vocab, int requests,
+                                const sili_logit_rules& rules, uintptr_t token, uintptr_t scratch, uintptr_t stream) {
+        check(sili_pick_tokens(dtype, (const void*)logits, stride, rows, vocab, requests, &rules, (int*)token,
+                               (void*)scratch, (void*)stream));
+    });
+    m.def("settle_drafts_ptr", [](uintptr_t drafted, uintptr_t parents, uintptr_t picked, bool picked64, uintptr_t starts,
+                                  uintptr_t lens, int requests, int64_t tokens, uintptr_t path, uintptr_t kept,
+                                  uintptr_t token, uintptr_t lens_out, uintptr_t table, int64_t stride, int width,
+                                  uintptr_t ring, int ring_size, uintptr_t pool, uintptr_t pool_out,
+                                  const std::vector<uintptr_t>& codes, const std::vector<uintptr_t>& scales,
+                                  int64_t n_pages, int page, int kv_heads, int dim, uintptr_t stream) {
+        if (codes.size() != scales.size()) throw std::invalid_argument("settle_drafts: codes and scales come in pairs");
+        check(sili_settle_drafts((const int*)drafted, (const int*)parents, (const void*)picked, picked64,
+                                 (const int*)starts, (const int*)lens, requests, tokens, (int*)path, (int*)kept,
+                                 (int*)token, (int*)lens_out, (const int*)table, stride, width, (int*)ring, ring_size,
+                                 (const int64_t*)pool, (int64_t*)pool_out, (int)codes.size(), (void* const*)codes.data(),
+                                 (void* const*)scales.data(), n_pages, page, kv_heads, dim, (void*)stream));
+    });
     m.def("fp32_fma_peak", [](int device, int iters) {
         double tf = 0, ms = 0;
         check(sili_fp32_fma_peak(device, iters, &tf, &ms));

@@ -626,3 +626,310 @@ def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, s
                                 1.0 / math.sqrt(dim) if scale is None else float(scale), window, out.data_ptr(),
                                 0 if lse is None else lse.data_ptr(), _workspace(dev, s).data_ptr(), s)
     return (out, lse) if return_lse else out
+
+
+# ── drafted tokens ───────────────────────────────────────────────────────────
+MASK_BITS = 64           # drafted tokens of a request that a mask word names
+MOST_DRAFTS = 256        # ... and a row's four words
+
+
+class DraftTree(NamedTuple):
+    """The plan of a step's trees (``draft_tree``)."""
+    masks: torch.Tensor       # int64 [tokens, words]: bit j: the row sees its request's row j
+    positions: torch.Tensor   # int32 [tokens]: committed + depth, -1: no row
+
+
+class Settled(NamedTuple):
+    """The end of a step (``settle_drafts``)."""
+    path: torch.Tensor        # int32 [tokens]: at starts[r] + j the j-th accepted row of request r, -1 after them
+    kept: torch.Tensor        # int32 [requests]: accepted rows
+    token: torch.Tensor       # int32 [requests]: the last one's pick, -1: no row
+    lens: torch.Tensor        # int32 [requests]: committed + kept
+    pool: torch.Tensor        # int64 [2]: the ring's pages taken and given, after this step
+
+
+def draft_tree(parents, starts, lens, most_new: int, window: int = 0) -> DraftTree:
+    """Masks and positions of a step's drafted tokens.
+
+    Request r's are the rows starts[r] .. starts[r + 1) (``starts``, ``lens``
+    int32 from ``page_tables``, which counts them as fresh tokens).
+    ``parents`` int32 [tokens]: the parent's place among the request's rows, a
+    smaller one, or -1 for a row that follows the committed tokens; a row with
+    another parent is none, and so are those that follow it.  ``most_new``: the
+    largest number of rows of a request, up to 256; rows past its next multiple
+    of 64 are none.  A row that is none, or of no request, has no mask bit and
+    position -1.  ``window`` > 0: only the nearest so many of a row and its
+    ancestors, for an attention with that window.  The positions go to
+    ``cache_append`` in place of ``page_tables``'s."""
+    who = "draft_tree"
+    tokens, requests = parents.numel(), lens.numel()
+    dev = parents.device
+    _contiguous(who, "parents", parents, _I32, (tokens,))
+    _contiguous(who, "lens", lens, _I32, (requests,))
+    _contiguous(who, "starts", starts, _I32, (requests + 1,))
+    if not 0 <= most_new <= MOST_DRAFTS:
+        raise ValueError(f"{who}: most_new must be 0 to {MOST_DRAFTS}, got {most_new}")
+    if window < 0:
+        raise ValueError(f"{who}: window must not be negative")
+    s = _on_device(who, dev, starts, lens)
+    words = max(-(-most_new // MASK_BITS), 1)
+    with _on(dev):
+        masks = torch.empty(tokens, words, dtype=_I64, device=dev)
+        positions = torch.empty(tokens, dtype=_I32, device=dev)
+        _cuda.draft_tree_ptr(parents.data_ptr(), starts.data_ptr(), lens.data_ptr(), requests, tokens, words,
+                             min(window, 0x7FFFFFFF), masks.data_ptr(), positions.data_ptr(), s)
+    return DraftTree(masks, positions)
+
+
+def _check_masks(who, masks, tokens):
+    if masks.dim() != 2 or not 1 <= masks.shape[1] <= MOST_DRAFTS // MASK_BITS:
+        raise ValueError(f"{who}: masks must be [tokens, 1 to {MOST_DRAFTS // MASK_BITS} words], got {list(masks.shape)}")
+    _contiguous(who, "masks", masks, _I64, (tokens, masks.shape[1]))
+
+
+def tree_attention(q, codes, scales, table, lens, starts, masks, most_new=None, scale=None, window: int = 0, out=None,
+                   return_lse: bool = False):
+    """``cache_attention`` of drafted tokens: row i of a request sees the
+    committed keys and, of the request's drafted ones (the last starts[r + 1] -
+    starts[r] of its lens[r] keys), those whose bits its mask has.
+
+    ``masks`` int64 [tokens, words] from ``draft_tree``, or any other; a row
+    without a bit sees nothing.  ``window`` > 0: as many of the committed keys,
+    the last ones, as the row's mask has bits fewer than that.  All else as in
+    ``cache_attention``."""
+    who = "tree_attention"
+    n_pages, hk, page, dim = _check_cache(who, codes, scales)
+    if page < 16 or page % 16:
+        raise ValueError(f"{who}: page size must be a multiple of 16, got {page}")
+    code = _dtype_code(q, who)
+    _heads(who, "q", q, None, dim)
+    tokens, heads, _ = q.shape
+    if heads < 1 or heads % hk:
+        raise ValueError(f"{who}: {hk} kv heads do not divide {heads} query heads")
+    requests = lens.numel()
+    _contiguous(who, "lens", lens, _I32, (requests,))
+    _check_block_table(who, table, requests)
+    _contiguous(who, "starts", starts, _I32, (requests + 1,))
+    _check_masks(who, masks, tokens)
+    if most_new is None:
+        most_new = -(-tokens // max(requests, 1))
+    if window < 0 or most_new < 0:
+        raise ValueError(f"{who}: window and most_new must not be negative")
+    window, most_new = min(window, 0x7FFFFFFF), min(most_new, 0x7FFFFFFF)
+    _no_gradient(who, q)
+    dev = q.device
+    s = _on_device(who, dev, codes, scales, table, lens, starts, masks, out)
+    with _on(dev):
+        if out is None:
+            out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
+        else:
+            _contiguous(who, "out", out, q.dtype, (tokens, heads, dim))
+        lse = torch.empty(tokens, heads, dtype=_F32, device=dev) if return_lse else None
+        _cuda.kv4_tree_attention_ptr(code, q.data_ptr(), q.stride(0), q.stride(1), tokens, heads, dim, codes.data_ptr(),
+                                     scales.data_ptr(), n_pages, page, hk, table.data_ptr(), _row_stride(table),
+                                     table.shape[1], lens.data_ptr(), requests, starts.data_ptr(), masks.data_ptr(),
+                                     masks.shape[1], most_new, 1.0 / math.sqrt(dim) if scale is None else float(scale),
+                                     window, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                     _workspace(dev, s).data_ptr(), s)
+    return (out, lse) if return_lse else out
+
+
+def _logit_rows(who, name, t):
+    """[rows, vocab] with the last axis contiguous and rows apart."""
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{who}: {name} must be [rows, vocab], got {list(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{who}: {name}'s last axis must be contiguous")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{who}: {name}'s rows overlap")
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _logit_rules(who, logits, starts, history, history_lens, prompt_lens, drafted, masks, repetition, presence, frequency,
+                 bias_tokens, bias_values, temperature, allowed, out=None):
+    """(type code, requests, rules, stream) of checked arguments."""
+    code = _dtype_code(logits, who)
+    _logit_rows(who, "logits", logits)
+    rows, vocab = logits.shape
+    if starts is None:
+        requests = rows
+    else:
+        requests = starts.numel() - 1
+        _contiguous(who, "starts", starts, _I32, (max(requests, 0) + 1,))
+    if (history is None) != (history_lens is None) or (history is None and prompt_lens is not None):
+        raise ValueError(f"{who}: history and history_lens come together, prompt_lens with them")
+    width = stride = 0
+    if history is not None:
+        _check_block_table(f"{who}: history as a", history, requests)
+        width, stride = history.shape[1], _row_stride(history)
+        _contiguous(who, "history_lens", history_lens, _I32, (requests,))
+        if prompt_lens is not None:
+            _contiguous(who, "prompt_lens", prompt_lens, _I32, (requests,))
+    if (drafted is None) != (masks is None):
+        raise ValueError(f"{who}: drafted and masks come together")
+    if drafted is not None:
+        if starts is None:
+            raise ValueError(f"{who}: drafted tokens need starts")
+        _contiguous(who, "drafted", drafted, _I32, (rows,))
+        _check_masks(who, masks, rows)
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency),
+                    ("temperature", temperature)):
+        if t is not None:
+            _contiguous(who, name, t, _F32, (requests,))
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError(f"{who}: bias_tokens and bias_values come together")
+    biases = 0
+    if bias_tokens is not None:
+        if bias_tokens.dim() != 2:
+            raise ValueError(f"{who}: bias_tokens must be [requests, biases], got {list(bias_tokens.shape)}")
+        biases = bias_tokens.shape[1]
+        _contiguous(who, "bias_tokens", bias_tokens, _I32, (requests, biases))
+        _contiguous(who, "bias_values", bias_values, _F32, (requests, biases))
+    words = 0
+    if allowed is not None:
+        _logit_rows(who, "allowed", allowed)
+        if allowed.dtype is not _I32 or allowed.shape != (rows, -(-vocab // 32)):
+            raise ValueError(f"{who}: allowed must be int32 {[rows, -(-vocab // 32)]}, got {allowed.dtype} "
+                             f"{list(allowed.shape)}")
+        words = allowed.stride(0) if rows > 1 else allowed.shape[1]
+    if out is not None:
+        _logit_rows(who, "out", out)
+        if out.shape != logits.shape or out.dtype is not logits.dtype:
+            raise ValueError(f"{who}: out must be {logits.dtype} {list(logits.shape)}, got {out.dtype} {list(out.shape)}")
+        if out.data_ptr() == logits.data_ptr():
+            if rows > 1 and out.stride(0) != logits.stride(0):
+                raise ValueError(f"{who}: out starts where the logits do, but its rows lie elsewhere")
+        elif _overlap(out, logits):
+            raise ValueError(f"{who}: out may be the logits, but not overlap them otherwise")
+    _no_gradient(who, logits, repetition, presence, frequency, temperature, bias_values)
+    s = _on_device(who, logits.device, starts, history, history_lens, prompt_lens, drafted, masks, repetition, presence,
+                   frequency, bias_tokens, bias_values, temperature, allowed, out)
+    rules = _cuda.LogitRules(_ptr(starts), _ptr(history), stride, width, _ptr(history_lens), _ptr(prompt_lens),
+                             _ptr(drafted), _ptr(masks), 0 if masks is None else masks.shape[1], _ptr(repetition),
+                             _ptr(presence), _ptr(frequency), _ptr(temperature), _ptr(bias_tokens), _ptr(bias_values),
+                             biases, _ptr(allowed), words)
+    return code, requests, rules, s
+
+
+def adjust_logits(logits, starts=None, history=None, history_lens=None, prompt_lens=None, drafted=None, masks=None,
+                  repetition=None, presence=None, frequency=None, bias_tokens=None, bias_values=None, temperature=None,
+                  allowed=None, out=None):
+    """Penalties for repeated tokens, biases, temperature and a grammar's mask
+    on ``logits`` [rows, vocab] (rows contiguous, any distance apart).
+
+    Request r's rows are starts[r] .. starts[r + 1) (int32; without it row r),
+    and ``history`` int32 [requests, width] holds the history_lens[r] tokens
+    behind which they stand, the first prompt_lens[r] of them (none by default)
+    the prompt's.  Rows of drafted tokens follow their own path, too: the
+    ``drafted`` int32 [rows] that their ``masks`` (``draft_tree``) name.  With
+    c(v) the times that token v stands in the history behind the prompt and on
+    the path, in fp32, each operation rounded::
+
+        x = x / repetition[r] if x > 0 else x * repetition[r]    # v in the history or on the path
+        x = x - frequency[r] * c(v) - presence[r]                # c(v) > 0
+        x = x + bias_values[r, j]                                # v = bias_tokens[r, j] (int32; outside the vocabulary: none)
+        x = x / temperature[r]                                   # temperature[r] > 0
+        x = -inf                                                 # bit v % 32 of allowed[row, v // 32] (int32) is not set
+
+    ``repetition``, ``presence``, ``frequency``, ``temperature``: float32
+    [requests]; every part may be left out.  A token that is listed twice gets
+    the sum of its biases.  Rows of no request are left as they are.  Returns
+    ``out`` (which may be the logits) in the logits' type."""
+    who = "adjust_logits"
+    code, requests, rules, s = _logit_rules(who, logits, starts, history, history_lens, prompt_lens, drafted, masks,
+                                            repetition, presence, frequency, bias_tokens, bias_values, temperature, allowed,
+                                            out)
+    dev = logits.device
+    rows, vocab = logits.shape
+    with _on(dev):
+        if out is None:
+            out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
+        _cuda.adjust_logits_ptr(code, logits.data_ptr(), logits.stride(0), rows, vocab, requests, rules, out.data_ptr(),
+                                out.stride(0), s)
+    return out
+
+
+def _overlap(a, b):
+    """Whether the memory between two [rows, vocab] arrays' first and last elements meets."""
+    if not a.numel() or not b.numel():
+        return False
+    size = lambda t: ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()  # noqa: E731
+    return a.data_ptr() < b.data_ptr() + size(b) and b.data_ptr() < a.data_ptr() + size(a)
+
+
+def pick_tokens(logits, starts=None, history=None, history_lens=None, prompt_lens=None, drafted=None, masks=None,
+                repetition=None, presence=None, frequency=None, bias_tokens=None, bias_values=None, temperature=None,
+                allowed=None):
+    """The token int32 [rows] with the largest value by the rules of
+    ``adjust_logits`` (in fp32, before any rounding to the logits' type): the
+    lowest one of equals, the first NaN where there is one, -1 where no token is
+    above -inf (a mask that allows none) and in rows of no request.  Writes no
+    logits."""
+    who = "pick_tokens"
+    code, requests, rules, s = _logit_rules(who, logits, starts, history, history_lens, prompt_lens, drafted, masks,
+                                            repetition, presence, frequency, bias_tokens, bias_values, temperature, allowed)
+    dev = logits.device
+    rows, vocab = logits.shape
+    with _on(dev):
+        token = torch.empty(rows, dtype=_I32, device=dev)
+        scratch = torch.empty(_cuda.pick_tokens_scratch(rows, vocab), dtype=_U8, device=dev)
+        _cuda.pick_tokens_ptr(code, logits.data_ptr(), logits.stride(0), rows, vocab, requests, rules, token.data_ptr(),
+                              scratch.data_ptr(), s)
+    return token
+
+
+def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, pool) -> Settled:
+    """Accepts drafted tokens and closes the step.
+
+    ``picked`` (int32 or int64 [tokens], as from ``pick_tokens`` or a sampler;
+    negative: none) is the model's own token behind each row.  A request's row 0
+    (parent -1: the token that the last step picked) is accepted, and from there
+    on the first row whose parent is the last accepted one and whose ``drafted``
+    token (int32 [tokens]) is that one's pick.  In every one of ``caches``
+    (``KVCache4`` or (codes, scales) pairs of one shape, all under ``table``:
+    the layers') the accepted rows' keys and values move up behind the committed
+    tokens; pages that only rejected rows had go back to the ring.
+
+    Pass the returned ``lens`` and ``pool`` on to the next ``page_tables``.  The
+    table's entries past a request's length are left as they are, and not read
+    again."""
+    who = "settle_drafts"
+    tokens, requests = drafted.numel(), lens.numel()
+    dev = lens.device
+    _contiguous(who, "drafted", drafted, _I32, (tokens,))
+    _contiguous(who, "parents", parents, _I32, (tokens,))
+    if picked.dtype not in (_I32, _I64):
+        raise ValueError(f"{who}: picked must be int32 or int64, got {picked.dtype}")
+    _contiguous(who, "picked", picked, picked.dtype, (tokens,))
+    _contiguous(who, "lens", lens, _I32, (requests,))
+    _contiguous(who, "starts", starts, _I32, (requests + 1,))
+    pairs = [(c.codes, c.scales) if isinstance(c, KVCache4) else tuple(c) for c in caches]
+    if not pairs:
+        raise ValueError(f"{who}: needs at least one cache")
+    n_pages, hk, page, dim = _check_cache(who, *pairs[0])
+    for codes, scales in pairs[1:]:
+        if codes.shape != pairs[0][0].shape:
+            raise ValueError(f"{who}: caches of different shapes: {list(codes.shape)} and {list(pairs[0][0].shape)}")
+        _check_cache(who, codes, scales)
+    _check_tables(who, table, ring, pool, page, requests)
+    if ring.numel() < 1:
+        raise ValueError(f"{who}: an empty ring")
+    codes, scales = [c for c, _ in pairs], [b for _, b in pairs]
+    at = [c.data_ptr() for c in codes], [b.data_ptr() for b in scales]
+    if n_pages and len(set(at[0])) < len(pairs):
+        raise ValueError(f"{who}: the same cache twice")
+    s = _on_device(who, dev, drafted, parents, picked, starts, table, ring, pool, *codes, *scales)
+    with _on(dev):
+        small = torch.empty(tokens + 3 * requests, dtype=_I32, device=dev)
+        pool_out = torch.empty(2, dtype=_I64, device=dev)
+        a = small.data_ptr()
+        b = a + 4 * tokens
+        _cuda.settle_drafts_ptr(drafted.data_ptr(), parents.data_ptr(), picked.data_ptr(), picked.dtype is _I64,
+                                starts.data_ptr(), lens.data_ptr(), requests, tokens, a, b, b + 4 * requests,
+                                b + 8 * requests, table.data_ptr(), _row_stride(table), table.shape[1], ring.data_ptr(),
+                                ring.numel(), pool.data_ptr(), pool_out.data_ptr(), *at, n_pages, page, hk, dim, s)
+        path, kept, token, lens_out = small.split_with_sizes((tokens, requests, requests, requests))
+    return Settled(path, kept, token, lens_out, pool_out)
