@@ -11,9 +11,12 @@
 // A CTA takes a tile of the vocabulary and a few consecutive rows.  The
 // tokens of a request's history that lie in the tile are counted in shared
 // memory, once for the rows that share it; a row's path (the drafted tokens
-// that its mask names) is counted on top and taken off again.  A bit a token
-// tells which need the penalties at all: the rest is one pass over the row
-// with 16-byte accesses, so the logits' bytes are what bounds it.
+// that its mask names) is counted on top and taken off again, where any of it
+// lies in the tile.  The tokens so touched are also listed, each once: they
+// are taken one by one, and the rest of a row is one pass over registers that
+// only divides by the temperature and masks.  A pick compares the rest before
+// the division, which keeps the order; what it may make equal is told apart
+// for the few elements next to the largest.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -21,7 +24,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 #include "sili_b200.h"
 
 namespace sili {
@@ -41,6 +44,9 @@ int bad(const char* who, const char* what) {
 }
 
 constexpr int kThreads = 256;
+constexpr int kEach = 16;                      // elements of a row that a thread holds in registers
+constexpr int kTile = kThreads * kEach;        // tokens of a tile
+constexpr int kGroup = 8;                      // rows of a CTA at most
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
 
 struct LogitArgs {
@@ -70,7 +76,7 @@ struct LogitArgs {
     int64_t allowed_stride;
     unsigned long long* best;  // [rows, tiles]: a tile's largest
     int* token;                // [rows]
-    int tile, tiles, group;    // tokens of a tile, tiles, rows of a CTA
+    int tiles, group;          // tiles, rows of a CTA
 };
 
 // A larger value, then a lower token, has the larger key; NaN is above all numbers (the first one is picked) and -inf below
@@ -82,31 +88,83 @@ __device__ __forceinline__ unsigned long long key_of(float y, int token) {
     return (unsigned long long)u << 32 | (0xFFFFFFFFu - (uint32_t)token);
 }
 
-struct Rules {
-    float rep, freq, pres, temp;
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+
+// Division by one number, many times: with r the rounded reciprocal of t, a quotient within a unit of x / t becomes the
+// rounded one by q + r (x - t q) in two fused steps (Markstein, 1990), where nothing on the way leaves the normal range.
+struct Divisor {
+    float t, r;
+    bool on, fast;
+    __device__ __forceinline__ void set(float temp) {
+        t = temp;
+        on = temp > 0.f && temp != 1.f;
+        fast = temp >= 0x1p-20f && temp <= 0x1p20f;
+        r = fast ? __frcp_rn(temp) : 0.f;
+    }
+    __device__ __forceinline__ bool takes(float x) const {     // 2^-60 <= |x| < 2^100
+        return fast && ((__float_as_uint(x) << 1) - (67u << 24)) < (160u << 24);
+    }
+    __device__ __forceinline__ float quick(float x) const {
+        float q = x * r;
+        q = fmaf(fmaf(-t, q, x), r, q);
+        return fmaf(fmaf(-t, q, x), r, q);
+    }
+    __device__ __forceinline__ float operator()(float x) const { return !on ? x : takes(x) ? quick(x) : x / t; }
+};
+
+struct Shared {
+    uint32_t cnt[kTile];                       // a token's count and marks
+    uint32_t touched[kTile / 32 + 1];          // a bit a token whose count is not 0
+    uint16_t list[kTile];                      // those tokens
+    uint16_t draft[256];                       // the request's drafted tokens, 0xFFFF: not in the tile
+    unsigned long long masks[kGroup][4];
+    unsigned long long top[kThreads / 32];
+    int listed, has_path[kGroup];
+    float value[1];                            // [kTile] biases, then (writing) [kTile] the listed tokens' results
 };
 
 template <typename T, bool WRITE>
 struct Logits {
-    static constexpr int kVec = 16 / sizeof(T);
+    static constexpr int kVec = 16 / sizeof(T), kPacks = kEach / kVec;
     using P = sili::Pack<T, kVec>;
     const LogitArgs& a;
-    uint32_t* cnt;        // [tile]
-    uint32_t* touched;    // [tile / 32 + 1]: a bit a token whose count is not 0
-    float* bias;          // [tile], where kBiased says so
+    Shared& s;
+    float *bias, *result;
     int t0, n;            // the tile's first token, its tokens
     const uint32_t* allow;
-    Rules w;
+    float rep, freq, pres;
+    Divisor by;
 
     __device__ __forceinline__ void note(uint32_t i, uint32_t what) const {
-        if (what & kCount) atomicAdd(cnt + i, what); else atomicOr(cnt + i, what);
-        atomicOr(touched + (i >> 5), 1u << (i & 31));
+        if (what & kCount) atomicAdd(s.cnt + i, what); else atomicOr(s.cnt + i, what);
+        const uint32_t bit = 1u << (i & 31);
+        if (!(atomicOr(s.touched + (i >> 5), bit) & bit)) s.list[atomicAdd(&s.listed, 1)] = (uint16_t)i;
     }
-    // the tokens of the request's history and bias list that lie in the tile
-    __device__ void count_request(int r) {
-        for (int i = threadIdx.x; i < n; i += kThreads) cnt[i] = 0;
-        for (int i = threadIdx.x; i <= a.tile / 32; i += kThreads) touched[i] = 0;
+    // the tokens of the request's history and bias list that lie in the tile, and which of rows [row, last) have a path there
+    __device__ void count_request(int r, int64_t row, int64_t last, int64_t row0, int64_t row1) {
+        for (int i = threadIdx.x; i < kTile; i += kThreads) s.cnt[i] = 0;
+        for (int i = threadIdx.x; i <= kTile / 32; i += kThreads) s.touched[i] = 0;
+        if (threadIdx.x == 0) s.listed = 0;
+        if (a.drafted) {
+            const uint32_t v = row0 + threadIdx.x < row1 && (int)threadIdx.x < 64 * a.words
+                                   ? (uint32_t)a.drafted[row0 + threadIdx.x] - (uint32_t)t0 : 0xFFFFFFFFu;
+            s.draft[threadIdx.x] = v < (uint32_t)n ? (uint16_t)v : (uint16_t)0xFFFFu;
+            const int64_t k = row + threadIdx.x / 4;
+            const int w = threadIdx.x & 3;
+            if (threadIdx.x < 4 * kGroup) {
+                s.masks[threadIdx.x / 4][w] = k < last && w < a.words ? (unsigned long long)a.masks[k * a.words + w] : 0;
+                s.has_path[threadIdx.x / 4] = 0;
+            }
+        }
         __syncthreads();
+        if (a.drafted && s.draft[threadIdx.x] != 0xFFFFu)
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+                if (s.masks[k][threadIdx.x >> 6] >> (threadIdx.x & 63) & 1) s.has_path[k] = 1;
         if (a.history) {
             const int* h = a.history + r * a.history_stride;
             const int len = min(max(a.history_lens[r], 0), a.history_width);
@@ -137,43 +195,33 @@ struct Logits {
         }
         __syncthreads();
     }
-    // the row's path on top of the counts, or off them again
-    __device__ void count_path(int64_t row, int64_t row0, int64_t row1, bool off) {
-        if (!a.drafted) return;
-        for (int j = threadIdx.x; j < 64 * a.words; j += kThreads) {
-            if (!((uint64_t)a.masks[row * a.words + (j >> 6)] >> (j & 63) & 1) || row0 + j >= row1) continue;
-            const uint32_t i = (uint32_t)a.drafted[row0 + j] - (uint32_t)t0;
-            if (i >= (uint32_t)n) continue;
+    // the path of the CTA's row k on top of the counts, or off them again (the list is then cut to what it was)
+    __device__ void count_path(int k, bool off, int listed) const {
+        const uint32_t i = s.draft[threadIdx.x];
+        if (i != 0xFFFFu && (s.masks[k][threadIdx.x >> 6] >> (threadIdx.x & 63) & 1)) {
             if (!off) note(i, 1u);
-            else if (atomicSub(cnt + i, 1u) == 1u) atomicAnd(touched + (i >> 5), ~(1u << (i & 31)));
+            else if (atomicSub(s.cnt + i, 1u) == 1u) atomicAnd(s.touched + (i >> 5), ~(1u << (i & 31)));
         }
+        if (off && threadIdx.x == 0) s.listed = listed;
         __syncthreads();
     }
 
     __device__ __forceinline__ float ruled(float x, uint32_t what, int i) const {
-        if (what) {
-            // (a count also makes it seen)
-            if (what & (kSeen | kCount)) x = x > 0.f ? x / w.rep : x * w.rep;
-            if (what & kCount) {
-                x = x - w.freq * (float)(what & kCount);
-                x = x - w.pres;
-            }
-            if (what & kBiased) x = x + bias[i];
+        // (a count also makes it seen)
+        if (what & (kSeen | kCount)) x = x > 0.f ? x / rep : x * rep;
+        if (what & kCount) {
+            x = x - freq * (float)(what & kCount);
+            x = x - pres;
         }
-        return w.temp > 0.f ? x / w.temp : x;
-    }
-    // bits [i, i + 8) of the tile's tokens, of which there is one word more than the tile needs
-    static __device__ __forceinline__ uint32_t bits8(const uint32_t* words, int i) {
-        return __funnelshift_r(words[i >> 5], words[(i >> 5) + 1], i & 31) & 0xFFu;
+        if (what & kBiased) x = x + bias[i];
+        return by(x);
     }
     __device__ __forceinline__ bool may(int i) const {
         const int v = t0 + i;
         return !allow || (__ldg(allow + (v >> 5)) >> (v & 31) & 1);
     }
-    __device__ __forceinline__ unsigned long long single(const T* x, T* y, int i) const {
-        const float v = may(i) ? ruled(sili::to_f32(x[i]), cnt[i], i) : -INFINITY;
-        if (WRITE) y[i] = sili::from_f32<T>(v);
-        return WRITE ? 0 : key_of(v, t0 + i);
+    __device__ __forceinline__ float single(T x, int i) const {
+        return may(i) ? ruled(sili::to_f32(x), s.cnt[i], i) : -INFINITY;
     }
 
     // one row of the tile; returns this thread's largest key
@@ -181,28 +229,97 @@ struct Logits {
         unsigned long long top = 0;
         // whole 16 bytes from the first aligned element on
         const int lead = (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
-        const bool vectors = (uintptr_t)x % sizeof(T) == 0 && (!WRITE || (uintptr_t)y % 16 == (uintptr_t)x % 16);
-        const int head = vectors ? min(lead, n) : n, packs = (n - head) / kVec, tail = head + packs * kVec;
-        for (int i = threadIdx.x; i < head; i += kThreads) top = max(top, single(x, y, i));
-        for (int i = tail + threadIdx.x; i < n; i += kThreads) top = max(top, single(x, y, i));
-        for (int p0 = threadIdx.x; p0 < packs; p0 += 4 * kThreads) {
-            P in[4];
+        const int head = !WRITE || (uintptr_t)y % 16 == (uintptr_t)x % 16 ? min(lead, n) : n;
+        const int packs = (n - head) / kVec, tail = head + packs * kVec;
+        P in[kPacks];
+        uint32_t words[kPacks][2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (p0 + k * kThreads < packs) in[k] = *(const P*)(x + head + (p0 + k * kThreads) * kVec);
+        for (int k = 0; k < kPacks; ++k) {
+            const int p = threadIdx.x + k * kThreads;
+            words[k][0] = words[k][1] = 0xFFFFFFFFu;
+            if (p < packs) {
+                in[k] = *(const P*)(x + head + p * kVec);
+                if (allow) {
+                    const int v = t0 + head + p * kVec;
+                    words[k][0] = __ldg(allow + (v >> 5));
+                    words[k][1] = __ldg(allow + ((v + kVec - 1) >> 5));
+                }
+            }
+        }
+        const int listed = s.listed;
+        for (int e = threadIdx.x; e < listed; e += kThreads) {
+            const int i = s.list[e];
+            const float v = single(x[i], i);
+            if (WRITE) result[e] = v; else top = max(top, key_of(v, t0 + i));
+        }
+        if (WRITE && listed) __syncthreads();     // (y may be x)
+        for (int i = threadIdx.x; i < n - packs * kVec; i += kThreads) {
+            const int j = i < head ? i : i - head + tail;
+            const float v = single(x[j], j);
+            if (WRITE) y[j] = sili::from_f32<T>(v); else top = max(top, key_of(v, t0 + j));
+        }
+        float most = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (p0 + k * kThreads >= packs) break;
-                const int i = head + (p0 + k * kThreads) * kVec;
-                const uint32_t some = bits8(touched, i);
+        for (int k = 0; k < kPacks; ++k) {
+            const int p = threadIdx.x + k * kThreads;
+            if (p >= packs) break;
+            const int i = head + p * kVec;
+            uint32_t take = __funnelshift_r(words[k][0], words[k][1], (t0 + i) & 31);
+            if (WRITE) {
                 P out;
+                bool quick = by.fast;
+                float v[kVec];
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    const float v = may(i + e) ? ruled(sili::to_f32(in[k].v[e]), some >> e & 1 ? cnt[i + e] : 0u, i + e) : -INFINITY;
-                    if (WRITE) out.v[e] = sili::from_f32<T>(v);
-                    else top = max(top, key_of(v, t0 + i + e));
+                    v[e] = sili::to_f32(in[k].v[e]);
+                    quick = quick && by.takes(v[e]);
                 }
-                if (WRITE) *(P*)(y + i) = out;
+                if (by.on) {
+                    if (quick)
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) v[e] = by.quick(v[e]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) v[e] = v[e] / by.t;
+                }
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) out.v[e] = sili::from_f32<T>(take >> e & 1 ? v[e] : -INFINITY);
+                *(P*)(y + i) = out;
+            } else {
+                take &= ~__funnelshift_r(s.touched[i >> 5], s.touched[(i >> 5) + 1], i & 31);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e)
+                    most = max_nan(most, take >> e & 1 ? sili::to_f32(in[k].v[e]) : -INFINITY);
+            }
+        }
+        if (WRITE) {
+            if (listed) {
+                __syncthreads();
+                for (int e = threadIdx.x; e < listed; e += kThreads) y[s.list[e]] = sili::from_f32<T>(result[e]);
+            }
+        } else {
+            // the warp's largest, and its first place: in the threads that hold it, next to it or the same after the division
+            const float best = by(most);
+            const uint32_t mine = (uint32_t)(key_of(best, 0) >> 32), all = __reduce_max_sync(0xffffffffu, mine);
+            if (all && mine == all) {
+                // (quotients that leave the normal range: any of them may be the same)
+                const float near = by.on && !by.takes(most) ? -INFINITY : most - fabsf(most) * 0x1p-20f;
+                bool found = false;
+#pragma unroll
+                for (int k = 0; k < kPacks; ++k) {
+                    const int i = head + (threadIdx.x + k * kThreads) * kVec;
+                    if (threadIdx.x + k * kThreads >= packs) break;
+                    const uint32_t take = __funnelshift_r(words[k][0], words[k][1], (t0 + i) & 31) &
+                                          ~__funnelshift_r(s.touched[i >> 5], s.touched[(i >> 5) + 1], i & 31);
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        const float v = sili::to_f32(in[k].v[e]);
+                        if (!found && (take >> e & 1) && !(v < near)) {
+                            const unsigned long long key = key_of(by(v), t0 + i + e);
+                            if ((uint32_t)(key >> 32) == all) { found = true; top = max(top, key); }
+                        }
+                    }
+                }
             }
         }
         return top;
@@ -211,20 +328,19 @@ struct Logits {
 
 template <typename T, bool WRITE>
 __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ LogitArgs a) {
-    extern __shared__ uint32_t smem[];
-    __shared__ unsigned long long s_top[kThreads / 32];
-    Logits<T, WRITE> k{a};
-    k.cnt = smem;
-    k.touched = smem + a.tile;
-    k.bias = (float*)(smem + a.tile + a.tile / 32 + 2);
-    k.t0 = blockIdx.x * a.tile;
-    k.n = min(a.tile, a.vocab - k.t0);
-    const int64_t first = (int64_t)blockIdx.y * a.group, last = min(first + a.group, a.rows);
-    int64_t row0 = 0, row1 = -1;      // the current request's rows
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared& s = *(Shared*)smem;
+    Logits<T, WRITE> k{a, s, s.value, s.value + (a.biases ? kTile : 0)};
+    const int tile = blockIdx.x % a.tiles;
+    k.t0 = tile * kTile;
+    k.n = min(kTile, a.vocab - k.t0);
+    const int64_t first = (int64_t)(blockIdx.x / a.tiles) * a.group, last = min(first + a.group, a.rows);
+    int64_t begin = first, row0 = 0, row1 = -1;      // the current request's rows, the first of them here
     int r = -1;
     for (int64_t row = first; row < last; ++row) {
         if (row >= row1) {
             // the request that holds the row, if any
+            begin = row;
             if (!a.starts) {
                 r = row < a.requests ? (int)row : -1;
                 row0 = row;
@@ -244,11 +360,12 @@ __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ Log
                 if (r < 0) { row0 = row; row1 = row + 1; }
             }
             if (r >= 0) {
-                k.count_request(r);
-                k.w.rep = a.repetition ? a.repetition[r] : 1.f;
-                k.w.freq = a.frequency ? a.frequency[r] : 0.f;
-                k.w.pres = a.presence ? a.presence[r] : 0.f;
-                k.w.temp = a.temperature ? a.temperature[r] : 0.f;
+                __syncthreads();     // the last request's counts have been read
+                k.count_request(r, row, min(last, row1), row0, row1);
+                k.rep = a.repetition ? a.repetition[r] : 1.f;
+                k.freq = a.frequency ? a.frequency[r] : 0.f;
+                k.pres = a.presence ? a.presence[r] : 0.f;
+                k.by.set(a.temperature ? a.temperature[r] : 0.f);
             }
         }
         const T* x = (const T*)a.x + row * a.x_stride + k.t0;
@@ -260,26 +377,30 @@ __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ Log
                 for (int i = threadIdx.x; i < k.n; i += kThreads) y[i] = x[i];
         } else {
             k.allow = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-            k.count_path(row, row0, row1, false);
-            top = k.row(x, y);
-            if (a.drafted) {
+            const bool path = a.drafted && s.has_path[row - begin];
+            const int listed = s.listed;
+            if (path) {
                 __syncthreads();
-                k.count_path(row, row0, row1, true);
+                k.count_path((int)(row - begin), false, 0);
+            }
+            top = k.row(x, y);
+            if (path) {
+                __syncthreads();
+                k.count_path((int)(row - begin), true, listed);
             }
         }
         if (!WRITE) {
 #pragma unroll
             for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             __syncthreads();
-            if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+            if ((threadIdx.x & 31) == 0) s.top[threadIdx.x >> 5] = top;
             __syncthreads();
             if (threadIdx.x == 0) {
 #pragma unroll
-                for (int i = 1; i < kThreads / 32; ++i) top = max(top, s_top[i]);
-                a.best[row * a.tiles + blockIdx.x] = top;
+                for (int i = 1; i < kThreads / 32; ++i) top = max(top, s.top[i]);
+                a.best[row * a.tiles + tile] = top;
             }
         }
-        if (row + 1 >= row1) __syncthreads();     // the next request's counts come over these
     }
 }
 
@@ -294,16 +415,13 @@ __global__ void __launch_bounds__(128) k_picked(const unsigned long long* best, 
     if ((threadIdx.x & 31) == 0) token[row] = top ? (int)(0xFFFFFFFFu - (uint32_t)top) : -1;
 }
 
-// Tokens of a tile, and rows of a CTA.
-constexpr int kTile = 8192;
-int tile_of(int vocab) { return std::min(kTile, (vocab + 31) / 32 * 32); }
-
 template <typename T, bool WRITE>
 int launch(LogitArgs& a, cudaStream_t s) {
-    const int smem = (a.tile + a.tile / 32 + 2 + (a.biases ? a.tile : 0)) * 4;
+    const int smem = (int)sizeof(Shared) + ((a.biases ? kTile : 0) + (WRITE ? kTile : 0)) * 4;
     auto kernel = k_logits<T, WRITE>;
-    if (smem > 48 * 1024) CKL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<dim3(a.tiles, (unsigned)((a.rows + a.group - 1) / a.group)), kThreads, smem, s>>>(a);
+    static std::atomic<uint64_t> set{0};
+    if (smem > 48 * 1024) CKL(sili::allow_smem(kernel, (int)sizeof(Shared) + 2 * kTile * 4, set));
+    kernel<<<(unsigned)((a.rows + a.group - 1) / a.group * a.tiles), kThreads, smem, s>>>(a);
     sili::count_launch();
     CKL(cudaGetLastError());
     return SILI_OK;
@@ -341,12 +459,11 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
     a = LogitArgs{logits, stride, nullptr, 0, rows, vocab, requests, q.starts, q.history_width ? q.history : nullptr,
                   q.history_stride, q.history_width, q.history_lens, q.prompt_lens, q.drafted, q.masks, q.words,
                   q.repetition, q.presence, q.frequency, q.temperature, q.bias_tokens, q.bias_values, q.biases, q.allowed,
-                  q.allowed_stride, nullptr, nullptr, tile_of(vocab), 0, 0};
-    a.tiles = (vocab + a.tile - 1) / a.tile;
+                  q.allowed_stride, nullptr, nullptr, (vocab + kTile - 1) / kTile, 0};
     // rows that share a request's counts, as far as the mean goes
     const int64_t mean = requests ? (rows + requests - 1) / requests : rows;
-    a.group = (int)std::min<int64_t>(8, std::max<int64_t>(1, mean));
-    if ((rows + a.group - 1) / a.group > 65535) a.group = (int)((rows + 65534) / 65535);
+    a.group = (int)std::min<int64_t>(kGroup, std::max<int64_t>(1, mean));
+    if ((rows + a.group - 1) / a.group * a.tiles > 0x7fffffffLL) return bad(who, "sizes out of range");
     return SILI_OK;
 }
 
@@ -371,7 +488,7 @@ int sili_adjust_logits(int dtype, const void* logits, int64_t stride, int64_t ro
 int sili_pick_tokens_scratch(int64_t rows, int vocab, int64_t* bytes) {
     if (!bytes) return bad("pick_tokens_scratch", "null array");
     if (rows < 0 || rows > 0x7fffffffLL || vocab < 1) return bad("pick_tokens_scratch", "sizes out of range");
-    *bytes = rows * ((vocab + tile_of(vocab) - 1) / tile_of(vocab)) * 8;
+    *bytes = rows * ((vocab + kTile - 1) / kTile) * 8;
     return SILI_OK;
 }
 
