@@ -47,6 +47,7 @@ constexpr int kThreads = 256;
 constexpr int kEach = 16;                      // elements of a row that a thread holds in registers
 constexpr int kTile = kThreads * kEach;        // tokens of a tile
 constexpr int kGroup = 8;                      // rows of a CTA at most
+static_assert(kGroup <= kThreads / 32, "a warp a row picks");
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
 
 struct LogitArgs {
@@ -113,7 +114,8 @@ struct Divisor {
         q = fmaf(fmaf(-t, q, x), r, q);
         return fmaf(fmaf(-t, q, x), r, q);
     }
-    __device__ __forceinline__ float operator()(float x) const { return !on ? x : takes(x) ? quick(x) : x / t; }
+    __device__ __forceinline__ float over(float x) const { return takes(x) ? quick(x) : x / t; }
+    __device__ __forceinline__ float operator()(float x) const { return on ? over(x) : x; }
 };
 
 struct Shared {
@@ -122,8 +124,9 @@ struct Shared {
     uint16_t list[kTile];                      // those tokens
     uint16_t draft[256];                       // the request's drafted tokens, 0xFFFF: not in the tile
     unsigned long long masks[kGroup][4];
-    unsigned long long top[kThreads / 32];
-    int listed, has_path[kGroup];
+    unsigned long long key[kGroup][kThreads / 32];     // picking: a warp's largest key of touched and single elements,
+    uint32_t y[kGroup][kThreads / 32];                 // and the upper half of that of the others
+    int listed, has_path[kGroup], twice;
     float value[1];                            // [kTile] biases, then (writing) [kTile] the listed tokens' results
 };
 
@@ -136,19 +139,20 @@ struct Logits {
     float *bias, *result;
     int t0, n;            // the tile's first token, its tokens
     const uint32_t* allow;
-    float rep, freq, pres;
-    Divisor by;
+    float freq, pres;
+    Divisor rep, by;
 
-    __device__ __forceinline__ void note(uint32_t i, uint32_t what) const {
-        if (what & kCount) atomicAdd(s.cnt + i, what); else atomicOr(s.cnt + i, what);
+    __device__ __forceinline__ uint32_t note(uint32_t i, uint32_t what) const {
+        const uint32_t was = what & kCount ? atomicAdd(s.cnt + i, what) : atomicOr(s.cnt + i, what);
         const uint32_t bit = 1u << (i & 31);
-        if (!(atomicOr(s.touched + (i >> 5), bit) & bit)) s.list[atomicAdd(&s.listed, 1)] = (uint16_t)i;
+        if (!was && !(atomicOr(s.touched + (i >> 5), bit) & bit)) s.list[atomicAdd(&s.listed, 1)] = (uint16_t)i;
+        return was;
     }
     // the tokens of the request's history and bias list that lie in the tile, and which of rows [row, last) have a path there
     __device__ void count_request(int r, int64_t row, int64_t last, int64_t row0, int64_t row1) {
         for (int i = threadIdx.x; i < kTile; i += kThreads) s.cnt[i] = 0;
         for (int i = threadIdx.x; i <= kTile / 32; i += kThreads) s.touched[i] = 0;
-        if (threadIdx.x == 0) s.listed = 0;
+        if (threadIdx.x == 0) s.listed = s.twice = 0;
         if (a.drafted) {
             const uint32_t v = row0 + threadIdx.x < row1 && (int)threadIdx.x < 64 * a.words
                                    ? (uint32_t)a.drafted[row0 + threadIdx.x] - (uint32_t)t0 : 0xFFFFFFFFu;
@@ -179,19 +183,26 @@ struct Logits {
             const int* list = a.bias_tokens + (int64_t)r * a.biases;
             const float* value = a.bias_values + (int64_t)r * a.biases;
             for (int j = threadIdx.x; j < a.biases; j += kThreads) {
-                const int v = list[j];
-                const uint32_t i = (uint32_t)v - (uint32_t)t0;
+                const uint32_t i = (uint32_t)list[j] - (uint32_t)t0;
                 if (i >= (uint32_t)n) continue;
-                // a token that is listed again: the first place adds them up, in order
-                bool first = true;
-                for (int k = 0; k < j; ++k) first = first && list[k] != v;
-                if (!first) continue;
-                float sum = value[j];
-                for (int k = j + 1; k < a.biases; ++k)
-                    if (list[k] == v) sum += value[k];
-                bias[i] = sum;
-                note(i, kBiased);
+                bias[i] = value[j];
+                if (note(i, kBiased) & kBiased) s.twice = 1;
             }
+            __syncthreads();
+            if (s.twice)
+                // a token is listed again: its first place adds all of them up, in order
+                for (int j = threadIdx.x; j < a.biases; j += kThreads) {
+                    const int v = list[j];
+                    const uint32_t i = (uint32_t)v - (uint32_t)t0;
+                    if (i >= (uint32_t)n) continue;
+                    bool first = true;
+                    for (int k = 0; k < j; ++k) first = first && list[k] != v;
+                    if (!first) continue;
+                    float sum = value[j];
+                    for (int k = j + 1; k < a.biases; ++k)
+                        if (list[k] == v) sum += value[k];
+                    bias[i] = sum;
+                }
         }
         __syncthreads();
     }
@@ -208,7 +219,7 @@ struct Logits {
 
     __device__ __forceinline__ float ruled(float x, uint32_t what, int i) const {
         // (a count also makes it seen)
-        if (what & (kSeen | kCount)) x = x > 0.f ? x / rep : x * rep;
+        if (what & (kSeen | kCount)) x = x > 0.f ? rep.over(x) : x * rep.t;
         if (what & kCount) {
             x = x - freq * (float)(what & kCount);
             x = x - pres;
@@ -224,8 +235,8 @@ struct Logits {
         return may(i) ? ruled(sili::to_f32(x), s.cnt[i], i) : -INFINITY;
     }
 
-    // one row of the tile; returns this thread's largest key
-    __device__ unsigned long long row(const T* x, T* y) const {
+    // one row of the tile, the CTA's row k of the request
+    __device__ void row(const T* x, T* y, int at) const {
         unsigned long long top = 0;
         // whole 16 bytes from the first aligned element on
         const int lead = (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
@@ -298,31 +309,60 @@ struct Logits {
                 for (int e = threadIdx.x; e < listed; e += kThreads) y[s.list[e]] = sili::from_f32<T>(result[e]);
             }
         } else {
-            // the warp's largest, and its first place: in the threads that hold it, next to it or the same after the division
-            const float best = by(most);
-            const uint32_t mine = (uint32_t)(key_of(best, 0) >> 32), all = __reduce_max_sync(0xffffffffu, mine);
-            if (all && mine == all) {
-                // (quotients that leave the normal range: any of them may be the same)
-                const float near = by.on && !by.takes(most) ? -INFINITY : most - fabsf(most) * 0x1p-20f;
-                bool found = false;
-#pragma unroll
-                for (int k = 0; k < kPacks; ++k) {
-                    const int i = head + (threadIdx.x + k * kThreads) * kVec;
-                    if (threadIdx.x + k * kThreads >= packs) break;
-                    const uint32_t take = __funnelshift_r(words[k][0], words[k][1], (t0 + i) & 31) &
-                                          ~__funnelshift_r(s.touched[i >> 5], s.touched[(i >> 5) + 1], i & 31);
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        const float v = sili::to_f32(in[k].v[e]);
-                        if (!found && (take >> e & 1) && !(v < near)) {
-                            const unsigned long long key = key_of(by(v), t0 + i + e);
-                            if ((uint32_t)(key >> 32) == all) { found = true; top = max(top, key); }
-                        }
-                    }
+            const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(top >> 32));
+            const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(top >> 32) == high ? (uint32_t)top : 0u);
+            const uint32_t most_y = __reduce_max_sync(0xffffffffu, (uint32_t)(key_of(by(most), 0) >> 32));
+            if ((threadIdx.x & 31) == 0) {
+                s.key[at][threadIdx.x >> 5] = (unsigned long long)high << 32 | low;
+                s.y[at][threadIdx.x >> 5] = most_y;
+            }
+        }
+    }
+
+    // picking: the row's first token of the largest value, by one warp.  The parts of the row whose largest it is are read
+    // again: after the division, elements next to it may be as large.
+    __device__ void settle(int64_t row, int at) const {
+        const int lane = threadIdx.x & 31, part = lane % (kThreads / 32);
+        const unsigned long long key = s.key[at][part];
+        const uint32_t y = s.y[at][part], high = (uint32_t)(key >> 32);
+        const uint32_t all = max(__reduce_max_sync(0xffffffffu, y), __reduce_max_sync(0xffffffffu, high));
+        unsigned parts = __ballot_sync(0xffffffffu, all && y == all) & ((1u << kThreads / 32) - 1u);
+        uint32_t low = high == all ? (uint32_t)key : 0u;
+        const T* x = (const T*)a.x + row * a.x_stride + t0;
+        const uint32_t* may = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+        const int head = min((int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)), n), packs = (n - head) / kVec;
+        for (; parts; parts &= parts - 1) {
+#pragma unroll 1
+            for (int k = 0; k < kPacks; ++k) {
+                const int p = (__ffs(parts) - 1) * 32 + lane + k * kThreads;
+                if (p >= packs) break;
+                const int i0 = head + p * kVec;
+                const P in = *(const P*)(x + i0);
+#pragma unroll 1
+                for (int e = 0; e < kVec; ++e) {
+                    const int i = i0 + e, v = t0 + i;
+                    const unsigned long long here = key_of(by(pick_of(in, e)), v);
+                    if ((uint32_t)(here >> 32) != all || (s.touched[i >> 5] >> (i & 31) & 1)) continue;
+                    if (may && !(__ldg(may + (v >> 5)) >> (v & 31) & 1)) continue;
+                    bool on_path = false;     // (the counts are those without the path)
+                    if (a.drafted && s.has_path[at])
+                        for (int j = 0; j < 64 * a.words; ++j)
+                            on_path = on_path || (s.draft[j] == i && (s.masks[at][j >> 6] >> (j & 63) & 1));
+                    if (!on_path) low = max(low, (uint32_t)here);
                 }
             }
         }
-        return top;
+        low = __reduce_max_sync(0xffffffffu, low);
+        if (lane == 0) a.best[row * a.tiles + blockIdx.x % a.tiles] = all ? (unsigned long long)all << 32 | low : 0;
+    }
+    // element e of a pack, from memory's order of bytes
+    static __device__ __forceinline__ float pick_of(const P& in, int e) {
+        const uint4 w = *(const uint4*)&in;
+        const int at = e * (int)sizeof(T) / 4;
+        const uint32_t u = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
+        if (sizeof(T) == 4) return __uint_as_float(u);
+        const unsigned short h = (unsigned short)(e & 1 ? u >> 16 : u);
+        return sili::to_f32(*(const T*)&h);
     }
 };
 
@@ -362,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ Log
             if (r >= 0) {
                 __syncthreads();     // the last request's counts have been read
                 k.count_request(r, row, min(last, row1), row0, row1);
-                k.rep = a.repetition ? a.repetition[r] : 1.f;
+                k.rep.set(a.repetition ? a.repetition[r] : 1.f);
                 k.freq = a.frequency ? a.frequency[r] : 0.f;
                 k.pres = a.presence ? a.presence[r] : 0.f;
                 k.by.set(a.temperature ? a.temperature[r] : 0.f);
@@ -370,7 +410,6 @@ __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ Log
         }
         const T* x = (const T*)a.x + row * a.x_stride + k.t0;
         T* y = WRITE ? (T*)a.y + row * a.y_stride + k.t0 : nullptr;
-        unsigned long long top = 0;
         if (r < 0) {
             // of no request: as it is
             if (WRITE)
@@ -383,23 +422,19 @@ __global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ Log
                 __syncthreads();
                 k.count_path((int)(row - begin), false, 0);
             }
-            top = k.row(x, y);
+            k.row(x, y, (int)(row - begin));
             if (path) {
                 __syncthreads();
                 k.count_path((int)(row - begin), true, listed);
             }
         }
-        if (!WRITE) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (!WRITE && (r < 0 || row + 1 == last || row + 1 >= row1)) {
+            // the end of the request's rows here
             __syncthreads();
-            if ((threadIdx.x & 31) == 0) s.top[threadIdx.x >> 5] = top;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-#pragma unroll
-                for (int i = 1; i < kThreads / 32; ++i) top = max(top, s.top[i]);
-                a.best[row * a.tiles + tile] = top;
-            }
+            const int64_t at = begin + (threadIdx.x >> 5);
+            if (r < 0) {
+                if (threadIdx.x == 0) a.best[row * a.tiles + tile] = 0;
+            } else if (at <= row) k.settle(at, (int)(at - begin));
         }
     }
 }
