@@ -587,15 +587,17 @@ typedef struct sili_logit_rules {
     const uint32_t* allowed;       /* [rows, allowed_stride]: bit v % 32 of word v / 32 */
     int64_t allowed_stride;
 } sili_logit_rules;
+/* The bytes of scratch space that a call of these sizes needs (pick: of
+ * sili_pick_tokens), 16-byte aligned; nothing in it outlives the call. */
+int sili_logits_scratch(int dtype, int64_t rows, int vocab, int requests, const sili_logit_rules* rules, int pick,
+                        int64_t* bytes);
 /* out [rows, vocab] (may be the logits) in the logits' type, rounded once.
  * Rows lie `stride` elements apart. */
 int sili_adjust_logits(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
-                       const sili_logit_rules* rules, void* out, int64_t out_stride, void* stream);
+                       const sili_logit_rules* rules, void* out, int64_t out_stride, void* scratch, void* stream);
 /* token[row]: the lowest of the tokens whose value by the rules is the largest
  * (in fp32; the first NaN where there is one), -1 where none is above -inf or
- * the row is no request's.  No logits are written.  scratch:
- * sili_pick_tokens_scratch bytes. */
-int sili_pick_tokens_scratch(int64_t rows, int vocab, int64_t* bytes);
+ * the row is no request's.  No logits are written. */
 int sili_pick_tokens(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
                      const sili_logit_rules* rules, int* token, void* scratch, void* stream);
 

@@ -8,18 +8,22 @@
 //   c(v) > 0 times in the history behind the prompt and on the path: - freq * c, - pres
 //   + bias(v);  / temp where temp > 0;  -inf where the mask's bit is not set.
 //
-// A CTA takes a tile of the vocabulary and a few consecutive rows.  The
-// tokens of a request's history that lie in the tile are counted in shared
-// memory, once for the rows that share it; a row's path (the drafted tokens
-// that its mask names) is counted on top and taken off again, where any of it
-// lies in the tile.  The tokens so touched are also listed, each once: they
-// are taken one by one, and the rest of a row is one pass over registers that
-// only divides by the temperature and masks.  A pick compares the rest before
-// the division, which keeps the order; what it may make equal is told apart
-// for the few elements next to the largest.
+// Three launches.  k_touch counts, for each request, the tokens of its history
+// and bias list in shared memory, a tile of the vocabulary at a time, and
+// leaves a bit a token and a list of those that it touched.  k_stream is one
+// pass over the logits in 16-byte accesses: it divides and masks what is not
+// touched, nor on the row's path (adjusting), or looks for the largest of it
+// before the division, which keeps the order (picking).  k_listed then takes
+// the touched tokens and the path one by one, a row a CTA, and, picking, finds
+// the first place of the largest: only where the division may have made
+// neighbours equal is a part of the row read again.  So the logits' bytes are
+// what bounds a large call; with the counts in the streaming CTAs, 32 trees
+// of 32 over 131072 tokens took 252 us in place of @PICK@ (a vocabulary's most
+// frequent tokens lie close together, and their CTAs were the last by far).
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "common.cuh"
@@ -44,11 +48,14 @@ int bad(const char* who, const char* what) {
 }
 
 constexpr int kThreads = 256;
-constexpr int kEach = 16;                      // elements of a row that a thread holds in registers
-constexpr int kTile = kThreads * kEach;        // tokens of a tile
-constexpr int kGroup = 8;                      // rows of a CTA at most
-static_assert(kGroup <= kThreads / 32, "a warp a row picks");
+constexpr int kWarps = kThreads / 32;
+constexpr int kTile = 8192;                    // tokens that a CTA of k_touch counts
+constexpr int kPacks = 8;                      // 16-byte accesses of a thread of k_stream
+constexpr int kMostDrafts = 256;
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
+// elements of a row that a CTA of k_stream takes, and a warp of it
+template <typename T> constexpr int kChunk = kThreads * kPacks * (16 / (int)sizeof(T));
+int chunk_of(int dtype) { return dtype == SILI_F32 ? kChunk<float> : kChunk<__half>; }
 
 struct LogitArgs {
     const void* x;
@@ -58,7 +65,7 @@ struct LogitArgs {
     int64_t rows;
     int vocab, requests;
     const int* starts;         // null: row r is request r's
-    const int* history;        // [requests, width]
+    const int* history;        // [requests, width] or null
     int64_t history_stride;
     int history_width;
     const int* history_lens;
@@ -75,24 +82,38 @@ struct LogitArgs {
     int biases;
     const uint32_t* allowed;   // [rows, allowed_stride] or null
     int64_t allowed_stride;
-    unsigned long long* best;  // [rows, tiles]: a tile's largest
     int* token;                // [rows]
-    int tiles, group;          // tiles, rows of a CTA
+    // scratch
+    int4* row_of;              // [rows]: the row's request, or -1, and its first row and the one past its last; null: the row itself
+    uint32_t* touched;         // [requests, touched_stride]: a bit a token; null: nothing is
+    int64_t touched_stride;
+    int2* listed;              // [requests, tiles]: where a tile's touched tokens lie in the list, and their number
+    uint2* list;               // [requests, cap]: token, count and marks
+    float* list_bias;          // [requests, cap]
+    int64_t cap;
+    int tiles;
+    uint32_t* most;            // picking: [rows, chunks, warps]: the order (below) of the largest element that is not touched
+    int chunks;
 };
 
-// A larger value, then a lower token, has the larger key; NaN is above all numbers (the first one is picked) and -inf below
-// every key (0).
-__device__ __forceinline__ unsigned long long key_of(float y, int token) {
-    uint32_t u = __float_as_uint(y + 0.f);     // -0 as 0
-    if (u == 0xFF800000u) return 0;
-    u = y != y ? 0xFFFFFFFFu : (int)u < 0 ? ~u : u | 0x80000000u;
-    return (unsigned long long)u << 32 | (0xFFFFFFFFu - (uint32_t)token);
+// x: the request, or -1; y, z: its rows
+__device__ __forceinline__ int4 request_of(const LogitArgs& a, int64_t row) {
+    return a.row_of ? a.row_of[row] : make_int4(row < a.requests ? (int)row : -1, (int)row, (int)row + 1, 0);
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float c;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-    return c;
+// top = x where bit e of `take` is set and x is larger, or not a number
+__device__ __forceinline__ void raise(float& top, float x, uint32_t take, int e) {
+    asm("{\n\t.reg .pred p;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 p, t, 0;\n\t@p max.NaN.f32 %0, %0, %1;\n\t}"
+        : "+f"(top) : "f"(x), "r"(take), "r"(1u << e));
+}
+// A number's place in the order (NaN above all, -0 as 0), 0 for -inf; and back.
+__device__ __forceinline__ uint32_t order_of(float y) {
+    const uint32_t u = __float_as_uint(y + 0.f);
+    return u == 0xFF800000u ? 0u : y != y ? 0xFFFFFFFFu : (int)u < 0 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_order(uint32_t u) {
+    return u == 0 ? -INFINITY : u == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u)
+                  : __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
 // Division by one number, many times: with r the rounded reciprocal of t, a quotient within a unit of x / t becomes the
@@ -118,387 +139,569 @@ struct Divisor {
     __device__ __forceinline__ float operator()(float x) const { return on ? over(x) : x; }
 };
 
-struct Shared {
-    uint32_t cnt[kTile];                       // a token's count and marks
-    uint32_t touched[kTile / 32 + 1];          // a bit a token whose count is not 0
-    uint16_t list[kTile];                      // those tokens
-    uint16_t draft[256];                       // the request's drafted tokens, 0xFFFF: not in the tile
-    unsigned long long masks[kGroup][4];
-    unsigned long long key[kGroup][kThreads / 32];     // picking: a warp's largest key of touched and single elements,
-    uint32_t y[kGroup][kThreads / 32];                 // and the upper half of that of the others
-    int listed, has_path[kGroup], twice;
-    float value[1];                            // [kTile] biases, then (writing) [kTile] the listed tokens' results
-};
+// ── the tokens that a request touches ───────────────────────────────────────
+// CTAs past the requests' tiles look up the rows' requests.
+__global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ LogitArgs a) {
+    const int64_t tiles = a.touched ? (int64_t)a.requests * a.tiles : 0;
+    if ((int64_t)blockIdx.x >= tiles) {
+        const int64_t step = (int64_t)(gridDim.x - tiles) * kThreads;
+        for (int64_t row = (int64_t)(blockIdx.x - tiles) * kThreads + threadIdx.x; row < a.rows; row += step) {
+            int lo = 0, hi = a.requests;       // the last request with starts[r] <= row
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.starts[mid] <= row) lo = mid; else hi = mid;
+            }
+            const int s0 = a.requests ? a.starts[lo] : 0, s1 = a.requests ? a.starts[lo + 1] : 0;
+            a.row_of[row] = make_int4(s0 <= row && row < s1 ? lo : -1, max(s0, 0), (int)min((int64_t)s1, a.rows), 0);
+        }
+        return;
+    }
+    __shared__ uint32_t cnt[kTile];
+    __shared__ int s_sum[kWarps], s_below[kWarps], s_twice;
+    extern __shared__ float bias[];            // [kTile], where there are biases
+    const int r = blockIdx.x / a.tiles, tile = blockIdx.x - r * a.tiles, t0 = tile * kTile, n = min(kTile, a.vocab - t0);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int len = a.history ? min(max(a.history_lens[r], 0), a.history_width) : 0;
+    const int prompt = a.history && a.prompt_lens ? a.prompt_lens[r] : 0;
+    for (int i = threadIdx.x; i < kTile / 4; i += kThreads) ((uint4*)cnt)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) s_twice = 0;
+    __syncthreads();
+    // a tile's part of the list begins behind as many places as the history and the biases have tokens before the tile
+    int below = 0;
+    const int* h = a.history + r * a.history_stride;
+    for (int j0 = threadIdx.x; j0 < len; j0 += 8 * kThreads) {
+        int v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = j0 + k * kThreads < len ? __ldg(h + j0 + k * kThreads) : -1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t i = (uint32_t)v[k] - (uint32_t)t0;
+            below += v[k] >= 0 && v[k] < t0;
+            if (v[k] < 0 || i >= (uint32_t)n) continue;
+            if (j0 + k * kThreads < prompt) atomicOr(cnt + i, kSeen); else atomicAdd(cnt + i, 1u);
+        }
+    }
+    if (a.biases) {
+        const int* list = a.bias_tokens + (int64_t)r * a.biases;
+        const float* value = a.bias_values + (int64_t)r * a.biases;
+        for (int j = threadIdx.x; j < a.biases; j += kThreads) {
+            const int v = list[j];
+            const uint32_t i = (uint32_t)v - (uint32_t)t0;
+            below += v >= 0 && v < t0;
+            if (i >= (uint32_t)n) continue;
+            bias[i] = value[j];
+            if (atomicOr(cnt + i, kBiased) & kBiased) s_twice = 1;
+        }
+        __syncthreads();
+        if (s_twice)
+            // a token is listed again: its first place adds all of them up, in order
+            for (int j = threadIdx.x; j < a.biases; j += kThreads) {
+                const int v = list[j];
+                const uint32_t i = (uint32_t)v - (uint32_t)t0;
+                if (i >= (uint32_t)n) continue;
+                bool first = true;
+                for (int k = 0; k < j; ++k) first = first && list[k] != v;
+                if (!first) continue;
+                float sum = value[j];
+                for (int k = j + 1; k < a.biases; ++k)
+                    if (list[k] == v) sum += value[k];
+                bias[i] = sum;
+            }
+    }
+    __syncthreads();
+    // a word of 32 tokens a thread and turn: a warp's ballots, token by token
+    static_assert(kTile == 32 * kThreads, "a word a thread");
+    uint32_t word = 0;
+    for (int k = 0; k < 32; ++k) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, cnt[(warp * 32 + k) * 32 + lane] != 0);
+        if (lane == k) word = bits;
+    }
+    if ((int)threadIdx.x * 32 < n) a.touched[r * a.touched_stride + t0 / 32 + threadIdx.x] = word;
+    int mine = __popc(word), before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += t;
+    }
+    if (lane == 31) s_sum[warp] = before;
+    below = sili::warp_sum(below);
+    if (lane == 0) s_below[warp] = below;
+    __syncthreads();
+    int all = 0;
+    below = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_sum[w];
+        all += s_sum[w];
+        below += s_below[w];
+    }
+    if (threadIdx.x == 0) a.listed[r * a.tiles + tile] = make_int2(below, all);
+    const int64_t at = r * a.cap + below;
+    int e = before - mine;
+    for (; word; word &= word - 1, ++e) {
+        const int i = (int)threadIdx.x * 32 + __ffs(word) - 1;
+        a.list[at + e] = make_uint2(t0 + i, cnt[i]);
+        if (a.biases) a.list_bias[at + e] = cnt[i] & kBiased ? bias[i] : 0.f;
+    }
+}
 
-template <typename T, bool WRITE>
-struct Logits {
-    static constexpr int kVec = 16 / sizeof(T), kPacks = kEach / kVec;
-    using P = sili::Pack<T, kVec>;
-    const LogitArgs& a;
-    Shared& s;
-    float *bias, *result;
-    int t0, n;            // the tile's first token, its tokens
-    const uint32_t* allow;
+// A row's rules.
+struct Rules {
     float freq, pres;
     Divisor rep, by;
-
-    __device__ __forceinline__ uint32_t note(uint32_t i, uint32_t what) const {
-        const uint32_t was = what & kCount ? atomicAdd(s.cnt + i, what) : atomicOr(s.cnt + i, what);
-        const uint32_t bit = 1u << (i & 31);
-        if (!was && !(atomicOr(s.touched + (i >> 5), bit) & bit)) s.list[atomicAdd(&s.listed, 1)] = (uint16_t)i;
-        return was;
+    __device__ __forceinline__ Rules(const LogitArgs& a, int r) {
+        rep.set(a.repetition ? a.repetition[r] : 1.f);
+        freq = a.frequency ? a.frequency[r] : 0.f;
+        pres = a.presence ? a.presence[r] : 0.f;
+        by.set(a.temperature ? a.temperature[r] : 0.f);
     }
-    // the tokens of the request's history and bias list that lie in the tile, and which of rows [row, last) have a path there
-    __device__ void count_request(int r, int64_t row, int64_t last, int64_t row0, int64_t row1) {
-        for (int i = threadIdx.x; i < kTile; i += kThreads) s.cnt[i] = 0;
-        for (int i = threadIdx.x; i <= kTile / 32; i += kThreads) s.touched[i] = 0;
-        if (threadIdx.x == 0) s.listed = s.twice = 0;
-        if (a.drafted) {
-            const uint32_t v = row0 + threadIdx.x < row1 && (int)threadIdx.x < 64 * a.words
-                                   ? (uint32_t)a.drafted[row0 + threadIdx.x] - (uint32_t)t0 : 0xFFFFFFFFu;
-            s.draft[threadIdx.x] = v < (uint32_t)n ? (uint16_t)v : (uint16_t)0xFFFFu;
-            const int64_t k = row + threadIdx.x / 4;
-            const int w = threadIdx.x & 3;
-            if (threadIdx.x < 4 * kGroup) {
-                s.masks[threadIdx.x / 4][w] = k < last && w < a.words ? (unsigned long long)a.masks[k * a.words + w] : 0;
-                s.has_path[threadIdx.x / 4] = 0;
-            }
-        }
-        __syncthreads();
-        if (a.drafted && s.draft[threadIdx.x] != 0xFFFFu)
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-                if (s.masks[k][threadIdx.x >> 6] >> (threadIdx.x & 63) & 1) s.has_path[k] = 1;
-        if (a.history) {
-            const int* h = a.history + r * a.history_stride;
-            const int len = min(max(a.history_lens[r], 0), a.history_width);
-            const int prompt = a.prompt_lens ? a.prompt_lens[r] : 0;
-#pragma unroll 4
-            for (int j = threadIdx.x; j < len; j += kThreads) {
-                const uint32_t i = (uint32_t)__ldg(h + j) - (uint32_t)t0;
-                if (i < (uint32_t)n) note(i, j < prompt ? kSeen : 1u);
-            }
-        }
-        if (a.biases) {
-            const int* list = a.bias_tokens + (int64_t)r * a.biases;
-            const float* value = a.bias_values + (int64_t)r * a.biases;
-            for (int j = threadIdx.x; j < a.biases; j += kThreads) {
-                const uint32_t i = (uint32_t)list[j] - (uint32_t)t0;
-                if (i >= (uint32_t)n) continue;
-                bias[i] = value[j];
-                if (note(i, kBiased) & kBiased) s.twice = 1;
-            }
-            __syncthreads();
-            if (s.twice)
-                // a token is listed again: its first place adds all of them up, in order
-                for (int j = threadIdx.x; j < a.biases; j += kThreads) {
-                    const int v = list[j];
-                    const uint32_t i = (uint32_t)v - (uint32_t)t0;
-                    if (i >= (uint32_t)n) continue;
-                    bool first = true;
-                    for (int k = 0; k < j; ++k) first = first && list[k] != v;
-                    if (!first) continue;
-                    float sum = value[j];
-                    for (int k = j + 1; k < a.biases; ++k)
-                        if (list[k] == v) sum += value[k];
-                    bias[i] = sum;
-                }
-        }
-        __syncthreads();
-    }
-    // the path of the CTA's row k on top of the counts, or off them again (the list is then cut to what it was)
-    __device__ void count_path(int k, bool off, int listed) const {
-        const uint32_t i = s.draft[threadIdx.x];
-        if (i != 0xFFFFu && (s.masks[k][threadIdx.x >> 6] >> (threadIdx.x & 63) & 1)) {
-            if (!off) note(i, 1u);
-            else if (atomicSub(s.cnt + i, 1u) == 1u) atomicAnd(s.touched + (i >> 5), ~(1u << (i & 31)));
-        }
-        if (off && threadIdx.x == 0) s.listed = listed;
-        __syncthreads();
-    }
-
-    __device__ __forceinline__ float ruled(float x, uint32_t what, int i) const {
+    __device__ __forceinline__ float operator()(float x, uint32_t what, float bias) const {
         // (a count also makes it seen)
         if (what & (kSeen | kCount)) x = x > 0.f ? rep.over(x) : x * rep.t;
         if (what & kCount) {
             x = x - freq * (float)(what & kCount);
             x = x - pres;
         }
-        if (what & kBiased) x = x + bias[i];
+        if (what & kBiased) x = x + bias;
         return by(x);
-    }
-    __device__ __forceinline__ bool may(int i) const {
-        const int v = t0 + i;
-        return !allow || (__ldg(allow + (v >> 5)) >> (v & 31) & 1);
-    }
-    __device__ __forceinline__ float single(T x, int i) const {
-        return may(i) ? ruled(sili::to_f32(x), s.cnt[i], i) : -INFINITY;
-    }
-
-    // one row of the tile, the CTA's row k of the request
-    __device__ void row(const T* x, T* y, int at) const {
-        unsigned long long top = 0;
-        // whole 16 bytes from the first aligned element on
-        const int lead = (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
-        const int head = !WRITE || (uintptr_t)y % 16 == (uintptr_t)x % 16 ? min(lead, n) : n;
-        const int packs = (n - head) / kVec, tail = head + packs * kVec;
-        P in[kPacks];
-        uint32_t words[kPacks][2];
-#pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            const int p = threadIdx.x + k * kThreads;
-            words[k][0] = words[k][1] = 0xFFFFFFFFu;
-            if (p < packs) {
-                in[k] = *(const P*)(x + head + p * kVec);
-                if (allow) {
-                    const int v = t0 + head + p * kVec;
-                    words[k][0] = __ldg(allow + (v >> 5));
-                    words[k][1] = __ldg(allow + ((v + kVec - 1) >> 5));
-                }
-            }
-        }
-        const int listed = s.listed;
-        for (int e = threadIdx.x; e < listed; e += kThreads) {
-            const int i = s.list[e];
-            const float v = single(x[i], i);
-            if (WRITE) result[e] = v; else top = max(top, key_of(v, t0 + i));
-        }
-        if (WRITE && listed) __syncthreads();     // (y may be x)
-        for (int i = threadIdx.x; i < n - packs * kVec; i += kThreads) {
-            const int j = i < head ? i : i - head + tail;
-            const float v = single(x[j], j);
-            if (WRITE) y[j] = sili::from_f32<T>(v); else top = max(top, key_of(v, t0 + j));
-        }
-        float most = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            const int p = threadIdx.x + k * kThreads;
-            if (p >= packs) break;
-            const int i = head + p * kVec;
-            uint32_t take = __funnelshift_r(words[k][0], words[k][1], (t0 + i) & 31);
-            if (WRITE) {
-                P out;
-                bool quick = by.fast;
-                float v[kVec];
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    v[e] = sili::to_f32(in[k].v[e]);
-                    quick = quick && by.takes(v[e]);
-                }
-                if (by.on) {
-                    if (quick)
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e) v[e] = by.quick(v[e]);
-                    else
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e) v[e] = v[e] / by.t;
-                }
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) out.v[e] = sili::from_f32<T>(take >> e & 1 ? v[e] : -INFINITY);
-                *(P*)(y + i) = out;
-            } else {
-                take &= ~__funnelshift_r(s.touched[i >> 5], s.touched[(i >> 5) + 1], i & 31);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e)
-                    most = max_nan(most, take >> e & 1 ? sili::to_f32(in[k].v[e]) : -INFINITY);
-            }
-        }
-        if (WRITE) {
-            if (listed) {
-                __syncthreads();
-                for (int e = threadIdx.x; e < listed; e += kThreads) y[s.list[e]] = sili::from_f32<T>(result[e]);
-            }
-        } else {
-            const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(top >> 32));
-            const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(top >> 32) == high ? (uint32_t)top : 0u);
-            const uint32_t most_y = __reduce_max_sync(0xffffffffu, (uint32_t)(key_of(by(most), 0) >> 32));
-            if ((threadIdx.x & 31) == 0) {
-                s.key[at][threadIdx.x >> 5] = (unsigned long long)high << 32 | low;
-                s.y[at][threadIdx.x >> 5] = most_y;
-            }
-        }
-    }
-
-    // picking: the row's first token of the largest value, by one warp.  The parts of the row whose largest it is are read
-    // again: after the division, elements next to it may be as large.
-    __device__ void settle(int64_t row, int at) const {
-        const int lane = threadIdx.x & 31, part = lane % (kThreads / 32);
-        const unsigned long long key = s.key[at][part];
-        const uint32_t y = s.y[at][part], high = (uint32_t)(key >> 32);
-        const uint32_t all = max(__reduce_max_sync(0xffffffffu, y), __reduce_max_sync(0xffffffffu, high));
-        unsigned parts = __ballot_sync(0xffffffffu, all && y == all) & ((1u << kThreads / 32) - 1u);
-        uint32_t low = high == all ? (uint32_t)key : 0u;
-        const T* x = (const T*)a.x + row * a.x_stride + t0;
-        const uint32_t* may = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-        const int head = min((int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)), n), packs = (n - head) / kVec;
-        for (; parts; parts &= parts - 1) {
-#pragma unroll 1
-            for (int k = 0; k < kPacks; ++k) {
-                const int p = (__ffs(parts) - 1) * 32 + lane + k * kThreads;
-                if (p >= packs) break;
-                const int i0 = head + p * kVec;
-                const P in = *(const P*)(x + i0);
-#pragma unroll 1
-                for (int e = 0; e < kVec; ++e) {
-                    const int i = i0 + e, v = t0 + i;
-                    const unsigned long long here = key_of(by(pick_of(in, e)), v);
-                    if ((uint32_t)(here >> 32) != all || (s.touched[i >> 5] >> (i & 31) & 1)) continue;
-                    if (may && !(__ldg(may + (v >> 5)) >> (v & 31) & 1)) continue;
-                    bool on_path = false;     // (the counts are those without the path)
-                    if (a.drafted && s.has_path[at])
-                        for (int j = 0; j < 64 * a.words; ++j)
-                            on_path = on_path || (s.draft[j] == i && (s.masks[at][j >> 6] >> (j & 63) & 1));
-                    if (!on_path) low = max(low, (uint32_t)here);
-                }
-            }
-        }
-        low = __reduce_max_sync(0xffffffffu, low);
-        if (lane == 0) a.best[row * a.tiles + blockIdx.x % a.tiles] = all ? (unsigned long long)all << 32 | low : 0;
-    }
-    // element e of a pack, from memory's order of bytes
-    static __device__ __forceinline__ float pick_of(const P& in, int e) {
-        const uint4 w = *(const uint4*)&in;
-        const int at = e * (int)sizeof(T) / 4;
-        const uint32_t u = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
-        if (sizeof(T) == 4) return __uint_as_float(u);
-        const unsigned short h = (unsigned short)(e & 1 ? u >> 16 : u);
-        return sili::to_f32(*(const T*)&h);
     }
 };
 
+// The draft that thread j stands for: its token where the row's path holds it, else -1.
+__device__ __forceinline__ int path_token(const LogitArgs& a, const int4& of, int j, uint64_t mask) {
+    return (mask >> (j & 63) & 1) && of.y + j < of.z ? a.drafted[of.y + j] : -1;
+}
+__device__ __forceinline__ uint64_t path_mask(const LogitArgs& a, int64_t row, int j) {
+    return a.drafted && j < 64 * a.words ? (uint64_t)a.masks[row * a.words + (j >> 6)] : 0;
+}
+
+// element e of a pack, from memory's order of bytes
+template <typename T>
+__device__ __forceinline__ float element(const sili::Pack<T, 16 / sizeof(T)>& in, int e) {
+    const uint4 w = *(const uint4*)&in;
+    const int at = e * (int)sizeof(T) / 4;
+    const uint32_t u = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
+    if (sizeof(T) == 4) return __uint_as_float(u);
+    const unsigned short h = (unsigned short)(e & 1 ? u >> 16 : u);
+    return sili::to_f32(*(const T*)&h);
+}
+
+// Where the 16-byte accesses of a chunk of a row lie: whole ones from the first aligned element on.
+template <typename T>
+struct Lay {
+    static constexpr int kVec = 16 / (int)sizeof(T);
+    int t0, n, head, packs;
+    __device__ __forceinline__ Lay(const LogitArgs& a, const T* row, int chunk) {
+        t0 = chunk * kChunk<T>;
+        n = min(kChunk<T>, a.vocab - t0);
+        head = min((int)((16 - (uintptr_t)(row + t0) % 16) % 16 / sizeof(T)), n);
+        packs = (n - head) / kVec;
+    }
+};
+
+// ── the pass over the logits ────────────────────────────────────────────────
+// A CTA takes a chunk of one row.  Touched tokens and the row's path are left as they are (adjusting), or aside (picking).
 template <typename T, bool WRITE>
-__global__ void __launch_bounds__(kThreads) k_logits(const __grid_constant__ LogitArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    Shared& s = *(Shared*)smem;
-    Logits<T, WRITE> k{a, s, s.value, s.value + (a.biases ? kTile : 0)};
-    const int tile = blockIdx.x % a.tiles;
-    k.t0 = tile * kTile;
-    k.n = min(kTile, a.vocab - k.t0);
-    const int64_t first = (int64_t)(blockIdx.x / a.tiles) * a.group, last = min(first + a.group, a.rows);
-    int64_t begin = first, row0 = 0, row1 = -1;      // the current request's rows, the first of them here
-    int r = -1;
-    for (int64_t row = first; row < last; ++row) {
-        if (row >= row1) {
-            // the request that holds the row, if any
-            begin = row;
-            if (!a.starts) {
-                r = row < a.requests ? (int)row : -1;
-                row0 = row;
-                row1 = row + 1;
-            } else {
-                int lo = 0, hi = a.requests;       // the last request with starts[r] <= row
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (a.starts[mid] <= row) lo = mid; else hi = mid;
-                }
-                r = a.requests ? lo : -1;
-                if (r >= 0) {
-                    row0 = max(a.starts[r], 0);
-                    row1 = min((int64_t)a.starts[r + 1], a.rows);
-                    if (row < row0 || row >= row1) r = -1;
-                }
-                if (r < 0) { row0 = row; row1 = row + 1; }
-            }
-            if (r >= 0) {
-                __syncthreads();     // the last request's counts have been read
-                k.count_request(r, row, min(last, row1), row0, row1);
-                k.rep.set(a.repetition ? a.repetition[r] : 1.f);
-                k.freq = a.frequency ? a.frequency[r] : 0.f;
-                k.pres = a.presence ? a.presence[r] : 0.f;
-                k.by.set(a.temperature ? a.temperature[r] : 0.f);
-            }
+__global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ LogitArgs a) {
+    constexpr int kVec = 16 / (int)sizeof(T), kStep = kThreads * kVec / 32;
+    static_assert(kChunk<T> % 32 == 0 && kThreads * kVec % 32 == 0, "whole words");
+    using P = sili::Pack<T, kVec>;
+    constexpr int kWords = kChunk<T> / 32;
+    // bits of the chunk's tokens: those to take (picking: allowed and not touched), and (adjusting) those to leave
+    __shared__ uint32_t s_take[kWords + 1], s_rest[WRITE ? kWords + 1 : 1];
+    const int64_t row = blockIdx.x / a.chunks;
+    const int chunk = blockIdx.x - (int)row * a.chunks, tid = threadIdx.x;
+    const T* x = (const T*)a.x + row * a.x_stride;
+    T* y = WRITE ? (T*)a.y + row * a.y_stride : nullptr;
+    Lay<T> lay(a, x, chunk);
+    if (WRITE && ((uintptr_t)y - (uintptr_t)x) % 16) { lay.head = lay.n; lay.packs = 0; }
+    const int t0 = lay.t0, n = lay.n, head = lay.head, packs = lay.packs;
+    x += t0;
+    y += t0;
+    const int first = head + tid * kVec;
+    P in[kPacks];
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k)
+        if (tid + k * kThreads < packs) in[k] = *(const P*)(x + first + k * kThreads * kVec);
+    const int4 of = request_of(a, row);
+    const uint64_t mask = path_mask(a, row, tid);
+    const int r = of.x;
+    if (r < 0) {
+        // of no request: as it is
+        if (WRITE && (const void*)x != (void*)y)
+            for (int i = tid; i < n; i += kThreads) y[i] = x[i];
+        return;
+    }
+    const uint32_t* allow = a.allowed ? a.allowed + row * a.allowed_stride + (t0 >> 5) : nullptr;
+    const uint32_t* touched = a.touched ? a.touched + r * a.touched_stride + (t0 >> 5) : nullptr;
+    const bool bits = a.allowed || a.touched || a.drafted;
+    Divisor by;
+    by.set(a.temperature ? a.temperature[r] : 0.f);
+    if (bits) {
+        uint32_t i = 0xFFFFFFFFu;
+        if (a.drafted) {
+            const int v = path_token(a, of, tid, mask);
+            if (v >= 0) i = (uint32_t)v - (uint32_t)t0;
         }
-        const T* x = (const T*)a.x + row * a.x_stride + k.t0;
-        T* y = WRITE ? (T*)a.y + row * a.y_stride + k.t0 : nullptr;
-        if (r < 0) {
-            // of no request: as it is
-            if (WRITE)
-                for (int i = threadIdx.x; i < k.n; i += kThreads) y[i] = x[i];
-        } else {
-            k.allow = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-            const bool path = a.drafted && s.has_path[row - begin];
-            const int listed = s.listed;
-            if (path) {
-                __syncthreads();
-                k.count_path((int)(row - begin), false, 0);
-            }
-            k.row(x, y, (int)(row - begin));
-            if (path) {
-                __syncthreads();
-                k.count_path((int)(row - begin), true, listed);
-            }
+        uint32_t word[2][kWords / kThreads];
+#pragma unroll
+        for (int k = 0; k < kWords / kThreads; ++k) {
+            const int w = tid + k * kThreads;
+            word[0][k] = allow && w * 32 < n ? __ldg(allow + w) : 0xFFFFFFFFu;
+            word[1][k] = touched && w * 32 < n ? touched[w] : 0u;
         }
-        if (!WRITE && (r < 0 || row + 1 == last || row + 1 >= row1)) {
-            // the end of the request's rows here
+#pragma unroll
+        for (int k = 0; k < kWords / kThreads; ++k) {
+            const int w = tid + k * kThreads;
+            s_take[w] = WRITE ? word[0][k] : word[0][k] & ~word[1][k];
+            if (WRITE) s_rest[w] = word[1][k];
+        }
+        if (__syncthreads_or(i < (uint32_t)n)) {
+            if (i < (uint32_t)n) {
+                if (WRITE) atomicOr(s_rest + (i >> 5), 1u << (i & 31)); else atomicAnd(s_take + (i >> 5), ~(1u << (i & 31)));
+            }
             __syncthreads();
-            const int64_t at = begin + (threadIdx.x >> 5);
-            if (r < 0) {
-                if (threadIdx.x == 0) a.best[row * a.tiles + tile] = 0;
-            } else if (at <= row) k.settle(at, (int)(at - begin));
         }
+    }
+    // a pack's bits lie in one word or two, whose places move by a constant from pack to pack
+    const int shift = first & 31, at0 = first >> 5, more = ((first + kVec - 1) >> 5) - at0;
+    auto bits_of = [&](const uint32_t* words, int k) {
+        return __funnelshift_r(words[at0 + k * kStep], words[at0 + k * kStep + more], shift);
+    };
+    float most = -INFINITY;
+    // elements before and behind the whole accesses
+    for (int i = tid; i < n - packs * kVec; i += kThreads) {
+        const int j = i < head ? i : i + packs * kVec, w = j >> 5;
+        const uint32_t may = bits ? s_take[w] >> (j & 31) & 1 : 1u;
+        if (WRITE) {
+            const bool left = bits && (s_rest[w] >> (j & 31) & 1);
+            y[j] = left ? x[j] : sili::from_f32<T>(may ? by(sili::to_f32(x[j])) : -INFINITY);
+        } else raise(most, sili::to_f32(x[j]), may, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+        if (tid + k * kThreads >= packs) break;
+        const uint32_t take = bits ? bits_of(s_take, k) : 0xFFFFFFFFu;
+        if (WRITE) {
+            const uint32_t rest = bits ? bits_of(s_rest, k) : 0u;
+            P out;
+            float v[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v[e] = sili::to_f32(in[k].v[e]);
+            if (by.on) {
+                bool quick = by.fast;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) quick = quick && by.takes(v[e]);
+                if (quick)
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) v[e] = by.quick(v[e]);
+                else
+#pragma unroll 1
+                    for (int e = 0; e < kVec; ++e) {
+                        const float u = element<T>(in[k], e) / by.t;
+#pragma unroll
+                        for (int f = 0; f < kVec; ++f) v[f] = f == e ? u : v[f];
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                out.v[e] = sili::from_f32<T>(take >> e & 1 ? v[e] : -INFINITY);
+                if (rest >> e & 1) out.v[e] = in[k].v[e];
+            }
+            *(P*)(y + first + k * kThreads * kVec) = out;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) raise(most, sili::to_f32(in[k].v[e]), take, e);
+        }
+    }
+    if (!WRITE) {
+        const uint32_t all = __reduce_max_sync(0xffffffffu, order_of(most));
+        if ((tid & 31) == 0) a.most[((int64_t)row * a.chunks + chunk) * kWarps + (tid >> 5)] = all;
     }
 }
 
-// the largest of a row's tiles, a warp a row
-__global__ void __launch_bounds__(128) k_picked(const unsigned long long* best, int64_t rows, int tiles, int* token) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    unsigned long long top = 0;
-    for (int i = threadIdx.x & 31; i < tiles; i += 32) top = max(top, best[row * tiles + i]);
+// ── the touched tokens, and the pick ────────────────────────────────────────
+// A CTA takes a row; adjusting, several may share its list.
+constexpr int kMostHeld = 64;
+struct Path {
+    uint32_t filter[256];          // a bit a token's hash
+    int token[kMostDrafts];
+    int n;
+};
+
+template <typename T, bool WRITE>
+__global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ LogitArgs a) {
+    __shared__ Path s;
+    __shared__ uint32_t s_red[kWarps][2];
+    __shared__ int s_first[65], s_base[64], s_hold[kMostHeld], s_held;
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int4 of = request_of(a, row);
+    const uint64_t mask = path_mask(a, row, tid);
+    const int r = of.x;
+    if (r < 0) {
+        if (!WRITE && tid == 0) a.token[row] = -1;
+        return;
+    }
+    const Rules rule(a, r);
+    // adjusting, what is touched still holds the logits
+    const T* x = WRITE ? (const T*)a.y + row * a.y_stride : (const T*)a.x + row * a.x_stride;
+    T* y = WRITE ? (T*)a.y + row * a.y_stride : nullptr;
+    const uint32_t* allow = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+    const uint32_t* touched = a.touched ? a.touched + r * a.touched_stride : nullptr;
+    auto may = [&](int v) { return !allow || (__ldg(allow + (v >> 5)) >> (v & 31) & 1); };
+    auto hash = [](int v) { return (uint32_t)v & 8191u; };
+    // the row's path
+    if (tid == 0) s.n = s_held = 0;
+    if (a.drafted) {
+        s.filter[tid] = 0;
+        __syncthreads();
+        const int v = path_token(a, of, tid, mask);
+        if (v >= 0 && v < a.vocab) {
+            s.token[atomicAdd(&s.n, 1)] = v;
+            atomicOr(s.filter + (hash(v) >> 5), 1u << (hash(v) & 31));
+        }
+    }
+    __syncthreads();
+    const int path = s.n;
+    auto times = [&](int v) {      // on the path
+        uint32_t c = 0;
+        if (path && (s.filter[hash(v) >> 5] >> (hash(v) & 31) & 1))
+            for (int k = 0; k < path; ++k) c += s.token[k] == v;
+        return c;
+    };
+    uint32_t high = 0, low = 0;    // the largest so far and its token, inverted
+    auto take = [&](int v, float value, bool is) {
+        const float z = is ? value : -INFINITY;
+        if (WRITE) y[v] = sili::from_f32<T>(z);
+        else {
+            const uint32_t u = order_of(z);
+            if (u > high) { high = u; low = ~(uint32_t)v; }
+            else if (u == high) low = max(low, ~(uint32_t)v);
+        }
+    };
+    // the listed tokens: of each 64 tiles, all places in a row
+    for (int tile0 = 0; touched && tile0 < a.tiles; tile0 += 64) {
+        const int m = min(64, a.tiles - tile0);
+        __syncthreads();
+        if (warp == 0) {
+            int carry = 0;
+            for (int b = 0; b < m; b += 32) {
+                const int2 c = b + lane < m ? a.listed[(int64_t)r * a.tiles + tile0 + b + lane] : make_int2(0, 0);
+                const uint32_t inc = sili::warp_inclusive_scan((uint32_t)c.y);
+                if (b + lane < m) {
+                    s_first[b + lane] = carry + (int)inc - c.y;
+                    s_base[b + lane] = c.x;
+                }
+                carry += (int)__shfl_sync(0xffffffffu, inc, 31);
+            }
+            if (lane == 0) s_first[m] = carry;
+        }
+        __syncthreads();
+        const int all = s_first[m], stride = kThreads * gridDim.y;
+        constexpr int kBatch = 4;
+        int t = 0;
+        for (int e0 = tid + blockIdx.y * kThreads; e0 < all; e0 += kBatch * stride) {
+            uint2 it[kBatch];
+            float bias[kBatch];
+            T v[kBatch];
+            bool is[kBatch];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) token[row] = top ? (int)(0xFFFFFFFFu - (uint32_t)top) : -1;
+            for (int b = 0; b < kBatch; ++b) {
+                const int e = e0 + b * stride;
+                if (e >= all) continue;
+                while (s_first[t + 1] <= e) ++t;
+                const int64_t at = r * a.cap + s_base[t] + (e - s_first[t]);
+                it[b] = a.list[at];
+                bias[b] = a.biases ? a.list_bias[at] : 0.f;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (e0 + b * stride < all) {
+                    v[b] = x[it[b].x];
+                    is[b] = may((int)it[b].x);
+                }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (e0 + b * stride < all)
+                    take((int)it[b].x, rule(sili::to_f32(v[b]), it[b].y + times((int)it[b].x), bias[b]), is[b]);
+        }
+    }
+    // the path's tokens that are on no list, at the first of their places
+    if (blockIdx.y == 0 && tid < path) {
+        const int v = s.token[tid];
+        bool first = !touched || !(touched[v >> 5] >> (v & 31) & 1);
+        for (int k = 0; k < tid; ++k) first = first && s.token[k] != v;
+        if (first) take(v, rule(sili::to_f32(x[v]), times(v), 0.f), may(v));
+    }
+    if (WRITE) return;
+    // the others' largest values, after the division
+    const uint32_t* most = a.most + row * a.chunks * kWarps;
+    const int parts = a.chunks * kWarps;
+    uint32_t other = 0;
+    int at_other = 0;              // the first of this thread's parts that hold its largest
+    for (int i = tid; i < parts; i += kThreads) {
+        const uint32_t u = order_of(rule.by(of_order(most[i])));
+        if (u > other) { other = u; at_other = i; }
+    }
+    auto reduce = [&](uint32_t u, int which) {
+        u = __reduce_max_sync(0xffffffffu, u);
+        __syncthreads();
+        if (lane == 0) s_red[warp][which] = u;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) all = max(all, s_red[w][which]);
+        return all;
+    };
+    const uint32_t all = reduce(max(other, high), 0);
+    if (high != all) low = 0;
+    if (all && __syncthreads_or(other == all)) {
+        // the parts that hold it are read again: after the division, elements next to the largest may be as large
+        constexpr int kVec = 16 / (int)sizeof(T);
+        using P = sili::Pack<T, kVec>;
+        auto candidate = [&](int v, float value) {
+            if (order_of(rule.by(value)) != all || (touched && (touched[v >> 5] >> (v & 31) & 1)) || times(v) || !may(v)) return;
+            low = max(low, ~(uint32_t)v);
+        };
+        for (int i = tid; i < parts; i += kThreads)
+            if (i >= at_other && other == all && order_of(rule.by(of_order(most[i]))) == all) {
+                const int k = atomicAdd(&s_held, 1);
+                if (k < kMostHeld) s_hold[k] = i;
+            }
+        __syncthreads();
+        // (more of them than there is room for, as where a row is one value: all parts are looked at)
+        const int held = s_held > kMostHeld ? parts : s_held;
+        for (int k = 0; k < held; ++k) {
+            const int i = s_held > kMostHeld ? k : s_hold[k];
+            const float top = of_order(most[i]);
+            if (s_held > kMostHeld && order_of(rule.by(top)) != all) continue;
+            // (quotients that leave the normal range: any of them may be the same)
+            const float near = rule.by.on && !rule.by.takes(top) ? -INFINITY : top - fabsf(top) * 0x1p-20f;
+            const int chunk = i / kWarps, w = i - chunk * kWarps;
+            const Lay<T> lay(a, x, chunk);
+            // the warp's whole accesses, and the single elements that were its own
+            static_assert(kPacks == kWarps, "a warp of this CTA an access of that one's");
+            const int p = w * 32 + lane + warp * kThreads;
+            if (p < lay.packs) {
+                const int at = lay.t0 + lay.head + p * kVec;
+                const P in = *(const P*)(x + at);
+                uint32_t some = 0;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) some |= !(sili::to_f32(in.v[e]) < near) ? 1u << e : 0u;
+                for (; some; some &= some - 1) candidate(at + __ffs(some) - 1, element<T>(in, __ffs(some) - 1));
+            }
+            if (warp == 0)
+                for (int k = w * 32 + lane; k < lay.n - lay.packs * kVec; k += kThreads) {
+                    const int j = lay.t0 + (k < lay.head ? k : k + lay.packs * kVec);
+                    candidate(j, sili::to_f32(x[j]));
+                }
+        }
+    }
+    low = reduce(low, 1);
+    if (tid == 0) a.token[row] = all ? (int)~low : -1;
+}
+
+// ── the entries ─────────────────────────────────────────────────────────────
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// The parts of the scratch space, one after the other from `base` on; returns its bytes.
+int64_t lay_out(LogitArgs& a, int dtype, bool counts, bool pick, uint8_t* base) {
+    int64_t at = 0;
+    auto part = [&](int64_t bytes) { const int64_t here = at; at += round16(bytes); return base + here; };
+    a.tiles = (a.vocab + kTile - 1) / kTile;
+    a.chunks = (a.vocab + chunk_of(dtype) - 1) / chunk_of(dtype);
+    a.cap = (int64_t)a.history_width + a.biases;
+    a.touched_stride = (int64_t)a.tiles * (kTile / 32) + 1;
+    a.row_of = a.starts ? (int4*)part(a.rows * 16) : nullptr;
+    a.touched = nullptr;
+    if (counts) {
+        a.touched = (uint32_t*)part(a.requests * a.touched_stride * 4);
+        a.listed = (int2*)part((int64_t)a.requests * a.tiles * 8);
+        a.list = (uint2*)part(a.requests * a.cap * 8);
+        a.list_bias = (float*)part(a.biases ? a.requests * a.cap * 4 : 0);
+    }
+    a.most = pick ? (uint32_t*)part(a.rows * a.chunks * kWarps * 4) : nullptr;
+    return at;
 }
 
 template <typename T, bool WRITE>
-int launch(LogitArgs& a, cudaStream_t s) {
-    const int smem = (int)sizeof(Shared) + ((a.biases ? kTile : 0) + (WRITE ? kTile : 0)) * 4;
-    auto kernel = k_logits<T, WRITE>;
-    static std::atomic<uint64_t> set{0};
-    if (smem > 48 * 1024) CKL(sili::allow_smem(kernel, (int)sizeof(Shared) + 2 * kTile * 4, set));
-    kernel<<<(unsigned)((a.rows + a.group - 1) / a.group * a.tiles), kThreads, smem, s>>>(a);
+int launch(const LogitArgs& a, cudaStream_t s) {
+    if (a.row_of || a.touched) {
+        const int64_t tiles = a.touched ? (int64_t)a.requests * a.tiles : 0;
+        const int64_t finders = a.row_of ? std::min<int64_t>((a.rows + kThreads - 1) / kThreads, 148) : 0;
+        const int smem = a.biases && tiles ? kTile * 4 : 0;
+        static std::atomic<uint64_t> set{0};
+        if (smem) CKL(sili::allow_smem(k_touch, smem, set));
+        k_touch<<<(unsigned)(tiles + finders), kThreads, smem, s>>>(a);
+        sili::count_launch();
+    }
+    k_stream<T, WRITE><<<(unsigned)(a.rows * a.chunks), kThreads, 0, s>>>(a);
     sili::count_launch();
+    if (!WRITE || a.touched || a.drafted) {
+        // (adjusting, long lists of few rows are shared)
+        const int64_t most = (int64_t)a.history_width + a.biases;
+        const int share = WRITE && a.touched ? (int)std::max<int64_t>(1, std::min<int64_t>(most / 1024, 1184 / std::max<int64_t>(a.rows, 1))) : 1;
+        k_listed<T, WRITE><<<dim3((unsigned)a.rows, share), kThreads, 0, s>>>(a);
+        sili::count_launch();
+    }
     CKL(cudaGetLastError());
     return SILI_OK;
 }
 template <bool WRITE>
-int by_type(int dtype, LogitArgs& a, cudaStream_t s) {
+int by_type(int dtype, const LogitArgs& a, cudaStream_t s) {
     return dtype == SILI_F32 ? launch<float, WRITE>(a, s)
          : dtype == SILI_F16 ? launch<__half, WRITE>(a, s) : launch<__nv_bfloat16, WRITE>(a, s);
 }
 
-int check(const char* who, int dtype, int64_t rows, int vocab, int requests, int history_width, int words, int biases) {
-    if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
-    if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || requests < 0 || history_width < 0 || biases < 0 || words < 0 || words > 4)
-        return bad(who, "sizes out of range");
-    return SILI_OK;
-}
-
 // Everything but where the result goes.
 int prepare(const char* who, int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
-            const sili_logit_rules* rules, LogitArgs& a) {
+            const sili_logit_rules* rules, bool pick, void* scratch, LogitArgs& a, int64_t* bytes) {
     if (!rules) return bad(who, "null array");
     const sili_logit_rules& q = *rules;
-    if (const int e = check(who, dtype, rows, vocab, requests, q.history_width, q.words, q.biases)) return e;
-    if (!logits && rows) return bad(who, "null array");
-    if (rows > 1 && stride < vocab) return bad(who, "rows overlap");
+    if (dtype < SILI_F32 || dtype > SILI_BF16) return bad(who, "unknown element type");
+    if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || requests < 0 || q.history_width < 0 || q.biases < 0 || q.words < 0 ||
+        q.words > 4)
+        return bad(who, "sizes out of range");
     if ((q.history != nullptr) != (q.history_lens != nullptr)) return bad(who, "history and its lengths come together");
     if (q.history && requests > 1 && q.history_stride < 0) return bad(who, "sizes out of range");
     if ((q.drafted != nullptr) != (q.masks != nullptr) || (q.drafted && (!q.starts || q.words < 1)))
         return bad(who, "drafted tokens, masks and starts come together");
-    if (q.biases && (!q.bias_tokens || !q.bias_values)) return bad(who, "null array");
+    if (q.biases && requests && (!q.bias_tokens || !q.bias_values)) return bad(who, "null array");
     if (q.allowed && q.allowed_stride < (vocab + 31) / 32 && rows > 1) return bad(who, "mask rows overlap");
     if (!q.starts && requests != rows) return bad(who, "without starts there is one row a request");
-    const int64_t item = dtype == SILI_F32 ? 4 : 2;
-    if ((uintptr_t)logits % item) return bad(who, "logits must be aligned to their type");
-    a = LogitArgs{logits, stride, nullptr, 0, rows, vocab, requests, q.starts, q.history_width ? q.history : nullptr,
-                  q.history_stride, q.history_width, q.history_lens, q.prompt_lens, q.drafted, q.masks, q.words,
-                  q.repetition, q.presence, q.frequency, q.temperature, q.bias_tokens, q.bias_values, q.biases, q.allowed,
-                  q.allowed_stride, nullptr, nullptr, (vocab + kTile - 1) / kTile, 0};
-    // rows that share a request's counts, as far as the mean goes
-    const int64_t mean = requests ? (rows + requests - 1) / requests : rows;
-    a.group = (int)std::min<int64_t>(kGroup, std::max<int64_t>(1, mean));
-    if ((rows + a.group - 1) / a.group * a.tiles > 0x7fffffffLL) return bad(who, "sizes out of range");
+    a = LogitArgs{};
+    a.x = logits;
+    a.x_stride = stride;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.requests = requests;
+    a.starts = q.starts;
+    a.history = q.history_width ? q.history : nullptr;
+    a.history_stride = q.history_stride;
+    a.history_width = a.history ? q.history_width : 0;
+    a.history_lens = q.history_lens;
+    a.prompt_lens = q.prompt_lens;
+    a.drafted = q.drafted;
+    a.masks = q.masks;
+    a.words = q.words;
+    a.repetition = q.repetition;
+    a.presence = q.presence;
+    a.frequency = q.frequency;
+    a.temperature = q.temperature;
+    a.bias_tokens = q.bias_tokens;
+    a.bias_values = q.bias_values;
+    a.biases = q.biases;
+    a.allowed = q.allowed;
+    a.allowed_stride = q.allowed_stride;
+    const int64_t need = lay_out(a, dtype, (a.history || a.biases) && requests, pick, (uint8_t*)scratch);
+    if (rows * a.chunks > 0x7fffffffLL || (int64_t)requests * a.tiles > 0x7fff0000LL) return bad(who, "sizes out of range");
+    if (bytes) { *bytes = need; return SILI_OK; }
+    if (rows == 0) return SILI_OK;
+    if (!logits || (need && !scratch)) return bad(who, "null array");
+    if (rows > 1 && stride < vocab) return bad(who, "rows overlap");
+    if ((uintptr_t)logits % (dtype == SILI_F32 ? 4 : 2)) return bad(who, "logits must be aligned to their type");
+    if ((uintptr_t)scratch % 16) return bad(who, "scratch must be 16-byte aligned");
     return SILI_OK;
 }
 
@@ -506,11 +709,18 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
 
 extern "C" {
 
+int sili_logits_scratch(int dtype, int64_t rows, int vocab, int requests, const sili_logit_rules* rules, int pick,
+                        int64_t* bytes) {
+    if (!bytes) return bad("logits_scratch", "null array");
+    LogitArgs a;
+    return prepare("logits_scratch", dtype, nullptr, vocab, rows, vocab, requests, rules, pick != 0, nullptr, a, bytes);
+}
+
 int sili_adjust_logits(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
-                       const sili_logit_rules* rules, void* out, int64_t out_stride, void* stream) {
+                       const sili_logit_rules* rules, void* out, int64_t out_stride, void* scratch, void* stream) {
     const char* who = "adjust_logits";
     LogitArgs a;
-    if (const int e = prepare(who, dtype, logits, stride, rows, vocab, requests, rules, a)) return e;
+    if (const int e = prepare(who, dtype, logits, stride, rows, vocab, requests, rules, false, scratch, a, nullptr)) return e;
     if (rows == 0) return SILI_OK;
     if (!out) return bad(who, "null array");
     if (rows > 1 && out_stride < vocab) return bad(who, "rows overlap");
@@ -520,29 +730,15 @@ int sili_adjust_logits(int dtype, const void* logits, int64_t stride, int64_t ro
     return by_type<true>(dtype, a, (cudaStream_t)stream);
 }
 
-int sili_pick_tokens_scratch(int64_t rows, int vocab, int64_t* bytes) {
-    if (!bytes) return bad("pick_tokens_scratch", "null array");
-    if (rows < 0 || rows > 0x7fffffffLL || vocab < 1) return bad("pick_tokens_scratch", "sizes out of range");
-    *bytes = rows * ((vocab + kTile - 1) / kTile) * 8;
-    return SILI_OK;
-}
-
 int sili_pick_tokens(int dtype, const void* logits, int64_t stride, int64_t rows, int vocab, int requests,
                      const sili_logit_rules* rules, int* token, void* scratch, void* stream) {
     const char* who = "pick_tokens";
     LogitArgs a;
-    if (const int e = prepare(who, dtype, logits, stride, rows, vocab, requests, rules, a)) return e;
+    if (const int e = prepare(who, dtype, logits, stride, rows, vocab, requests, rules, true, scratch, a, nullptr)) return e;
     if (rows == 0) return SILI_OK;
-    if (!token || !scratch) return bad(who, "null array");
-    if ((uintptr_t)scratch % 8) return bad(who, "scratch must be 8-byte aligned");
-    a.best = (unsigned long long*)scratch;
+    if (!token) return bad(who, "null array");
     a.token = token;
-    cudaStream_t s = (cudaStream_t)stream;
-    if (const int e = by_type<false>(dtype, a, s)) return e;
-    k_picked<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a.best, rows, a.tiles, token);
-    sili::count_launch();
-    CKL(cudaGetLastError());
-    return SILI_OK;
+    return by_type<false>(dtype, a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -879,13 +879,14 @@ PYBIND11_MODULE(_cuda, m) {
                                 (const float*)bias_values, biases, (const uint32_t*)allowed, allowed_stride};
     }));
     m.def("adjust_logits_ptr", [](int dtype, uintptr_t logits, int64_t stride, int64_t rows, int vocab, int requests,
-                                  const sili_logit_rules& rules, uintptr_t out, int64_t out_stride, uintptr_t stream) {
+                                  const sili_logit_rules& rules, uintptr_t out, int64_t out_stride, uintptr_t scratch,
+                                  uintptr_t stream) {
         check(sili_adjust_logits(dtype, (const void*)logits, stride, rows, vocab, requests, &rules, (void*)out, out_stride,
-                                 (void*)stream));
+                                 (void*)scratch, (void*)stream));
     });
-    m.def("pick_tokens_scratch", [](int64_t rows, int vocab) {
+    m.def("logits_scratch", [](int dtype, int64_t rows, int vocab, int requests, const sili_logit_rules& rules, bool pick) {
         int64_t n = 0;
-        check(sili_pick_tokens_scratch(rows, vocab, &n));
+        check(sili_logits_scratch(dtype, rows, vocab, requests, &rules, pick, &n));
         return n;
     });
     m.def("pick_tokens_ptr", [](int dtype, uintptr_t logits, int64_t stride, int64_t rows, int vocab, int requests,

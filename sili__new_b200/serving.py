@@ -847,8 +847,9 @@ def adjust_logits(logits, starts=None, history=None, history_lens=None, prompt_l
     with _on(dev):
         if out is None:
             out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
+        scratch = torch.empty(_cuda.logits_scratch(code, rows, vocab, requests, rules, False), dtype=_U8, device=dev)
         _cuda.adjust_logits_ptr(code, logits.data_ptr(), logits.stride(0), rows, vocab, requests, rules, out.data_ptr(),
-                                out.stride(0), s)
+                                out.stride(0), scratch.data_ptr(), s)
     return out
 
 
@@ -875,7 +876,7 @@ def pick_tokens(logits, starts=None, history=None, history_lens=None, prompt_len
     rows, vocab = logits.shape
     with _on(dev):
         token = torch.empty(rows, dtype=_I32, device=dev)
-        scratch = torch.empty(_cuda.pick_tokens_scratch(rows, vocab), dtype=_U8, device=dev)
+        scratch = torch.empty(_cuda.logits_scratch(code, rows, vocab, requests, rules, True), dtype=_U8, device=dev)
         _cuda.pick_tokens_ptr(code, logits.data_ptr(), logits.stride(0), rows, vocab, requests, rules, token.data_ptr(),
                               scratch.data_ptr(), s)
     return token
