@@ -23,12 +23,11 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <string>
 
 #include "common.cuh"
 #include "kernels.cuh"
-#include "kv4_attention.cuh"
+#include "kv4.cuh"
 #include "sili_b200.h"
 
 namespace sili {
@@ -158,7 +157,8 @@ __global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ Logi
     }
     __shared__ uint32_t cnt[kTile];
     __shared__ int s_sum[kWarps], s_below[kWarps], s_twice;
-    extern __shared__ float bias[];            // [kTile], where there are biases
+    __shared__ uint32_t s_word[kThreads];
+    __shared__ int s_before[kThreads];
     const int r = blockIdx.x / a.tiles, tile = blockIdx.x - r * a.tiles, t0 = tile * kTile, n = min(kTile, a.vocab - t0);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int len = a.history ? min(max(a.history_lens[r], 0), a.history_width) : 0;
@@ -183,30 +183,13 @@ __global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ Logi
     }
     if (a.biases) {
         const int* list = a.bias_tokens + (int64_t)r * a.biases;
-        const float* value = a.bias_values + (int64_t)r * a.biases;
         for (int j = threadIdx.x; j < a.biases; j += kThreads) {
             const int v = list[j];
             const uint32_t i = (uint32_t)v - (uint32_t)t0;
             below += v >= 0 && v < t0;
             if (i >= (uint32_t)n) continue;
-            bias[i] = value[j];
             if (atomicOr(cnt + i, kBiased) & kBiased) s_twice = 1;
         }
-        __syncthreads();
-        if (s_twice)
-            // a token is listed again: its first place adds all of them up, in order
-            for (int j = threadIdx.x; j < a.biases; j += kThreads) {
-                const int v = list[j];
-                const uint32_t i = (uint32_t)v - (uint32_t)t0;
-                if (i >= (uint32_t)n) continue;
-                bool first = true;
-                for (int k = 0; k < j; ++k) first = first && list[k] != v;
-                if (!first) continue;
-                float sum = value[j];
-                for (int k = j + 1; k < a.biases; ++k)
-                    if (list[k] == v) sum += value[k];
-                bias[i] = sum;
-            }
     }
     __syncthreads();
     // a word of 32 tokens a thread and turn: a warp's ballots, token by token
@@ -217,6 +200,7 @@ __global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ Logi
         if (lane == k) word = bits;
     }
     if ((int)threadIdx.x * 32 < n) a.touched[r * a.touched_stride + t0 / 32 + threadIdx.x] = word;
+    const uint32_t kept = word;
     int mine = __popc(word), before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -241,7 +225,28 @@ __global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ Logi
     for (; word; word &= word - 1, ++e) {
         const int i = (int)threadIdx.x * 32 + __ffs(word) - 1;
         a.list[at + e] = make_uint2(t0 + i, cnt[i]);
-        if (a.biases) a.list_bias[at + e] = cnt[i] & kBiased ? bias[i] : 0.f;
+    }
+    if (!a.biases) return;
+    s_word[threadIdx.x] = kept;
+    s_before[threadIdx.x] = before - mine;
+    __syncthreads();
+    const int* list = a.bias_tokens + (int64_t)r * a.biases;
+    const float* value = a.bias_values + (int64_t)r * a.biases;
+    for (int j = threadIdx.x; j < a.biases; j += kThreads) {
+        const int v = list[j];
+        const uint32_t i = (uint32_t)v - (uint32_t)t0;
+        if (i >= (uint32_t)n) continue;
+        float sum = value[j];
+        if (s_twice) {
+            // a token that is listed again: its first place adds all of them up, in order
+            bool first = true;
+            for (int k = 0; k < j; ++k) first = first && list[k] != v;
+            if (!first) continue;
+            for (int k = j + 1; k < a.biases; ++k)
+                if (list[k] == v) sum += value[k];
+        }
+        // its place in the list: the touched tokens before it
+        a.list_bias[at + s_before[i >> 5] + __popc(s_word[i >> 5] & ((1u << (i & 31)) - 1u))] = sum;
     }
 }
 
@@ -480,6 +485,29 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
             else if (u == high) low = max(low, ~(uint32_t)v);
         }
     };
+    // picking: the others' largest, and what is certainly below it
+    const uint32_t* most = WRITE ? nullptr : a.most + row * a.chunks * kWarps;
+    const int parts = WRITE ? 0 : a.chunks * kWarps;
+    uint32_t other = 0;            // the order of this thread's parts' largest, before the division
+    for (int i = tid; i < parts; i += kThreads) other = max(other, most[i]);
+    // (quotients that leave the normal range: any of them may be the same)
+    auto below = [&](float top) { return rule.by.on && !rule.by.takes(top) ? -INFINITY : top - fabsf(top) * 0x1p-20f; };
+    auto reduce = [&](uint32_t u, int which) {
+        u = __reduce_max_sync(0xffffffffu, u);
+        __syncthreads();
+        if (lane == 0) s_red[warp][which] = u;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) all = max(all, s_red[w][which]);
+        return all;
+    };
+    float near = -INFINITY;
+    bool lowers = false;           // the penalties raise no logit: one below the others' largest stays there
+    if (!WRITE) {
+        near = below(of_order(reduce(other, 0)));
+        lowers = rule.rep.t >= 1.f && rule.freq >= 0.f && rule.pres >= 0.f;
+    }
     // the listed tokens: of each 64 tiles, all places in a row
     for (int tile0 = 0; touched && tile0 < a.tiles; tile0 += 64) {
         const int m = min(64, a.tiles - tile0);
@@ -505,7 +533,8 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
             uint2 it[kBatch];
             float bias[kBatch];
             T v[kBatch];
-            bool is[kBatch];
+            uint32_t word[kBatch];
+            // (several in flight: no load is used before all of them have been asked for)
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int e = e0 + b * stride;
@@ -519,12 +548,13 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
             for (int b = 0; b < kBatch; ++b)
                 if (e0 + b * stride < all) {
                     v[b] = x[it[b].x];
-                    is[b] = may((int)it[b].x);
+                    word[b] = allow ? __ldg(allow + (it[b].x >> 5)) : 0xFFFFFFFFu;
                 }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
-                if (e0 + b * stride < all)
-                    take((int)it[b].x, rule(sili::to_f32(v[b]), it[b].y + times((int)it[b].x), bias[b]), is[b]);
+                if (e0 + b * stride < all && !(!WRITE && lowers && !(it[b].y & kBiased) && sili::to_f32(v[b]) < near))
+                    take((int)it[b].x, rule(sili::to_f32(v[b]), it[b].y + times((int)it[b].x), bias[b]),
+                         word[b] >> (it[b].x & 31) & 1);
         }
     }
     // the path's tokens that are on no list, at the first of their places
@@ -535,26 +565,8 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
         if (first) take(v, rule(sili::to_f32(x[v]), times(v), 0.f), may(v));
     }
     if (WRITE) return;
-    // the others' largest values, after the division
-    const uint32_t* most = a.most + row * a.chunks * kWarps;
-    const int parts = a.chunks * kWarps;
-    uint32_t other = 0;
-    int at_other = 0;              // the first of this thread's parts that hold its largest
-    for (int i = tid; i < parts; i += kThreads) {
-        const uint32_t u = order_of(rule.by(of_order(most[i])));
-        if (u > other) { other = u; at_other = i; }
-    }
-    auto reduce = [&](uint32_t u, int which) {
-        u = __reduce_max_sync(0xffffffffu, u);
-        __syncthreads();
-        if (lane == 0) s_red[warp][which] = u;
-        __syncthreads();
-        uint32_t all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all = max(all, s_red[w][which]);
-        return all;
-    };
-    const uint32_t all = reduce(max(other, high), 0);
+    other = order_of(rule.by(of_order(other)));
+    const uint32_t all = reduce(max(other, high), 1);
     if (high != all) low = 0;
     if (all && __syncthreads_or(other == all)) {
         // the parts that hold it are read again: after the division, elements next to the largest may be as large
@@ -565,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
             low = max(low, ~(uint32_t)v);
         };
         for (int i = tid; i < parts; i += kThreads)
-            if (i >= at_other && other == all && order_of(rule.by(of_order(most[i]))) == all) {
+            if (other == all && order_of(rule.by(of_order(most[i]))) == all) {
                 const int k = atomicAdd(&s_held, 1);
                 if (k < kMostHeld) s_hold[k] = i;
             }
@@ -576,8 +588,7 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
             const int i = s_held > kMostHeld ? k : s_hold[k];
             const float top = of_order(most[i]);
             if (s_held > kMostHeld && order_of(rule.by(top)) != all) continue;
-            // (quotients that leave the normal range: any of them may be the same)
-            const float near = rule.by.on && !rule.by.takes(top) ? -INFINITY : top - fabsf(top) * 0x1p-20f;
+            const float near = below(top);
             const int chunk = i / kWarps, w = i - chunk * kWarps;
             const Lay<T> lay(a, x, chunk);
             // the warp's whole accesses, and the single elements that were its own
@@ -598,7 +609,7 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
                 }
         }
     }
-    low = reduce(low, 1);
+    low = reduce(low, 0);
     if (tid == 0) a.token[row] = all ? (int)~low : -1;
 }
 
@@ -630,10 +641,7 @@ int launch(const LogitArgs& a, cudaStream_t s) {
     if (a.row_of || a.touched) {
         const int64_t tiles = a.touched ? (int64_t)a.requests * a.tiles : 0;
         const int64_t finders = a.row_of ? std::min<int64_t>((a.rows + kThreads - 1) / kThreads, 148) : 0;
-        const int smem = a.biases && tiles ? kTile * 4 : 0;
-        static std::atomic<uint64_t> set{0};
-        if (smem) CKL(sili::allow_smem(k_touch, smem, set));
-        k_touch<<<(unsigned)(tiles + finders), kThreads, smem, s>>>(a);
+        k_touch<<<(unsigned)(tiles + finders), kThreads, 0, s>>>(a);
         sili::count_launch();
     }
     k_stream<T, WRITE><<<(unsigned)(a.rows * a.chunks), kThreads, 0, s>>>(a);
