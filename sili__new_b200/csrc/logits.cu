@@ -8,18 +8,19 @@
 //   c(v) > 0 times in the history behind the prompt and on the path: - freq * c, - pres
 //   + bias(v);  / temp where temp > 0;  -inf where the mask's bit is not set.
 //
-// Three launches.  k_touch counts, for each request, the tokens of its history
-// and bias list in shared memory, a tile of the vocabulary at a time, and
-// leaves a bit a token and a list of those that it touched.  k_stream is one
-// pass over the logits in 16-byte accesses: it divides and masks what is not
-// touched, nor on the row's path (adjusting), or looks for the largest of it
-// before the division, which keeps the order (picking).  k_listed then takes
-// the touched tokens and the path one by one, a row a CTA, and, picking, finds
-// the first place of the largest: only where the division may have made
-// neighbours equal is a part of the row read again.  So the logits' bytes are
-// what bounds a large call; with the counts in the streaming CTAs, 32 trees
-// of 32 over 131072 tokens took 252 us in place of @PICK@ (a vocabulary's most
-// frequent tokens lie close together, and their CTAs were the last by far).
+// k_touch counts, for each request, the tokens of its history and bias list in
+// shared memory, a tile of the vocabulary at a time, and leaves a bit a token
+// and a list of those that it touched.  k_stream takes a tile of a row: one
+// pass in 16-byte accesses divides and masks what is neither touched nor on
+// the row's path (adjusting), or looks for the largest of it before the
+// division, which keeps the order (picking); then come the touched tokens, one
+// by one, from the list.  k_pick finds a row's largest and its first place: a
+// part of the row is read again, since the division may have made neighbours
+// equal.  So the logits' bytes are what should bound a large call.  With the
+// counts in the streaming CTAs, 32 trees of 32 over 131072 tokens took 252 us
+// in place of 125 (a vocabulary's most frequent tokens lie close together, and
+// their CTAs were the last by far); with the touched tokens in a launch of
+// their own, which fetches them once more, 140.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -49,12 +50,10 @@ int bad(const char* who, const char* what) {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                    // tokens that a CTA of k_touch counts
-constexpr int kPacks = 8;                      // 16-byte accesses of a thread of k_stream
 constexpr int kMostDrafts = 256;
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
-// elements of a row that a CTA of k_stream takes, and a warp of it
-template <typename T> constexpr int kChunk = kThreads * kPacks * (16 / (int)sizeof(T));
-int chunk_of(int dtype) { return dtype == SILI_F32 ? kChunk<float> : kChunk<__half>; }
+// 16-byte accesses of a thread of k_stream, whose CTAs take a tile of a row each
+template <typename T> constexpr int kPacksOf = kTile / kThreads * (int)sizeof(T) / 16;
 
 struct LogitArgs {
     const void* x;
@@ -91,8 +90,8 @@ struct LogitArgs {
     float* list_bias;          // [requests, cap]
     int64_t cap;
     int tiles;
-    uint32_t* most;            // picking: [rows, chunks, warps]: the order (below) of the largest element that is not touched
-    int chunks;
+    uint4* parts;              // picking: [rows, chunks, warps]: the order (below) of a warp's largest element that is not
+                               // touched; of its largest touched one, after the rules, and that one's token, inverted
 };
 
 // x: the request, or -1; y, z: its rows
@@ -250,6 +249,12 @@ __global__ void __launch_bounds__(kThreads) k_touch(const __grid_constant__ Logi
     }
 }
 
+// What is certainly smaller than `top`, and stays so after the division (where a quotient leaves the normal range, any two
+// may become the same).
+__device__ __forceinline__ float surely_below(const Divisor& by, float top) {
+    return by.on && !by.takes(top) ? -INFINITY : top - fabsf(top) * 0x1p-20f;
+}
+
 // A row's rules.
 struct Rules {
     float freq, pres;
@@ -297,8 +302,8 @@ struct Lay {
     static constexpr int kVec = 16 / (int)sizeof(T);
     int t0, n, head, packs;
     __device__ __forceinline__ Lay(const LogitArgs& a, const T* row, int chunk) {
-        t0 = chunk * kChunk<T>;
-        n = min(kChunk<T>, a.vocab - t0);
+        t0 = chunk * kTile;
+        n = min(kTile, a.vocab - t0);
         head = min((int)((16 - (uintptr_t)(row + t0) % 16) % 16 / sizeof(T)), n);
         packs = (n - head) / kVec;
     }
@@ -307,15 +312,16 @@ struct Lay {
 // ── the pass over the logits ────────────────────────────────────────────────
 // A CTA takes a chunk of one row.  Touched tokens and the row's path are left as they are (adjusting), or aside (picking).
 template <typename T, bool WRITE>
-__global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ LogitArgs a) {
-    constexpr int kVec = 16 / (int)sizeof(T), kStep = kThreads * kVec / 32;
-    static_assert(kChunk<T> % 32 == 0 && kThreads * kVec % 32 == 0, "whole words");
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 5) k_stream(const __grid_constant__ LogitArgs a) {
+    constexpr int kVec = 16 / (int)sizeof(T), kPacks = kPacksOf<T>, kStep = kThreads * kVec / 32;
+    static_assert(kThreads * kVec % 32 == 0, "whole words");
     using P = sili::Pack<T, kVec>;
-    constexpr int kWords = kChunk<T> / 32;
-    // bits of the chunk's tokens: those to take (picking: allowed and not touched), and (adjusting) those to leave
-    __shared__ uint32_t s_take[kWords + 1], s_rest[WRITE ? kWords + 1 : 1];
-    const int64_t row = blockIdx.x / a.chunks;
-    const int chunk = blockIdx.x - (int)row * a.chunks, tid = threadIdx.x;
+    constexpr int kWords = kTile / 32;
+    // bits of the tile's tokens: those that are allowed; adjusting, those to leave, and picking, those to take
+    __shared__ uint32_t s_allow[kWords + 1], s_rest[kWords + 1], s_path[kWords];
+    __shared__ int s_tok[kMostDrafts], s_n;        // the path's tokens that lie in the tile
+    const int64_t row = blockIdx.x / a.tiles;
+    const int chunk = blockIdx.x - (int)row * a.tiles, tid = threadIdx.x;
     const T* x = (const T*)a.x + row * a.x_stride;
     T* y = WRITE ? (T*)a.y + row * a.y_stride : nullptr;
     Lay<T> lay(a, x, chunk);
@@ -340,8 +346,10 @@ __global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ Log
     const uint32_t* allow = a.allowed ? a.allowed + row * a.allowed_stride + (t0 >> 5) : nullptr;
     const uint32_t* touched = a.touched ? a.touched + r * a.touched_stride + (t0 >> 5) : nullptr;
     const bool bits = a.allowed || a.touched || a.drafted;
-    Divisor by;
-    by.set(a.temperature ? a.temperature[r] : 0.f);
+    const int2 listed = touched ? a.listed[r * a.tiles + chunk] : make_int2(0, 0);
+    const Rules rule(a, r);
+    const Divisor& by = rule.by;
+    bool path = false;
     if (bits) {
         uint32_t i = 0xFFFFFFFFu;
         if (a.drafted) {
@@ -358,15 +366,29 @@ __global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ Log
 #pragma unroll
         for (int k = 0; k < kWords / kThreads; ++k) {
             const int w = tid + k * kThreads;
-            s_take[w] = WRITE ? word[0][k] : word[0][k] & ~word[1][k];
-            if (WRITE) s_rest[w] = word[1][k];
+            s_allow[w] = word[0][k];
+            s_rest[w] = WRITE ? word[1][k] : word[0][k] & ~word[1][k];
         }
-        if (__syncthreads_or(i < (uint32_t)n)) {
+        path = __syncthreads_or(i < (uint32_t)n);
+        if (path) {
+            for (int w = tid; w < kWords; w += kThreads) s_path[w] = 0;
+            if (tid == 0) s_n = 0;
+            __syncthreads();
             if (i < (uint32_t)n) {
-                if (WRITE) atomicOr(s_rest + (i >> 5), 1u << (i & 31)); else atomicAnd(s_take + (i >> 5), ~(1u << (i & 31)));
+                atomicOr(s_path + (i >> 5), 1u << (i & 31));
+                s_tok[atomicAdd(&s_n, 1)] = (int)i;
+                if (WRITE) atomicOr(s_rest + (i >> 5), 1u << (i & 31)); else atomicAnd(s_rest + (i >> 5), ~(1u << (i & 31)));
             }
             __syncthreads();
         }
+    }
+    // this thread's first touched token, on its way during the pass
+    const int64_t list_at = r * a.cap + listed.x;
+    uint2 next = make_uint2((uint32_t)t0, 0);
+    float next_bias = 0.f;
+    if (tid < listed.y) {
+        next = a.list[list_at + tid];
+        if (a.biases) next_bias = a.list_bias[list_at + tid];
     }
     // a pack's bits lie in one word or two, whose places move by a constant from pack to pack
     const int shift = first & 31, at0 = first >> 5, more = ((first + kVec - 1) >> 5) - at0;
@@ -377,16 +399,15 @@ __global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ Log
     // elements before and behind the whole accesses
     for (int i = tid; i < n - packs * kVec; i += kThreads) {
         const int j = i < head ? i : i + packs * kVec, w = j >> 5;
-        const uint32_t may = bits ? s_take[w] >> (j & 31) & 1 : 1u;
         if (WRITE) {
-            const bool left = bits && (s_rest[w] >> (j & 31) & 1);
+            const bool left = bits && (s_rest[w] >> (j & 31) & 1), may = !bits || (s_allow[w] >> (j & 31) & 1);
             y[j] = left ? x[j] : sili::from_f32<T>(may ? by(sili::to_f32(x[j])) : -INFINITY);
-        } else raise(most, sili::to_f32(x[j]), may, 0);
+        } else raise(most, sili::to_f32(x[j]), bits ? s_rest[w] >> (j & 31) : 1u, 0);
     }
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) {
         if (tid + k * kThreads >= packs) break;
-        const uint32_t take = bits ? bits_of(s_take, k) : 0xFFFFFFFFu;
+        const uint32_t take = bits ? bits_of(WRITE ? s_allow : s_rest, k) : 0xFFFFFFFFu;
         if (WRITE) {
             const uint32_t rest = bits ? bits_of(s_rest, k) : 0u;
             P out;
@@ -419,183 +440,140 @@ __global__ void __launch_bounds__(kThreads) k_stream(const __grid_constant__ Log
             for (int e = 0; e < kVec; ++e) raise(most, sili::to_f32(in[k].v[e]), take, e);
         }
     }
-    if (!WRITE) {
-        const uint32_t all = __reduce_max_sync(0xffffffffu, order_of(most));
-        if ((tid & 31) == 0) a.most[((int64_t)row * a.chunks + chunk) * kWarps + (tid >> 5)] = all;
-    }
-}
-
-// ── the touched tokens, and the pick ────────────────────────────────────────
-// A CTA takes a row; adjusting, several may share its list.
-constexpr int kMostHeld = 64;
-struct Path {
-    uint32_t filter[256];          // a bit a token's hash
-    int token[kMostDrafts];
-    int n;
-};
-
-template <typename T, bool WRITE>
-__global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ LogitArgs a) {
-    __shared__ Path s;
-    __shared__ uint32_t s_red[kWarps][2];
-    __shared__ int s_first[65], s_base[64], s_hold[kMostHeld], s_held;
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int4 of = request_of(a, row);
-    const uint64_t mask = path_mask(a, row, tid);
-    const int r = of.x;
-    if (r < 0) {
-        if (!WRITE && tid == 0) a.token[row] = -1;
-        return;
-    }
-    const Rules rule(a, r);
-    // adjusting, what is touched still holds the logits
-    const T* x = WRITE ? (const T*)a.y + row * a.y_stride : (const T*)a.x + row * a.x_stride;
-    T* y = WRITE ? (T*)a.y + row * a.y_stride : nullptr;
-    const uint32_t* allow = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    const uint32_t* touched = a.touched ? a.touched + r * a.touched_stride : nullptr;
-    auto may = [&](int v) { return !allow || (__ldg(allow + (v >> 5)) >> (v & 31) & 1); };
-    auto hash = [](int v) { return (uint32_t)v & 8191u; };
-    // the row's path
-    if (tid == 0) s.n = s_held = 0;
-    if (a.drafted) {
-        s.filter[tid] = 0;
-        __syncthreads();
-        const int v = path_token(a, of, tid, mask);
-        if (v >= 0 && v < a.vocab) {
-            s.token[atomicAdd(&s.n, 1)] = v;
-            atomicOr(s.filter + (hash(v) >> 5), 1u << (hash(v) & 31));
-        }
-    }
-    __syncthreads();
-    const int path = s.n;
-    auto times = [&](int v) {      // on the path
-        uint32_t c = 0;
-        if (path && (s.filter[hash(v) >> 5] >> (hash(v) & 31) & 1))
-            for (int k = 0; k < path; ++k) c += s.token[k] == v;
-        return c;
-    };
-    uint32_t high = 0, low = 0;    // the largest so far and its token, inverted
-    auto take = [&](int v, float value, bool is) {
-        const float z = is ? value : -INFINITY;
-        if (WRITE) y[v] = sili::from_f32<T>(z);
-        else {
-            const uint32_t u = order_of(z);
-            if (u > high) { high = u; low = ~(uint32_t)v; }
-            else if (u == high) low = max(low, ~(uint32_t)v);
-        }
-    };
-    // picking: the others' largest, and what is certainly below it
-    const uint32_t* most = WRITE ? nullptr : a.most + row * a.chunks * kWarps;
-    const int parts = WRITE ? 0 : a.chunks * kWarps;
-    uint32_t other = 0;            // the order of this thread's parts' largest, before the division
-    for (int i = tid; i < parts; i += kThreads) other = max(other, most[i]);
-    // (quotients that leave the normal range: any of them may be the same)
-    auto below = [&](float top) { return rule.by.on && !rule.by.takes(top) ? -INFINITY : top - fabsf(top) * 0x1p-20f; };
-    auto reduce = [&](uint32_t u, int which) {
-        u = __reduce_max_sync(0xffffffffu, u);
-        __syncthreads();
-        if (lane == 0) s_red[warp][which] = u;
-        __syncthreads();
-        uint32_t all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all = max(all, s_red[w][which]);
-        return all;
-    };
-    float near = -INFINITY;
-    bool lowers = false;           // the penalties raise no logit: one below the others' largest stays there
-    if (!WRITE) {
-        near = below(of_order(reduce(other, 0)));
-        lowers = rule.rep.t >= 1.f && rule.freq >= 0.f && rule.pres >= 0.f;
-    }
-    // the listed tokens: of each 64 tiles, all places in a row
-    for (int tile0 = 0; touched && tile0 < a.tiles; tile0 += 64) {
-        const int m = min(64, a.tiles - tile0);
-        __syncthreads();
-        if (warp == 0) {
-            int carry = 0;
-            for (int b = 0; b < m; b += 32) {
-                const int2 c = b + lane < m ? a.listed[(int64_t)r * a.tiles + tile0 + b + lane] : make_int2(0, 0);
-                const uint32_t inc = sili::warp_inclusive_scan((uint32_t)c.y);
-                if (b + lane < m) {
-                    s_first[b + lane] = carry + (int)inc - c.y;
-                    s_base[b + lane] = c.x;
-                }
-                carry += (int)__shfl_sync(0xffffffffu, inc, 31);
+    const uint32_t all = WRITE ? 0u : __reduce_max_sync(0xffffffffu, order_of(most));
+    uint32_t high = 0, low = 0;    // picking: the largest touched one and its token, inverted
+    if (touched || path) {
+        if (WRITE) __syncthreads();        // (what is touched has been written as it was, with what lies beside it)
+        // picking, where the penalties raise no logit: one below the warp's largest other stays there
+        const bool lowers = !WRITE && rule.rep.t >= 1.f && rule.freq >= 0.f && rule.pres >= 0.f;
+        const float near = WRITE ? 0.f : surely_below(by, of_order(all));
+        auto times = [&](int i) {          // on the path
+            uint32_t c = 0;
+            if (path && (s_path[i >> 5] >> (i & 31) & 1))
+                for (int k = 0; k < s_n; ++k) c += s_tok[k] == i;
+            return c;
+        };
+        auto one = [&](int i, T raw, uint32_t what, float bias) {
+            const float v = sili::to_f32(raw);
+            if (!WRITE && lowers && !(what & kBiased) && v < near) return;
+            const bool may = s_allow[i >> 5] >> (i & 31) & 1;
+            const float z = may ? rule(v, what + times(i), bias) : -INFINITY;
+            if (WRITE) y[i] = sili::from_f32<T>(z);
+            else {
+                const uint32_t u = order_of(z);
+                if (u > high) { high = u; low = ~(uint32_t)(t0 + i); }
+                else if (u == high) low = max(low, ~(uint32_t)(t0 + i));
             }
-            if (lane == 0) s_first[m] = carry;
-        }
-        __syncthreads();
-        const int all = s_first[m], stride = kThreads * gridDim.y;
-        constexpr int kBatch = 4;
-        int t = 0;
-        for (int e0 = tid + blockIdx.y * kThreads; e0 < all; e0 += kBatch * stride) {
+        };
+        if (tid < listed.y) one((int)next.x - t0, x[(int)next.x - t0], next.y, next_bias);
+        constexpr int kBatch = 4;      // in flight: no load is used before all of them have been asked for
+        for (int e0 = tid + kThreads; e0 < listed.y; e0 += kBatch * kThreads) {
             uint2 it[kBatch];
             float bias[kBatch];
             T v[kBatch];
-            uint32_t word[kBatch];
-            // (several in flight: no load is used before all of them have been asked for)
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int e = e0 + b * stride;
-                if (e >= all) continue;
-                while (s_first[t + 1] <= e) ++t;
-                const int64_t at = r * a.cap + s_base[t] + (e - s_first[t]);
-                it[b] = a.list[at];
-                bias[b] = a.biases ? a.list_bias[at] : 0.f;
-            }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
-                if (e0 + b * stride < all) {
-                    v[b] = x[it[b].x];
-                    word[b] = allow ? __ldg(allow + (it[b].x >> 5)) : 0xFFFFFFFFu;
+                if (e0 + b * kThreads < listed.y) {
+                    it[b] = a.list[list_at + e0 + b * kThreads];
+                    bias[b] = a.biases ? a.list_bias[list_at + e0 + b * kThreads] : 0.f;
                 }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
-                if (e0 + b * stride < all && !(!WRITE && lowers && !(it[b].y & kBiased) && sili::to_f32(v[b]) < near))
-                    take((int)it[b].x, rule(sili::to_f32(v[b]), it[b].y + times((int)it[b].x), bias[b]),
-                         word[b] >> (it[b].x & 31) & 1);
+                if (e0 + b * kThreads < listed.y) v[b] = x[(int)it[b].x - t0];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (e0 + b * kThreads < listed.y) one((int)it[b].x - t0, v[b], it[b].y, bias[b]);
+        }
+        // the path's tokens that are on no list, at the first of their places
+        if (path && tid < s_n) {
+            const int i = s_tok[tid];
+            bool is = !touched || !(touched[i >> 5] >> (i & 31) & 1);
+            for (int k = 0; k < tid; ++k) is = is && s_tok[k] != i;
+            if (is) one(i, x[i], 0u, 0.f);
+        }
+        if (!WRITE) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, high);
+            low = __reduce_max_sync(0xffffffffu, high == top ? low : 0u);
+            high = top;
         }
     }
-    // the path's tokens that are on no list, at the first of their places
-    if (blockIdx.y == 0 && tid < path) {
-        const int v = s.token[tid];
-        bool first = !touched || !(touched[v >> 5] >> (v & 31) & 1);
-        for (int k = 0; k < tid; ++k) first = first && s.token[k] != v;
-        if (first) take(v, rule(sili::to_f32(x[v]), times(v), 0.f), may(v));
+    if (!WRITE && (tid & 31) == 0) a.parts[((int64_t)row * a.tiles + chunk) * kWarps + (tid >> 5)] = make_uint4(all, high, low, 0);
+}
+
+// ── the pick ────────────────────────────────────────────────────────────────
+// A row a CTA: the largest of its parts, and the first place of it.
+constexpr int kPickThreads = 128, kMostHeld = 64;
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ LogitArgs a) {
+    __shared__ uint32_t s_red[2][kPickThreads / 32];
+    __shared__ int s_hold[kMostHeld], s_held;
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int4 of = request_of(a, row);
+    const int r = of.x;
+    if (r < 0) {
+        if (tid == 0) a.token[row] = -1;
+        return;
     }
-    if (WRITE) return;
-    other = order_of(rule.by(of_order(other)));
-    const uint32_t all = reduce(max(other, high), 1);
+    if (tid == 0) s_held = 0;
+    Divisor by;
+    by.set(a.temperature ? a.temperature[r] : 0.f);
+    auto reduce = [&](uint32_t u, int which) {
+        u = __reduce_max_sync(0xffffffffu, u);
+        if (lane == 0) s_red[which][warp] = u;
+        __syncthreads();
+        uint32_t top = 0;
+#pragma unroll
+        for (int w = 0; w < kPickThreads / 32; ++w) top = max(top, s_red[which][w]);
+        return top;
+    };
+    const uint4* parts = a.parts + row * a.tiles * kWarps;
+    const int n_parts = a.tiles * kWarps;
+    uint32_t other = 0, high = 0, low = 0;
+    for (int i = tid; i < n_parts; i += kPickThreads) {
+        const uint4 p = parts[i];
+        other = max(other, p.x);
+        if (p.y > high) { high = p.y; low = p.z; }
+        else if (p.y == high) low = max(low, p.z);
+    }
+    other = order_of(by(of_order(other)));
+    const uint32_t all = reduce(max(other, high), 0);
     if (high != all) low = 0;
     if (all && __syncthreads_or(other == all)) {
         // the parts that hold it are read again: after the division, elements next to the largest may be as large
-        constexpr int kVec = 16 / (int)sizeof(T);
-        using P = sili::Pack<T, kVec>;
+        const T* x = (const T*)a.x + row * a.x_stride;
+        const uint32_t* allow = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+        const uint32_t* touched = a.touched ? a.touched + r * a.touched_stride : nullptr;
         auto candidate = [&](int v, float value) {
-            if (order_of(rule.by(value)) != all || (touched && (touched[v >> 5] >> (v & 31) & 1)) || times(v) || !may(v)) return;
+            if (order_of(by(value)) != all || (touched && (touched[v >> 5] >> (v & 31) & 1))) return;
+            if (allow && !(__ldg(allow + (v >> 5)) >> (v & 31) & 1)) return;
+            if (a.drafted)
+                for (int j = 0; j < 64 * a.words; ++j)
+                    if (path_token(a, of, j, path_mask(a, row, j)) == v) return;
             low = max(low, ~(uint32_t)v);
         };
-        for (int i = tid; i < parts; i += kThreads)
-            if (other == all && order_of(rule.by(of_order(most[i]))) == all) {
+        for (int i = tid; i < n_parts; i += kPickThreads)
+            if (order_of(by(of_order(parts[i].x))) == all) {
                 const int k = atomicAdd(&s_held, 1);
                 if (k < kMostHeld) s_hold[k] = i;
             }
         __syncthreads();
         // (more of them than there is room for, as where a row is one value: all parts are looked at)
-        const int held = s_held > kMostHeld ? parts : s_held;
+        const int held = s_held > kMostHeld ? n_parts : s_held;
+        using P = sili::Pack<T, 16 / sizeof(T)>;
+        constexpr int kVec = 16 / (int)sizeof(T), kPacks = kPacksOf<T>;
         for (int k = 0; k < held; ++k) {
             const int i = s_held > kMostHeld ? k : s_hold[k];
-            const float top = of_order(most[i]);
-            if (s_held > kMostHeld && order_of(rule.by(top)) != all) continue;
-            const float near = below(top);
+            const float top = of_order(parts[i].x), near = surely_below(by, top);
+            if (s_held > kMostHeld && order_of(by(top)) != all) continue;
+            // the warp's whole accesses, and the single elements that were its own
             const int chunk = i / kWarps, w = i - chunk * kWarps;
             const Lay<T> lay(a, x, chunk);
-            // the warp's whole accesses, and the single elements that were its own
-            static_assert(kPacks == kWarps, "a warp of this CTA an access of that one's");
-            const int p = w * 32 + lane + warp * kThreads;
-            if (p < lay.packs) {
-                const int at = lay.t0 + lay.head + p * kVec;
+#pragma unroll
+            for (int b = 0; b < kPacks; b += kPickThreads / 32) {
+                const int p = w * 32 + lane + (b + warp) * kThreads, at = lay.t0 + lay.head + p * kVec;
+                if (p >= lay.packs) continue;
                 const P in = *(const P*)(x + at);
                 uint32_t some = 0;
 #pragma unroll
@@ -603,13 +581,13 @@ __global__ void __launch_bounds__(kThreads) k_listed(const __grid_constant__ Log
                 for (; some; some &= some - 1) candidate(at + __ffs(some) - 1, element<T>(in, __ffs(some) - 1));
             }
             if (warp == 0)
-                for (int k = w * 32 + lane; k < lay.n - lay.packs * kVec; k += kThreads) {
-                    const int j = lay.t0 + (k < lay.head ? k : k + lay.packs * kVec);
+                for (int e = w * 32 + lane; e < lay.n - lay.packs * kVec; e += kThreads) {
+                    const int j = lay.t0 + (e < lay.head ? e : e + lay.packs * kVec);
                     candidate(j, sili::to_f32(x[j]));
                 }
         }
     }
-    low = reduce(low, 0);
+    low = reduce(low, 1);
     if (tid == 0) a.token[row] = all ? (int)~low : -1;
 }
 
@@ -621,7 +599,6 @@ int64_t lay_out(LogitArgs& a, int dtype, bool counts, bool pick, uint8_t* base) 
     int64_t at = 0;
     auto part = [&](int64_t bytes) { const int64_t here = at; at += round16(bytes); return base + here; };
     a.tiles = (a.vocab + kTile - 1) / kTile;
-    a.chunks = (a.vocab + chunk_of(dtype) - 1) / chunk_of(dtype);
     a.cap = (int64_t)a.history_width + a.biases;
     a.touched_stride = (int64_t)a.tiles * (kTile / 32) + 1;
     a.row_of = a.starts ? (int4*)part(a.rows * 16) : nullptr;
@@ -632,7 +609,7 @@ int64_t lay_out(LogitArgs& a, int dtype, bool counts, bool pick, uint8_t* base) 
         a.list = (uint2*)part(a.requests * a.cap * 8);
         a.list_bias = (float*)part(a.biases ? a.requests * a.cap * 4 : 0);
     }
-    a.most = pick ? (uint32_t*)part(a.rows * a.chunks * kWarps * 4) : nullptr;
+    a.parts = pick ? (uint4*)part(a.rows * a.tiles * kWarps * 16) : nullptr;
     return at;
 }
 
@@ -644,13 +621,10 @@ int launch(const LogitArgs& a, cudaStream_t s) {
         k_touch<<<(unsigned)(tiles + finders), kThreads, 0, s>>>(a);
         sili::count_launch();
     }
-    k_stream<T, WRITE><<<(unsigned)(a.rows * a.chunks), kThreads, 0, s>>>(a);
+    k_stream<T, WRITE><<<(unsigned)(a.rows * a.tiles), kThreads, 0, s>>>(a);
     sili::count_launch();
-    if (!WRITE || a.touched || a.drafted) {
-        // (adjusting, long lists of few rows are shared)
-        const int64_t most = (int64_t)a.history_width + a.biases;
-        const int share = WRITE && a.touched ? (int)std::max<int64_t>(1, std::min<int64_t>(most / 1024, 1184 / std::max<int64_t>(a.rows, 1))) : 1;
-        k_listed<T, WRITE><<<dim3((unsigned)a.rows, share), kThreads, 0, s>>>(a);
+    if (!WRITE) {
+        k_pick<T><<<(unsigned)a.rows, kPickThreads, 0, s>>>(a);
         sili::count_launch();
     }
     CKL(cudaGetLastError());
@@ -703,7 +677,7 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
     a.allowed = q.allowed;
     a.allowed_stride = q.allowed_stride;
     const int64_t need = lay_out(a, dtype, (a.history || a.biases) && requests, pick, (uint8_t*)scratch);
-    if (rows * a.chunks > 0x7fffffffLL || (int64_t)requests * a.tiles > 0x7fff0000LL) return bad(who, "sizes out of range");
+    if (rows * a.tiles > 0x7fffffffLL || (int64_t)requests * a.tiles > 0x7fff0000LL) return bad(who, "sizes out of range");
     if (bytes) { *bytes = need; return SILI_OK; }
     if (rows == 0) return SILI_OK;
     if (!logits || (need && !scratch)) return bad(who, "null array");
