@@ -553,7 +553,11 @@ int sili_draft_tree(const int* parents, const int* starts, const int* lens, int 
 /* sili_kv4_attention for such a step: row i of a request sees the committed
  * keys, with window > 0 only the last window - (bits of its mask) of them, and
  * the request's drafted keys whose bits its mask has.  A row without a bit sees
- * nothing.  masks [tokens, words], words 1 to 4. */
+ * nothing.  masks [tokens, words], words 1 to 4.  workspace:
+ * sili_kv4_tree_attention_workspace bytes, kept as that of
+ * sili_kv4_attention is (and looked at by sili_kv4_attention_status), for
+ * calls of the same answer only. */
+int sili_kv4_tree_attention_workspace(int dtype, int dim, int heads, int kv_heads, int most_new, int64_t* bytes);
 int sili_kv4_tree_attention(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
                             int heads, int dim, const uint8_t* codes, const uint8_t* scales, int64_t n_pages, int page,
                             int kv_heads, const int* table, int64_t table_stride, int width, const int* lens, int requests,

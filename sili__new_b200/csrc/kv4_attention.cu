@@ -858,6 +858,15 @@ int sili_kv4_attention_workspace(int64_t* bytes) {
     return SILI_OK;
 }
 
+int sili_kv4_tree_attention_workspace(int dtype, int dim, int heads, int kv_heads, int most_new, int64_t* bytes) {
+    const char* who = "kv4_tree_attention_workspace";
+    if (!bytes) return bad(who, "null array");
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads || most_new < 0) return bad(who, "sizes out of range");
+    const int64_t rows = (int64_t)std::max(most_new, 1) * (heads / kv_heads);
+    *bytes = sili::kv4_tree_takes(dtype, dim, rows) ? sili::kv4_tree_workspace(dim, rows) : workspace_bytes();
+    return SILI_OK;
+}
+
 int sili_kv4_attention_long_prompt(int dtype, int dim, int64_t tokens, int heads, int kv_heads, int most_new, int* yes) {
     const char* who = "kv4_attention_long_prompt";
     if (!yes) return bad(who, "null array");

@@ -207,6 +207,7 @@ int kv4_prompt_launch(int dtype, int dim, const AttendArgs& a, cudaStream_t s);
 void kv4_polls(AttendArgs& a);
 // Trees with many 16-bit rows a request (kv4_tree.cu).
 bool kv4_tree_takes(int dtype, int dim, int64_t rows);
+int64_t kv4_tree_workspace(int dim, int64_t rows);
 int kv4_tree_launch(int dtype, int dim, const AttendArgs& a, int64_t rows, cudaStream_t s);
 
 }  // namespace sili

@@ -857,6 +857,11 @@ PYBIND11_MODULE(_cuda, m) {
         check(sili_draft_tree((const int*)parents, (const int*)starts, (const int*)lens, requests, tokens, words, window,
                               (int64_t*)masks, (int*)positions, (void*)stream));
     });
+    m.def("kv4_tree_attention_workspace", [](int dtype, int dim, int heads, int kv_heads, int most_new) {
+        int64_t n = 0;
+        check(sili_kv4_tree_attention_workspace(dtype, dim, heads, kv_heads, most_new, &n));
+        return n;
+    });
     m.def("kv4_tree_attention_ptr", [](int dtype, uintptr_t q, int64_t qt, int64_t qh, int64_t tokens, int heads, int dim,
                                        uintptr_t codes, uintptr_t scales, int64_t n_pages, int page, int kv_heads,
                                        uintptr_t table, int64_t stride, int width, uintptr_t lens, int requests,

@@ -542,33 +542,43 @@ def cache_read(codes, scales, slots, dtype=torch.float32):
 _workspaces: dict = {}
 
 
-def _workspace(dev, stream):
+def _workspace(dev, stream, size=None):
+    """``size``: the bytes of a tree's workspace, which has a place of its own; None: cache_attention's."""
     if torch._C._cuda_isCurrentStreamCapturing():
         # a graph owns its workspace: it may be replayed on any stream, beside eager calls
-        return _new_workspace(dev)
-    w = _workspaces.get((dev.index, stream))
+        return _new_workspace(dev, size)
+    key = (dev.index, stream) if size is None else (dev.index, stream, size)
+    w = _workspaces.get(key)
     if w is None:
-        w = _workspaces[(dev.index, stream)] = _new_workspace(dev)
+        w = _workspaces[key] = _new_workspace(dev, size)
     return w
 
 
-def _new_workspace(dev):
-    w = torch.empty(_cuda.kv4_attention_workspace(), dtype=torch.uint8, device=dev)
+def _new_workspace(dev, size):
+    w = torch.empty(_cuda.kv4_attention_workspace() if size is None else size, dtype=torch.uint8, device=dev)
     w[:4096].zero_()      # the counters; the rest is written before it is read
     return w
 
 
 def check_attention(device=None):
     """Raises RuntimeError if a device-side wait of an eager ``cache_attention``
-    on the current stream gave up since the last check (its rows are NaN).
-    Waits for the stream; a captured call's rows tell by themselves."""
+    or ``tree_attention`` on the current stream gave up since the last check
+    (its rows are NaN).  Waits for the stream; a captured call's rows tell by
+    themselves."""
     dev = torch.device("cuda" if device is None else device)
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    w = _workspaces.get((dev.index, _raw_stream(dev.index)))
-    if w is not None:
-        with _on(dev):
-            _cuda.kv4_attention_status_ptr(w.data_ptr(), _raw_stream(dev.index))
+    at = dev.index, _raw_stream(dev.index)
+    failed = None
+    with _on(dev):
+        for key, w in list(_workspaces.items()):
+            if key[:2] == at:
+                try:
+                    _cuda.kv4_attention_status_ptr(w.data_ptr(), at[1])
+                except RuntimeError as e:
+                    failed = e
+    if failed is not None:
+        raise failed
 
 
 def cache_attention(q, codes, scales, table, lens, starts=None, most_new=None, scale=None, window: int = 0, out=None,
@@ -725,12 +735,13 @@ def tree_attention(q, codes, scales, table, lens, starts, masks, most_new=None, 
         else:
             _contiguous(who, "out", out, q.dtype, (tokens, heads, dim))
         lse = torch.empty(tokens, heads, dtype=_F32, device=dev) if return_lse else None
+        size = _cuda.kv4_tree_attention_workspace(code, dim, heads, hk, most_new)
         _cuda.kv4_tree_attention_ptr(code, q.data_ptr(), q.stride(0), q.stride(1), tokens, heads, dim, codes.data_ptr(),
                                      scales.data_ptr(), n_pages, page, hk, table.data_ptr(), _row_stride(table),
                                      table.shape[1], lens.data_ptr(), requests, starts.data_ptr(), masks.data_ptr(),
                                      masks.shape[1], most_new, 1.0 / math.sqrt(dim) if scale is None else float(scale),
                                      window, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                                     _workspace(dev, s).data_ptr(), s)
+                                     _workspace(dev, s, size).data_ptr(), s)
     return (out, lse) if return_lse else out
 
 
