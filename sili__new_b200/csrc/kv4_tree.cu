@@ -102,7 +102,40 @@ struct Smem {
 
 // true when the phase of this parity is complete; false, at once, when any role has given up
 __device__ __forceinline__ bool wait(unsigned long long* b, uint32_t parity, int* dead, int polls) {
-    return !*(volatile int*)dead && bar_wait(b, parity, dead, polls);
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(addr(b)), "r"(parity) : "memory");
+    return done || (!*(volatile int*)dead && bar_wait(b, parity, dead, polls));
+}
+// one arrival a warp
+__device__ __forceinline__ void warp_arrive(unsigned long long* b) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
+// two floats at a time
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void halves(uint64_t d, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); }
 __device__ __forceinline__ bool softmax_any(bool is) {
@@ -337,7 +370,7 @@ struct Tree {
                 for (int k = 0; k < kSub; k += 16) tmem_ld16(s_col(t) + lanes + k, reinterpret_cast<float(&)[16]>(x[k]));
                 tmem_wait(x);
                 asm volatile("tcgen05.fence::before_thread_sync;");
-                bar_arrive(&s.s_free[t]);          // the next scores may come while these are worked on
+                warp_arrive(&s.s_free[t]);         // the next scores may come while these are worked on
                 const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
                 const bool masked = there != 0x01010101u || key0 + kSub > all_to || key0 < all_from;
                 uint64_t bits = ~0ull;
@@ -350,11 +383,11 @@ struct Tree {
                 }
                 // The running maximum moves when a logit exceeds it by 2^7: P stays within a half, and O is seldom read and
                 // written back.
-                float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
+                float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int k = 4; k < kSub; k += 4) {
-                    top = fmaxf(top, fmaxf(x[k], x[k + 1]));
-                    top1 = fmaxf(top1, fmaxf(x[k + 2], x[k + 3]));
+                for (int k = 0; k < kSub; k += 4) {
+                    top = max3(top, x[k], x[k + 1]);
+                    top1 = max3(top1, x[k + 2], x[k + 3]);
                 }
                 top = fmaxf(top, top1);
                 if (top != -INFINITY) top = top * r.cf - kLift;
@@ -373,15 +406,21 @@ struct Tree {
                 const float shift = base == -INFINITY ? 0.f : base;
                 // P's buffer was last read by the product two steps ago, which was queued before these scores
                 uint32_t p[2][16];
-                float sum0 = 0.f, sum1 = 0.f;
+                const uint64_t cf2 = two(r.cf, r.cf), shift2 = two(-shift, -shift);
+                uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < kSub; k += 2) {
-                    const float y = ex2(fmaf(x[k], r.cf, -shift)), z = ex2(fmaf(x[k + 1], r.cf, -shift));
-                    sum0 += y; sum1 += z;
+                    float y, z;
+                    halves(fma2(two(x[k], x[k + 1]), cf2, shift2), y, z);
+                    y = ex2(y);
+                    z = ex2(z);
+                    sum[k / 2 & 3] = add2(sum[k / 2 & 3], two(y, z));
                     p[k / 32][k / 2 % 16] = pack2(y, z);
                 }
                 tmem_st16(p_col(t) + lanes + (at & 1) * (kSub / 2), p[0]);
                 tmem_st16(p_col(t) + lanes + (at & 1) * (kSub / 2) + 16, p[1]);
+                float sum0, sum1;
+                halves(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sum0, sum1);
                 l += sum0 + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 if (*(volatile int*)&s.odd[st] == n + 1) {
@@ -393,7 +432,7 @@ struct Tree {
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;");
-                bar_arrive(&s.p_full[t][at & 1]);
+                warp_arrive(&s.p_full[t][at & 1]);
             }
             u += steps;
             // (a barrier of its own: p_free may be one or two phases behind here, which a parity does not tell apart)
@@ -543,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree(const __grid_constant__ At
             bar_init(&s.s_full[i], 1);
             bar_init(&s.o_full[i], 1);
             bar_init(&s.drained[i], 1);
-            bar_init(&s.s_free[i], kM);
-            bar_init(&s.p_full[i][0], kM);
-            bar_init(&s.p_full[i][1], kM);
+            bar_init(&s.s_free[i], kM / 32);
+            bar_init(&s.p_full[i][0], kM / 32);
+            bar_init(&s.p_full[i][1], kM / 32);
             bar_init(&s.p_free[i], 1);
             s.odd[i] = 0;
         }
