@@ -175,13 +175,15 @@ struct Attend {
     float l[NT][2], o[kSteps][NT][4];
     int to[NT][2], from[NT][2];        // the columns' keys [from, to)
     int any_from, any_to, all_from, all_to;   // keys that any of the rows sees, that every row sees
-    int own, token[TREE ? NT : 1][2];         // TREE: the first drafted key, the columns' rows of q
+    int own;                                  // TREE: the first drafted key
+    unsigned long long (*masks)[4];           // TREE: the row tile's masks, in shared memory
 
-    __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, float* factors)
+    __device__ __forceinline__ Attend(const AttendArgs& args, uint8_t* smem, float* factors, unsigned long long (*tree)[4])
         : a(args), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
         ring = smem + warp * (kStages * L::kStage);
         ring_at = (uint32_t)__cvta_generic_to_shared(ring);
         s_cf = factors;
+        masks = tree;
         step_pages = kUnit / a.page;
         step_off = kUnit - step_pages * a.page;
         join = (float*)(smem + L::kRing);
@@ -264,8 +266,8 @@ struct Attend {
         auto span = [&](int row, int& from_, int& to_) {
             if constexpr (TREE) {
                 int some = 0;
-                for (int i = 0; i < a.words; ++i)
-                    some += __popcll((unsigned long long)a.masks[(int64_t)(c.q.row0 + row / group) * a.words + i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) some += __popcll(masks[row - row0][i]);
                 to_ = some ? (int)min(max(c.q.pos0, (int64_t)0), (int64_t)c.q.len) : 0;
                 from_ = a.window ? (int)min(max(c.q.pos0 + some - a.window, (int64_t)0), (int64_t)0x7FFFFFFF) : 0;
             } else {
@@ -277,6 +279,13 @@ struct Attend {
         if constexpr (!TREE) {
             span(row0, any_from, all_to);
             span(min(row0 + kRows, rows) - 1, all_from, any_to);
+        } else {
+            if (threadIdx.x < kRows * 4) {
+                const int row = row0 + (threadIdx.x >> 2), word = threadIdx.x & 3;
+                masks[threadIdx.x >> 2][word] = row < rows && word < a.words
+                    ? (unsigned long long)a.masks[(int64_t)(c.q.row0 + row / group) * a.words + word] : 0;
+            }
+            __syncthreads();
         }
         if (kShared) __syncthreads();    // the last segment's fragments have been read
 #pragma unroll
@@ -336,9 +345,7 @@ struct Attend {
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int row = min(row0 + n * 8 + 2 * t + j, rows - 1);
-                span(row, from[n][j], to[n][j]);
-                if constexpr (TREE) token[n][j] = c.q.row0 + row / group;
+                span(min(row0 + n * 8 + 2 * t + j, rows - 1), from[n][j], to[n][j]);
                 base[n][j] = kNoMaximum;
                 l[n][j] = 0.f;
             }
@@ -383,8 +390,7 @@ struct Attend {
         if constexpr (TREE) {
             if (key >= own) {
                 const uint32_t d = (uint32_t)key - (uint32_t)own;
-                return key < any_to && d < 64u * a.words &&
-                       (a.masks[(int64_t)token[n][j] * a.words + (d >> 6)] >> (d & 63) & 1);
+                return key < any_to && d < 256u && (masks[n * 8 + 2 * t + j][d >> 6] >> (d & 63) & 1);
             }
         }
         return key < to[n][j] && key >= from[n][j];
@@ -764,12 +770,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && E < 8 ? 2 : 1) k_atten
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_factors[8 * 4];
     __shared__ int s_last;
+    __shared__ unsigned long long s_masks[TREE ? 8 * NT : 1][4];
     blank_rows<T>(a, 32 * E);
     Cursor<8 * NT> c;
     int64_t begin, end;
     const int64_t all = locate<8 * NT, kWarps>(a, c, blockIdx.x, gridDim.x, begin, end);
     if (begin >= end) return;
-    Attend<T, E, NT, TREE> k(a, smem, s_factors);
+    Attend<T, E, NT, TREE> k(a, smem, s_factors, s_masks);
     k.run(c, begin, end, all, &s_last);
 }
 
@@ -793,8 +800,10 @@ int launch(const AttendArgs& a, cudaStream_t s) {
 template <typename T, int E, bool TREE>
 int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
     if (rows <= 8) return launch<T, E, 1, TREE>(a, s);
-    if (rows <= 16 || E == 8) return launch<T, E, 2, TREE>(a, s);
-    return launch<T, E, E == 8 ? 2 : 4, TREE>(a, s);
+    // (a tree's rows in fp32, whose two terms and masks leave 32 of them no registers: 24 requests of 16 drafts over up to
+    // 8192 keys took 463 us, in tiles of 16 rows 376)
+    if (rows <= 16 || E == 8 || (TREE && sizeof(T) == 4)) return launch<T, E, 2, TREE>(a, s);
+    return launch<T, E, E == 8 || (TREE && sizeof(T) == 4) ? 2 : 4, TREE>(a, s);
 }
 template <typename T, bool TREE>
 int by_dim(const AttendArgs& a, int dim, int64_t rows, cudaStream_t s) {
