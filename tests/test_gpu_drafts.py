@@ -630,3 +630,101 @@ def test_drafted_decoding_gives_the_tokens_of_plain_decoding(S, dtype=torch.floa
     for r in range(n):
         m = min(len(got[r]), len(told[r]))
         assert got[r][:m] == told[r][:m]
+
+
+# ── the kernel of many 16-bit rows ───────────────────────────────────────────
+def _own_kernel(dtype, dim, h, hk, most_new):
+    from sili__new_b200 import _cuda
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    return _cuda.kv4_tree_attention_workspace(code, dim, h, hk, most_new) != _cuda.kv4_attention_workspace()
+
+
+def test_which_calls_have_a_kernel_of_their_own():
+    assert not _own_kernel(torch.float32, 128, 32, 8, 64) and not _own_kernel(torch.bfloat16, 256, 32, 8, 64)
+    assert not _own_kernel(torch.float16, 64, 8, 8, 32) and _own_kernel(torch.float16, 64, 8, 8, 33)
+    assert _own_kernel(torch.bfloat16, 128, 32, 8, 9) and not _own_kernel(torch.bfloat16, 128, 32, 8, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h,hk,dim,page,most,longest", [(8, 2, 64, 16, 60, 200), (4, 2, 128, 48, 64, 150), (20, 4, 64, 32, 51, 90)])
+def test_many_short_trees(S, dtype, h, hk, dim, page, most, longest):
+    """A CTA's run goes over many segments of one or two units, of one row tile or two."""
+    rng = np.random.default_rng(most)
+    counts = [int(c) for c in rng.integers(0, most + 1, 70)]
+    counts[3], counts[7] = most, 1
+    committed = [int(c) for c in rng.integers(0, longest, 70)]
+    assert _own_kernel(dtype, dim, h, hk, most)
+    case = _tree_case(committed, counts, h, hk, dim, page, dtype, most, extra_rows=4)
+    _check_tree(S, case, dtype, most_new=most)
+    _check_tree(S, case, dtype, most_new=most, window=25)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,h,hk,dim", [([130], 2, 1, 128), ([256, 3, 200], 8, 8, 64), ([33, 40], 4, 4, 128)])
+def test_trees_over_long_caches(S, dtype, counts, h, hk, dim):
+    """Segments that many CTAs share."""
+    assert _own_kernel(dtype, dim, h, hk, max(counts))
+    case = _tree_case([6000, 2500, 3000][:len(counts)], counts, h, hk, dim, 64, dtype, 4)
+    _check_tree(S, case, dtype, most_new=max(counts))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-4, 30.0, 3000.0])
+def test_tree_query_sizes(S, dtype, size):
+    """Flat to one-hot softmaxes, maxima that move late; rows of very different sizes in one tile."""
+    case = _tree_case([900, 90], [40, 36], 8, 2, 128, 16, dtype, 13, scale_q=size)
+    _check_tree(S, case, dtype)
+    _check_tree(S, case, dtype, scale=-0.3 / size)
+    q = case[0].clone()
+    q[::3] *= 2.0 ** -12
+    _check_tree(S, (q, *case[1:]), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tree_sums_of_long_runs_hold(S, dtype):
+    """Runs of more units than a row's sums stay in tensor memory for (fp16): V is the same in every key, so the output is V.
+    |out - V| <= u |V| + 2^-11 |V| (probabilities rounded) + 2^-19 |V| (fp32 sums)."""
+    from test_gpu_serving_long import _one_v
+    keys, hk, d, n = 420000, 8, 64, 40
+    assert _own_kernel(dtype, d, hk, hk, n) and keys * hk // 128 // 148 > 128
+    codes, scales, want = _one_v(keys, hk, d, 3)
+    table = torch.arange(codes.shape[0], dtype=torch.int32, device="cuda")[None]
+    masks = torch.from_numpy(D.draft_tree(D.random_tree(n, np.random.default_rng(2)), [0, n], [keys], n, 1, 0)[0]).cuda()
+    q = (torch.randn(n, hk, d, generator=_gen(1), device="cuda") * 0.3).to(dtype)
+    args = (codes, scales, table, _dev([keys]), _dev([0, n]), masks)
+    out, lse = S.tree_attention(q, *args, return_lse=True)
+    S.check_attention()
+    off = out.double() / want[None] - 1
+    assert float(off.abs().max()) <= HALF_UNIT[dtype] + 2.0 ** -11 + 2.0 ** -19
+    assert abs(float(off.mean())) <= 2.0 ** -12
+    # each row's lse against the kernel for single rows (fp32 sums of the same probabilities in another order)
+    few = S.tree_attention(q[:3], codes, scales, table, _dev([keys]), _dev([0, n]), masks[:3].clone(), most_new=1, return_lse=True)[1]
+    assert float((few - lse[:3]).abs().max()) <= 2.0 ** -18 * (1 + float(few.abs().max()))
+
+
+@pytest.mark.parametrize("counts,h,hk,dim", [([40, 12], 32, 8, 64), ([30, 20], 8, 4, 128)])
+def test_a_tree_wait_that_runs_out_is_reported(S, counts, h, hk, dim):
+    """Every role's first wait gives up: the rows are NaN, the status says so, and the next call is whole again."""
+    from sili__new_b200 import _cuda
+    q, codes, scales, table, lens, starts, masks = _tree_case([700, 300], counts, h, hk, dim, 16, torch.bfloat16, dim)
+    assert _own_kernel(torch.bfloat16, dim, h, hk, max(counts))
+
+    def call():
+        return S.tree_attention(q, codes, scales, table, lens, _dev(starts), masks, most_new=max(counts), return_lse=True)
+
+    S.check_attention()
+    want, want_lse = call()
+    S.check_attention()
+    try:
+        _cuda.kv4_attention_wait_limit(polls=0)
+        out, lse = call()
+        torch.cuda.synchronize()
+    finally:
+        _cuda.kv4_attention_wait_limit()
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    with pytest.raises(RuntimeError, match="gave up"):
+        S.check_attention()
+    S.check_attention()
+    again, again_lse = call()
+    S.check_attention()
+    assert torch.equal(again, want) and torch.equal(again_lse, want_lse)
