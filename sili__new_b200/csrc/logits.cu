@@ -549,8 +549,9 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ L
             if (order_of(by(value)) != all || (touched && (touched[v >> 5] >> (v & 31) & 1))) return;
             if (allow && !(__ldg(allow + (v >> 5)) >> (v & 31) & 1)) return;
             if (a.drafted)
-                for (int j = 0; j < 64 * a.words; ++j)
-                    if (path_token(a, of, j, path_mask(a, row, j)) == v) return;
+                for (int w = 0; w < a.words; ++w)
+                    for (uint64_t left = path_mask(a, row, 64 * w); left; left &= left - 1)
+                        if (path_token(a, of, 64 * w + __ffsll((long long)left) - 1, left) == v) return;
             low = max(low, ~(uint32_t)v);
         };
         for (int i = tid; i < n_parts; i += kPickThreads)
