@@ -9,6 +9,16 @@ projections are this library's sparse layers goes::
                      positions=t.positions, q=q)
     y = cache_attention(q, cache.codes, cache.scales, table, t.lens, starts=t.starts)
 
+A step that verifies trees of drafted tokens goes::
+
+    t = page_tables(cached, drafts, table, ring, pool, cache.page, max_tokens)
+    tree = draft_tree(parents, t.starts, t.lens, most_drafts)
+    ... cache_append(..., positions=tree.positions), then in place of cache_attention
+    y = tree_attention(q, cache.codes, cache.scales, table, t.lens, t.starts, tree.masks)
+    ... the logits of all rows
+    picked = pick_tokens(logits, t.starts, history, history_lens, drafted=drafted, masks=tree.masks, ...)
+    end = settle_drafts(drafted, parents, picked, t.starts, t.lens, table, caches, ring, t.pool)
+
 Everything stays on the device: no call reads a length back to the host, so a
 step can be captured in a CUDA graph.  All work is enqueued on torch's current
 stream of the arrays' device; arrays made on another stream are ordered by the
@@ -705,8 +715,8 @@ def tree_attention(q, codes, scales, table, lens, starts, masks, most_new=None, 
 
     ``masks`` int64 [tokens, words] from ``draft_tree``, or any other; a row
     without a bit sees nothing.  ``window`` > 0: as many of the committed keys,
-    the last ones, as the row's mask has bits fewer than that.  All else as in
-    ``cache_attention``."""
+    the last ones, as the row's mask has bits fewer than that.  ``out`` shares
+    no memory with q.  All else as in ``cache_attention``."""
     who = "tree_attention"
     n_pages, hk, page, dim = _check_cache(who, codes, scales)
     if page < 16 or page % 16:
@@ -725,6 +735,8 @@ def tree_attention(q, codes, scales, table, lens, starts, masks, most_new=None, 
         most_new = -(-tokens // max(requests, 1))
     if window < 0 or most_new < 0:
         raise ValueError(f"{who}: window and most_new must not be negative")
+    if out is not None and _meet(out, q):
+        raise ValueError(f"{who}: out must not overlap q")
     window, most_new = min(window, 0x7FFFFFFF), min(most_new, 0x7FFFFFFF)
     _no_gradient(who, q)
     dev = q.device
@@ -813,7 +825,7 @@ def _logit_rules(who, logits, starts, history, history_lens, prompt_lens, drafte
         if out.data_ptr() == logits.data_ptr():
             if rows > 1 and out.stride(0) != logits.stride(0):
                 raise ValueError(f"{who}: out starts where the logits do, but its rows lie elsewhere")
-        elif _overlap(out, logits):
+        elif _meet(out, logits):
             raise ValueError(f"{who}: out may be the logits, but not overlap them otherwise")
     _no_gradient(who, logits, repetition, presence, frequency, temperature, bias_values)
     s = _on_device(who, logits.device, starts, history, history_lens, prompt_lens, drafted, masks, repetition, presence,
@@ -864,11 +876,11 @@ def adjust_logits(logits, starts=None, history=None, history_lens=None, prompt_l
     return out
 
 
-def _overlap(a, b):
-    """Whether the memory between two [rows, vocab] arrays' first and last elements meets."""
+def _meet(a, b):
+    """Whether the memory between two arrays' first and last elements overlaps."""
     if not a.numel() or not b.numel():
         return False
-    size = lambda t: ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()  # noqa: E731
+    size = lambda t: (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()  # noqa: E731
     return a.data_ptr() < b.data_ptr() + size(b) and b.data_ptr() < a.data_ptr() + size(a)
 
 
@@ -919,8 +931,8 @@ def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, p
     _contiguous(who, "lens", lens, _I32, (requests,))
     _contiguous(who, "starts", starts, _I32, (requests + 1,))
     pairs = [(c.codes, c.scales) if isinstance(c, KVCache4) else tuple(c) for c in caches]
-    if not pairs:
-        raise ValueError(f"{who}: needs at least one cache")
+    if not pairs or any(len(c) != 2 for c in pairs):
+        raise ValueError(f"{who}: needs at least one cache, a KVCache4 or (codes, scales) each")
     n_pages, hk, page, dim = _check_cache(who, *pairs[0])
     for codes, scales in pairs[1:]:
         if codes.shape != pairs[0][0].shape:

@@ -96,6 +96,21 @@ def test_an_output_that_meets_the_logits_is_refused():
             _logits(logits=x, out=out)
 
 
+def test_an_output_that_meets_the_queries_is_refused():
+    flat = torch.zeros(6 * 4 * 64)
+    q = flat[:5 * 256].view(5, 4, 64)
+    for out in (q, flat[256:].view(5, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            _attend(q=q, out=out)
+    with pytest.raises(ValueError, match="CUDA"):
+        _attend(q=q, out=torch.zeros(5, 4, 64))
+
+
+def test_a_cache_is_a_pair():
+    with pytest.raises(ValueError, match="codes, scales"):
+        _settle(caches=[(torch.zeros(3, 2, 2, 16, 32, dtype=torch.uint8),)])
+
+
 @pytest.mark.parametrize("name,call", [("q", _attend), ("logits", _logits), ("repetition", _logits), ("bias_values", _logits),
                                        ("logits", lambda **k: _logits(S.pick_tokens, **k))])
 def test_a_gradient_that_would_be_lost_is_refused(name, call):
