@@ -33,6 +33,13 @@
 // keep a ring of cp.async stages; the page of the next tile is fetched one
 // step ahead.
 //
+// Drafted tokens' trees (TREE): a row sees the committed keys, as its window
+// leaves them, and of the request's own those that its mask names; the masks of
+// a row tile lie in shared memory.  16-bit trees of more than 32 rows a request
+// run in kv4_tree.cu.  24 requests of up to 16 drafts over up to 8192 keys in fp32
+// (121 MB, 18 us at the copy rate): 360 us, bound by instructions: every tile
+// of 16 rows decodes the keys again and multiplies two terms.
+//
 // What bounds it, 96 requests of 2k-16k keys, 32 heads over 8, dim 128, bf16
 // (0.96 GB, 146 us at the card's copy rate): 271 us, 3.5 TB/s.  A warp's 16
 // keys x 136 bytes take about 400 instructions, 266 of them the tile's own

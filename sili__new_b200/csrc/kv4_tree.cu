@@ -19,6 +19,15 @@
 // of a warp's rows see whole gets its 64 bits from those two.  Roundings as in
 // kv4_prompt.cu; a row's sums leave tensor memory every kPiece units.
 //
+// What bounds it, 40 requests of up to 64 drafts over 2k-12k keys, 32 heads over
+// 8, dim 128, bf16 (233 GFLOP, 143 us at the card's matrix rate): 453 us, 515
+// TFLOP/s, tensor pipe 35 %, issue 50 %.  With the conversions, loads,
+// exponentials and most products left out it took 328: a step is the softmax
+// warps' chain (scores' barrier, tensor-memory load, maximum, exponentials,
+// store), two of its warps a scheduler.  24 drafts over 131071 keys (52 GFLOP):
+// 172 us; there the conversion of the keys, for 96 rows, weighs as much (125
+// without it).
+//
 // Every wait is bounded: one that gives up sets the workspace's error word; the
 // rows of the CTA's run, and its parts of shared segments, become NaN.
 #include <cuda_runtime.h>
@@ -704,6 +713,12 @@ int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
 
 namespace sili {
 
+// us of this kernel | the one of kv4_attention.cu, by rows a request (32 heads over 8 x 128):
+//   1 request, 131071 keys, fp16:    32 rows 167 | 121, 36: 168 | 198, 64: 170 | 200, 128: 179 | 364
+//   40 requests, 2k-12k keys, bf16:  32 rows 348 | 268, 36: 350 | 328, 48: 347 | 409, 128: 376 | 850, 256: 453 | 1618
+//   the same up to 1000 keys:        32 rows 119 | 111, 36: 117 | 118, 64: 122 | 201
+//   4 requests up to 700 keys:       32 rows  28 |  24, 48:  28 |  26, 64:  28 |  42
+// The other one walks tiles of up to 32 rows, so it is taken up to there.
 bool kv4_tree_takes(int dtype, int dim, int64_t rows) { return dtype != SILI_F32 && (dim == 64 || dim == 128) && rows > 32; }
 
 int64_t kv4_tree_workspace(int dim, int64_t rows) {
