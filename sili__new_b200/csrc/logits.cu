@@ -56,6 +56,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                    // tokens that a CTA of k_touch counts
 constexpr int kMostDrafts = 256;
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
+constexpr int kMostListed = 1 << 29;    // tokens of a history, or biases: with the path's, their number stays within kCount
 // 16-byte accesses of a thread of k_stream, whose CTAs take a tile of a row each
 template <typename T> constexpr int kPacksOf = kTile / kThreads * (int)sizeof(T) / 16;
 
@@ -651,6 +652,7 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
         q.words > 4)
         return bad(who, "sizes out of range");
     if ((q.history != nullptr) != (q.history_lens != nullptr)) return bad(who, "history and its lengths come together");
+    if (q.history_width > kMostListed || q.biases > kMostListed) return bad(who, "history or biases too long");
     if (q.history && requests > 1 && q.history_stride < 0) return bad(who, "sizes out of range");
     if ((q.drafted != nullptr) != (q.masks != nullptr) || (q.drafted && (!q.starts || q.words < 1)))
         return bad(who, "drafted tokens, masks and starts come together");

@@ -106,6 +106,15 @@ def test_an_output_that_meets_the_queries_is_refused():
         _attend(q=q, out=torch.zeros(5, 4, 64))
 
 
+@pytest.mark.parametrize("width,biases", [(2 ** 29 + 1, 0), (2 ** 31 - 1, 0), (0, 2 ** 29 + 1), (0, 2 ** 31 - 1)])
+def test_lists_too_long_to_count_are_refused(width, biases):
+    # (the sizes are looked at, not the arrays)
+    rules = S._cuda.LogitRules(0, 8 if width else 0, width, width, 8 if width else 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                               8 if biases else 0, 8 if biases else 0, biases, 0, 0)
+    with pytest.raises(ValueError, match="too long"):
+        S._cuda.logits_scratch(0, 1, 64, 1, rules, False)
+
+
 def test_a_cache_is_a_pair():
     with pytest.raises(ValueError, match="codes, scales"):
         _settle(caches=[(torch.zeros(3, 2, 2, 16, 32, dtype=torch.uint8),)])
