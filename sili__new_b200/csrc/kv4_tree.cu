@@ -20,7 +20,7 @@
 // kv4_prompt.cu; a row's sums leave tensor memory every kPiece units.
 //
 // What bounds it, 40 requests of up to 64 drafts over 2k-12k keys, 32 heads over
-// 8, dim 128, bf16 (233 GFLOP, 143 us at the card's matrix rate): 453 us, 515
+// 8, dim 128, bf16 (233 GFLOP, 143 us at the card's matrix rate): 443 us, 526
 // TFLOP/s, tensor pipe 35 %, issue 50 %.  With the conversions, loads,
 // exponentials and most products left out it took 328: a step is the softmax
 // warps' chain (scores' barrier, tensor-memory load, maximum, exponentials,
@@ -374,13 +374,15 @@ struct Tree {
                 ok = __all_sync(0xffffffffu, wait(&s.s_full[t], at & 1, &s.dead, a.polls));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
+                // (both were written before the stage was given to the products; asked for here, they come beside the scores)
+                const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
+                const int odd_stage = *(const volatile int*)&s.odd[st];
                 float x[kSub];
 #pragma unroll
                 for (int k = 0; k < kSub; k += 16) tmem_ld16(s_col(t) + lanes + k, reinterpret_cast<float(&)[16]>(x[k]));
                 tmem_wait(x);
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 warp_arrive(&s.s_free[t]);         // the next scores may come while these are worked on
-                const uint32_t there = *(const volatile uint32_t*)&s.there[st][4 * half];
                 const bool masked = there != 0x01010101u || key0 + kSub > all_to || key0 < all_from;
                 uint64_t bits = ~0ull;
                 if (masked) {
@@ -392,13 +394,10 @@ struct Tree {
                 }
                 // The running maximum moves when a logit exceeds it by 2^7: P stays within a half, and O is seldom read and
                 // written back.
-                float top = -INFINITY, top1 = -INFINITY;
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < kSub; k += 4) {
-                    top = max3(top, x[k], x[k + 1]);
-                    top1 = max3(top1, x[k + 2], x[k + 3]);
-                }
-                top = fmaxf(top, top1);
+                for (int k = 0; k < kSub; k += 2) tops[k / 2 & 3] = max3(tops[k / 2 & 3], x[k], x[k + 1]);
+                float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
                 if (top != -INFINITY) top = top * r.cf - kLift;
                 if (__any_sync(0xffffffffu, top > base + kSlack)) {       // (NaN compares false)
                     const float fresh = fmaxf(base, top);
@@ -432,7 +431,7 @@ struct Tree {
                 halves(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sum0, sum1);
                 l += sum0 + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                if (*(volatile int*)&s.odd[st] == n + 1) {
+                if (odd_stage == n + 1) {
                     if (!masked) bits = visible(r, key0, there);
                     for (int g = 0; g < E; ++g) {
                         uint64_t odd = 0;
