@@ -575,7 +575,7 @@ typedef struct sili_logit_rules {
     const int* starts;             /* [requests + 1] or NULL */
     const int* history;            /* [requests, history_width], rows history_stride apart; tokens outside the vocabulary are passed over */
     int64_t history_stride;
-    int history_width;
+    int history_width;             /* 0: no history, whatever the pointers are */
     const int* history_lens;       /* [requests] */
     const int* prompt_lens;        /* [requests]: so many of them are the prompt's; NULL: none */
     const int* drafted;            /* [rows]: the rows' own tokens; a row's path is those that its mask names */

@@ -651,7 +651,9 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
     if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || requests < 0 || q.history_width < 0 || q.biases < 0 || q.words < 0 ||
         q.words > 4)
         return bad(who, "sizes out of range");
-    if ((q.history != nullptr) != (q.history_lens != nullptr)) return bad(who, "history and its lengths come together");
+    // (an array of no columns may have no address)
+    if (q.history_width && (q.history != nullptr) != (q.history_lens != nullptr))
+        return bad(who, "history and its lengths come together");
     if (q.history_width > kMostListed || q.biases > kMostListed) return bad(who, "history or biases too long");
     if (q.history && requests > 1 && q.history_stride < 0) return bad(who, "sizes out of range");
     if ((q.drafted != nullptr) != (q.masks != nullptr) || (q.drafted && (!q.starts || q.words < 1)))

@@ -844,9 +844,9 @@ def adjust_logits(logits, starts=None, history=None, history_lens=None, prompt_l
     on ``logits`` [rows, vocab] (rows contiguous, any distance apart).
 
     Request r's rows are starts[r] .. starts[r + 1) (int32; without it row r),
-    and ``history`` int32 [requests, width] holds the history_lens[r] tokens
-    behind which they stand, the first prompt_lens[r] of them (none by default)
-    the prompt's.  Rows of drafted tokens follow their own path, too: the
+    and ``history`` int32 [requests, width] (any width, 0 too) holds the
+    history_lens[r] tokens behind which they stand, the first prompt_lens[r] of
+    them (none by default) the prompt's.  Rows of drafted tokens follow their own path, too: the
     ``drafted`` int32 [rows] that their ``masks`` (``draft_tree``) name.  With
     c(v) the times that token v stands in the history behind the prompt and on
     the path, in fp32, each operation rounded::
