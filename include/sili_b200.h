@@ -616,12 +616,22 @@ int sili_pick_tokens(int dtype, const void* logits, int64_t stride, int64_t rows
  * one table).  Pages that lens took and lens_out does not go back to the ring
  * in request order; the table keeps their entries, which nothing reads past a
  * request's length.  But for the caches, the same inputs write the same values
- * again. */
+ * again.  Every row counts as one that the attention saw. */
 int sili_settle_drafts(const int* drafted, const int* parents, const void* picked, int picked64, const int* starts,
                        const int* lens, int requests, int64_t tokens, int* path, int* kept, int* token, int* lens_out,
                        const int* table, int64_t table_stride, int width, int* ring, int ring_size, const int64_t* pool,
                        int64_t* pool_out, int n_caches, void* const* codes, void* const* scales, int64_t n_pages, int page,
                        int kv_heads, int dim, void* stream);
+/* The same for a step whose attention saw what masks [tokens, words] (words 1
+ * to 4, or masks NULL) name: a row without a bit, or past its request's 64 *
+ * words first ones, is none, as in sili_draft_tree.  It has no key, and is not
+ * accepted. */
+int sili_settle_masked_drafts(const int* drafted, const int* parents, const int64_t* masks, int words, const void* picked,
+                              int picked64, const int* starts, const int* lens, int requests, int64_t tokens, int* path,
+                              int* kept, int* token, int* lens_out, const int* table, int64_t table_stride, int width,
+                              int* ring, int ring_size, const int64_t* pool, int64_t* pool_out, int n_caches,
+                              void* const* codes, void* const* scales, int64_t n_pages, int page, int kv_heads, int dim,
+                              void* stream);
 
 #ifdef __cplusplus
 }

@@ -148,6 +148,8 @@ constexpr int kCachesOfLaunch = 64;
 struct SettleArgs {
     const int* drafted;
     const int* parents;
+    const int64_t* masks;      // [tokens, words] or null: rows without a bit, or past the masks' bits, are none
+    int words;
     const void* picked;
     int picked64;
     const int* starts;
@@ -186,7 +188,13 @@ __global__ void __launch_bounds__(128) k_accept(SettleArgs a) {
     auto pick = [&](int i) {
         return a.picked64 ? ((const int64_t*)a.picked)[q.row0 + i] : (int64_t)((const int*)a.picked)[q.row0 + i];
     };
-    int node = q.n > 0 && a.parents[q.row0] == -1 ? 0 : -1, kept = 0;
+    auto there = [&](int i) {
+        if (!a.masks) return true;
+        int64_t any = 0;
+        for (int w = 0; w < a.words; ++w) any |= a.masks[(q.row0 + i) * a.words + w];
+        return any != 0 && i < 64 * a.words;
+    };
+    int node = q.n > 0 && a.parents[q.row0] == -1 && there(0) ? 0 : -1, kept = 0;
     int64_t want = -1;
     while (node >= 0) {
         if (lane == 0) a.path[q.row0 + kept] = node;
@@ -196,7 +204,7 @@ __global__ void __launch_bounds__(128) k_accept(SettleArgs a) {
         if (want >= 0)
             for (int at = (node + 1) & ~31; at < q.n; at += 32) {
                 const int i = at + lane;
-                const bool is = i > node && i < q.n && a.parents[q.row0 + i] == node && a.drafted[q.row0 + i] == want;
+                const bool is = i > node && i < q.n && a.parents[q.row0 + i] == node && a.drafted[q.row0 + i] == want && there(i);
                 const unsigned hit = __ballot_sync(0xffffffffu, is);
                 if (hit) { child = at + __ffs(hit) - 1; break; }
             }
@@ -342,12 +350,14 @@ int sili_draft_tree(const int* parents, const int* starts, const int* lens, int 
     return SILI_OK;
 }
 
-int sili_settle_drafts(const int* drafted, const int* parents, const void* picked, int picked64, const int* starts,
-                       const int* lens, int requests, int64_t tokens, int* path, int* kept, int* token, int* lens_out,
-                       const int* table, int64_t table_stride, int width, int* ring, int ring_size, const int64_t* pool,
-                       int64_t* pool_out, int n_caches, void* const* codes, void* const* scales, int64_t n_pages, int page,
-                       int kv_heads, int dim, void* stream) {
+int sili_settle_masked_drafts(const int* drafted, const int* parents, const int64_t* masks, int words, const void* picked,
+                              int picked64, const int* starts, const int* lens, int requests, int64_t tokens, int* path,
+                              int* kept, int* token, int* lens_out, const int* table, int64_t table_stride, int width,
+                              int* ring, int ring_size, const int64_t* pool, int64_t* pool_out, int n_caches,
+                              void* const* codes, void* const* scales, int64_t n_pages, int page, int kv_heads, int dim,
+                              void* stream) {
     const char* who = "settle_drafts";
+    if (masks && (words < 1 || words > kMostWords)) return bad(who, "masks must have 1 to 4 words a row");
     if (requests < 0 || tokens < 0 || tokens > 0x7fffffffLL || width < 0 || ring_size < 1 || n_caches < 0 || n_pages < 0 ||
         page < 1 || kv_heads < 1)
         return bad(who, "sizes out of range");
@@ -363,7 +373,7 @@ int sili_settle_drafts(const int* drafted, const int* parents, const void* picke
         if (!codes[i] || !scales[i]) return bad(who, "null array");
         if ((uintptr_t)codes[i] % 16 || (uintptr_t)scales[i] % 16) return bad(who, "codes and scales must be 16-byte aligned");
     }
-    SettleArgs a{drafted, parents, picked, picked64, starts, lens, requests, tokens, path, kept, token, lens_out, table,
+    SettleArgs a{drafted, parents, masks, words, picked, picked64, starts, lens, requests, tokens, path, kept, token, lens_out, table,
                  table_stride, width, ring, ring_size, pool, pool_out, page, n_pages, kv_heads, dim};
     cudaStream_t s = (cudaStream_t)stream;
     k_accept<<<(unsigned)((requests + 3) / 4 + 1), 128, 0, s>>>(a);
@@ -379,6 +389,16 @@ int sili_settle_drafts(const int* drafted, const int* parents, const void* picke
     sili::count_launch();
     CKD(cudaGetLastError());
     return SILI_OK;
+}
+
+int sili_settle_drafts(const int* drafted, const int* parents, const void* picked, int picked64, const int* starts,
+                       const int* lens, int requests, int64_t tokens, int* path, int* kept, int* token, int* lens_out,
+                       const int* table, int64_t table_stride, int width, int* ring, int ring_size, const int64_t* pool,
+                       int64_t* pool_out, int n_caches, void* const* codes, void* const* scales, int64_t n_pages, int page,
+                       int kv_heads, int dim, void* stream) {
+    return sili_settle_masked_drafts(drafted, parents, nullptr, 0, picked, picked64, starts, lens, requests, tokens, path, kept,
+                                     token, lens_out, table, table_stride, width, ring, ring_size, pool, pool_out, n_caches,
+                                     codes, scales, n_pages, page, kv_heads, dim, stream);
 }
 
 }  // extern "C"

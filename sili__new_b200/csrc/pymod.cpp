@@ -899,18 +899,20 @@ PYBIND11_MODULE(_cuda, m) {
         check(sili_pick_tokens(dtype, (const void*)logits, stride, rows, vocab, requests, &rules, (int*)token,
                                (void*)scratch, (void*)stream));
     });
-    m.def("settle_drafts_ptr", [](uintptr_t drafted, uintptr_t parents, uintptr_t picked, bool picked64, uintptr_t starts,
-                                  uintptr_t lens, int requests, int64_t tokens, uintptr_t path, uintptr_t kept,
+    m.def("settle_drafts_ptr", [](uintptr_t drafted, uintptr_t parents, uintptr_t masks, int words, uintptr_t picked,
+                                  bool picked64, uintptr_t starts, uintptr_t lens, int requests, int64_t tokens,
+                                  uintptr_t path, uintptr_t kept,
                                   uintptr_t token, uintptr_t lens_out, uintptr_t table, int64_t stride, int width,
                                   uintptr_t ring, int ring_size, uintptr_t pool, uintptr_t pool_out,
                                   const std::vector<uintptr_t>& codes, const std::vector<uintptr_t>& scales,
                                   int64_t n_pages, int page, int kv_heads, int dim, uintptr_t stream) {
         if (codes.size() != scales.size()) throw std::invalid_argument("settle_drafts: codes and scales come in pairs");
-        check(sili_settle_drafts((const int*)drafted, (const int*)parents, (const void*)picked, picked64,
-                                 (const int*)starts, (const int*)lens, requests, tokens, (int*)path, (int*)kept,
-                                 (int*)token, (int*)lens_out, (const int*)table, stride, width, (int*)ring, ring_size,
-                                 (const int64_t*)pool, (int64_t*)pool_out, (int)codes.size(), (void* const*)codes.data(),
-                                 (void* const*)scales.data(), n_pages, page, kv_heads, dim, (void*)stream));
+        check(sili_settle_masked_drafts((const int*)drafted, (const int*)parents, (const int64_t*)masks, words,
+                                        (const void*)picked, picked64, (const int*)starts, (const int*)lens, requests,
+                                        tokens, (int*)path, (int*)kept, (int*)token, (int*)lens_out, (const int*)table,
+                                        stride, width, (int*)ring, ring_size, (const int64_t*)pool, (int64_t*)pool_out,
+                                        (int)codes.size(), (void* const*)codes.data(), (void* const*)scales.data(),
+                                        n_pages, page, kv_heads, dim, (void*)stream));
     });
     m.def("fp32_fma_peak", [](int device, int iters) {
         double tf = 0, ms = 0;

@@ -17,7 +17,7 @@ A step that verifies trees of drafted tokens goes::
     y = tree_attention(q, cache.codes, cache.scales, table, t.lens, t.starts, tree.masks)
     ... the logits of all rows
     picked = pick_tokens(logits, t.starts, history, history_lens, drafted=drafted, masks=tree.masks, ...)
-    end = settle_drafts(drafted, parents, picked, t.starts, t.lens, table, caches, ring, t.pool)
+    end = settle_drafts(drafted, parents, picked, t.starts, t.lens, table, caches, ring, t.pool, tree.masks)
 
 Everything stays on the device: no call reads a length back to the host, so a
 step can be captured in a CUDA graph.  All work is enqueued on torch's current
@@ -677,7 +677,8 @@ def draft_tree(parents, starts, lens, most_new: int, window: int = 0) -> DraftTr
     smaller one, or -1 for a row that follows the committed tokens; a row with
     another parent is none, and so are those that follow it.  ``most_new``: the
     largest number of rows of a request, up to 256; rows past its next multiple
-    of 64 are none.  A row that is none, or of no request, has no mask bit and
+    of 64 are none (``settle_drafts`` leaves them out, too, where it is given
+    the masks).  A row that is none, or of no request, has no mask bit and
     position -1.  ``window`` > 0: only the nearest so many of a row and its
     ancestors, for an attention with that window.  The positions go to
     ``cache_append`` in place of ``page_tables``'s."""
@@ -905,7 +906,7 @@ def pick_tokens(logits, starts=None, history=None, history_lens=None, prompt_len
     return token
 
 
-def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, pool) -> Settled:
+def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, pool, masks=None) -> Settled:
     """Accepts drafted tokens and closes the step.
 
     ``picked`` (int32 or int64 [tokens], as from ``pick_tokens`` or a sampler;
@@ -917,6 +918,12 @@ def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, p
     the layers') the accepted rows' keys and values move up behind the committed
     tokens; pages that only rejected rows had go back to the ring.
 
+    ``masks``: the ones that the step's attention took.  A row without a bit, or
+    past the masks' 64 * words places, is none: it has no key that could be
+    accepted, and no row follows it.  Leave them out only where the attention
+    saw every row (chains under ``cache_attention``); ``draft_tree`` makes such
+    rows of bad parents, of an understated ``most_new`` and past 256 drafts.
+
     Pass the returned ``lens`` and ``pool`` on to the next ``page_tables``.  The
     table's entries past a request's length are left as they are, and not read
     again."""
@@ -925,6 +932,8 @@ def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, p
     dev = lens.device
     _contiguous(who, "drafted", drafted, _I32, (tokens,))
     _contiguous(who, "parents", parents, _I32, (tokens,))
+    if masks is not None:
+        _check_masks(who, masks, tokens)
     if picked.dtype not in (_I32, _I64):
         raise ValueError(f"{who}: picked must be int32 or int64, got {picked.dtype}")
     _contiguous(who, "picked", picked, picked.dtype, (tokens,))
@@ -945,15 +954,16 @@ def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, p
     at = [c.data_ptr() for c in codes], [b.data_ptr() for b in scales]
     if n_pages and len(set(at[0])) < len(pairs):
         raise ValueError(f"{who}: the same cache twice")
-    s = _on_device(who, dev, drafted, parents, picked, starts, table, ring, pool, *codes, *scales)
+    s = _on_device(who, dev, drafted, parents, picked, starts, table, ring, pool, masks, *codes, *scales)
     with _on(dev):
         small = torch.empty(tokens + 3 * requests, dtype=_I32, device=dev)
         pool_out = torch.empty(2, dtype=_I64, device=dev)
         a = small.data_ptr()
         b = a + 4 * tokens
-        _cuda.settle_drafts_ptr(drafted.data_ptr(), parents.data_ptr(), picked.data_ptr(), picked.dtype is _I64,
-                                starts.data_ptr(), lens.data_ptr(), requests, tokens, a, b, b + 4 * requests,
-                                b + 8 * requests, table.data_ptr(), _row_stride(table), table.shape[1], ring.data_ptr(),
-                                ring.numel(), pool.data_ptr(), pool_out.data_ptr(), *at, n_pages, page, hk, dim, s)
+        _cuda.settle_drafts_ptr(drafted.data_ptr(), parents.data_ptr(), _ptr(masks), 0 if masks is None else masks.shape[1],
+                                picked.data_ptr(), picked.dtype is _I64, starts.data_ptr(), lens.data_ptr(), requests,
+                                tokens, a, b, b + 4 * requests, b + 8 * requests, table.data_ptr(), _row_stride(table),
+                                table.shape[1], ring.data_ptr(), ring.numel(), pool.data_ptr(), pool_out.data_ptr(), *at,
+                                n_pages, page, hk, dim, s)
         path, kept, token, lens_out = small.split_with_sizes((tokens, requests, requests, requests))
     return Settled(path, kept, token, lens_out, pool_out)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from sili__new_b200 import serving as S
-from test_drafts import I32, _logits
+from test_drafts import I32, I64, _logits, _settle
 
 
 def _rules(history=0, width=0, lens=0, prompts=0):
@@ -26,3 +26,15 @@ def test_a_history_without_a_column_is_none(pick):
 def test_a_history_without_a_column_passes_the_checks(call):
     with pytest.raises(ValueError, match="CUDA"):
         _logits(call, history=torch.zeros(3, 9, dtype=I32)[:, :0], prompt_lens=torch.zeros(3, dtype=I32))
+
+
+@pytest.mark.parametrize("masks", [torch.zeros(5, dtype=I64), torch.zeros(5, 5, dtype=I64), torch.zeros(4, 1, dtype=I64),
+                                   torch.zeros(5, 1, dtype=I32), torch.zeros(5, 4, dtype=I64)[:, ::2]])
+def test_settling_takes_the_masks_of_its_rows(masks):
+    with pytest.raises(ValueError, match="masks"):
+        _settle(masks=masks)
+
+
+def test_settling_takes_masks():
+    with pytest.raises(ValueError, match="CUDA"):
+        _settle(masks=torch.zeros(5, 2, dtype=I64))
