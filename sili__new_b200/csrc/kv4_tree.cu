@@ -444,7 +444,8 @@ struct Tree {
             }
             u += steps;
             // (a barrier of its own: p_free may be one or two phases behind here, which a parity does not tell apart)
-            if (ok) ok = wait(&s.o_full[t], filled & 1, &s.dead, a.output_polls);
+            // (voted as the others are: the barrier and the loads that follow take a warp's lanes together)
+            if (ok) ok = __all_sync(0xffffffffu, wait(&s.o_full[t], filled & 1, &s.dead, a.output_polls));
             ++filled;
             asm volatile("tcgen05.fence::after_thread_sync;");
             end_piece(c, r, base, l, poisoned, steps, softmax_any(!ok), again, left, begin + done - (c.u - c.q.k0));
@@ -515,6 +516,7 @@ struct Tree {
 #pragma unroll 1
             for (int d = 0; d < D; d += 16) {
                 float x[16];
+                __syncwarp();          // (lanes without a row left the last turn early)
                 if (steps > 0) {
                     tmem_ld16(o_col(t) + lanes + d, x);
                     tmem_wait(x);
@@ -557,6 +559,7 @@ struct Tree {
                 to.parts = (int)((seg1 * ctas - 1) / all) - lead + 1;
             }
         }
+        __syncwarp();
         if (!PAIR) softmax_sync();         // (the next segment's queries come over the sums)
     }
 };

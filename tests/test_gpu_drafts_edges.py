@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import drafts_ref as D
-from test_gpu_drafts import DTYPES, S, _dev, _logit_case, _on_gpu      # noqa: F401  (S: the fixture)
+from test_gpu_drafts import DTYPES, S, _dev, _logit_case, _on_gpu, _own_kernel, _tree_case      # noqa: F401  (S: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,46 @@ def test_a_chain_past_the_plan_goes_on_where_it_ended(S):
         q = x[:1, 4:8].contiguous()
         outs.append((end.lens, end.token, S.cache_attention(q, c.codes, c.scales, table, end.lens)))
     assert outs[0][0].tolist() == [69] and all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+# ── waits that run out ───────────────────────────────────────────────────────
+def _runs_out(S, case, most_new, **limits):
+    """(a call's out and lse, those of a call under these limits); each of its rows is NaN or whole, the status tells which
+    there were, and the next call is whole again."""
+    from sili__new_b200 import _cuda
+    q, codes, scales, table, lens, starts, masks = case
+
+    def call():
+        return S.tree_attention(q, codes, scales, table, lens, _dev(starts), masks, most_new=most_new, return_lse=True)
+
+    S.check_attention()
+    want = call()
+    S.check_attention()
+    try:
+        _cuda.kv4_attention_wait_limit(**limits)
+        got = call()
+        torch.cuda.synchronize()
+    finally:
+        _cuda.kv4_attention_wait_limit()
+    nan = torch.isnan(got[1])
+    assert torch.equal(torch.isnan(got[0]), nan[..., None].expand_as(got[0]))
+    assert all(torch.equal(a[~nan], b[~nan]) for a, b in zip(got, want))
+    if nan.any():
+        with pytest.raises(RuntimeError, match="gave up"):
+            S.check_attention()
+    S.check_attention()
+    again = call()
+    S.check_attention()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    return want, got
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,h,hk,dim", [([40, 12], 32, 8, 64), ([30, 20], 8, 4, 128), ([9, 11], 32, 8, 128), ([33], 1, 1, 64)])
+def test_the_last_wait_of_a_piece_runs_out(S, dtype, counts, h, hk, dim):
+    """The softmax warps' wait for the output gives up by itself, in some lanes and not in others: whole warps go on.  One
+    row tile and two, with rows to spare in each."""
+    case = _tree_case([700, 300][:len(counts)], counts, h, hk, dim, 16, dtype, dim)
+    assert _own_kernel(dtype, dim, h, hk, max(counts))
+    for _ in range(4):
+        _runs_out(S, case, max(counts), output_polls=0)
