@@ -28,8 +28,8 @@
 // 172 us; there the conversion of the keys, for 96 rows, weighs as much (125
 // without it).
 //
-// Every wait is bounded: one that gives up sets the workspace's error word; the
-// rows of the CTA's run, and its parts of shared segments, become NaN.
+// Every wait is bounded: one that gives up sets the workspace's error word; from
+// there on the rows of the CTA's run, and its parts of shared segments, become NaN.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -361,14 +361,15 @@ struct Tree {
         const int t = threadIdx.x >> 7;
         const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;     // this warp's quarter of the tensor memory's lanes
         int u = 0, filled = 0;                                         // steps and pieces done
+        bool alive = true;     // no wait has given up: behind one that has, a barrier's parity says nothing about its phase
         pieces(c0, [&](const Cur& c, const Work& w, bool again, int left, int done) {
             const Row r = begin_segment(c, w);
             const int all_from = __reduce_max_sync(0xffffffffu, r.from), all_to = __reduce_min_sync(0xffffffffu, r.to);
             float base = -INFINITY, l = 0.f;       // base: the running maximum - lift
             uint32_t poisoned = 0;                 // groups of 32 elements in which the row saw a NaN
             const int steps = steps_of(c, t, w.last - w.j0);
-            bool ok = true;
-            for (int i = 0; i < steps; ++i) {
+            bool ok = alive;
+            for (int i = 0; ok && i < steps; ++i) {
                 const int n = done + (PAIR ? i >> 1 : i), st = n & 1, half = PAIR ? i & 1 : t, at = u + i;
                 const int key0 = (w.j0 + (PAIR ? i >> 1 : i)) * kKeys + half * kSub;
                 ok = __all_sync(0xffffffffu, wait(&s.s_full[t], at & 1, &s.dead, a.polls));
@@ -448,7 +449,8 @@ struct Tree {
             if (ok) ok = __all_sync(0xffffffffu, wait(&s.o_full[t], filled & 1, &s.dead, a.output_polls));
             ++filled;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            end_piece(c, r, base, l, poisoned, steps, softmax_any(!ok), again, left, begin + done - (c.u - c.q.k0));
+            alive = !softmax_any(!ok);
+            end_piece(c, r, base, l, poisoned, steps, !alive, again, left, begin + done - (c.u - c.q.k0));
             return true;
         });
     }

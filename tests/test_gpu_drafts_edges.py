@@ -143,3 +143,19 @@ def test_the_last_wait_of_a_piece_runs_out(S, dtype, counts, h, hk, dim):
     assert _own_kernel(dtype, dim, h, hk, max(counts))
     for _ in range(4):
         _runs_out(S, case, max(counts), output_polls=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h,hk,dim,page,most,longest", [(8, 2, 64, 16, 60, 200), (4, 2, 128, 48, 64, 150), (20, 4, 64, 32, 51, 90)])
+def test_segments_behind_a_wait_that_ran_out_are_nan(S, dtype, h, hk, dim, page, most, longest):
+    """CTAs whose runs go on over many segments: behind a wait that gave up none of them passes for whole."""
+    rng = np.random.default_rng(most)
+    counts = [int(c) for c in rng.integers(1, most + 1, 90)]
+    counts[3] = most
+    assert _own_kernel(dtype, dim, h, hk, most)
+    case = _tree_case([int(c) for c in rng.integers(0, longest, 90)], counts, h, hk, dim, page, dtype, most)
+    assert 90 * hk > 148          # more segments than CTAs
+    want, got = _runs_out(S, case, most, polls=0)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[1]).all()
+    for _ in range(3):
+        _runs_out(S, case, most, output_polls=0)
