@@ -952,7 +952,7 @@ def settle_drafts(drafted, parents, picked, starts, lens, table, caches, ring, p
         raise ValueError(f"{who}: an empty ring")
     codes, scales = [c for c, _ in pairs], [b for _, b in pairs]
     at = [c.data_ptr() for c in codes], [b.data_ptr() for b in scales]
-    if n_pages and len(set(at[0])) < len(pairs):
+    if n_pages and any(len(set(a)) < len(pairs) for a in at):
         raise ValueError(f"{who}: the same cache twice")
     s = _on_device(who, dev, drafted, parents, picked, starts, table, ring, pool, masks, *codes, *scales)
     with _on(dev):

@@ -38,3 +38,14 @@ def test_settling_takes_the_masks_of_its_rows(masks):
 def test_settling_takes_masks():
     with pytest.raises(ValueError, match="CUDA"):
         _settle(masks=torch.zeros(5, 2, dtype=I64))
+
+
+def test_caches_must_not_share_an_array():
+    """Each array is moved once: two caches with one array of codes, or of scales, would move it twice."""
+    codes = [torch.zeros(3, 2, 2, 16, 32, dtype=torch.uint8) for _ in range(2)]
+    scales = [torch.zeros(3, 2, 2, 16, 2, dtype=torch.uint8) for _ in range(2)]
+    for caches in ([(codes[0], scales[0]), (codes[1], scales[0])], [(codes[0], scales[0]), (codes[0], scales[1])]):
+        with pytest.raises(ValueError, match="twice"):
+            _settle(caches=caches)
+    with pytest.raises(ValueError, match="CUDA"):
+        _settle(caches=list(zip(codes, scales)))
