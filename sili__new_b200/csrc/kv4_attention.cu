@@ -344,15 +344,18 @@ struct Attend {
                 }
                 // undo the scaling (the scale's sign is in q; not 0, which would undo a mask's -inf); the thread's columns are rows 2t and 2t + 1, held by lanes of g = 2t, 2t + 1
                 const float back = fmaxf(fabsf(a.scale) * kLog2e * __int_as_float((127 - e) << 23), 0x1p-126f);
-                // (shared: all threads read them below.  Stored here too, by the one warp of each tile, they made the
-                // compiler keep a thread's state in local memory where there are two tiles: 40 requests of 4 drafts 276 us
-                // in place of 170, 20 of 16 drafts at dim 256 1513 in place of 419.)
-                if (!kShared) {
+                // (shared: all threads read them below.  Whether the one warp of a tile takes them here as well changes
+                // how the compiler spreads the registers, so both were measured.  With two tiles it made it keep a thread's
+                // state in local memory: 40 requests of 4 drafts 276 us in place of 170, 20 of 16 drafts at dim 256 1513
+                // in place of 419.  With four of dim 128 it is slower: chunks over a window in fp32 250.4 for 246.8 us.
+                // With one tile it is faster: 64 fp32 requests 142.0 for 143.2 us (a spill less), and with four of dim 64:
+                // 6 chunks of 100 rows in fp32 199.4 for 208.2, in fp16 151.2 for 152.6.)
+                constexpr bool kTakes = !kShared || NT == 1 || (NT == 4 && E == 2);
+                if (kTakes) {
                     cf[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
                     cf[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-                } else if (t == 0) {
-                    s_cf[n * 8 + g] = back;
                 }
+                if (kShared && t == 0) s_cf[n * 8 + g] = back;
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
