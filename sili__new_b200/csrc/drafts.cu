@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(128) k_accept(SettleArgs a) {
     auto there = [&](int i) {
         if (!a.masks) return true;
         int64_t any = 0;
-        for (int w = 0; w < a.words; ++w) any |= a.masks[(q.row0 + i) * a.words + w];
+#pragma unroll
+        for (int w = 0; w < kMostWords; ++w) any |= w < a.words ? a.masks[(q.row0 + i) * a.words + w] : 0;
         return any != 0 && i < 64 * a.words;
     };
     int node = q.n > 0 && a.parents[q.row0] == -1 && there(0) ? 0 : -1, kept = 0;
@@ -204,7 +205,10 @@ __global__ void __launch_bounds__(128) k_accept(SettleArgs a) {
         if (want >= 0)
             for (int at = (node + 1) & ~31; at < q.n; at += 32) {
                 const int i = at + lane;
-                const bool is = i > node && i < q.n && a.parents[q.row0 + i] == node && a.drafted[q.row0 + i] == want && there(i);
+                const bool in = i > node && i < q.n;       // (all of a row's loads are asked for at once: a step waits for one)
+                const int up = in ? a.parents[q.row0 + i] : -2;
+                const int64_t own = in ? a.drafted[q.row0 + i] : -2;
+                const bool is = in & there(in ? i : 0) & (up == node) & (own == want);
                 const unsigned hit = __ballot_sync(0xffffffffu, is);
                 if (hit) { child = at + __ffs(hit) - 1; break; }
             }
