@@ -569,8 +569,8 @@ int sili_kv4_tree_attention(int dtype, const void* q, int64_t q_token_stride, in
  *   seen in the request's history, or on the row's path: x > 0 ? x / repetition : x * repetition
  *   c > 0 times in the history behind the prompt and on the path: x - frequency * c - presence
  *   + the bias of v;  / temperature, where that is above 0;  -inf where v is not allowed.
- * Any part may be NULL.  Without starts row r is request r's one row; rows of
- * no request are left as they are. */
+ * Any part may be NULL; repetition and temperature are finite.  Without starts
+ * row r is request r's one row; rows of no request are left as they are. */
 typedef struct sili_logit_rules {
     const int* starts;             /* [requests + 1] or NULL */
     const int* history;            /* [requests, history_width], rows history_stride apart; tokens outside the vocabulary are passed over */

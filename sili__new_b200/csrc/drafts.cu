@@ -5,9 +5,11 @@
 // row's parent before it.  All of it is integer work on little data: bound by
 // launches and the latency of a few loads, except that the accepted rows' keys
 // and values move in every layer's cache.  Calls take what their host side does:
-// 11 us for the plan of 192 requests of up to 250 drafts, 24 for the end of a
-// small step, 41 for one of 96 requests in 12 layers (whose 24 arrays are
-// checked).
+// 11 us for the plan of 192 requests of up to 250 drafts, 25 for the end of a
+// small step, 43 for one of 96 requests in 12 layers (whose 24 arrays are
+// checked).  Two take longer: an accepted way is walked a row at a time (64 rows
+// 32 us, 256 rows 109; 27 and 91 without masks), and the rows of no request are
+// one CTA's beside the requests' (24000 of them: the plan 21 us; 4000: 11).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -345,7 +347,7 @@ int sili_draft_tree(const int* parents, const int* starts, const int* lens, int 
     if (tokens == 0) return SILI_OK;
     if (!parents || !masks || !positions || (requests && (!starts || !lens))) return bad(who, "null array");
     PlanArgs a{parents, starts, lens, requests, tokens, words, window, masks, positions};
-    // one CTA a request, and some for the rows of none (seldom many)
+    // one CTA a request, and for the rows of none one more, or as many as they fill where there are no requests
     const int64_t extra = requests ? 1 : std::min<int64_t>((tokens + 255) / 256, 148);
     if (requests + extra > 0x7fffffffLL) return bad(who, "sizes out of range");
     k_draft_tree<<<(unsigned)(requests + extra), 64 * words, 0, (cudaStream_t)stream>>>(a);

@@ -35,10 +35,13 @@
 //
 // Drafted tokens' trees (TREE): a row sees the committed keys, as its window
 // leaves them, and of the request's own those that its mask names; the masks of
-// a row tile lie in shared memory.  16-bit trees of more than 32 rows a request
-// run in kv4_tree.cu.  24 requests of up to 16 drafts over up to 8192 keys in fp32
-// (121 MB, 18 us at the copy rate): 360 us, bound by instructions: every tile
-// of 16 rows decodes the keys again and multiplies two terms.
+// a row tile lie in shared memory.  16-bit trees of dim 64 and 128 with more than
+// 32 rows a request run in kv4_tree.cu.  24 requests of up to 16 drafts over up to
+// 8192 keys in fp32 (121 MB, 18 us at the copy rate): 367 us, bound by
+// instructions: every tile of 16 rows decodes the keys again and multiplies two
+// terms.  40 requests over 2k-12k keys in bf16 (32 heads over 8, dim 128): of 2
+// drafts 106 us, 4 165, 8 263, against 48 for the bytes: the instructions above,
+// and wider tiles' products, with a CTA an SM in place of two from 4 drafts on.
 //
 // What bounds it, 96 requests of 2k-16k keys, 32 heads over 8, dim 128, bf16
 // (0.96 GB, 146 us at the card's copy rate): 271 us, 3.5 TB/s.  A warp's 16
@@ -814,8 +817,11 @@ int launch(const AttendArgs& a, cudaStream_t s) {
 template <typename T, int E, bool TREE>
 int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
     if (rows <= 8) return launch<T, E, 1, TREE>(a, s);
-    // (a tree's rows in fp32, whose two terms and masks leave 32 of them no registers: 24 requests of 16 drafts over up to
-    // 8192 keys took 463 us, in tiles of 16 rows 376)
+    // (A tree's rows in fp32, whose two terms and masks leave 32 of them no registers, go in tiles of 16.  us in tiles of 16 |
+    // 32, 32 heads over 8: dim 128, 24 requests of 16 drafts over up to 8192 keys 367 | 393, 40 over 2k-12k keys of 5 drafts
+    // 297 | 372, of 8 396 | 384; dim 64, the same 40 of 5 drafts 212 | 213, of 8 283 | 220, of 64 1707 | 1312, 4 of 16 over up
+    // to 700 keys 24 | 34.  So at dim 64 the other side would be the better one for long batches, whose lengths are not known
+    // here.)
     if (rows <= 16 || E == 8 || (TREE && sizeof(T) == 4)) return launch<T, E, 2, TREE>(a, s);
     return launch<T, E, E == 8 || (TREE && sizeof(T) == 4) ? 2 : 4, TREE>(a, s);
 }

@@ -20,12 +20,12 @@
 // kv4_prompt.cu; a row's sums leave tensor memory every kPiece units.
 //
 // What bounds it, 40 requests of up to 64 drafts over 2k-12k keys, 32 heads over
-// 8, dim 128, bf16 (233 GFLOP, 143 us at the card's matrix rate): 443 us, 526
-// TFLOP/s, tensor pipe 35 %, issue 50 %.  With the conversions, loads,
+// 8, dim 128, bf16 (233 GFLOP, 143 us at the card's matrix rate): 444-459 us
+// from card to card, 520 TFLOP/s, tensor pipe 35 %, issue 50 %.  With the conversions, loads,
 // exponentials and most products left out it took 328: a step is the softmax
 // warps' chain (scores' barrier, tensor-memory load, maximum, exponentials,
 // store), two of its warps a scheduler.  24 drafts over 131071 keys (52 GFLOP):
-// 172 us; there the conversion of the keys, for 96 rows, weighs as much (125
+// 173 us; there the conversion of the keys, for 96 rows, weighs as much (125
 // without it).
 //
 // Every wait is bounded: one that gives up sets the workspace's error word; from
@@ -717,12 +717,17 @@ int by_rows(const AttendArgs& a, int64_t rows, cudaStream_t s) {
 
 namespace sili {
 
-// us of this kernel | the one of kv4_attention.cu, by rows a request (32 heads over 8 x 128):
-//   1 request, 131071 keys, fp16:    32 rows 167 | 121, 36: 168 | 198, 64: 170 | 200, 128: 179 | 364
-//   40 requests, 2k-12k keys, bf16:  32 rows 348 | 268, 36: 350 | 328, 48: 347 | 409, 128: 376 | 850, 256: 453 | 1618
-//   the same up to 1000 keys:        32 rows 119 | 111, 36: 117 | 118, 64: 122 | 201
-//   4 requests up to 700 keys:       32 rows  28 |  24, 48:  28 |  26, 64:  28 |  42
-// The other one walks tiles of up to 32 rows, so it is taken up to there.
+// us of this kernel | the one of kv4_attention.cu, by rows that every request has (32 heads over 8):
+//   dim 128, 1 request, 131071 keys, fp16:    32 rows 166 | 119, 36: 166 | 200, 64: 168 | 200, 128: 178 | 368
+//   dim 128, 40 requests, 2k-12k keys, bf16:  32 rows 344 | 264, 36: 343 | 487, 64: 349 | 495, 128: 378 | 978, 256: 460 | 1898
+//   dim 128, the same up to 1000 keys:        32 rows 124 | 114, 36: 127 | 181, 64: 121 | 181, 256: 209 | 799
+//   dim 128, 4 requests up to 700 keys:       32 rows  30 |  27, 36:  30 |  41, 64:  30 |  44, 256:  40 |  59
+//   dim 64, 1 request, 131071 keys, fp16:     32 rows 114 |  78, 36: 114 | 126, 64: 116 | 126, 128: 121 | 226
+//   dim 64, 40 requests, 2k-12k keys, bf16:   32 rows 237 | 170, 36: 235 | 307, 64: 239 | 314, 256: 365 | 1178
+//   dim 64, the same up to 1000 keys:         32 rows  79 |  83, 36:  81 | 130, 64:  77 | 130, 256: 127 | 546
+//   dim 64, 4 requests up to 700 keys:        32 rows  24 |  22, 36:  24 |  33, 64:  24 |  34, 256:  32 |  44
+// The other one walks tiles of up to 32 rows, so it is taken up to there.  `rows` comes from the caller's largest number of
+// queries (or their average, without a hint); requests that have fewer, up to 32 rows, would be faster in the other one.
 bool kv4_tree_takes(int dtype, int dim, int64_t rows) { return dtype != SILI_F32 && (dim == 64 || dim == 128) && rows > 32; }
 
 int64_t kv4_tree_workspace(int dim, int64_t rows) {

@@ -18,13 +18,14 @@
 // part of the row is read again, since the division may have made neighbours
 // equal.  So the logits' bytes are what should bound a large call.  With the
 // counts in the streaming CTAs, 32 trees of 32 over 131072 tokens took 252 us
-// in place of 125 (a vocabulary's most frequent tokens lie close together, and
-// their CTAs were the last by far); with the touched tokens in a launch of
-// their own, which fetches them once more, 140. Now 120: the pass 97, 4.2
+// (a vocabulary's most frequent tokens lie close together, and their CTAs were
+// the last by far); with the touched tokens in a launch of their own, which fetches them once more, 140.  Now 120: the pass 97, 4.2
 // TB/s, with the chain of loads before a row's (its request, bits, rules, list)
 // and 20 instructions an element and warp, a quarter of them the most frequent
 // tokens' rules; without history, drafts and mask it takes 65.  444 rows of
-// 131072 adjusted in bf16: 78 us.
+// 131072 adjusted in bf16: 78 us.  A decode step takes what its host side and
+// its launches take, 24 us for 16 rows of 32000 adjusted; as one launch without
+// scratch space, which took 324 us in place of those 78, it was 18.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ L
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // The parts of the scratch space, one after the other from `base` on; returns its bytes.
-int64_t lay_out(LogitArgs& a, int dtype, bool counts, bool pick, uint8_t* base) {
+int64_t lay_out(LogitArgs& a, bool counts, bool pick, uint8_t* base) {
     int64_t at = 0;
     auto part = [&](int64_t bytes) { const int64_t here = at; at += round16(bytes); return base + here; };
     a.tiles = (a.vocab + kTile - 1) / kTile;
@@ -685,7 +686,7 @@ int prepare(const char* who, int dtype, const void* logits, int64_t stride, int6
     a.biases = q.biases;
     a.allowed = q.allowed;
     a.allowed_stride = q.allowed_stride;
-    const int64_t need = lay_out(a, dtype, (a.history || a.biases) && requests, pick, (uint8_t*)scratch);
+    const int64_t need = lay_out(a, (a.history || a.biases) && requests, pick, (uint8_t*)scratch);
     if (rows * a.tiles > 0x7fffffffLL || (int64_t)requests * a.tiles > 0x7fff0000LL) return bad(who, "sizes out of range");
     if (bytes) { *bytes = need; return SILI_OK; }
     if (rows == 0) return SILI_OK;

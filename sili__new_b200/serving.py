@@ -859,7 +859,7 @@ def adjust_logits(logits, starts=None, history=None, history_lens=None, prompt_l
         x = -inf                                                 # bit v % 32 of allowed[row, v // 32] (int32) is not set
 
     ``repetition``, ``presence``, ``frequency``, ``temperature``: float32
-    [requests]; every part may be left out.  A token that is listed twice gets
+    [requests], the first and the last finite; every part may be left out.  A token that is listed twice gets
     the sum of its biases.  Rows of no request are left as they are.  Returns
     ``out`` (which may be the logits) in the logits' type."""
     who = "adjust_logits"
