@@ -5,8 +5,8 @@
 // row's parent before it.  All of it is integer work on little data: bound by
 // launches and the latency of a few loads, except that the accepted rows' keys
 // and values move in every layer's cache.  Calls take what their host side does:
-// 11 us for the plan of 192 requests of up to 250 drafts, 25 for the end of a
-// small step, 43 for one of 96 requests in 12 layers (whose 24 arrays are
+// 11 us for the plan of 192 requests of up to 250 drafts, 26 for the end of a
+// small step, 44 for one of 96 requests in 12 layers (whose 24 arrays are
 // checked).  Two take longer: an accepted way is walked a row at a time (64 rows
 // 32 us, 256 rows 109; 27 and 91 without masks), and the rows of no request are
 // one CTA's beside the requests' (24000 of them: the plan 21 us; 4000: 11).

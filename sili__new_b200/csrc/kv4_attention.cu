@@ -37,7 +37,7 @@
 // leaves them, and of the request's own those that its mask names; the masks of
 // a row tile lie in shared memory.  16-bit trees of dim 64 and 128 with more than
 // 32 rows a request run in kv4_tree.cu.  24 requests of up to 16 drafts over up to
-// 8192 keys in fp32 (121 MB, 18 us at the copy rate): 367 us, bound by
+// 8192 keys in fp32 (121 MB, 18 us at the copy rate): 371 us, bound by
 // instructions: every tile of 16 rows decodes the keys again and multiplies two
 // terms.  40 requests over 2k-12k keys in bf16 (32 heads over 8, dim 128): of 2
 // drafts 106 us, 4 165, 8 263, against 48 for the bytes: the instructions above,

@@ -19,10 +19,10 @@
 // equal.  So the logits' bytes are what should bound a large call.  With the
 // counts in the streaming CTAs, 32 trees of 32 over 131072 tokens took 252 us
 // (a vocabulary's most frequent tokens lie close together, and their CTAs were
-// the last by far); with the touched tokens in a launch of their own, which fetches them once more, 140.  Now 120: the pass 97, 4.2
-// TB/s, with the chain of loads before a row's (its request, bits, rules, list)
-// and 20 instructions an element and warp, a quarter of them the most frequent
-// tokens' rules; without history, drafts and mask it takes 65.  444 rows of
+// the last by far); with the touched tokens in a launch of their own, which
+// fetches them once more, 140.  Now 120: the pass 97, 4.2 TB/s, with the chain
+// of loads before a row's (its request, bits, rules, list) and 20 instructions
+// an element and warp, a quarter of them the most frequent tokens' rules; without history, drafts and mask it takes 65.  444 rows of
 // 131072 adjusted in bf16: 78 us.  A decode step takes what its host side and
 // its launches take, 24 us for 16 rows of 32000 adjusted; as one launch without
 // scratch space, which took 324 us in place of those 78, it was 18.
